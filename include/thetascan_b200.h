@@ -537,6 +537,80 @@ typedef struct ts_gn_prep_args {
 int ts_b200_gn_prep_fwd(const ts_gn_prep_args* args, ts_stream_t stream);
 int ts_b200_gn_prep_bwd(const ts_gn_prep_args* args, ts_stream_t stream);
 
+/* ------------------------------------------------------------------ norm
+ * Root-mean-square norm of `rows` rows of `width` channels, with the
+ * residual's addition: s = round(x + residual) (x itself without a residual),
+ * y = s * rstd * weight, rstd = (mean s^2 + eps)^(-1/2).  No reference
+ * counterpart (its host model's norm): the rest of a block around the mixer.
+ * Rows have contiguous channels and any row stride; outputs are contiguous.
+ * With `scales`, y receives e4m3 codes of y / scale, scale = max(max|y|,
+ * 2^-100) / 448 over the row (group 0) or over each 128 columns (group 128,
+ * scales [rows, ceil(width/128)]).  The backward reads as x the STORED sum. */
+typedef struct ts_norm_args {
+  long long rows;
+  int width;                /* 1..16384 */
+  int dtype;                /* of x, residual, y, sum */
+  int weight_dtype;
+  float eps;
+  const void* x;
+  const void* residual;     /* or NULL */
+  const void* weight;       /* [width] */
+  long long x_stride, residual_stride;   /* elements between rows */
+  void* y;                  /* [rows,width], dtype (or 8-bit codes with scales) */
+  void* sum;                /* [rows,width], dtype: required with a residual */
+  float* rstd;              /* [rows]: written by the forward (or NULL), read by the backward */
+  float* scales;
+  int group;                /* 0 or 128 */
+} ts_norm_args;
+
+typedef struct ts_norm_grad_args {
+  const void* dy;           /* dtype */
+  const void* dsum;         /* dtype, gradient of the stored sum, or NULL */
+  long long dy_stride, dsum_stride;
+  void* dx;                 /* [rows,width], dtype: the gradient of x and of the residual */
+  void* dweight;            /* [width], weight_dtype */
+  void* workspace;
+  size_t workspace_bytes;
+} ts_norm_grad_args;
+
+int ts_b200_norm_fwd(const ts_norm_args* args, ts_stream_t stream);
+size_t ts_b200_norm_bwd_workspace_bytes(const ts_norm_args* args);
+int ts_b200_norm_bwd(const ts_norm_args* args, const ts_norm_grad_args* grads, ts_stream_t stream);
+
+/* ----------------------------------------------------------------- adamw
+ * One AdamW step (decoupled weight decay) over `count` tensors of one kind:
+ *   m <- b1 m + (1-b1) g, v <- b2 v + (1-b2) g^2,
+ *   p <- p (1 - lr wd) - lr/(1-b1^t) m / (sqrt(v/(1-b2^t)) + eps).
+ * state_bits 32: f32 m and v.  state_bits 8: e4m3 codes of m and of sqrt(v)
+ * with an f32 scale (max|x|/448) for each 256 elements, rounded
+ * stochastically by a hash of (seed, step, ordinal, element).  Tensors are
+ * flat memory of n elements; n = 0 is allowed.  Nothing is kept between
+ * calls.  No reference counterpart (its host's optimizer). */
+typedef struct ts_adamw_tensor {
+  void* param;              /* param_dtype */
+  const void* grad;         /* grad_dtype */
+  float* master;            /* f32 value behind a bf16 parameter (args.master), else NULL */
+  void* exp_avg;            /* f32, or e4m3 codes */
+  void* exp_avg_sq;         /* f32 v, or e4m3 codes of sqrt(v) */
+  float* exp_avg_scale;     /* [ceil(n/256)] with 8-bit states */
+  float* exp_avg_sq_scale;
+  long long n;
+  int ordinal;              /* the tensor's place in the whole step (keys its rounding) */
+} ts_adamw_tensor;
+
+typedef struct ts_adamw_args {
+  int count;
+  const ts_adamw_tensor* tensors;   /* HOST memory, read during the call */
+  int param_dtype, grad_dtype;
+  int master;               /* nonzero: bf16 parameters with f32 masters */
+  int state_bits;           /* 32 or 8 */
+  long long step;           /* t >= 1 */
+  double lr, beta1, beta2, eps, weight_decay;
+  long long seed;
+} ts_adamw_args;
+
+int ts_b200_adamw(const ts_adamw_args* args, ts_stream_t stream);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif

@@ -1,0 +1,271 @@
+"""The AdamW step's kernel against its formula in float64.
+
+Bounds, derived before any run: the step is a few f32 operations (the quotient
+by an approximate division, 2 units in the last place), so the parameter's
+change is within 1e-6 of itself and the result within a unit in the last
+place of its type; the moments are two products and a sum, within 2^-22.  An
+8-bit code lies within one of its steps (1/8 of the value, or 2^-9 of the
+scale) of the f32 value.
+"""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+gpu = pytest.mark.gpu
+BF16, F32, E4M3 = torch.bfloat16, torch.float32, torch.float8_e4m3fn
+HYPER = dict(lr=3e-3, betas=(0.9, 0.95), eps=1e-8, weight_decay=0.1)
+SIZES = (1, 7, 8, 255, 256, 257, 1000, 4096, 4099, 70001)
+
+
+@pytest.fixture(scope="module")
+def optim():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a CUDA device")
+    from thetascan_b200 import optim
+    return optim
+
+
+def _formula(p, g, m, v, step, lr, betas, eps, weight_decay):
+    b1, b2 = betas
+    m = b1 * m + (1 - b1) * g
+    v = b2 * v + (1 - b2) * g * g
+    return p - lr * weight_decay * p - lr / (1 - b1 ** step) * m / ((v / (1 - b2 ** step)).sqrt() + eps), m, v
+
+
+def _case(sizes, pdtype, gdtype, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    r = lambda n, s=1.0: (torch.randn(n, generator=gen) * s).cuda()  # noqa: E731
+    ps = [r(n) for n in sizes]
+    gs = [r(n, 0.01).to(gdtype) for n in sizes]
+    ms = [r(n, 0.01) for n in sizes]
+    vs = [r(n, 0.01).square() for n in sizes]
+    return [p.to(pdtype) for p in ps], gs, ms, vs, ps
+
+
+def _within_ulp(got, want, dtype, slack):
+    ulp = want.abs() * (2.0 ** -8 if dtype == BF16 else 2.0 ** -23)
+    assert ((got.double() - want).abs() <= ulp + slack).all()
+
+
+@gpu
+@pytest.mark.parametrize("pdtype,gdtype", [(F32, F32), (F32, BF16), (BF16, BF16), (BF16, F32)])
+@pytest.mark.parametrize("master", [False, True])
+def test_step_is_the_formulas(optim, pdtype, gdtype, master):
+    if master and pdtype == F32:
+        pytest.skip("masters belong to bf16 parameters")
+    ps, gs, ms, vs, p32 = _case(SIZES, pdtype, gdtype)
+    start = [(p32[i] if master else ps[i]).double() for i in range(len(SIZES))]
+    want = [_formula(p, g.double(), m.double(), v.double(), 5, **HYPER) for p, g, m, v in zip(start, gs, ms, vs)]
+    optim.adamw_step(ps, gs, ms, vs, step=5, **HYPER, masters=p32 if master else None)
+    for i, (p, m, v) in enumerate(want):
+        change = (p - start[i]).abs()
+        _within_ulp(ps[i], p, pdtype, 1e-6 * change)
+        if master:
+            _within_ulp(p32[i], p, F32, 1e-6 * change)
+        assert ((ms[i].double() - m).abs() <= 2.0 ** -22 * (m.abs() + 0.02)).all()
+        assert ((vs[i].double() - v).abs() <= 2.0 ** -22 * v + 1e-40).all()
+
+
+def _decode(codes, scales):
+    return codes.double() * scales.double().repeat_interleave(256)[:codes.numel()]
+
+
+@gpu
+@pytest.mark.parametrize("pdtype,gdtype,master", [(F32, F32, False), (BF16, BF16, False), (BF16, F32, True)])
+def test_8bit_step(optim, pdtype, gdtype, master):
+    ps, gs, _, _, p32 = _case(SIZES, pdtype, gdtype, seed=2)
+    zeros = lambda k: [torch.zeros(n, device="cuda", dtype=k) for n in SIZES]  # noqa: E731
+    scales = lambda: [torch.zeros(optim.state_scales(n), device="cuda") for n in SIZES]  # noqa: E731
+    m, r, ms, rs = zeros(E4M3), zeros(E4M3), scales(), scales()
+    for step in (1, 2, 3):
+        start = [(p32[i] if master else ps[i]).double() for i in range(len(SIZES))]
+        want = [_formula(p, g.double(), _decode(a, sa), _decode(b, sb).square(), step, **HYPER)
+                for p, g, a, sa, b, sb in zip(start, gs, m, ms, r, rs)]
+        optim.adamw_step(ps, gs, m, r, step=step, **HYPER, masters=p32 if master else None, exp_avg_scales=ms,
+                         exp_avg_sq_scales=rs, seed=11)
+        for i, (p, first, second) in enumerate(want):
+            _within_ulp(ps[i], p, pdtype, 2e-6 * (p - start[i]).abs())
+            for value, codes, scale in ((first, m[i], ms[i]), (second.sqrt(), r[i], rs[i])):
+                top = torch.stack([b.abs().max() for b in value.split(256)])
+                assert ((scale.double() * 448 - top).abs() <= 1e-6 * top).all()
+                each = scale.double().repeat_interleave(256)[:value.numel()]
+                off = (_decode(codes, scale) - value).abs()
+                assert (off <= (value.abs() / 8).maximum(each * 2.0 ** -9) * (1 + 1e-5)).all()
+            assert ((r[i].float() > 0) | (second == 0)).all()
+
+
+@gpu
+def test_8bit_rounding_is_right_on_average(optim):
+    # one value 0.3 of the block's largest in every element but one: its code is one of two neighbours; over n
+    # elements the mean is within 5 standard deviations, 5 * step / 2 / sqrt(n), of the value
+    n = 256 * 400
+    g = torch.full((n,), 0.3, device="cuda")
+    g[::256] = 1.0
+    args = [[torch.zeros(n, device="cuda", dtype=E4M3)] for _ in range(2)]
+    scales = [[torch.zeros(n // 256, device="cuda")] for _ in range(2)]
+    p = [torch.zeros(n, device="cuda")]
+    optim.adamw_step(p, [g], *args, step=1, **HYPER, exp_avg_scales=scales[0], exp_avg_sq_scales=scales[1], seed=5)
+    for codes, scale, value in ((args[0][0], scales[0][0], 0.1 * 0.3), (args[1][0], scales[1][0], math.sqrt(0.05) * 0.3)):
+        x = _decode(codes, scale).view(-1, 256)[:, 1:]
+        step = float(x.max() - x.min())
+        assert 0 < step <= value / 8 * 1.001
+        assert abs(float(x.mean()) - value) <= 5 * step / 2 / math.sqrt(x.numel())
+
+
+@gpu
+def test_8bit_rounding_follows_its_key(optim):
+    def once(seed, ordinals):
+        ps, gs, _, _, _ = _case((5000, 5000), F32, F32)
+        gs[1] = gs[0]
+        m, r = ([torch.zeros(5000, device="cuda", dtype=E4M3) for _ in range(2)] for _ in range(2))
+        ms, rs = ([torch.zeros(20, device="cuda") for _ in range(2)] for _ in range(2))
+        optim.adamw_step(ps, gs, m, r, step=1, **HYPER, exp_avg_scales=ms, exp_avg_sq_scales=rs, seed=seed,
+                         ordinals=ordinals)
+        return [t.view(torch.uint8) for t in m + r]
+
+    a = once(1, [0, 1])
+    assert all(torch.equal(x, y) for x, y in zip(a, once(1, [0, 1])))
+    assert not torch.equal(a[0], a[1]) and not torch.equal(a[0], once(2, [0, 1])[0])
+    assert torch.equal(a[1], once(1, [1, 0])[0])
+
+
+@gpu
+def test_many_tensors_mixed_kinds_and_alignment(optim):
+    # more tensors than one launch takes, sizes of zero among them, views that start at odd elements
+    gen = torch.Generator().manual_seed(8)
+    sizes = [int(torch.randint(0, 700, (1,), generator=gen)) for _ in range(900)]
+    flat = [torch.randn(sum(sizes) + 900, generator=gen).cuda() for _ in range(3)]
+    flat.append(torch.rand(sum(sizes) + 900, generator=gen).cuda())
+    lists, at = [[] for _ in flat], 0
+    for i, n in enumerate(sizes):
+        for x, f in zip(lists, flat):
+            x.append(f[at + i:at + i + n])
+        at += n
+    ps = [p.to(BF16) if i % 3 == 0 else p.clone() for i, p in enumerate(lists[0])]
+    want = [_formula(p.double(), g.double(), m.double(), v.double(), 2, **HYPER) for p, g, m, v in zip(ps, *lists[1:])]
+    start = [p.double() for p in ps]
+    optim.adamw_step(ps, lists[1], lists[2], lists[3], step=2, **HYPER)
+    for p, m, v, (wp, wm, wv), s in zip(ps, lists[2], lists[3], want, start):
+        _within_ulp(p, wp, p.dtype, 1e-6 * (wp - s).abs())
+        assert ((m.double() - wm).abs() <= 2.0 ** -22 * (wm.abs() + 2)).all()
+        assert ((v.double() - wv).abs() <= 2.0 ** -21 * wv).all()
+
+
+@gpu
+def test_8bit_special_values(optim):
+    n = 1024
+    g = torch.zeros(n, device="cuda")
+    g[300] = float("nan")
+    g[600] = 1e-30
+    m, r = (torch.zeros(n, device="cuda", dtype=E4M3) for _ in range(2))
+    ms, rs = (torch.zeros(4, device="cuda") for _ in range(2))
+    p = torch.ones(n, device="cuda")
+    optim.adamw_step([p], [g], [m], [r], step=1, **HYPER, exp_avg_scales=[ms], exp_avg_sq_scales=[rs])
+    bad = torch.zeros(n, dtype=torch.bool, device="cuda")
+    bad[300] = True
+    assert torch.equal(p.isnan(), bad) and torch.equal(m.float().isnan(), bad) and torch.equal(r.float().isnan(), bad)
+    assert ms.isfinite().all() and rs.isfinite().all()
+    assert (m.float()[:256] == 0).all() and (r.float()[:256] == 0).all()
+
+
+@gpu
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype,master", [(F32, False), (BF16, True)])
+def test_optimizer_learns_and_resumes(optim, bits, dtype, master):
+    # a quadratic bowl from the origin: Adam moves about lr a step, so 300 steps of 1e-2 reach targets within 1
+    torch.manual_seed(0)
+    target = torch.rand(33, 65, device="cuda") * 2 - 1
+    make = lambda ps: optim.AdamW(ps, lr=1e-2, betas=(0.9, 0.95), weight_decay=0.0, state_bits=bits, master_weights=master)  # noqa: E731
+
+    def steps(p, frozen, opt, count):
+        for _ in range(count):
+            opt.zero_grad()
+            ((p.float() - target).square().sum() * 0.5).backward()
+            opt.step()
+
+    p = torch.zeros(33, 65, device="cuda", dtype=dtype, requires_grad=True)
+    frozen = torch.zeros(4, device="cuda", requires_grad=True)
+    opt = make([p, frozen])
+    steps(p, frozen, opt, 300)
+    assert float((p.float() - target).abs().mean()) < 0.02 and (frozen == 0).all()
+    q = p.detach().clone().requires_grad_(True)
+    again = make([q, frozen])
+    again.load_state_dict(opt.state_dict())
+    for k, v in opt.state[p].items():
+        w = again.state[q][k]
+        assert w == v if k == "step" else (w.dtype == v.dtype and w is not v and torch.equal(w.view(torch.uint8), v.view(torch.uint8)))
+    steps(p, frozen, opt, 3)
+    steps(q, frozen, again, 3)
+    assert torch.equal(p, q)
+
+
+@gpu
+def test_optimizer_groups_follow_torch(optim):
+    # the same steps as torch.optim.AdamW on its single-tensor path; both are f32, so a few units in the last place apart
+    torch.manual_seed(1)
+    a = [torch.randn(n, device="cuda", requires_grad=True) for n in (5, 300, 4097)]
+    b = [t.detach().clone().requires_grad_(True) for t in a]
+    groups = lambda x: [dict(params=x[:2], lr=1e-3), dict(params=x[2:], weight_decay=0.0)]  # noqa: E731
+    ours, theirs = optim.AdamW(groups(a), lr=2e-3), torch.optim.AdamW(groups(b), lr=2e-3, foreach=False)
+    for i in range(5):
+        for x, y in zip(a, b):
+            x.grad = torch.randn_like(x)
+            y.grad = x.grad.clone()
+        if i == 2:
+            a[1].grad = b[1].grad = None   # its count of steps falls behind the others'
+        ours.step()
+        theirs.step()
+    for x, y in zip(a, b):
+        assert ((x - y).abs() <= 1e-6 * (1 + y.abs())).all()
+
+
+@gpu
+def test_refusals(optim):
+    p, g, m, v = ([torch.ones(300, device="cuda")] for _ in range(4))
+    ok = dict(step=1, **HYPER)
+    optim.adamw_step([], [], [], [], **ok)
+    for bad in (dict(step=0), dict(step=1.5), dict(betas=(1.0, 0.9)), dict(lr=-1.0), dict(eps=-1.0)):
+        with pytest.raises(ValueError):
+            optim.adamw_step(p, g, m, v, **{**ok, **bad})
+    for lists in ((p, [], m, v), (p, g, [], v), (p, [g[0][:299]], m, v), (p, g, [m[0].bfloat16()], v), ([p[0].half()], g, m, v),
+                  (p, [g[0].half()], m, v), ([torch.ones(10, 30, device="cuda").T], g, m, v), (p, [g[0].cpu()], m, v)):
+        with pytest.raises(ValueError):
+            optim.adamw_step(*lists, **ok)
+    with pytest.raises(ValueError):
+        optim.adamw_step(p, g, m, v, **ok, masters=[p[0].clone()])
+    with pytest.raises(ValueError):
+        optim.adamw_step(p, g, m, v, **ok, exp_avg_scales=[m[0][:2]], exp_avg_sq_scales=[m[0][:2]])
+    code = [torch.zeros(300, device="cuda", dtype=E4M3)]
+    with pytest.raises(ValueError):
+        optim.adamw_step(p, g, code, code, **ok)
+    with pytest.raises(ValueError):
+        optim.adamw_step(p, g, code, code, **ok, exp_avg_scales=[m[0][:1]], exp_avg_sq_scales=[m[0][:2]])
+    assert (p[0] == 1).all()
+    for bad in (dict(state_bits=16), dict(lr=-1.0), dict(betas=(0.9, 1.0))):
+        with pytest.raises(ValueError):
+            optim.AdamW([torch.ones(3, device="cuda", requires_grad=True)], **bad)
+    with pytest.raises(ValueError):
+        optim.AdamW([torch.ones(3, 4, device="cuda").T.requires_grad_(True)])
+    with pytest.raises(RuntimeError):
+        optim.adamw_step([torch.ones(3)], [torch.ones(3)], [torch.ones(3)], [torch.ones(3)], **ok)
+
+
+def test_c_entry_refuses_bad_arguments():
+    import ctypes
+    from thetascan_b200 import _lib
+    lib = _lib.load()
+    assert lib.ts_b200_adamw(None, None) == _lib.TS_ERR_VALUE
+    t = _lib.AdamWTensor()
+    t.n = 4
+    a = _lib.AdamWArgs()
+    a.count, a.tensors, a.step, a.state_bits = 1, ctypes.addressof(t), 1, 32
+    assert lib.ts_b200_adamw(ctypes.byref(a), None) == _lib.TS_ERR_VALUE      # null pointers
+    a.state_bits = 16
+    assert lib.ts_b200_adamw(ctypes.byref(a), None) == _lib.TS_ERR_NOT_IMPLEMENTED
+    a.state_bits, a.step = 32, 0
+    assert lib.ts_b200_adamw(ctypes.byref(a), None) == _lib.TS_ERR_VALUE
+    a.step, a.master = 1, 1
+    assert lib.ts_b200_adamw(ctypes.byref(a), None) == _lib.TS_ERR_VALUE      # a master behind an f32 parameter

@@ -6,6 +6,8 @@ Public surface (mirrors the reference package ``thetascan``):
   its configuration, state-dict compatible with the reference;
 * ``scan``: the scan-backend contract (``linattn_views`` / ``linattn``);
 * ``kernel.kernel_core``: the fused kernel-family hot path;
+* ``rms_norm`` / ``add_rms_norm`` / ``rms_norm_8bit``: the norms around it;
+* ``AdamW`` / ``adamw_step``: the optimizer step over many tensors;
 * ``integration.install()``: register ``backend="b200"`` in an installed
   reference package.
 
@@ -16,9 +18,12 @@ from __future__ import annotations
 from .config import (GNConfig, KernelConfig, RegularizationConfig, RoPEConfig, RuntimeConfig,
                      TemporalConfig, ThetaScanConfig)
 from .mixer import ThetaScan
+from .norm import add_rms_norm, rms_norm, rms_norm_8bit
+from .optim import AdamW, adamw_step
 
 __version__ = "0.1.0"
 BACKEND_NAME = "b200"
 
 __all__ = ["GNConfig", "KernelConfig", "RegularizationConfig", "RoPEConfig", "RuntimeConfig",
-           "TemporalConfig", "ThetaScan", "ThetaScanConfig", "BACKEND_NAME"]
+           "TemporalConfig", "ThetaScan", "ThetaScanConfig", "BACKEND_NAME",
+           "AdamW", "adamw_step", "add_rms_norm", "rms_norm", "rms_norm_8bit"]

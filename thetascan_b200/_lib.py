@@ -10,6 +10,8 @@ import ctypes
 import os
 import threading
 
+import torch
+
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libthetascan_b200.so")
 
@@ -184,6 +186,54 @@ SIGNATURES.update({
     "ts_b200_gn_prep_bwd": (ctypes.c_int, [ctypes.POINTER(GnPrepArgs), ctypes.c_void_p]),
 })
 
+
+
+class NormArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", ctypes.c_longlong), ("width", ctypes.c_int), ("dtype", ctypes.c_int),
+        ("weight_dtype", ctypes.c_int), ("eps", ctypes.c_float),
+        ("x", ctypes.c_void_p), ("residual", ctypes.c_void_p), ("weight", ctypes.c_void_p),
+        ("x_stride", ctypes.c_longlong), ("residual_stride", ctypes.c_longlong),
+        ("y", ctypes.c_void_p), ("sum", ctypes.c_void_p), ("rstd", ctypes.c_void_p),
+        ("scales", ctypes.c_void_p), ("group", ctypes.c_int),
+    ]
+
+
+class NormGradArgs(ctypes.Structure):
+    _fields_ = [
+        ("dy", ctypes.c_void_p), ("dsum", ctypes.c_void_p),
+        ("dy_stride", ctypes.c_longlong), ("dsum_stride", ctypes.c_longlong),
+        ("dx", ctypes.c_void_p), ("dweight", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class AdamWTensor(ctypes.Structure):
+    _fields_ = [
+        ("param", ctypes.c_void_p), ("grad", ctypes.c_void_p), ("master", ctypes.c_void_p),
+        ("exp_avg", ctypes.c_void_p), ("exp_avg_sq", ctypes.c_void_p),
+        ("exp_avg_scale", ctypes.c_void_p), ("exp_avg_sq_scale", ctypes.c_void_p),
+        ("n", ctypes.c_longlong), ("ordinal", ctypes.c_int),
+    ]
+
+
+class AdamWArgs(ctypes.Structure):
+    _fields_ = [
+        ("count", ctypes.c_int), ("tensors", ctypes.c_void_p),
+        ("param_dtype", ctypes.c_int), ("grad_dtype", ctypes.c_int),
+        ("master", ctypes.c_int), ("state_bits", ctypes.c_int), ("step", ctypes.c_longlong),
+        ("lr", ctypes.c_double), ("beta1", ctypes.c_double), ("beta2", ctypes.c_double),
+        ("eps", ctypes.c_double), ("weight_decay", ctypes.c_double), ("seed", ctypes.c_longlong),
+    ]
+
+
+SIGNATURES.update({
+    "ts_b200_adamw": (ctypes.c_int, [ctypes.POINTER(AdamWArgs), ctypes.c_void_p]),
+    "ts_b200_norm_fwd": (ctypes.c_int, [ctypes.POINTER(NormArgs), ctypes.c_void_p]),
+    "ts_b200_norm_bwd_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(NormArgs)]),
+    "ts_b200_norm_bwd": (ctypes.c_int, [ctypes.POINTER(NormArgs), ctypes.POINTER(NormGradArgs), ctypes.c_void_p]),
+})
+
 _lock = threading.Lock()
 _lib = None
 
@@ -208,6 +258,29 @@ def load():
                 fn.argtypes = argtypes
             _lib = lib
     return _lib
+
+
+def stream() -> int:
+    """Handle of the current stream of the current device."""
+    return torch.cuda.current_stream().cuda_stream
+
+
+class _SameDevice:
+    """A context that changes nothing."""
+
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *_):
+        return False
+
+
+_same_device = _SameDevice()
+
+
+def on_device(t):
+    """A context in which the current device is that of the CUDA tensor ``t``."""
+    return _same_device if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
 def last_error() -> tuple[int, str]:

@@ -1,0 +1,212 @@
+"""AdamW over many tensors in one launch, with states in 32 or in 8 bits.
+
+* :func:`adamw_step` -- one step on lists of tensors, in place;
+* :class:`AdamW` -- the ``torch.optim.Optimizer`` that keeps the states.
+
+One kernel launch updates up to 400 tensors of one kind (``csrc/adamw.cu``);
+their addresses travel with the launch, so nothing is kept between calls.
+
+8-bit states hold e4m3 codes of the first moment and of the square root of
+the second, and an f32 scale for each 256 elements of a tensor (its largest
+magnitude / 448).  The step uses f32 values; the codes are rounded
+stochastically, because a moving average moves by less than half a code per
+step and rounding to nearest would hold it in place.  The random words are a
+hash of ``(seed, step, place of the tensor, element)``: a step is a function of
+its arguments.  A NaN stays in its element; an infinite value makes its block
+of 256 non-finite.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+
+BLOCK = 256
+_DTYPES = {torch.float32: _lib.TS_DTYPE_F32, torch.bfloat16: _lib.TS_DTYPE_BF16}
+
+
+def state_scales(n: int) -> int:
+    """Scales of an 8-bit state of ``n`` elements."""
+    return -(-n // BLOCK)
+
+
+def _require(ok, message):
+    if not ok:
+        raise ValueError(f"adamw: {message}")
+
+
+def _same(lists, sizes, dtype, device, what):
+    """Check that the tensors of ``lists`` are contiguous, of ``dtype``, on ``device`` and of the given sizes."""
+    _require(len(lists) == len(sizes), f"{len(sizes)} parameters but {len(lists)} {what}")
+    _require({t.dtype for t in lists} <= {dtype}, f"{what} must be {dtype}")
+    _require([t.numel() for t in lists] == sizes, f"{what} have other sizes than the parameters")
+    _require({t.get_device() for t in lists} <= {device}, f"{what} must be on the parameters' device")
+    _require(all(t.is_contiguous() for t in lists), f"{what} must be contiguous")
+
+
+def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step: int, lr: float, betas=(0.9, 0.999), eps: float = 1e-8,
+               weight_decay: float = 1e-2, masters=None, exp_avg_scales=None, exp_avg_sq_scales=None,
+               seed: int = 0, ordinals=None) -> None:
+    """One AdamW step, in place, on lists of CUDA tensors of one device.
+
+    ``params`` are f32 or bf16 and contiguous, ``grads`` f32 or bf16 of the
+    same shapes.  ``masters`` (f32) belong to bf16 parameters and carry their
+    values.  States are f32 tensors, or ``float8_e4m3fn`` codes (of the first
+    moment, and of the root of the second) with f32 scales of
+    ``state_scales(numel)`` entries.  ``step`` counts from 1; ``ordinals`` are
+    the tensors' places in the whole step (default 0, 1, ...), which key the
+    stochastic rounding of 8-bit states with ``seed``."""
+    _require(isinstance(step, int) and step >= 1, f"step must be an integer >= 1, got {step!r}")
+    b1, b2 = betas
+    _require(0 <= b1 < 1 and 0 <= b2 < 1, f"betas must lie in [0, 1), got {betas}")
+    _require(lr >= 0 and eps >= 0 and weight_decay >= 0, "lr, eps and weight_decay must be >= 0")
+    n = len(params)
+    if n == 0:
+        return
+    if not all(t.is_cuda for t in params):
+        raise RuntimeError("b200 backend requires CUDA tensors")
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("adamw: a captured step would repeat its step count; call it outside the graph")
+    device, sizes = params[0].get_device(), [t.numel() for t in params]
+    kinds = {t.dtype for t in params}
+    _require(kinds <= _DTYPES.keys(), "parameters must be float32 or bfloat16")
+    _require(len(grads) == n, f"{n} parameters but {len(grads)} gradients")
+    grad_kinds = {t.dtype for t in grads}
+    ordinals = range(n) if ordinals is None else ordinals
+    if len(kinds) > 1 or len(grad_kinds) > 1:
+        # one launch for each kind
+        groups = {}
+        for i in range(n):
+            groups.setdefault((params[i].dtype, grads[i].dtype), []).append(i)
+        _require(masters is None, "masters need parameters and gradients of one kind")
+        optional = (exp_avg_scales, exp_avg_sq_scales)
+        for at in groups.values():
+            lists = [[x[i] for i in at] for x in (params, grads, exp_avgs, exp_avg_sqs)]
+            m_scales, v_scales = (None if x is None else [x[i] for i in at] for x in optional)
+            adamw_step(*lists, step=step, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay,
+                       exp_avg_scales=m_scales, exp_avg_sq_scales=v_scales, seed=seed,
+                       ordinals=[ordinals[i] for i in at])
+        return
+    kind, grad_kind = kinds.pop(), grad_kinds.pop()
+    _require(grad_kind in _DTYPES, "gradients must be float32 or bfloat16")
+    eight = exp_avgs[0].dtype == torch.float8_e4m3fn if len(exp_avgs) else False
+    _same(params, sizes, kind, device, "parameters")
+    if not all(t.is_contiguous() for t in grads):
+        grads = [t.contiguous() for t in grads]
+    _same(grads, sizes, grad_kind, device, "gradients")
+    state_kind = torch.float8_e4m3fn if eight else torch.float32
+    _same(exp_avgs, sizes, state_kind, device, "first moments")
+    _same(exp_avg_sqs, sizes, state_kind, device, "second moments")
+    columns = [[t.data_ptr() for t in x] for x in (params, grads)]
+    none = [0] * n
+    if masters is not None:
+        _require(kind == torch.bfloat16, "masters belong to bfloat16 parameters")
+        _same(masters, sizes, torch.float32, device, "masters")
+        columns.append([t.data_ptr() for t in masters])
+    else:
+        columns.append(none)
+    columns += [[t.data_ptr() for t in x] for x in (exp_avgs, exp_avg_sqs)]
+    if eight:
+        _require(exp_avg_scales is not None and exp_avg_sq_scales is not None, "8-bit states need their scales")
+        blocks = [state_scales(k) for k in sizes]
+        _same(exp_avg_scales, blocks, torch.float32, device, "scales")
+        _same(exp_avg_sq_scales, blocks, torch.float32, device, "scales")
+        columns += [[t.data_ptr() for t in x] for x in (exp_avg_scales, exp_avg_sq_scales)]
+    else:
+        _require(exp_avg_scales is None and exp_avg_sq_scales is None, "scales belong to 8-bit states")
+        columns += [none, none]
+    # ts_adamw_tensor: seven pointers, the size, and the place (with its padding one more 64-bit word)
+    words = [w for row in zip(*columns, sizes, ordinals, strict=True) for w in row]
+    table = (ctypes.c_longlong * len(words))(*words)
+    a = _lib.AdamWArgs()
+    a.count, a.tensors = n, ctypes.addressof(table)
+    a.param_dtype, a.grad_dtype = _DTYPES[kind], _DTYPES[grad_kind]
+    a.master, a.state_bits, a.step = masters is not None, 8 if eight else 32, step
+    a.lr, a.beta1, a.beta2, a.eps, a.weight_decay, a.seed = lr, b1, b2, eps, weight_decay, seed
+    with _lib.on_device(params[0]):
+        _lib.check(_lib.load().ts_b200_adamw(ctypes.byref(a), _lib.stream()))
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW with decoupled weight decay over :func:`adamw_step`.
+
+    ``state_bits=8`` keeps the moments in 8 bits; ``master_weights=True`` keeps
+    an f32 value behind every bf16 parameter.  Parameters are contiguous CUDA
+    tensors in f32 or bf16; gradients may be either type.  ``seed`` keys the
+    rounding of 8-bit states."""
+
+    def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, *,
+                 state_bits: int = 32, master_weights: bool = False, seed: int = 0):
+        if state_bits not in (8, 32):
+            raise ValueError(f"adamw: state_bits must be 8 or 32, got {state_bits}")
+        _require(lr >= 0 and eps >= 0 and weight_decay >= 0, "lr, eps and weight_decay must be >= 0")
+        _require(0 <= betas[0] < 1 and 0 <= betas[1] < 1, f"betas must lie in [0, 1), got {betas}")
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay,
+                                      state_bits=state_bits, master_weights=master_weights, seed=seed))
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        for p in self.param_groups[-1]["params"]:
+            _require(p.dtype in _DTYPES, f"parameters must be float32 or bfloat16, got {p.dtype}")
+            _require(p.is_contiguous(), "parameters must be contiguous")
+
+    def _new_state(self, p, group):
+        state = {"step": 0}
+        if group["state_bits"] == 8:
+            for name in ("exp_avg", "exp_avg_sq"):
+                state[name] = torch.zeros(p.shape, dtype=torch.float8_e4m3fn, device=p.device)
+                state[name + "_scale"] = torch.zeros(state_scales(p.numel()), device=p.device)
+        else:
+            for name in ("exp_avg", "exp_avg_sq"):
+                state[name] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+        if group["master_weights"] and p.dtype == torch.bfloat16:
+            state["master"] = p.detach().float()
+        return state
+
+    def load_state_dict(self, state_dict):
+        """States keep the types that they were saved in (the base class would
+        give them the parameters')."""
+        super().load_state_dict(state_dict)
+        saved = state_dict["state"]
+        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        for i, p in zip(ids, (p for g in self.param_groups for p in g["params"]), strict=True):
+            if i in saved:
+                self.state[p] = {k: v.detach().to(p.device, copy=True) if torch.is_tensor(v) else v
+                                 for k, v in saved[i].items()}
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        ordinal = 0
+        for group in self.param_groups:
+            calls = {}
+            for p in group["params"]:
+                ordinal += 1
+                if p.grad is None:
+                    continue
+                if p.grad.is_sparse:
+                    raise RuntimeError("adamw: sparse gradients are not supported")
+                state = self.state[p]
+                if not state:
+                    state.update(self._new_state(p, group))
+                state["step"] += 1
+                # tensors of one step count and device go together, those with a master apart
+                master = "master" in state
+                key = (state["step"], p.device, master, (p.dtype, p.grad.dtype) if master else None)
+                calls.setdefault(key, []).append((ordinal - 1, p, state))
+            for (count, _, master, _), entries in calls.items():
+                ordinals, params, states = zip(*entries)
+                eight = group["state_bits"] == 8
+                adamw_step(params, [p.grad for p in params], [s["exp_avg"] for s in states],
+                           [s["exp_avg_sq"] for s in states], step=count, lr=float(group["lr"]), betas=group["betas"],
+                           eps=group["eps"], weight_decay=group["weight_decay"],
+                           masters=[s["master"] for s in states] if master else None,
+                           exp_avg_scales=[s["exp_avg_scale"] for s in states] if eight else None,
+                           exp_avg_sq_scales=[s["exp_avg_sq_scale"] for s in states] if eight else None,
+                           seed=group["seed"], ordinals=ordinals)
+        return loss

@@ -611,6 +611,44 @@ typedef struct ts_adamw_args {
 
 int ts_b200_adamw(const ts_adamw_args* args, ts_stream_t stream);
 
+/* ------------------------------------------------------------------- ffn
+ * Gated feed-forward block on `rows` rows:
+ *   y = (act(x Wg^T) * (x Wu^T)) Wd^T
+ * x [rows,width], Wg and Wu [hidden,width], Wd [width_out,hidden], all bf16
+ * with contiguous columns, 16-byte aligned bases and row strides that are
+ * multiples of 8; widths are multiples of 8.  y and the gradients are
+ * contiguous bf16.  The backward needs the inputs and dy only (it forms the
+ * projections again).  No reference counterpart (its host model's MLP). */
+enum { TS_FFN_SILU = 0, TS_FFN_GELU = 1 /* exact, by erf */, TS_FFN_RELU2 = 2 /* max(g,0)^2 */ };
+
+typedef struct ts_ffn_args {
+  long long rows;
+  int width, hidden, width_out;
+  int activation;
+  const void* x;
+  const void* w_gate;
+  const void* w_up;
+  const void* w_down;
+  long long x_stride, w_gate_stride, w_up_stride, w_down_stride;  /* elements between rows */
+  void* y;                  /* [rows,width_out] (forward) */
+  void* workspace;
+  size_t workspace_bytes;
+} ts_ffn_args;
+
+typedef struct ts_ffn_grad_args {
+  const void* dy;
+  long long dy_stride;
+  void* dx;                 /* [rows,width]; any of the four gradients may be NULL (not wanted) */
+  void* dw_gate;            /* [hidden,width] */
+  void* dw_up;              /* [hidden,width] */
+  void* dw_down;            /* [width_out,hidden] */
+} ts_ffn_grad_args;
+
+size_t ts_b200_ffn_fwd_workspace_bytes(const ts_ffn_args* args);
+int ts_b200_ffn_fwd(const ts_ffn_args* args, ts_stream_t stream);
+size_t ts_b200_ffn_bwd_workspace_bytes(const ts_ffn_args* args);
+int ts_b200_ffn_bwd(const ts_ffn_args* args, const ts_ffn_grad_args* grads, ts_stream_t stream);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif

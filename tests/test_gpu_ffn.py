@@ -1,0 +1,280 @@
+"""The gated feed-forward block's kernels against its formula in float64.
+
+Bounds, derived before any run.  bf16 rounds a value by at most 2^-8 of it (U).
+The kernels round the hidden values (h, dg, du) and each result once and
+accumulate in f32, so a result sum_j a_j b_j with rounded a_j is off by at most
+U sum_j |a_j b_j| + U |result|, and f32 sums and the activation's fast
+exponential add less than 1e-5 sum_j |a_j b_j| (with what cancels inside a_j
+counted by its terms).  Over many entries the roundings are independent, each
+of root mean square at most U / sqrt(3), so the norm of the error is within
+U sqrt(2/3) = 3.2e-3 of the result's (checked at 3.3e-3).
+"""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+gpu = pytest.mark.gpu
+BF16 = torch.bfloat16
+U = 2.0 ** -8
+
+
+@pytest.fixture(scope="module")
+def ffn():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a CUDA device")
+    from thetascan_b200 import _lib, ffn
+    yield ffn
+    assert _lib.device_status(torch.cuda.current_stream().cuda_stream) == 0
+
+
+def _make(rows, width, hidden, out, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    r = lambda *s, scale=1.0: (torch.randn(*s, generator=g) * scale).to(BF16).cuda()  # noqa: E731
+    return (r(rows, width), r(hidden, width, scale=1.5 / math.sqrt(width)), r(hidden, width, scale=1 / math.sqrt(width)),
+            r(out, hidden, scale=1 / math.sqrt(hidden)), r(rows, out))
+
+
+def _act(g, kind):
+    if kind == "silu":
+        s = torch.sigmoid(g)
+        return g * s, s * (1 + g * (1 - s))
+    if kind == "gelu":
+        s = 0.5 * (1 + torch.erf(g / math.sqrt(2)))
+        return g * s, s + g * torch.exp(-g * g / 2) / math.sqrt(2 * math.pi)
+    return g.clamp_min(0).square(), 2 * g.clamp_min(0)
+
+
+def _formula(x, wg, wu, wd, dy, kind):
+    """Outputs, and for each the sum of magnitudes that its bound is made of."""
+    x, wg, wu, wd, dy = (t.double() for t in (x, wg, wu, wd, dy))
+    g, u = x @ wg.T, x @ wu.T
+    a, slope = _act(g, kind)
+    h = a * u
+    dh = dy @ wd
+    du, dg = dh * a, dh * u * slope
+    # f32 error inside the hidden values is relative to the terms of their sums
+    terms_dh = dy.abs() @ wd.abs()
+    t = dict(h=a.abs() * (x.abs() @ wu.abs().T) + slope.abs() * u.abs() * (x.abs() @ wg.abs().T),
+             du=terms_dh * a.abs() + dh.abs() * slope.abs() * (x.abs() @ wg.abs().T),
+             dg=terms_dh * (u * slope).abs() + dh.abs() * (x.abs() @ wu.abs().T) * slope.abs()
+             + (dh * u).abs() * 2 * (x.abs() @ wg.abs().T))
+    want = (h @ wd.T, dg @ wg + du @ wu, dg.T @ x, du.T @ x, dy.T @ h)
+    rounded = (h.abs() @ wd.abs().T, dg.abs() @ wg.abs() + du.abs() @ wu.abs(), dg.abs().T @ x.abs(), du.abs().T @ x.abs(),
+               dy.abs().T @ h.abs())
+    summed = (t["h"] @ wd.abs().T, t["dg"] @ wg.abs() + t["du"] @ wu.abs(), t["dg"].T @ x.abs(), t["du"].T @ x.abs(),
+              dy.abs().T @ t["h"])
+    return want, [U * r + 1e-5 * (r + s) for r, s in zip(rounded, summed)]
+
+
+def _close(got, want, bound, what):
+    assert got.dtype == BF16 and got.shape == want.shape
+    off = (got.double() - want).abs()
+    assert (off <= bound + U * want.abs() + 1e-30).all(), (what, float((off - bound - U * want.abs()).max()))
+    if want.numel() >= 4096:
+        assert float(off.norm()) <= 3.3e-3 * float(want.norm()), (what, float(off.norm() / want.norm()))
+
+
+NAMES = ("y", "dx", "dw_gate", "dw_up", "dw_down")
+SHAPES = [
+    # rows, width, hidden, width_out: one token, few rows, tile edges, ragged everything
+    (1, 8, 8, 8), (1, 512, 1024, 512), (2, 64, 128, 64), (5, 264, 136, 72), (8, 1024, 2056, 1024), (9, 128, 512, 128),
+    (16, 520, 1032, 520), (17, 72, 264, 8), (31, 256, 256, 256), (33, 256, 256, 256), (64, 512, 512, 512), (65, 192, 320, 448),
+    (127, 64, 128, 256), (128, 64, 256, 264), (129, 136, 120, 64), (255, 256, 384, 256), (256, 512, 1024, 512), (257, 256, 256, 512),
+    # a long inner length and few tiles: split products, forward and backward
+    (100, 64, 4096, 64), (5000, 64, 72, 64), (3001, 128, 384, 320),
+    # several tiles for each pair of SMs
+    (20011, 64, 264, 136), (9000, 328, 1304, 328),
+]
+
+
+@gpu
+@pytest.mark.parametrize("rows,width,hidden,out", SHAPES)
+@pytest.mark.parametrize("kind", ["silu", "gelu", "relu2"])
+def test_block_is_the_formulas(ffn, rows, width, hidden, out, kind):
+    *inputs, dy = _make(rows, width, hidden, out, seed=rows + width)
+    want, bound = _formula(*inputs, dy, kind)
+    with torch.no_grad():
+        _close(ffn.gated_ffn(*inputs, kind), want[0], bound[0], "inference")
+    leaves = [t.requires_grad_(True) for t in inputs]
+    y = ffn.gated_ffn(*leaves, kind)
+    got = (y, *torch.autograd.grad(y, leaves, dy))
+    for name, g, w, b in zip(NAMES, got, want, bound):
+        _close(g.detach(), w, b, name)
+
+
+@gpu
+def test_gradient_is_the_difference_of_the_forward(ffn):
+    # along the gradient, a step of 5 % of x: the difference of two forwards of N rounded outputs is off by at most
+    # 5 deviations of their noise (3.2e-3 |y| |dy| / sqrt(N) each), and by 2 % for its own curvature
+    x, wg, wu, wd, dy = _make(300, 128, 256, 128, seed=5)
+    leaf = x.clone().requires_grad_(True)
+    y = ffn.gated_ffn(leaf, wg, wu, wd)
+    grad = torch.autograd.grad(y, leaf, dy)[0].double()
+    step = grad / grad.norm() * x.double().norm() * 0.05
+    up, down = (x.double() + step).to(BF16), (x.double() - step).to(BF16)
+    loss = lambda t: (ffn.gated_ffn(t, wg, wu, wd).double() * dy.double()).sum()  # noqa: E731
+    change, slope = float(loss(up) - loss(down)), float((grad * (up.double() - down.double())).sum())
+    noise = 5 * 2 * 3.2e-3 * float(y.double().norm() * dy.double().norm()) / math.sqrt(y.numel())
+    assert noise < 0.1 * abs(slope)
+    assert abs(change - slope) <= noise + 0.02 * abs(slope)
+
+
+@gpu
+def test_only_wanted_gradients(ffn):
+    x, wg, wu, wd, dy = _make(300, 64, 128, 64)
+    leaves = [t.clone().requires_grad_(True) for t in (x, wg, wu, wd)]
+    every = torch.autograd.grad(ffn.gated_ffn(*leaves), leaves, dy)
+    for i in range(4):
+        some = [t.clone().requires_grad_(j == i) for j, t in enumerate((x, wg, wu, wd))]
+        only, = torch.autograd.grad(ffn.gated_ffn(*some), some[i], dy)
+        assert torch.equal(only, every[i])
+
+
+@gpu
+def test_results_do_not_depend_on_timing(ffn):
+    x, wg, wu, wd, dy = _make(5000, 64, 264, 64)
+
+    def once():
+        leaves = [t.clone().requires_grad_(True) for t in (x, wg, wu, wd)]
+        y = ffn.gated_ffn(*leaves)
+        return (y.detach(), *torch.autograd.grad(y, leaves, dy))
+
+    a = once()
+    for _ in range(5):
+        assert all(torch.equal(p, q) for p, q in zip(a, once()))
+
+
+@gpu
+def test_rows_are_independent(ffn):
+    # a NaN or infinite row stays its own: the others are what they are without it
+    x, wg, wu, wd, _ = _make(300, 128, 256, 128)
+    want = ffn.gated_ffn(x, wg, wu, wd)
+    bad = x.clone()
+    bad[7, 3], bad[260, 0] = float("nan"), float("inf")
+    got = ffn.gated_ffn(bad, wg, wu, wd)
+    keep = torch.ones(300, dtype=torch.bool, device="cuda")
+    keep[7] = keep[260] = False
+    assert torch.equal(got[keep], want[keep]) and got[7].isnan().all()
+    y = ffn.gated_ffn(bad[:8], wg, wu, wd)
+    assert torch.isfinite(y[:7]).all() and y[7].isnan().all()
+
+
+@gpu
+@pytest.mark.parametrize("rows", [3, 70])
+def test_strides_leading_dimensions_and_alignment(ffn, rows):
+    g = torch.Generator().manual_seed(3)
+    big = torch.randn(2, rows, 3, 160, generator=g).to(BF16).cuda()
+    _, wg, wu, wd, _ = _make(1, 128, 256, 128)
+    wide = torch.zeros(256, 200, dtype=BF16, device="cuda")
+    wide[:, 8:136] = wg
+    turned = wd.T.contiguous().T
+    for x in (big[..., :128], big[..., 8:136], big[..., 1:129], big[:, :, 1, 32:], big.transpose(0, 2)[..., :128],
+              big[:, :1, :, :128].expand(2, rows, 3, 128), big[0, 0, 0, :128]):
+        want, bound = _formula(x.reshape(-1, 128), wg, wu, wd, torch.zeros(x.reshape(-1, 128).shape, device="cuda"), "silu")
+        for weights in ((wg, wu, wd), (wide[:, 8:136], wu, turned)):
+            got = ffn.gated_ffn(x, *weights)
+            assert got.shape == x.shape
+            _close(got.reshape(-1, 128), want[0], bound[0], "y")
+    x = big[..., 1:129].requires_grad_(True)
+    dx, = torch.autograd.grad(ffn.gated_ffn(x, wg, wu, wd).float().sum(), x)   # an expanded gradient
+    want, bound = _formula(x.detach().reshape(-1, 128), wg, wu, wd, torch.ones(x.numel() // 128, 128, device="cuda"), "silu")
+    _close(dx.reshape(-1, 128), want[1], bound[1], "dx")
+
+
+@gpu
+def test_empty(ffn):
+    _, wg, wu, wd, _ = _make(1, 64, 128, 64)
+    leaves = [torch.zeros(2, 0, 64, dtype=BF16, device="cuda", requires_grad=True), wg.requires_grad_(True)]
+    y = ffn.gated_ffn(leaves[0], leaves[1], wu, wd)
+    dx, dw = torch.autograd.grad(y.sum(), leaves)
+    assert y.shape == (2, 0, 64) and dx.shape == (2, 0, 64) and (dw == 0).all()
+
+
+@gpu
+def test_on_another_stream_and_in_a_graph(ffn):
+    for rows in (4, 700):
+        x, wg, wu, wd, _ = _make(rows, 128, 256, 128)
+        want = ffn.gated_ffn(x, wg, wu, wd)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            got = ffn.gated_ffn(x, wg, wu, wd)
+        torch.cuda.current_stream().wait_stream(side)
+        assert torch.equal(got, want)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = ffn.gated_ffn(x, wg, wu, wd)
+        x.copy_(x.flip(0))
+        for _ in range(2):
+            graph.replay()
+        assert torch.equal(got, want.flip(0))
+
+
+@gpu
+def test_module_rounds_wider_weights(ffn):
+    torch.manual_seed(0)
+    m = ffn.GatedFFN(64, 128, "gelu").cuda()
+    x = torch.randn(50, 64, device="cuda", requires_grad=True)
+    y = m(x)
+    assert y.dtype == torch.float32
+    y.sum().backward()
+    want = ffn.gated_ffn(x.detach().to(BF16), *(l.weight.detach().to(BF16) for l in (m.gate, m.up, m.down)), "gelu")
+    assert torch.equal(y.detach(), want.float())
+    assert all(p.grad.dtype == torch.float32 and p.grad.abs().sum() > 0 for p in m.parameters()) and x.grad.dtype == torch.float32
+
+
+@gpu
+def test_compiles_into_one_graph(ffn):
+    x, wg, wu, wd, _ = _make(64, 64, 128, 64)
+    leaves = [t.requires_grad_(True) for t in (x, wg, wu, wd)]
+    f = lambda *t: ffn.gated_ffn(*t).float().square().sum()  # noqa: E731
+    want = torch.autograd.grad(f(*leaves), leaves)
+    got = torch.autograd.grad(torch.compile(f, fullgraph=True, backend="aot_eager")(*leaves), leaves)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+@gpu
+def test_refusals(ffn):
+    x, wg, wu, wd, _ = _make(4, 64, 128, 64)
+    for bad in ((x.float(), wg, wu, wd), (x, wg.half(), wu, wd), (x, wg[:64], wu, wd), (x, wg, wu, wd[:, :64]), (x[:, :32], wg, wu, wd),
+                (x, wg[0], wu[0], wd)):
+        with pytest.raises(ValueError):
+            ffn.gated_ffn(*bad)
+    with pytest.raises(ValueError):
+        ffn.gated_ffn(x, wg, wu, wd, "tanh")
+    with pytest.raises(NotImplementedError):
+        ffn.gated_ffn(x, wg[:100], wu[:100], wd[:, :100])
+    with pytest.raises(RuntimeError):
+        ffn.gated_ffn(x, wg.cpu(), wu, wd)
+
+
+def test_refuses_cpu_tensors_and_widths():
+    from thetascan_b200 import GatedFFN, gated_ffn
+    with pytest.raises(RuntimeError):
+        gated_ffn(*(torch.zeros(8, 8, dtype=BF16) for _ in range(4)))
+    with pytest.raises(NotImplementedError):
+        GatedFFN(60, 128)
+    with pytest.raises(ValueError):
+        GatedFFN(64, 128, "tanh")
+
+
+def test_c_entry_refuses_bad_arguments():
+    import ctypes
+    from thetascan_b200 import _lib
+    lib = _lib.load()
+    assert lib.ts_b200_ffn_fwd(None, None) == _lib.TS_ERR_VALUE
+    a = _lib.FfnArgs()
+    a.rows, a.width, a.hidden, a.width_out = 4, 64, 100, 64
+    assert lib.ts_b200_ffn_fwd(ctypes.byref(a), None) == _lib.TS_ERR_NOT_IMPLEMENTED
+    assert lib.ts_b200_ffn_fwd_workspace_bytes(ctypes.byref(a)) == 0
+    a.hidden = 128
+    assert lib.ts_b200_ffn_fwd(ctypes.byref(a), None) == _lib.TS_ERR_VALUE      # null pointers
+    assert lib.ts_b200_ffn_bwd_workspace_bytes(ctypes.byref(a)) > lib.ts_b200_ffn_fwd_workspace_bytes(ctypes.byref(a)) > 0
+    a.x = a.w_gate = a.w_up = a.w_down = a.y = 256
+    assert lib.ts_b200_ffn_fwd(ctypes.byref(a), None) == _lib.TS_ERR_VALUE      # no workspace
+    a.activation = 9
+    assert lib.ts_b200_ffn_fwd(ctypes.byref(a), None) == _lib.TS_ERR_VALUE

@@ -7,6 +7,7 @@ Public surface (mirrors the reference package ``thetascan``):
 * ``scan``: the scan-backend contract (``linattn_views`` / ``linattn``);
 * ``kernel.kernel_core``: the fused kernel-family hot path;
 * ``rms_norm`` / ``add_rms_norm`` / ``rms_norm_8bit``: the norms around it;
+* ``gated_ffn`` / ``GatedFFN``: the gated feed-forward block;
 * ``AdamW`` / ``adamw_step``: the optimizer step over many tensors;
 * ``integration.install()``: register ``backend="b200"`` in an installed
   reference package.
@@ -17,6 +18,7 @@ from __future__ import annotations
 
 from .config import (GNConfig, KernelConfig, RegularizationConfig, RoPEConfig, RuntimeConfig,
                      TemporalConfig, ThetaScanConfig)
+from .ffn import GatedFFN, gated_ffn
 from .mixer import ThetaScan
 from .norm import add_rms_norm, rms_norm, rms_norm_8bit
 from .optim import AdamW, adamw_step
@@ -26,4 +28,4 @@ BACKEND_NAME = "b200"
 
 __all__ = ["GNConfig", "KernelConfig", "RegularizationConfig", "RoPEConfig", "RuntimeConfig",
            "TemporalConfig", "ThetaScan", "ThetaScanConfig", "BACKEND_NAME",
-           "AdamW", "adamw_step", "add_rms_norm", "rms_norm", "rms_norm_8bit"]
+           "AdamW", "GatedFFN", "adamw_step", "add_rms_norm", "gated_ffn", "rms_norm", "rms_norm_8bit"]

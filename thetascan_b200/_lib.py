@@ -227,7 +227,31 @@ class AdamWArgs(ctypes.Structure):
     ]
 
 
+class FfnArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", ctypes.c_longlong), ("width", ctypes.c_int), ("hidden", ctypes.c_int), ("width_out", ctypes.c_int),
+        ("activation", ctypes.c_int),
+        ("x", ctypes.c_void_p), ("w_gate", ctypes.c_void_p), ("w_up", ctypes.c_void_p), ("w_down", ctypes.c_void_p),
+        ("x_stride", ctypes.c_longlong), ("w_gate_stride", ctypes.c_longlong), ("w_up_stride", ctypes.c_longlong),
+        ("w_down_stride", ctypes.c_longlong),
+        ("y", ctypes.c_void_p), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class FfnGradArgs(ctypes.Structure):
+    _fields_ = [
+        ("dy", ctypes.c_void_p), ("dy_stride", ctypes.c_longlong), ("dx", ctypes.c_void_p),
+        ("dw_gate", ctypes.c_void_p), ("dw_up", ctypes.c_void_p), ("dw_down", ctypes.c_void_p),
+    ]
+
+
+TS_FFN_SILU, TS_FFN_GELU, TS_FFN_RELU2 = 0, 1, 2
+
 SIGNATURES.update({
+    "ts_b200_ffn_fwd_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(FfnArgs)]),
+    "ts_b200_ffn_fwd": (ctypes.c_int, [ctypes.POINTER(FfnArgs), ctypes.c_void_p]),
+    "ts_b200_ffn_bwd_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(FfnArgs)]),
+    "ts_b200_ffn_bwd": (ctypes.c_int, [ctypes.POINTER(FfnArgs), ctypes.POINTER(FfnGradArgs), ctypes.c_void_p]),
     "ts_b200_adamw": (ctypes.c_int, [ctypes.POINTER(AdamWArgs), ctypes.c_void_p]),
     "ts_b200_norm_fwd": (ctypes.c_int, [ctypes.POINTER(NormArgs), ctypes.c_void_p]),
     "ts_b200_norm_bwd_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(NormArgs)]),

@@ -75,7 +75,6 @@ struct FfnParams {
   FfnProblem p[kCount];
   int count;
   int units;
-  int activation;
 };
 
 // ---- pair-of-CTAs forms of the tensor-core instructions
@@ -221,13 +220,14 @@ __device__ __forceinline__ void tmem_ld16x3(uint32_t a, uint32_t b, uint32_t c, 
 
 constexpr int kSilu = TS_FFN_SILU, kGelu = TS_FFN_GELU, kRelu2 = TS_FFN_RELU2;
 
-__device__ __forceinline__ float ffn_act(int kind, float g, float& slope) {
-  if (kind == kSilu) {
+template <int kAct>
+__device__ __forceinline__ float ffn_act(float g, float& slope) {
+  if (kAct == kSilu) {
     const float s = __fdividef(1.f, 1.f + __expf(-g));
     slope = s * fmaf(g, 1.f - s, 1.f);
     return g * s;
   }
-  if (kind == kGelu) {
+  if (kAct == kGelu) {
     // by erfc: 1 + erf would cancel where g is negative
     const float s = 0.5f * erfcf(g * -0.70710678118654752f);
     slope = fmaf(g * 0.39894228040143268f, __expf(-0.5f * g * g), s);
@@ -287,7 +287,7 @@ __device__ __forceinline__ void stage16(uint32_t block, int lane, int c16, const
   st_shared_v4(block + sw128_offset(lane, 2 * c16 + 1), pack8(v + 8));
 }
 
-template <int kMode, int kCount>
+template <int kMode, int kAct, int kCount>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
     ffn_kernel(const __grid_constant__ FfnParams<kCount> q) {
   extern __shared__ uint8_t smem_raw[];
@@ -494,12 +494,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
       } else if (kMode == kGateFwd) {
         const uint32_t acc = tmem + 256u * buf + lanes + 64 * half;
         const uint32_t block = next_block();
-#pragma unroll
+        // rolled: the unrolled code of the activations outgrows the instruction cache
+#pragma unroll 1
         for (int c = 0; c < 4; ++c) {
           float g[16], v[16], slope;
           tmem_ld16x2(acc + 16 * c, acc + 128 + 16 * c, g, v);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) v[e] *= ffn_act(q.activation, g[e], slope);
+          for (int e = 0; e < 16; ++e) v[e] *= ffn_act<kAct>(g[e], slope);
           stage16(block, lane, c, v);
         }
         tc_fence_before();
@@ -517,7 +518,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
 #pragma unroll
           for (int e = 0; e < 16; e += 2) {
             float s0, s1;
-            const float a0 = ffn_act(q.activation, g[e], s0), a1 = ffn_act(q.activation, g[e + 1], s1);
+            const float a0 = ffn_act<kAct>(g[e], s0), a1 = ffn_act<kAct>(g[e + 1], s1);
             h[c][e / 2] = pack_bf16(a0 * v[e], a1 * v[e + 1]);
             du[c][e / 2] = pack_bf16(dh[e] * a0, dh[e + 1] * a1);
             g[e] = dh[e] * v[e] * s0;
@@ -616,18 +617,25 @@ void ffn_place(FfnProblem* p, float*& partial, int*& counters) {
   counters += p->units / p->splits * 2;
 }
 
-template <int kMode, int kCount>
+template <int kMode, int kAct, int kCount>
 int ffn_launch(FfnParams<kCount>& q, cudaStream_t s, const char* what) {
   q.units = 0;
   for (int i = 0; i < q.count; ++i) q.units += q.p[i].units;
   if (q.units == 0) return TS_OK;
   // an attribute of the function on the current device
-  const cudaError_t set = cudaFuncSetAttribute(ffn_kernel<kMode, kCount>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               kFfnSmem);
+  const cudaError_t set = cudaFuncSetAttribute(ffn_kernel<kMode, kAct, kCount>,
+                                               cudaFuncAttributeMaxDynamicSharedMemorySize, kFfnSmem);
   if (set != cudaSuccess) return set_error(TS_ERR_CUDA, "%s: %s", what, cudaGetErrorString(set));
   const int pairs = q.units < kPairs ? q.units : kPairs;
-  ffn_kernel<kMode, kCount><<<2 * pairs, kFfnThreads, kFfnSmem, s>>>(q);
+  ffn_kernel<kMode, kAct, kCount><<<2 * pairs, kFfnThreads, kFfnSmem, s>>>(q);
   return check_launch(what);
+}
+
+template <int kMode>
+int ffn_launch_gate(FfnParams<1>& q, int activation, cudaStream_t s, const char* what) {
+  if (activation == kSilu) return ffn_launch<kMode, kSilu>(q, s, what);
+  if (activation == kGelu) return ffn_launch<kMode, kGelu>(q, s, what);
+  return ffn_launch<kMode, kRelu2>(q, s, what);
 }
 
 size_t ffn_align(size_t x) { return (x + 1023) & ~static_cast<size_t>(1023); }
@@ -707,7 +715,6 @@ int ts_b200_ffn_fwd(const ts_ffn_args* a, ts_stream_t stream) {
   void* h = ws;
   FfnParams<1> gate = {};
   gate.count = 1;
-  gate.activation = a->activation;
   FfnProblem& p = gate.p[0];
   p.rows = static_cast<int>(a->rows);
   p.cols = a->hidden;
@@ -734,8 +741,8 @@ int ts_b200_ffn_fwd(const ts_ffn_args* a, ts_stream_t stream) {
       !ffn_map(&down.p[0].b[0], a->w_down, a->width_out, a->hidden, a->w_down_stride, 128) ||
       !ffn_map(&down.p[0].out[0], a->y, a->rows, a->width_out, a->width_out, 32))
     return set_error(TS_ERR_VALUE, kFfnLayout);
-  if (const int rc = ffn_launch<kGateFwd>(gate, stream, "ffn_gate_fwd")) return rc;
-  return ffn_launch<kProduct>(down, stream, "ffn_down");
+  if (const int rc = ffn_launch_gate<kGateFwd>(gate, a->activation, stream, "ffn_gate_fwd")) return rc;
+  return ffn_launch<kProduct, 0>(down, stream, "ffn_down");
 }
 
 size_t ts_b200_ffn_bwd_workspace_bytes(const ts_ffn_args* a) {
@@ -756,7 +763,6 @@ int ts_b200_ffn_bwd(const ts_ffn_args* a, const ts_ffn_grad_args* g, ts_stream_t
   const int D = a->width, H = a->hidden, O = a->width_out;
   FfnParams<1> gate = {};
   gate.count = 1;
-  gate.activation = a->activation;
   FfnProblem& p = gate.p[0];
   p.rows = static_cast<int>(M);
   p.cols = H;
@@ -804,8 +810,8 @@ int ts_b200_ffn_bwd(const ts_ffn_args* a, const ts_ffn_grad_args* g, ts_stream_t
   }
   if (!ok) return set_error(TS_ERR_VALUE, kFfnLayout);
   if (grads.count == 0) return TS_OK;
-  if (const int rc = ffn_launch<kGateBwd>(gate, stream, "ffn_gate_bwd")) return rc;
-  return ffn_launch<kProduct>(grads, stream, "ffn_grads");
+  if (const int rc = ffn_launch_gate<kGateBwd>(gate, a->activation, stream, "ffn_gate_bwd")) return rc;
+  return ffn_launch<kProduct, 0>(grads, stream, "ffn_grads");
 }
 
 }  // extern "C"

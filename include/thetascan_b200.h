@@ -617,8 +617,9 @@ int ts_b200_adamw(const ts_adamw_args* args, ts_stream_t stream);
  * x [rows,width], Wg and Wu [hidden,width], Wd [width_out,hidden], all bf16
  * with contiguous columns, 16-byte aligned bases and row strides that are
  * multiples of 8; widths are multiples of 8.  y and the gradients are
- * contiguous bf16.  The backward needs the inputs and dy only (it forms the
- * projections again).  No reference counterpart (its host model's MLP). */
+ * contiguous bf16.  A forward whose backward will run also writes h and kept
+ * (the projections in 24 bits, ts_b200_ffn_kept_bytes), which the backward
+ * reads.  No reference counterpart (its host model's MLP). */
 enum { TS_FFN_SILU = 0, TS_FFN_GELU = 1 /* exact, by erf */, TS_FFN_RELU2 = 2 /* max(g,0)^2 */ };
 
 typedef struct ts_ffn_args {
@@ -631,6 +632,8 @@ typedef struct ts_ffn_args {
   const void* w_down;
   long long x_stride, w_gate_stride, w_up_stride, w_down_stride;  /* elements between rows */
   void* y;                  /* [rows,width_out] (forward) */
+  void* h;                  /* bf16 [rows,hidden], with kept; both NULL in inference */
+  void* kept;
   void* workspace;
   size_t workspace_bytes;
 } ts_ffn_args;
@@ -644,6 +647,7 @@ typedef struct ts_ffn_grad_args {
   void* dw_down;            /* [width_out,hidden] */
 } ts_ffn_grad_args;
 
+size_t ts_b200_ffn_kept_bytes(const ts_ffn_args* args);
 size_t ts_b200_ffn_fwd_workspace_bytes(const ts_ffn_args* args);
 int ts_b200_ffn_fwd(const ts_ffn_args* args, ts_stream_t stream);
 size_t ts_b200_ffn_bwd_workspace_bytes(const ts_ffn_args* args);

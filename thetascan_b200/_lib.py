@@ -234,7 +234,8 @@ class FfnArgs(ctypes.Structure):
         ("x", ctypes.c_void_p), ("w_gate", ctypes.c_void_p), ("w_up", ctypes.c_void_p), ("w_down", ctypes.c_void_p),
         ("x_stride", ctypes.c_longlong), ("w_gate_stride", ctypes.c_longlong), ("w_up_stride", ctypes.c_longlong),
         ("w_down_stride", ctypes.c_longlong),
-        ("y", ctypes.c_void_p), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+        ("y", ctypes.c_void_p), ("h", ctypes.c_void_p), ("kept", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
     ]
 
 
@@ -248,6 +249,7 @@ class FfnGradArgs(ctypes.Structure):
 TS_FFN_SILU, TS_FFN_GELU, TS_FFN_RELU2 = 0, 1, 2
 
 SIGNATURES.update({
+    "ts_b200_ffn_kept_bytes": (ctypes.c_size_t, [ctypes.POINTER(FfnArgs)]),
     "ts_b200_ffn_fwd_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(FfnArgs)]),
     "ts_b200_ffn_fwd": (ctypes.c_int, [ctypes.POINTER(FfnArgs), ctypes.c_void_p]),
     "ts_b200_ffn_bwd_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(FfnArgs)]),

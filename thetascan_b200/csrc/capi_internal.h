@@ -25,6 +25,10 @@ int selftest_tma_mma(const void* A, const void* B, float* D, int N, int K, int a
 bool make_tmap_bf16_sw128(CUtensorMap* map, const void* base, int rank, const uint64_t* dims,
                           const int64_t* strides, const uint32_t* box);
 
+// The same with a swizzle of the caller's choice.
+bool make_tmap_bf16(CUtensorMap* map, const void* base, int rank, const uint64_t* dims, const int64_t* strides,
+                    const uint32_t* box, CUtensorMapSwizzle swizzle);
+
 inline int round_up(int x, int m) { return (x + m - 1) / m * m; }
 inline int ceil_div(int x, int m) { return (x + m - 1) / m; }
 

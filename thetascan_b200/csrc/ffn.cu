@@ -5,30 +5,38 @@
 //   dx = dg Wg + du Wu, dWg = dg^T x, dWu = du^T x, dWd = dy^T h
 //
 // bf16 operands, f32 accumulators in tensor memory; every stored value (h, y,
-// dg, du and the gradients) is rounded once, from f32.  Four launches:
+// dg, du and the gradients) is rounded once, from f32.  Launches:
 //
-//   kGateFwd   both projections, the activation and the product: h
+//   kGateFwd   both projections, the activation and the product: h; for a
+//              backward pass also g and u, in 24 bits (the f32 without its last
+//              byte, within 2^-16: a bf16 copy would double the error of dg
+//              and du, an f32 copy costs a third more traffic)
 //   kProduct   y = h Wd^T
-//   kGateBwd   dh, and g and u AGAIN, in one tile: dg, du and h.  Keeping g and
-//              u from the forward would either round them (their error then
-//              enters dg and du on top of dg's own rounding) or cost 16 bytes
-//              of traffic per hidden element in f32; the two products cost
-//              4 D operations per hidden element, which is as long as that
-//              traffic at D = 900 and buys that nothing of the block is kept
-//              for the backward but its input.
+//   kGateGrad  dh = dy Wd and, from g and u, dg and du
 //   kProduct   dx, dWg, dWu and dWd: one launch over all their tiles
+//
+// Forming g and u again in the backward instead of keeping them was built
+// first and measured slower: dh, g and u then share a tile of 128 hidden
+// columns, and the N = 128 instructions of dh run at half the rate of N = 256
+// ones (65536 x 512 x 1024: 261 us; 8192 x 2048 x 5632: 632 us).
 //
 // A pair of CTAs (cta_group::2) computes a tile of 256 x 256: each loads its
 // own 128 rows of A and its half of B's 256 rows, so an SM reads each operand
-// byte for twice the arithmetic of a single CTA's tile.  Gate tiles are 256 x
-// 128 hidden columns: one CTA of the pair loads rows of Wg, the other of Wu,
-// and one N = 256 instruction forms g and u side by side, in the same lanes,
-// where the epilogue needs them.  Warp 0 feeds a ring of kStages stages by
-// TMA, a thread of warp 1 (of the leading CTA) issues the instructions, warps
-// 4-11 take accumulators out of tensor memory while the next tile's are formed
-// in the other half of it.  In kGateBwd three accumulators of 128 columns do
-// not fit twice; the next tile's dh (two columns blocks in turn) is formed
-// while this tile's epilogue still reads g and u.
+// byte for twice the arithmetic of a single CTA's tile.  kGateFwd's tiles are
+// 256 x 128 hidden columns: one CTA of the pair loads rows of Wg, the other of
+// Wu, and one N = 256 instruction forms g and u side by side, in the same
+// lanes, where the epilogue needs them.  Warp 0 feeds a ring of kStages stages
+// by TMA, a thread of warp 1 (of the leading CTA) issues the instructions,
+// sixteen more warps take accumulators out of tensor memory while the next
+// tile's are formed in the other half of it.
+//
+// What bounds it: with loads left out the instructions alone take 246 us of
+// the 290 of kGateFwd at 8192 x 2048 x 5632 (1.53 PFLOP/s), the loads alone
+// 174 us (63 bytes a cycle into each SM).  An operand whose tile is 64 rows of
+// the inner dimension comes as one copy of two column blocks (a map of three
+// dimensions) where its columns are a multiple of 64, else as two copies: the
+// loads of the weight gradients alone take 571 us one way and 648 the other
+// at that size.
 //
 // A product of few tiles and a long inner length (the weight gradients: the
 // inner length is the number of tokens) is split along it; partial tiles go to
@@ -45,29 +53,34 @@ namespace ts {
 
 namespace {
 
-constexpr int kFfnThreads = 384;             // warps: 0 loads, 1 issues, 2 tensor memory, 4-11 epilogue
+constexpr int kEpiWarps = 16;
+constexpr int kFfnThreads = 128 + 32 * kEpiWarps;  // warps: 0 loads, 1 issues, 2 tensor memory, 4.. epilogue
 constexpr int kStages = 5;
 constexpr uint32_t kStageBytes = 32768;      // a CTA's part: 16 KB of A, 16 KB of B
-constexpr uint32_t kOutBlock = 4096;         // 32 rows x 64 bf16 columns
-constexpr uint32_t kFfnSmem = kStages * kStageBytes + 8 * 2 * kOutBlock + 1024;
+constexpr uint32_t kOutBlock = 2048;         // 32 rows x 32 bf16 columns
+constexpr uint32_t kFfnSmem = kStages * kStageBytes + kEpiWarps * 2 * kOutBlock + 1024;
 constexpr int kPairs = 74;
 constexpr int kMinSplitSteps = 8;
 
-enum FfnMode { kGateFwd = 0, kGateBwd = 1, kProduct = 2 };
+enum FfnMode { kGateFwd = 0, kGateGrad = 1, kProduct = 2 };
+
+// How an operand lies in memory: inner dimension contiguous; or M (N)
+// contiguous, loaded as two boxes of 64 columns or as one of 2 x 64.
+enum FfnLayout { kInner = 0, kOuter = 1, kOuterBlocks = 2 };
 
 // One product of a launch: C[M, N] = sum over segments A_i B_i^T.
 struct FfnProblem {
-  CUtensorMap a[2], b[2];    // per segment; gate modes: a = {x, dy}, b = {Wg, Wu}
-  CUtensorMap out[3];        // product: {C}; gate modes: {h, dg, du}
-  CUtensorMap b_down;        // kGateBwd: Wd
+  CUtensorMap a[2], b[2];    // per segment; kGateFwd: a[0] = x, b = {Wg, Wu}
+  CUtensorMap out[2];        // {C}; kGateGrad: {dg, du}
   int rows, cols;            // of C
   int tiles_n;
-  int steps[2];              // 64-wide inner steps of each segment (kGateBwd: of x, of dy)
+  int steps[2];              // 64-wide inner steps of each segment
   int splits;
   int units;                 // tiles * splits
-  int a_mn, b_mn;            // operands stored with M (N) contiguous
+  int a_layout, b_layout;
   float* partial;
   int* counters;
+  uint8_t* kept;             // g and u (see keep_at), or null
 };
 
 template <int kCount>
@@ -155,6 +168,24 @@ __device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* m
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
       : "memory");
 }
+__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+      : "memory");
+}
+// This CTA's 128 rows (from `row`, a multiple of 64) of an operand at inner step `k`.
+__device__ __forceinline__ void ffn_load(uint32_t dst, const CUtensorMap* map, int layout, int row, int k, uint32_t bar) {
+  if (layout == kInner) {
+    tma_load_pair(dst, map, 64 * k, row, bar);
+  } else if (layout == kOuterBlocks) {
+    tma_load_pair(dst, map, 0, 64 * k, row >> 6, bar);
+  } else {
+    tma_load_pair(dst, map, row, 64 * k, bar);
+    tma_load_pair(dst + 8192, map, row + 64, 64 * k, bar);
+  }
+}
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, int x, int y, uint32_t src) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
                    reinterpret_cast<uint64_t>(map)),
@@ -168,52 +199,35 @@ __device__ __forceinline__ void tma_store_read_wait() {
   asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kLeft) : "memory");
 }
 
-// 16 columns of this lane's row at each of two (three) column addresses, one wait for all.
-__device__ __forceinline__ void tmem_ld16x2(uint32_t a, uint32_t b, float (&x)[16], float (&y)[16]) {
-  uint32_t r[32];
+// 32 (16) columns of this lane's row from `addr` on; valid after tmem_wait()
+// and tie() of the registers (which keeps their uses behind the wait).
+__device__ __forceinline__ void tmem_ld(uint32_t addr, uint32_t (&r)[32]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%32];\n\t"
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%33];\n\t"
-      "tcgen05.wait::ld.sync.aligned;"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,"
+      "%29,%30,%31}, [%32];"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
         "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
         "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
         "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(a), "r"(b)
+      : "r"(addr)
       : "memory");
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    x[i] = __uint_as_float(r[i]);
-    y[i] = __uint_as_float(r[16 + i]);
-  }
 }
-__device__ __forceinline__ void tmem_ld16x3(uint32_t a, uint32_t b, uint32_t c, float (&x)[16], float (&y)[16],
-                                            float (&z)[16]) {
-  uint32_t r[48];
+__device__ __forceinline__ void tmem_ld(uint32_t addr, uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%48];\n\t"
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%49];\n\t"
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47}, [%50];\n\t"
-      "tcgen05.wait::ld.sync.aligned;"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
-        "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
-        "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47])
-      : "r"(a), "r"(b), "r"(c)
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr)
       : "memory");
+}
+__device__ __forceinline__ void tmem_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+template <int kN>
+__device__ __forceinline__ void tie(uint32_t (&r)[kN]) {
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    x[i] = __uint_as_float(r[i]);
-    y[i] = __uint_as_float(r[16 + i]);
-    z[i] = __uint_as_float(r[32 + i]);
-  }
+  for (int i = 0; i < kN; i += 8)
+    asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]),
+                 "+r"(r[i + 6]), "+r"(r[i + 7]));
 }
 
 // ---- activations: value and slope
@@ -238,6 +252,56 @@ __device__ __forceinline__ float ffn_act(float g, float& slope) {
   return s * s;
 }
 
+// ---- g and u between the passes
+//
+// Blocks of 32 rows x 32 columns, a lane's row as twelve 16-byte vectors
+// [vector][lane] (a warp's access is 512 contiguous bytes); for each half of
+// 16 columns: the upper halves of g's words, two vectors, their third bytes,
+// one vector, and the same of u.
+
+__device__ __forceinline__ uint8_t* keep_at(uint8_t* base, int cols, int row, int col, int lane) {
+  const size_t blocks = static_cast<size_t>((cols + 31) >> 5);
+  return base + ((row >> 5) * blocks + (col >> 5)) * 6144 + 16 * lane;
+}
+
+// 16 values from r[c] on, as three vectors.
+__device__ __forceinline__ void keep16(uint8_t* to, const uint32_t (&r)[32], int c) {
+  uint32_t high[8], low[4];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) high[i] = __byte_perm(r[c + 2 * i], r[c + 2 * i + 1], 0x7632);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    low[i] = __byte_perm(__byte_perm(r[c + 4 * i], r[c + 4 * i + 1], 0x0051),
+                         __byte_perm(r[c + 4 * i + 2], r[c + 4 * i + 3], 0x0051), 0x5410);
+  uint4* q = reinterpret_cast<uint4*>(to);
+  __stcs(q, make_uint4(high[0], high[1], high[2], high[3]));
+  __stcs(q + 32, make_uint4(high[4], high[5], high[6], high[7]));
+  __stcs(q + 64, make_uint4(low[0], low[1], low[2], low[3]));
+}
+
+// g and u of 16 columns of a lane's row.
+struct KeptHalf {
+  uint32_t high[2][8], low[2][4];
+  __device__ __forceinline__ void load(const uint8_t* from) {
+    const uint4* q = reinterpret_cast<const uint4*>(from);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint4 a = __ldcs(q + 96 * i), b = __ldcs(q + 96 * i + 32), c = __ldcs(q + 96 * i + 64);
+      high[i][0] = a.x; high[i][1] = a.y; high[i][2] = a.z; high[i][3] = a.w;
+      high[i][4] = b.x; high[i][5] = b.y; high[i][6] = b.z; high[i][7] = b.w;
+      low[i][0] = c.x; low[i][1] = c.y; low[i][2] = c.z; low[i][3] = c.w;
+    }
+  }
+  // The word again, with its third byte in the place of the lost fourth too:
+  // nearer to the middle of what was cut off than zero.
+  __device__ __forceinline__ float value(int i, int e) const {
+    const uint32_t byte = 4 + (e & 3), half = e & 1 ? 0x3200 : 0x1000;
+    return __uint_as_float(__byte_perm(high[i][e >> 1], low[i][e >> 2], half | byte << 4 | byte));
+  }
+  __device__ __forceinline__ float gate(int e) const { return value(0, e); }
+  __device__ __forceinline__ float up(int e) const { return value(1, e); }
+};
+
 // ---- one unit of work
 
 struct FfnUnit {
@@ -260,20 +324,20 @@ __device__ __forceinline__ FfnUnit ffn_unit(const FfnParams<kCount>& q, int unit
   u.tile = unit / splits;
   u.split = unit - u.tile * splits;
   u.m = u.tile / u.p->tiles_n * 256;
-  u.n = u.tile % u.p->tiles_n * (kMode == kProduct ? 256 : 128);
+  u.n = u.tile % u.p->tiles_n * (kMode == kGateFwd ? 128 : 256);
   const int steps = u.p->steps[0] + u.p->steps[1];
   u.begin = static_cast<int>(static_cast<long long>(steps) * u.split / splits);
   u.end = static_cast<int>(static_cast<long long>(steps) * (u.split + 1) / splits);
   return u;
 }
 
-// Whether `ok` holds in all of the CTA's 256 epilogue threads (a barrier among them).
+// Whether `ok` holds in all of the CTA's 512 epilogue threads (a barrier among them).
 __device__ __forceinline__ bool epilogue_all(bool ok) {
   uint32_t all;
   asm volatile(
       "{\n\t.reg .pred p, r;\n\t"
       "setp.ne.u32 p, %1, 0;\n\t"
-      "barrier.cta.red.and.pred r, 1, 256, p;\n\t"
+      "barrier.cta.red.and.pred r, 1, 512, p;\n\t"
       "selp.u32 %0, 1, 0, r;\n\t}"
       : "=r"(all)
       : "r"(static_cast<uint32_t>(ok))
@@ -281,10 +345,10 @@ __device__ __forceinline__ bool epilogue_all(bool ok) {
   return all != 0;
 }
 
-// 16 bf16 columns of a lane's row into its staging block (128-byte rows, swizzled as the store expects).
-__device__ __forceinline__ void stage16(uint32_t block, int lane, int c16, const float (&v)[16]) {
-  st_shared_v4(block + sw128_offset(lane, 2 * c16), pack8(v));
-  st_shared_v4(block + sw128_offset(lane, 2 * c16 + 1), pack8(v + 8));
+// 16 bytes (8 bf16 columns) of a lane's row into its warp's staging block: 64-byte rows, swizzled as the store
+// expects (the 16-byte chunk's index XORed with bits 1-2 of the row).
+__device__ __forceinline__ void stage8(uint32_t block, int lane, int chunk, uint4 v) {
+  st_shared_v4(block + 64 * lane + ((chunk ^ ((lane >> 1) & 3)) << 4), v);
 }
 
 template <int kMode, int kAct, int kCount>
@@ -305,7 +369,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_empty[i], 16);   // the epilogue warps of both CTAs
+      mbar_init(&acc_empty[i], 2 * kEpiWarps);   // the epilogue warps of both CTAs
     }
     fence_mbar_init();
   }
@@ -329,32 +393,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
         if (!(ok = wait_cluster(&empty[s], ((it / kStages) & 1) ^ 1, kErrMmaTimeout))) break;
         const uint32_t a = base + s * kStageBytes, b = a + 16384;
         const uint32_t bar = leader_addr(&full[s]);
-        if (kMode == kProduct) {
-          const int seg = k < p.steps[0] ? 0 : 1;
-          const int x = 64 * (k - (seg ? p.steps[0] : 0));
-          const int col = u.n + 128 * static_cast<int>(rank);
-          if (rank == 0) mbar_expect_tx(&full[s], 2 * kStageBytes);
-          if (p.a_mn) {
-            tma_load_pair(a, &p.a[seg], row, x, bar);
-            tma_load_pair(a + 8192, &p.a[seg], row + 64, x, bar);
-          } else {
-            tma_load_pair(a, &p.a[seg], x, row, bar);
-          }
-          if (p.b_mn) {
-            tma_load_pair(b, &p.b[seg], col, x, bar);
-            tma_load_pair(b + 8192, &p.b[seg], col + 64, x, bar);
-          } else {
-            tma_load_pair(b, &p.b[seg], x, col, bar);
-          }
-        } else if (kMode == kGateBwd && k < p.steps[1]) {
-          if (rank == 0) mbar_expect_tx(&full[s], 2 * 24576);
-          tma_load_pair(a, &p.a[1], 64 * k, row, bar);
-          tma_load_pair(b, &p.b_down, u.n + 64 * static_cast<int>(rank), 64 * k, bar);
+        if (rank == 0) mbar_expect_tx(&full[s], 2 * kStageBytes);
+        if (kMode == kGateFwd) {
+          ffn_load(a, &p.a[0], kInner, row, k, bar);
+          ffn_load(b, &p.b[rank], kInner, u.n, k, bar);
         } else {
-          const int x = 64 * (kMode == kGateBwd ? k - p.steps[1] : k);
-          if (rank == 0) mbar_expect_tx(&full[s], 2 * kStageBytes);
-          tma_load_pair(a, &p.a[0], x, row, bar);
-          tma_load_pair(b, &p.b[rank], x, u.n, bar);
+          const int seg = k < p.steps[0] ? 0 : 1;
+          const int step = k - (seg ? p.steps[0] : 0);
+          ffn_load(a, &p.a[seg], p.a_layout, row, step, bar);
+          ffn_load(b, &p.b[seg], p.b_layout, u.n + 128 * static_cast<int>(rank), step, bar);
         }
       }
     }
@@ -371,46 +418,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
     for (int w = pair; w < q.units && ok; w += pairs, ++n_unit) {
       const FfnUnit u = ffn_unit<kMode>(q, w);
       const FfnProblem& p = *u.p;
-      const bool a_mn = kMode == kProduct && p.a_mn, b_mn = kMode == kProduct && p.b_mn;
-      const int buf = kMode == kGateBwd ? 0 : n_unit & 1;
-      const uint32_t free_parity = ((kMode == kGateBwd ? n_unit : n_unit >> 1) & 1) ^ 1;
-      uint32_t acc = tmem + (kMode == kGateBwd ? 256u : 256u * buf);
-      bool waited = false;
+      const bool a_mn = p.a_layout != kInner, b_mn = p.b_layout != kInner;
+      const int buf = n_unit & 1;
+      const uint32_t acc = tmem + 256u * buf, id = idesc_bf16(256, 256, a_mn, b_mn);
+      const uint32_t a_step = a_mn ? 2048 : 32, b_step = b_mn ? 2048 : 32;
+      const uint32_t a_lbo = a_mn ? 8192 : 16, b_lbo = b_mn ? 8192 : 16;
+      if (!(ok = wait_cluster(&acc_empty[buf], ((n_unit >> 1) & 1) ^ 1, kErrMmaTimeout))) break;
       for (int k = u.begin; k < u.end; ++k, ++it) {
         const int s = it % kStages;
-        const bool down = kMode == kGateBwd && k < p.steps[1];
-        if (!down && !waited) {
-          // dh's own columns were free before: the epilogue that read them had
-          // ended when the tile in between could form its g and u
-          waited = true;
-          if (!(ok = wait_cluster(&acc_empty[buf], free_parity, kErrMmaTimeout))) break;
-        }
         if (!(ok = wait_cluster(&full[s], (it / kStages) & 1, kErrCopyTimeout))) break;
         tc_fence_after();
         const uint32_t a = base + s * kStageBytes, b = a + 16384;
-        if (down) {
-          const uint32_t id = idesc_bf16(256, 128, false, true);
-          const uint32_t d = tmem + 128u * (n_unit & 1);
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            mma_pair(d, smem_desc_sw128(a + 32 * j, 16, 1024), smem_desc_sw128(b + 2048 * j, 8192, 1024), id,
-                     k > u.begin || j > 0);
-        } else {
-          const uint32_t id = idesc_bf16(256, 256, a_mn, b_mn);
-          const int first = kMode == kGateBwd ? p.steps[1] : u.begin;
-          const uint32_t a_step = a_mn ? 2048 : 32, b_step = b_mn ? 2048 : 32;
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            mma_pair(acc, smem_desc_sw128(a + a_step * j, a_mn ? 8192 : 16, 1024),
-                     smem_desc_sw128(b + b_step * j, b_mn ? 8192 : 16, 1024), id, k > first || j > 0);
-        }
+        for (int j = 0; j < 4; ++j)
+          mma_pair(acc, smem_desc_sw128(a + a_step * j, a_lbo, 1024), smem_desc_sw128(b + b_step * j, b_lbo, 1024), id,
+                   k > u.begin || j > 0);
         mma_commit_pair(&empty[s]);
       }
       if (ok) mma_commit_pair(&acc_full[buf]);
     }
   } else if (warp >= 4) {
-    // ---- accumulators out
-    const int quad = warp & 3, half = (warp - 4) >> 2;
+    // ---- accumulators out: a warp takes the 32 rows of its quarter of tensor memory (warp % 4) and a quarter of
+    // the columns
+    const int quad = warp & 3, part = (warp - 4) >> 2;
     const uint32_t stage = base + kStages * kStageBytes + (warp - 4) * 2 * kOutBlock;
     const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
     uint32_t turn = 0;
@@ -433,113 +463,143 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
     for (int w = pair; w < q.units; w += pairs, ++n_unit) {
       const FfnUnit u = ffn_unit<kMode>(q, w);
       const FfnProblem& p = *u.p;
-      const int buf = kMode == kGateBwd ? 0 : n_unit & 1;
-      bool ok = wait_cluster(&acc_full[buf], (kMode == kGateBwd ? n_unit : n_unit >> 1) & 1, kErrMmaTimeout);
+      const int buf = n_unit & 1;
+      auto release = [&]() {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) arrive_cluster(leader_addr(&acc_empty[buf]));
+      };
+      const int row0 = u.m + 128 * static_cast<int>(rank) + 32 * quad;
+      KeptHalf kept;
+      const uint8_t* from = nullptr;
+      if (kMode == kGateGrad) {
+        // 64 columns of g and u: two blocks, the first half-block ahead of the wait
+        from = keep_at(p.kept, p.cols, row0, u.n + 64 * part, lane);
+        if (row0 < p.rows && u.n + 64 * part < p.cols) kept.load(from);
+      }
+      bool ok = wait_cluster(&acc_full[buf], (n_unit >> 1) & 1, kErrMmaTimeout);
       // the warps of a product meet in barriers below: they go on, or give up, together
       if (kMode == kProduct) ok = epilogue_all(ok);
       if (!ok) break;
       tc_fence_after();
-      const int row0 = u.m + 128 * static_cast<int>(rank) + 32 * quad;
       if (kMode == kProduct) {
-        const uint32_t acc = tmem + 256u * buf + lanes;
-        float* part = p.partial + (static_cast<size_t>(u.tile) * p.splits * 2 + rank) * 32768;
+        const uint32_t acc = tmem + 256u * buf + lanes + 64 * part;
+        float* sums = p.partial + (static_cast<size_t>(u.tile) * p.splits * 2 + rank) * 32768 + 64 * part * 128 +
+                      32 * quad + lane;   // [split][rank][column][row]
         if (p.splits > 1) {
-          float* mine = part + static_cast<size_t>(u.split) * 65536 + 32 * quad + lane;
+          float* mine = sums + static_cast<size_t>(u.split) * 65536;
+#pragma unroll 1
+          for (int c = 0; c < 64; c += 32) {
+            uint32_t v[32];
+            tmem_ld(acc + c, v);
+            tmem_wait();
+            tie(v);
 #pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            float v[16];
-            tmem_ld16(acc + 128 * half + 16 * c, v);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) __stcg(mine + (128 * half + 16 * c + e) * 128, v[e]);
+            for (int e = 0; e < 32; ++e) __stcg(mine + (c + e) * 128, __uint_as_float(v[e]));
           }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) arrive_cluster(leader_addr(&acc_empty[buf]));
+          release();
           __threadfence();
-          asm volatile("bar.sync 1, 256;" ::: "memory");
+          asm volatile("bar.sync 1, 512;" ::: "memory");
           if (threadIdx.x == 128) is_last = atomicAdd(&p.counters[u.tile * 2 + rank], 1) == p.splits - 1;
-          asm volatile("bar.sync 1, 256;" ::: "memory");
+          asm volatile("bar.sync 1, 512;" ::: "memory");
           const bool last = is_last != 0;
-          asm volatile("bar.sync 1, 256;" ::: "memory");
+          asm volatile("bar.sync 1, 512;" ::: "memory");
           if (!last) continue;
           __threadfence();
         }
-#pragma unroll
-        for (int half64 = 0; half64 < 2; ++half64) {
+#pragma unroll 1
+        for (int c = 0; c < 64; c += 32) {
           const uint32_t block = next_block();
-          const int c0 = 128 * half + 64 * half64;
+          float v[32];
+          if (p.splits > 1) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            float v[16];
-            if (p.splits > 1) {
+            for (int e = 0; e < 32; ++e) v[e] = 0.f;
+            for (int i = 0; i < p.splits; ++i) {
+              const float* from = sums + static_cast<size_t>(i) * 65536 + c * 128;
+              float a[32];
 #pragma unroll
-              for (int e = 0; e < 16; ++e) v[e] = 0.f;
-              for (int i = 0; i < p.splits; ++i) {
-                const float* from = part + static_cast<size_t>(i) * 65536 + (c0 + 16 * c) * 128 + 32 * quad + lane;
+              for (int e = 0; e < 32; ++e) a[e] = __ldcg(from + e * 128);
 #pragma unroll
-                for (int e = 0; e < 16; ++e) v[e] += __ldcg(from + e * 128);
-              }
-            } else {
-              tmem_ld16(acc + c0 + 16 * c, v);
+              for (int e = 0; e < 32; ++e) v[e] += a[e];
             }
-            stage16(block, lane, c, v);
+          } else {
+            uint32_t r[32];
+            tmem_ld(acc + c, r);
+            tmem_wait();
+            tie(r);
+            if (c == 32) release();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(r[e]);
           }
-          if (p.splits == 1 && half64 == 1) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) arrive_cluster(leader_addr(&acc_empty[buf]));
-          }
-          store_block(&p.out[0], block, u.n + c0, row0, p);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) stage8(block, lane, i, pack8(v + 8 * i));
+          store_block(&p.out[0], block, u.n + 64 * part + c, row0, p);
         }
       } else if (kMode == kGateFwd) {
-        const uint32_t acc = tmem + 256u * buf + lanes + 64 * half;
+        const uint32_t acc = tmem + 256u * buf + lanes + 32 * part;
+        uint32_t g[32], v[32];
+        tmem_ld(acc, g);
+        tmem_ld(acc + 128, v);
+        tmem_wait();
+        tie(g);
+        tie(v);
+        release();
+        const int col = u.n + 32 * part;
+        if (p.kept && row0 < p.rows && col < p.cols) {
+          uint8_t* to = keep_at(p.kept, p.cols, row0, col, lane);
+#pragma unroll
+          for (int c = 0; c < 32; c += 16) {
+            keep16(to + 6 * 512 * (c / 16), g, c);
+            keep16(to + 6 * 512 * (c / 16) + 3 * 512, v, c);
+          }
+        }
         const uint32_t block = next_block();
-        // rolled: the unrolled code of the activations outgrows the instruction cache
-#pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          float g[16], v[16], slope;
-          tmem_ld16x2(acc + 16 * c, acc + 128 + 16 * c, g, v);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) v[e] *= ffn_act<kAct>(g[e], slope);
-          stage16(block, lane, c, v);
+        for (int i = 0; i < 4; ++i) {
+          float h[8], slope;
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            h[e] = ffn_act<kAct>(__uint_as_float(g[8 * i + e]), slope) * __uint_as_float(v[8 * i + e]);
+          stage8(block, lane, i, pack8(h));
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) arrive_cluster(leader_addr(&acc_empty[buf]));
-        store_block(&p.out[0], block, u.n + 64 * half, row0, p);
+        store_block(&p.out[0], block, col, row0, p);
       } else {
-        const uint32_t dh_at = tmem + 128u * (n_unit & 1) + lanes + 64 * half, acc = tmem + 256u + lanes + 64 * half;
-        uint32_t du[4][8], h[4][8];
-        uint32_t block = next_block();
+        const uint32_t acc = tmem + 256u * buf + lanes + 64 * part;
+        // blocks of 32 columns, in halves of 16; the next half's g and u are on their way meanwhile
+#pragma unroll 1
+        for (int c = 0; c < 64; c += 32) {
+          const int col = u.n + 64 * part + c;
+          if (lane == 0) tma_store_read_wait<0>();
+          __syncwarp();
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          float dh[16], g[16], v[16];
-          tmem_ld16x3(dh_at + 16 * c, acc + 16 * c, acc + 128 + 16 * c, dh, g, v);
+          for (int o = 0; o < 32; o += 16) {
+            uint32_t d[16];
+            tmem_ld(acc + c + o, d);
+            tmem_wait();
+            tie(d);
+            if (c + o == 48) release();
+            KeptHalf next;
+            const int ahead = c + o + 16;   // the columns after this half, where they are this tile's and inside
+            if (ahead < 64 && row0 < p.rows && u.n + 64 * part + (ahead & 32) < p.cols)
+              next.load(from + (ahead >> 5) * 6144 + ((ahead >> 4) & 1) * (6 * 512));
 #pragma unroll
-          for (int e = 0; e < 16; e += 2) {
-            float s0, s1;
-            const float a0 = ffn_act<kAct>(g[e], s0), a1 = ffn_act<kAct>(g[e + 1], s1);
-            h[c][e / 2] = pack_bf16(a0 * v[e], a1 * v[e + 1]);
-            du[c][e / 2] = pack_bf16(dh[e] * a0, dh[e + 1] * a1);
-            g[e] = dh[e] * v[e] * s0;
-            g[e + 1] = dh[e + 1] * v[e + 1] * s1;
+            for (int i = 0; i < 2; ++i) {
+              float x[8], y[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const float dh = __uint_as_float(d[8 * i + e]);
+                float slope;
+                const float act = ffn_act<kAct>(kept.gate(8 * i + e), slope);
+                x[e] = dh * kept.up(8 * i + e) * slope;
+                y[e] = dh * act;
+              }
+              stage8(stage, lane, o / 8 + i, pack8(x));
+              stage8(stage + kOutBlock, lane, o / 8 + i, pack8(y));
+            }
+            kept = next;
           }
-          stage16(block, lane, c, g);
-        }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) arrive_cluster(leader_addr(&acc_empty[buf]));
-        store_block(&p.out[1], block, u.n + 64 * half, row0, p);
-#pragma unroll
-        for (int o = 0; o < 2; ++o) {
-          block = next_block();
-          const uint32_t(&x)[4][8] = o ? h : du;
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            st_shared_v4(block + sw128_offset(lane, 2 * c), make_uint4(x[c][0], x[c][1], x[c][2], x[c][3]));
-            st_shared_v4(block + sw128_offset(lane, 2 * c + 1), make_uint4(x[c][4], x[c][5], x[c][6], x[c][7]));
-          }
-          store_block(&p.out[o ? 0 : 2], block, u.n + 64 * half, row0, p);
+          store_block(&p.out[0], stage, col, row0, p);
+          store_block(&p.out[1], stage + kOutBlock, col, row0, p);
         }
       }
     }
@@ -578,6 +638,24 @@ bool ffn_map(CUtensorMap* map, const void* base, long long outer, int inner, lon
   const int64_t strides[1] = {stride};
   const uint32_t boxes[2] = {64, box};
   return make_tmap_bf16_sw128(map, base, 2, dims, strides, boxes);
+}
+
+// Operand of a product whose inner dimension is its rows: [inner, cols], columns contiguous.
+bool ffn_outer_map(CUtensorMap* map, int* layout, const void* base, long long inner, int cols, long long stride) {
+  *layout = cols % 64 ? kOuter : kOuterBlocks;
+  if (*layout == kOuter) return ffn_map(map, base, inner, cols, stride, 64);
+  const uint64_t dims[3] = {64, static_cast<uint64_t>(inner), static_cast<uint64_t>(cols / 64)};
+  const int64_t strides[2] = {stride, 64};
+  const uint32_t boxes[3] = {64, 64, 2};
+  return make_tmap_bf16_sw128(map, base, 3, dims, strides, boxes);
+}
+
+// Output [rows, cols], contiguous: boxes of 32 x 32.
+bool ffn_out_map(CUtensorMap* map, const void* base, long long rows, int cols) {
+  const uint64_t dims[2] = {static_cast<uint64_t>(cols), static_cast<uint64_t>(rows)};
+  const int64_t strides[1] = {cols};
+  const uint32_t boxes[2] = {32, 32};
+  return make_tmap_bf16(map, base, 2, dims, strides, boxes, CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
 // Splits of a product's inner length: enough units for every pair of SMs where
@@ -658,16 +736,18 @@ int ffn_check(const ts_ffn_args* a) {
 
 const char* const kFfnLayout = "ffn: every matrix needs a 16-byte aligned base and a row stride that is a multiple of 8";
 
+size_t ffn_hidden_bytes(const ts_ffn_args* a) { return static_cast<size_t>(a->rows) * a->hidden * 2; }
+
 struct FfnForward {
   FfnProblem down = {};
   FfnSpace space;
-  size_t h = 0, partial = 0, counters = 0, total = 0;
+  size_t partial = 0, counters = 0, total = 0;   // offsets; h is at 0 where the caller keeps none
 };
 
 FfnForward ffn_forward(const ts_ffn_args* a) {
   FfnForward f;
   ffn_product(&f.down, a->rows, a->width_out, a->hidden, 0, &f.space);
-  f.partial = ffn_align(static_cast<size_t>(a->rows) * a->hidden * 2);
+  f.partial = ffn_align(ffn_hidden_bytes(a));
   f.counters = f.partial + ffn_align(f.space.partial * 4);
   f.total = f.counters + ffn_align(f.space.counters * 4);
   return f;
@@ -676,7 +756,7 @@ FfnForward ffn_forward(const ts_ffn_args* a) {
 struct FfnBackward {
   FfnProblem p[4] = {};   // dWg, dWu, dWd, dx
   FfnSpace space;
-  size_t dg = 0, du = 0, h = 0, partial = 0, counters = 0, total = 0;
+  size_t du = 0, partial = 0, counters = 0, total = 0;   // offsets; dg at 0
 };
 
 FfnBackward ffn_backward(const ts_ffn_args* a) {
@@ -685,13 +765,33 @@ FfnBackward ffn_backward(const ts_ffn_args* a) {
   ffn_product(&b.p[1], a->hidden, a->width, a->rows, 0, &b.space);
   ffn_product(&b.p[2], a->width_out, a->hidden, a->rows, 0, &b.space);
   ffn_product(&b.p[3], a->rows, a->width, a->hidden, a->hidden, &b.space);
-  const size_t one = ffn_align(static_cast<size_t>(a->rows) * a->hidden * 2);
+  const size_t one = ffn_align(ffn_hidden_bytes(a));
   b.du = one;
-  b.h = 2 * one;
-  b.partial = 3 * one;
+  b.partial = 2 * one;
   b.counters = b.partial + ffn_align(b.space.partial * 4);
   b.total = b.counters + ffn_align(b.space.counters * 4);
   return b;
+}
+
+// A gate launch: tiles of 256 rows x `tile` hidden columns, not split.
+FfnParams<1> ffn_gate(const ts_ffn_args* a, int tile, int inner) {
+  FfnParams<1> q = {};
+  q.count = 1;
+  FfnProblem& p = q.p[0];
+  p.rows = static_cast<int>(a->rows);
+  p.cols = a->hidden;
+  p.tiles_n = static_cast<int>(ffn_tiles(a->hidden, tile));
+  p.steps[0] = ffn_steps(inner);
+  p.splits = 1;
+  p.units = static_cast<int>(ffn_tiles(a->rows, 256)) * p.tiles_n;
+  p.kept = static_cast<uint8_t*>(a->kept);
+  return q;
+}
+
+int ffn_clear(int* counters, size_t n, cudaStream_t s) {
+  if (n == 0) return TS_OK;
+  const cudaError_t e = cudaMemsetAsync(counters, 0, n * sizeof(int), s);
+  return e == cudaSuccess ? TS_OK : set_error(TS_ERR_CUDA, "ffn: %s", cudaGetErrorString(e));
 }
 
 }  // namespace
@@ -699,6 +799,11 @@ FfnBackward ffn_backward(const ts_ffn_args* a) {
 }  // namespace ts
 
 extern "C" {
+
+size_t ts_b200_ffn_kept_bytes(const ts_ffn_args* a) {
+  if (ts::ffn_check(a)) return 0;
+  return static_cast<size_t>((a->rows + 31) / 32) * ((a->hidden + 31) / 32) * 6144;
+}
 
 size_t ts_b200_ffn_fwd_workspace_bytes(const ts_ffn_args* a) {
   return ts::ffn_check(a) ? 0 : ts::ffn_forward(a).total;
@@ -708,38 +813,28 @@ int ts_b200_ffn_fwd(const ts_ffn_args* a, ts_stream_t stream) {
   using namespace ts;
   if (const int rc = ffn_check(a)) return rc;
   if (!a->x || !a->w_gate || !a->w_up || !a->w_down || !a->y) return set_error(TS_ERR_VALUE, "ffn_fwd: null pointer");
+  if (!a->kept != !a->h) return set_error(TS_ERR_VALUE, "ffn_fwd: h and kept belong together");
   FfnForward f = ffn_forward(a);
   if (!a->workspace || a->workspace_bytes < f.total) return set_error(TS_ERR_VALUE, "ffn_fwd: workspace too small");
   if (!ffn_bind_context()) return set_error(TS_ERR_CUDA, "ffn_fwd: no context on the current device");
   uint8_t* ws = static_cast<uint8_t*>(a->workspace);
-  void* h = ws;
-  FfnParams<1> gate = {};
-  gate.count = 1;
+  void* h = a->h ? a->h : ws;
+  FfnParams<1> gate = ffn_gate(a, 128, a->width);
   FfnProblem& p = gate.p[0];
-  p.rows = static_cast<int>(a->rows);
-  p.cols = a->hidden;
-  p.tiles_n = static_cast<int>(ffn_tiles(a->hidden, 128));
-  p.steps[0] = ffn_steps(a->width);
-  p.splits = 1;
-  p.units = static_cast<int>(ffn_tiles(a->rows, 256)) * p.tiles_n;
+  FfnParams<1> down = {};
+  down.count = 1;
+  FfnProblem& d = down.p[0];
+  d = f.down;
+  float* partial = reinterpret_cast<float*>(ws + f.partial);
+  int* counters = reinterpret_cast<int*>(ws + f.counters);
+  if (const int rc = ffn_clear(counters, f.space.counters, stream)) return rc;
+  ffn_place(&d, partial, counters);
   if (!ffn_map(&p.a[0], a->x, a->rows, a->width, a->x_stride, 128) ||
       !ffn_map(&p.b[0], a->w_gate, a->hidden, a->width, a->w_gate_stride, 128) ||
       !ffn_map(&p.b[1], a->w_up, a->hidden, a->width, a->w_up_stride, 128) ||
-      !ffn_map(&p.out[0], h, a->rows, a->hidden, a->hidden, 32))
-    return set_error(TS_ERR_VALUE, kFfnLayout);
-  FfnParams<1> down = {};
-  down.count = 1;
-  down.p[0] = f.down;
-  float* partial = reinterpret_cast<float*>(ws + f.partial);
-  int* counters = reinterpret_cast<int*>(ws + f.counters);
-  if (f.space.counters) {
-    const cudaError_t e = cudaMemsetAsync(counters, 0, f.space.counters * sizeof(int), stream);
-    if (e != cudaSuccess) return set_error(TS_ERR_CUDA, "ffn_fwd: %s", cudaGetErrorString(e));
-  }
-  ffn_place(&down.p[0], partial, counters);
-  if (!ffn_map(&down.p[0].a[0], h, a->rows, a->hidden, a->hidden, 128) ||
-      !ffn_map(&down.p[0].b[0], a->w_down, a->width_out, a->hidden, a->w_down_stride, 128) ||
-      !ffn_map(&down.p[0].out[0], a->y, a->rows, a->width_out, a->width_out, 32))
+      !ffn_out_map(&p.out[0], h, a->rows, a->hidden) || !ffn_map(&d.a[0], h, a->rows, a->hidden, a->hidden, 128) ||
+      !ffn_map(&d.b[0], a->w_down, a->width_out, a->hidden, a->w_down_stride, 128) ||
+      !ffn_out_map(&d.out[0], a->y, a->rows, a->width_out))
     return set_error(TS_ERR_VALUE, kFfnLayout);
   if (const int rc = ffn_launch_gate<kGateFwd>(gate, a->activation, stream, "ffn_gate_fwd")) return rc;
   return ffn_launch<kProduct, 0>(down, stream, "ffn_down");
@@ -752,65 +847,49 @@ size_t ts_b200_ffn_bwd_workspace_bytes(const ts_ffn_args* a) {
 int ts_b200_ffn_bwd(const ts_ffn_args* a, const ts_ffn_grad_args* g, ts_stream_t stream) {
   using namespace ts;
   if (const int rc = ffn_check(a)) return rc;
-  if (!g || !a->x || !a->w_gate || !a->w_up || !a->w_down || !g->dy)
+  if (!g || !a->x || !a->w_gate || !a->w_up || !a->w_down || !a->h || !a->kept || !g->dy)
     return set_error(TS_ERR_VALUE, "ffn_bwd: null pointer");
   FfnBackward b = ffn_backward(a);
   if (!a->workspace || a->workspace_bytes < b.total) return set_error(TS_ERR_VALUE, "ffn_bwd: workspace too small");
   if (!ffn_bind_context()) return set_error(TS_ERR_CUDA, "ffn_bwd: no context on the current device");
   uint8_t* ws = static_cast<uint8_t*>(a->workspace);
-  void *dg = ws + b.dg, *du = ws + b.du, *h = ws + b.h;
+  void *dg = ws, *du = ws + b.du;
   const long long M = a->rows;
   const int D = a->width, H = a->hidden, O = a->width_out;
-  FfnParams<1> gate = {};
-  gate.count = 1;
+  FfnParams<1> gate = ffn_gate(a, 256, O);
   FfnProblem& p = gate.p[0];
-  p.rows = static_cast<int>(M);
-  p.cols = H;
-  p.tiles_n = static_cast<int>(ffn_tiles(H, 128));
-  p.steps[0] = ffn_steps(D);
-  p.steps[1] = ffn_steps(O);
-  p.splits = 1;
-  p.units = static_cast<int>(ffn_tiles(M, 256)) * p.tiles_n;
-  bool ok = ffn_map(&p.a[0], a->x, M, D, a->x_stride, 128) && ffn_map(&p.a[1], g->dy, M, O, g->dy_stride, 128) &&
-            ffn_map(&p.b[0], a->w_gate, H, D, a->w_gate_stride, 128) &&
-            ffn_map(&p.b[1], a->w_up, H, D, a->w_up_stride, 128) &&
-            ffn_map(&p.b_down, a->w_down, O, H, a->w_down_stride, 64) && ffn_map(&p.out[0], h, M, H, H, 32) &&
-            ffn_map(&p.out[1], dg, M, H, H, 32) && ffn_map(&p.out[2], du, M, H, H, 32);
-  if (!ok) return set_error(TS_ERR_VALUE, kFfnLayout);
+  bool ok = ffn_map(&p.a[0], g->dy, M, O, g->dy_stride, 128) &&
+            ffn_outer_map(&p.b[0], &p.b_layout, a->w_down, O, H, a->w_down_stride) &&
+            ffn_out_map(&p.out[0], dg, M, H) && ffn_out_map(&p.out[1], du, M, H);
   FfnParams<4> grads = {};
   float* partial = reinterpret_cast<float*>(ws + b.partial);
   int* counters = reinterpret_cast<int*>(ws + b.counters);
-  if (b.space.counters) {
-    const cudaError_t e = cudaMemsetAsync(counters, 0, b.space.counters * sizeof(int), stream);
-    if (e != cudaSuccess) return set_error(TS_ERR_CUDA, "ffn_bwd: %s", cudaGetErrorString(e));
-  }
+  if (const int rc = ffn_clear(counters, b.space.counters, stream)) return rc;
   // dWg = dg^T x, dWu = du^T x, dWd = dy^T h: the inner dimension is the tokens, outside in every operand
-  auto weight = [&](FfnProblem& w, const void* left, long long left_cols, long long left_stride, const void* right,
+  auto weight = [&](FfnProblem& w, const void* left, int left_cols, long long left_stride, const void* right,
                     int right_cols, long long right_stride, void* out) {
     if (!out) return true;
-    w.a_mn = w.b_mn = 1;
     ffn_place(&w, partial, counters);
-    const bool mapped = ffn_map(&w.a[0], left, M, static_cast<int>(left_cols), left_stride, 64) &&
-                        ffn_map(&w.b[0], right, M, right_cols, right_stride, 64) &&
-                        ffn_map(&w.out[0], out, left_cols, right_cols, right_cols, 32);
+    const bool mapped = ffn_outer_map(&w.a[0], &w.a_layout, left, M, left_cols, left_stride) &&
+                        ffn_outer_map(&w.b[0], &w.b_layout, right, M, right_cols, right_stride) &&
+                        ffn_out_map(&w.out[0], out, left_cols, right_cols);
     grads.p[grads.count++] = w;
     return mapped;
   };
-  ok = weight(b.p[0], dg, H, H, a->x, D, a->x_stride, g->dw_gate) &&
+  ok = ok && weight(b.p[0], dg, H, H, a->x, D, a->x_stride, g->dw_gate) &&
        weight(b.p[1], du, H, H, a->x, D, a->x_stride, g->dw_up) &&
-       weight(b.p[2], g->dy, O, g->dy_stride, h, H, H, g->dw_down);
+       weight(b.p[2], g->dy, O, g->dy_stride, a->h, H, H, g->dw_down);
   if (ok && g->dx) {
     FfnProblem& x = b.p[3];
-    x.b_mn = 1;
     ffn_place(&x, partial, counters);
     ok = ffn_map(&x.a[0], dg, M, H, H, 128) && ffn_map(&x.a[1], du, M, H, H, 128) &&
-         ffn_map(&x.b[0], a->w_gate, H, D, a->w_gate_stride, 64) &&
-         ffn_map(&x.b[1], a->w_up, H, D, a->w_up_stride, 64) && ffn_map(&x.out[0], g->dx, M, D, D, 32);
+         ffn_outer_map(&x.b[0], &x.b_layout, a->w_gate, H, D, a->w_gate_stride) &&
+         ffn_outer_map(&x.b[1], &x.b_layout, a->w_up, H, D, a->w_up_stride) && ffn_out_map(&x.out[0], g->dx, M, D);
     grads.p[grads.count++] = x;
   }
   if (!ok) return set_error(TS_ERR_VALUE, kFfnLayout);
   if (grads.count == 0) return TS_OK;
-  if (const int rc = ffn_launch_gate<kGateBwd>(gate, a->activation, stream, "ffn_gate_bwd")) return rc;
+  if (const int rc = ffn_launch_gate<kGateGrad>(gate, a->activation, stream, "ffn_gate_grad")) return rc;
   return ffn_launch<kProduct, 0>(grads, stream, "ffn_grads");
 }
 

@@ -26,8 +26,8 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
 
 }  // namespace
 
-bool make_tmap_bf16_sw128(CUtensorMap* map, const void* base, int rank, const uint64_t* dims,
-                          const int64_t* strides, const uint32_t* box) {
+bool make_tmap_bf16(CUtensorMap* map, const void* base, int rank, const uint64_t* dims, const int64_t* strides,
+                    const uint32_t* box, CUtensorMapSwizzle swizzle) {
   const PFN_cuTensorMapEncodeTiled_v12000 encode = encode_fn();
   if (encode == nullptr || rank < 2 || rank > 5) return false;
   if (reinterpret_cast<uintptr_t>(base) % 16 != 0) return false;
@@ -46,9 +46,14 @@ bool make_tmap_bf16_sw128(CUtensorMap* map, const void* base, int rank, const ui
   }
   const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, static_cast<cuuint32_t>(rank),
                             const_cast<void*>(base), gdim, gstride, bdim, estride, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS;
+}
+
+bool make_tmap_bf16_sw128(CUtensorMap* map, const void* base, int rank, const uint64_t* dims,
+                          const int64_t* strides, const uint32_t* box) {
+  return make_tmap_bf16(map, base, rank, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 }  // namespace ts

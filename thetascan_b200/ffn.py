@@ -4,10 +4,11 @@
 * :class:`GatedFFN` -- the module, with ``torch.nn.Linear`` weight layouts.
 
 The kernels (``csrc/ffn.cu``) form both projections, the activation and the
-product in one launch and the down projection in a second; the backward forms
-the projections again instead of keeping them, so nothing of the block is kept
-but its input.  bf16 operands with f32 accumulators and one rounding for every
-stored value.  Any number of rows; widths that are multiples of 8.
+product in one launch and the down projection in a second.  For a backward
+pass the block keeps its input and 8 bytes per hidden value: ``h`` in bf16 and
+both projections in 24 bits.  bf16 operands with f32 accumulators and one
+rounding for every stored value.  Any number of rows; widths that are
+multiples of 8.
 """
 from __future__ import annotations
 
@@ -73,21 +74,36 @@ def _workspace(a, query, device):
     return ws
 
 
-def _ffn_fwd_impl(x, w_gate, w_up, w_down, activation):
+def _hidden(rows, hidden):
+    """Bytes of the projections that a forward keeps (``ts_b200_ffn_kept_bytes``, from shapes alone)."""
+    return -(-rows // 32) * -(-hidden // 32) * 6144
+
+
+def _rows_of(x):
+    return x.numel() // x.shape[-1]
+
+
+def _ffn_fwd_impl(x, w_gate, w_up, w_down, activation, keep):
+    """(y, h, kept); the last two are empty unless ``keep``."""
     with _lib.on_device(x):
         y = torch.empty(*x.shape[:-1], w_down.shape[0], dtype=x.dtype, device=x.device)
+        rows, hidden = _rows_of(x), w_gate.shape[0]
+        h = torch.empty((rows, hidden) if keep else 0, dtype=x.dtype, device=x.device)
+        kept = torch.empty(_hidden(rows, hidden) if keep else 0, dtype=torch.uint8, device=x.device)
         if x.numel():
             lib = _lib.load()
             m = [_matrix(t) for t in (x, w_gate, w_up, w_down)]
             a = _args(*m, activation)
             a.y = y.data_ptr()
+            if keep:
+                a.h, a.kept = h.data_ptr(), kept.data_ptr()
             ws = _workspace(a, lib.ts_b200_ffn_fwd_workspace_bytes, x.device)
             _lib.check(lib.ts_b200_ffn_fwd(ctypes.byref(a), _lib.stream()))
             del ws
-        return y
+        return y, h, kept
 
 
-def _ffn_bwd_impl(dy, x, w_gate, w_up, w_down, activation, wanted):
+def _ffn_bwd_impl(dy, x, w_gate, w_up, w_down, h, kept, activation, wanted):
     """Gradients of x and the three weights; an empty tensor where not wanted."""
     with _lib.on_device(x):
         inputs = (x, w_gate, w_up, w_down)
@@ -98,6 +114,7 @@ def _ffn_bwd_impl(dy, x, w_gate, w_up, w_down, activation, wanted):
         m = [_matrix(t) for t in inputs]
         dy2 = _matrix(dy)
         a = _args(*m, activation)
+        a.h, a.kept = h.data_ptr(), kept.data_ptr()
         ws = _workspace(a, lib.ts_b200_ffn_bwd_workspace_bytes, x.device)
         g = _lib.FfnGradArgs()
         g.dy, g.dy_stride = dy2.data_ptr(), dy2.stride(0)
@@ -108,24 +125,28 @@ def _ffn_bwd_impl(dy, x, w_gate, w_up, w_down, activation, wanted):
 
 
 @torch.library.custom_op(f"{LIB}::gated_ffn_fwd", mutates_args=())
-def gated_ffn_fwd(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, activation: str) -> Tensor:
-    return _ffn_fwd_impl(x, w_gate, w_up, w_down, activation)
+def gated_ffn_fwd(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, activation: str,
+                  keep: bool) -> tuple[Tensor, Tensor, Tensor]:
+    """The block's output, and what its backward reads: h and the projections (empty unless ``keep``)."""
+    return _ffn_fwd_impl(x, w_gate, w_up, w_down, activation, keep)
 
 
 @gated_ffn_fwd.register_fake
-def _(x, w_gate, w_up, w_down, activation):
-    return x.new_empty(*x.shape[:-1], w_down.shape[0])
+def _(x, w_gate, w_up, w_down, activation, keep):
+    rows, hidden = _rows_of(x), w_gate.shape[0]
+    return (x.new_empty(*x.shape[:-1], w_down.shape[0]), x.new_empty((rows, hidden) if keep else (0,)),
+            x.new_empty(_hidden(rows, hidden) if keep else 0, dtype=torch.uint8))
 
 
 @torch.library.custom_op(f"{LIB}::gated_ffn_bwd", mutates_args=())
-def gated_ffn_bwd(dy: Tensor, x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, activation: str,
-                  wanted: list[bool]) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+def gated_ffn_bwd(dy: Tensor, x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, h: Tensor, kept: Tensor,
+                  activation: str, wanted: list[bool]) -> tuple[Tensor, Tensor, Tensor, Tensor]:
     """Gradients of x, w_gate, w_up, w_down (empty where not wanted)."""
-    return _ffn_bwd_impl(dy, x, w_gate, w_up, w_down, activation, wanted)
+    return _ffn_bwd_impl(dy, x, w_gate, w_up, w_down, h, kept, activation, wanted)
 
 
 @gated_ffn_bwd.register_fake
-def _(dy, x, w_gate, w_up, w_down, activation, wanted):
+def _(dy, x, w_gate, w_up, w_down, h, kept, activation, wanted):
     return tuple(t.new_empty(t.shape if need else (0,)) for t, need in zip((x, w_gate, w_up, w_down), wanted))
 
 
@@ -135,10 +156,11 @@ class _GatedFFN(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, w_gate, w_up, w_down, activation):
-        ctx.activation = activation
-        ctx.save_for_backward(x, w_gate, w_up, w_down)
         fwd = gated_ffn_fwd if torch.compiler.is_compiling() else _ffn_fwd_impl
-        return fwd(x, w_gate, w_up, w_down, activation)
+        y, h, kept = fwd(x, w_gate, w_up, w_down, activation, True)
+        ctx.activation = activation
+        ctx.save_for_backward(x, w_gate, w_up, w_down, h, kept)
+        return y
 
     @staticmethod
     def backward(ctx, dy):
@@ -157,7 +179,7 @@ def gated_ffn(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, activatio
     if torch.is_grad_enabled() and any(t.requires_grad for t in (x, w_gate, w_up, w_down)):
         return _GatedFFN.apply(x, w_gate, w_up, w_down, activation)
     fwd = gated_ffn_fwd if torch.compiler.is_compiling() else _ffn_fwd_impl
-    return fwd(x, w_gate, w_up, w_down, activation)
+    return fwd(x, w_gate, w_up, w_down, activation, False)[0]
 
 
 class GatedFFN(nn.Module):

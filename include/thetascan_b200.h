@@ -622,6 +622,9 @@ int ts_b200_adamw(const ts_adamw_args* args, ts_stream_t stream);
  * reads.  No reference counterpart (its host model's MLP). */
 enum { TS_FFN_SILU = 0, TS_FFN_GELU = 1 /* exact, by erf */, TS_FFN_RELU2 = 2 /* max(g,0)^2 */ };
 
+/* Bytes of `kept` for each 32 rows x 32 hidden columns (both rounded up). */
+#define TS_FFN_KEPT_BLOCK 6144
+
 typedef struct ts_ffn_args {
   long long rows;
   int width, hidden, width_out;

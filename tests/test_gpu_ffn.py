@@ -281,6 +281,6 @@ def test_c_entry_refuses_bad_arguments():
     a.rows, a.hidden = 33, 136
     assert lib.ts_b200_ffn_kept_bytes(ctypes.byref(a)) == 2 * 5 * 6144
     from thetascan_b200 import ffn
-    assert ffn._hidden(33, 136) == 2 * 5 * 6144
+    assert ffn._kept_bytes(33, 136) == 2 * 5 * 6144
     a.activation = 9
     assert lib.ts_b200_ffn_fwd(ctypes.byref(a), None) == _lib.TS_ERR_VALUE

@@ -10,10 +10,9 @@ import ctypes
 import os
 import threading
 
-import torch
-
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libthetascan_b200.so")
+HOST_PATH = os.path.join(HERE, "_host.so")
 
 TS_OK, TS_ERR_VALUE, TS_ERR_NOT_IMPLEMENTED, TS_ERR_CUDA, TS_ERR_DEVICE = range(5)
 TS_DTYPE_F32, TS_DTYPE_BF16 = 0, 1
@@ -262,6 +261,7 @@ SIGNATURES.update({
 
 _lock = threading.Lock()
 _lib = None
+_host = None
 
 
 class ThetaScanB200Error(RuntimeError):
@@ -286,27 +286,17 @@ def load():
     return _lib
 
 
-def stream() -> int:
-    """Handle of the current stream of the current device."""
-    return torch.cuda.current_stream().cuda_stream
-
-
-class _SameDevice:
-    """A context that changes nothing."""
-
-    def __enter__(self):
-        return None
-
-    def __exit__(self, *_):
-        return False
-
-
-_same_device = _SameDevice()
-
-
-def on_device(t):
-    """A context in which the current device is that of the CUDA tensor ``t``."""
-    return _same_device if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+def host():
+    """The Python extension over the C ABI (``csrc/host.cpp``); loaded once."""
+    global _host
+    if _host is None:
+        load()
+        if not os.path.exists(HOST_PATH):
+            raise ImportError(
+                f"thetascan_b200: {HOST_PATH} is missing; build it with `python -m thetascan_b200.build`")
+        from . import _host as module
+        _host = module
+    return _host
 
 
 def last_error() -> tuple[int, str]:

@@ -261,7 +261,7 @@ __device__ __forceinline__ float ffn_act(float g, float& slope) {
 
 __device__ __forceinline__ uint8_t* keep_at(uint8_t* base, int cols, int row, int col, int lane) {
   const size_t blocks = static_cast<size_t>((cols + 31) >> 5);
-  return base + ((row >> 5) * blocks + (col >> 5)) * 6144 + 16 * lane;
+  return base + ((row >> 5) * blocks + (col >> 5)) * TS_FFN_KEPT_BLOCK + 16 * lane;
 }
 
 // 16 values from r[c] on, as three vectors.
@@ -581,7 +581,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
             KeptHalf next;
             const int ahead = c + o + 16;   // the columns after this half, where they are this tile's and inside
             if (ahead < 64 && row0 < p.rows && u.n + 64 * part + (ahead & 32) < p.cols)
-              next.load(from + (ahead >> 5) * 6144 + ((ahead >> 4) & 1) * (6 * 512));
+              next.load(from + (ahead >> 5) * TS_FFN_KEPT_BLOCK + ((ahead >> 4) & 1) * (6 * 512));
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               float x[8], y[8];
@@ -802,7 +802,7 @@ extern "C" {
 
 size_t ts_b200_ffn_kept_bytes(const ts_ffn_args* a) {
   if (ts::ffn_check(a)) return 0;
-  return static_cast<size_t>((a->rows + 31) / 32) * ((a->hidden + 31) / 32) * 6144;
+  return static_cast<size_t>((a->rows + 31) / 32) * ((a->hidden + 31) / 32) * TS_FFN_KEPT_BLOCK;
 }
 
 size_t ts_b200_ffn_fwd_workspace_bytes(const ts_ffn_args* a) {

@@ -17,14 +17,12 @@ of 256 non-finite.
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import _lib
 
 BLOCK = 256
-_DTYPES = {torch.float32: _lib.TS_DTYPE_F32, torch.bfloat16: _lib.TS_DTYPE_BF16}
+_DTYPES = (torch.float32, torch.bfloat16)
 
 
 def state_scales(n: int) -> int:
@@ -35,15 +33,6 @@ def state_scales(n: int) -> int:
 def _require(ok, message):
     if not ok:
         raise ValueError(f"adamw: {message}")
-
-
-def _same(lists, sizes, dtype, device, what):
-    """Check that the tensors of ``lists`` are contiguous, of ``dtype``, on ``device`` and of the given sizes."""
-    _require(len(lists) == len(sizes), f"{len(sizes)} parameters but {len(lists)} {what}")
-    _require({t.dtype for t in lists} <= {dtype}, f"{what} must be {dtype}")
-    _require([t.numel() for t in lists] == sizes, f"{what} have other sizes than the parameters")
-    _require({t.get_device() for t in lists} <= {device}, f"{what} must be on the parameters' device")
-    _require(all(t.is_contiguous() for t in lists), f"{what} must be contiguous")
 
 
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step: int, lr: float, betas=(0.9, 0.999), eps: float = 1e-8,
@@ -62,71 +51,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step: int, lr: float, be
     b1, b2 = betas
     _require(0 <= b1 < 1 and 0 <= b2 < 1, f"betas must lie in [0, 1), got {betas}")
     _require(lr >= 0 and eps >= 0 and weight_decay >= 0, "lr, eps and weight_decay must be >= 0")
-    n = len(params)
-    if n == 0:
-        return
-    if not all(t.is_cuda for t in params):
-        raise RuntimeError("b200 backend requires CUDA tensors")
-    if torch.cuda.is_current_stream_capturing():
-        raise RuntimeError("adamw: a captured step would repeat its step count; call it outside the graph")
-    device, sizes = params[0].get_device(), [t.numel() for t in params]
-    kinds = {t.dtype for t in params}
-    _require(kinds <= _DTYPES.keys(), "parameters must be float32 or bfloat16")
-    _require(len(grads) == n, f"{n} parameters but {len(grads)} gradients")
-    grad_kinds = {t.dtype for t in grads}
-    ordinals = range(n) if ordinals is None else ordinals
-    if len(kinds) > 1 or len(grad_kinds) > 1:
-        # one launch for each kind
-        groups = {}
-        for i in range(n):
-            groups.setdefault((params[i].dtype, grads[i].dtype), []).append(i)
-        _require(masters is None, "masters need parameters and gradients of one kind")
-        optional = (exp_avg_scales, exp_avg_sq_scales)
-        for at in groups.values():
-            lists = [[x[i] for i in at] for x in (params, grads, exp_avgs, exp_avg_sqs)]
-            m_scales, v_scales = (None if x is None else [x[i] for i in at] for x in optional)
-            adamw_step(*lists, step=step, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay,
-                       exp_avg_scales=m_scales, exp_avg_sq_scales=v_scales, seed=seed,
-                       ordinals=[ordinals[i] for i in at])
-        return
-    kind, grad_kind = kinds.pop(), grad_kinds.pop()
-    _require(grad_kind in _DTYPES, "gradients must be float32 or bfloat16")
-    eight = exp_avgs[0].dtype == torch.float8_e4m3fn if len(exp_avgs) else False
-    _same(params, sizes, kind, device, "parameters")
-    if not all(t.is_contiguous() for t in grads):
-        grads = [t.contiguous() for t in grads]
-    _same(grads, sizes, grad_kind, device, "gradients")
-    state_kind = torch.float8_e4m3fn if eight else torch.float32
-    _same(exp_avgs, sizes, state_kind, device, "first moments")
-    _same(exp_avg_sqs, sizes, state_kind, device, "second moments")
-    columns = [[t.data_ptr() for t in x] for x in (params, grads)]
-    none = [0] * n
-    if masters is not None:
-        _require(kind == torch.bfloat16, "masters belong to bfloat16 parameters")
-        _same(masters, sizes, torch.float32, device, "masters")
-        columns.append([t.data_ptr() for t in masters])
-    else:
-        columns.append(none)
-    columns += [[t.data_ptr() for t in x] for x in (exp_avgs, exp_avg_sqs)]
-    if eight:
-        _require(exp_avg_scales is not None and exp_avg_sq_scales is not None, "8-bit states need their scales")
-        blocks = [state_scales(k) for k in sizes]
-        _same(exp_avg_scales, blocks, torch.float32, device, "scales")
-        _same(exp_avg_sq_scales, blocks, torch.float32, device, "scales")
-        columns += [[t.data_ptr() for t in x] for x in (exp_avg_scales, exp_avg_sq_scales)]
-    else:
-        _require(exp_avg_scales is None and exp_avg_sq_scales is None, "scales belong to 8-bit states")
-        columns += [none, none]
-    # ts_adamw_tensor: seven pointers, the size, and the place (with its padding one more 64-bit word)
-    words = [w for row in zip(*columns, sizes, ordinals, strict=True) for w in row]
-    table = (ctypes.c_longlong * len(words))(*words)
-    a = _lib.AdamWArgs()
-    a.count, a.tensors = n, ctypes.addressof(table)
-    a.param_dtype, a.grad_dtype = _DTYPES[kind], _DTYPES[grad_kind]
-    a.master, a.state_bits, a.step = masters is not None, 8 if eight else 32, step
-    a.lr, a.beta1, a.beta2, a.eps, a.weight_decay, a.seed = lr, b1, b2, eps, weight_decay, seed
-    with _lib.on_device(params[0]):
-        _lib.check(_lib.load().ts_b200_adamw(ctypes.byref(a), _lib.stream()))
+    _lib.host().adamw(params, grads, exp_avgs, exp_avg_sqs, masters, exp_avg_scales, exp_avg_sq_scales, ordinals, step, lr,
+                      b1, b2, eps, weight_decay, seed)
 
 
 class AdamW(torch.optim.Optimizer):

@@ -172,6 +172,37 @@ def test_8bit_special_values(optim):
 
 
 @gpu
+@pytest.mark.parametrize("size", [1e-21, 1e-12, 1e6, 1e12])
+def test_8bit_step_at_extreme_magnitudes(optim, size):
+    # the first step moves by lr (with eps = 0) whatever the gradient's size; v itself is 1e-42 to 1e24
+    gen = torch.Generator().manual_seed(3)
+    g = (size * (1 + torch.rand(700, generator=gen))).cuda()
+    m, r = (torch.zeros(700, device="cuda", dtype=E4M3) for _ in range(2))
+    ms, rs = (torch.zeros(3, device="cuda") for _ in range(2))
+    p = torch.zeros(700, device="cuda")
+    optim.adamw_step([p], [g], [m], [r], step=1, lr=1.0, betas=(0.9, 0.95), eps=0.0, weight_decay=0.0, exp_avg_scales=[ms],
+                     exp_avg_sq_scales=[rs])
+    assert ((p + 1).abs() <= 1e-5).all()
+    for codes, scale, c in ((m, ms, 0.1), (r, rs, math.sqrt(0.05))):
+        off = (_decode(codes, scale) - c * g.double()).abs()
+        assert (off <= c * g.double() / 8 * 1.0001).all()
+
+
+@gpu
+def test_8bit_infinite_value_makes_its_block_non_finite(optim):
+    g = torch.ones(600, device="cuda")
+    g[10] = float("inf")
+    m, r = (torch.zeros(600, device="cuda", dtype=E4M3) for _ in range(2))
+    ms, rs = (torch.zeros(3, device="cuda") for _ in range(2))
+    p = torch.ones(600, device="cuda")
+    optim.adamw_step([p], [g], [m], [r], step=1, **HYPER, exp_avg_scales=[ms], exp_avg_sq_scales=[rs])
+    assert not p[10].isfinite() and p[:10].isfinite().all() and p[11:].isfinite().all()
+    for codes, scale in ((m, ms), (r, rs)):
+        x = _decode(codes, scale)
+        assert not x[:256].isfinite().any() and x[256:].isfinite().all() and (x[256:] > 0).all()
+
+
+@gpu
 @pytest.mark.parametrize("bits", [32, 8])
 @pytest.mark.parametrize("dtype,master", [(F32, False), (BF16, True)])
 def test_optimizer_learns_and_resumes(optim, bits, dtype, master):

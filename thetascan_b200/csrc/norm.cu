@@ -15,9 +15,11 @@
 //
 // Bound by HBM: every stream is read once and written once.  kTpr threads own
 // a row and keep its values (in their own type) in registers between the
-// reduction and the output, so nothing is read twice; a thread has up to 16
-// values of each stream (32 above 8192 columns), which keeps two or more CTAs
-// on an SM and some 64 KB of loads in flight there.  CTAs walk over rows, so a
+// reduction and the output, so nothing is read twice; a thread has up to 8
+// values of each stream (16 above 8192 columns), which leaves registers for
+// 1024 to 1536 threads on an SM and 32 to 98 KB of loads in flight there
+// (with 16 values the compiler keeps as many weights in registers too, and
+// 8-bit output and backward ran at half of this).  CTAs walk over rows, so a
 // thread meets the same columns in every row and the weight gradient is a
 // register sum; one partial row per CTA goes to a workspace, and a second
 // kernel adds the partials in a fixed order (no atomics: the result does not
@@ -103,7 +105,7 @@ __device__ __forceinline__ float row_reduce(float v, float* red, int& turn) {
     v = kMax ? fmaxf(v, other) : v + other;
   }
   if (kTpr > 32) {
-    float* buf = red + turn * 16;
+    float* buf = red + turn * 32;
     turn ^= 1;
     const int warp = threadIdx.x >> 5;
     if ((threadIdx.x & 31) == 0) buf[warp] = v;
@@ -120,14 +122,27 @@ __device__ __forceinline__ float row_reduce(float v, float* red, int& turn) {
 template <int kTpr>
 constexpr int norm_threads() { return kTpr < 256 ? 256 : kTpr; }
 
+// CTAs of a kernel that an SM holds at once: threads that fit beside `regs`
+// registers each.  The kernels are compiled to it and the grids made for it
+// (a grid of more CTAs than are resident leaves a ragged last wave).
+template <int kTpr>
+constexpr int norm_resident(int regs) {
+  return 65536 / regs / norm_threads<kTpr>() > 0 ? 65536 / regs / norm_threads<kTpr>() : 1;
+}
+template <int kTpr>
+constexpr int norm_fwd_resident() { return norm_resident<kTpr>(64); }
+template <int kTpr>
+constexpr int norm_bwd_resident() { return norm_resident<kTpr>(64); }
+
 __device__ __forceinline__ uint8_t to_e4m3(float x) {
   return static_cast<uint8_t>(__nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3));
 }
 
 template <typename T, int kVec, int kPacks, int kTpr, bool kCodes>
-__global__ void __launch_bounds__(norm_threads<kTpr>()) norm_fwd_kernel(const NormParams p) {
+__global__ void __launch_bounds__(norm_threads<kTpr>(), (norm_fwd_resident<kTpr>()))
+    norm_fwd_kernel(const NormParams p) {
   constexpr int kRows = norm_threads<kTpr>() / kTpr;
-  __shared__ float red[32];
+  __shared__ float red[64];
   __shared__ int group_max[kCodes && kVec == 1 ? kRows * (kNormMaxWidth / kNormGroup) : 1];
   const int t = threadIdx.x % kTpr, slot = threadIdx.x / kTpr;
   const float inv_width = 1.f / static_cast<float>(p.width);
@@ -194,7 +209,7 @@ __global__ void __launch_bounds__(norm_threads<kTpr>()) norm_fwd_kernel(const No
     constexpr int kLanes = kNormGroup / kVec < 32 ? kNormGroup / kVec : 32;
     const int n_groups = p.group ? (p.width + kNormGroup - 1) / kNormGroup : 1;
     int* gmax = group_max + slot * (kNormMaxWidth / kNormGroup);
-    float y[kPacks][kVec], top[kPacks], row_top = 0.f;
+    float top[kPacks], row_top = 0.f;
     if (kVec == 1 && p.group) {
       __syncthreads();
       for (int i = t; i < n_groups; i += kTpr) gmax[i] = 0;
@@ -209,8 +224,7 @@ __global__ void __launch_bounds__(norm_threads<kTpr>()) norm_fwd_kernel(const No
         load_weight<kVec>(p.w, p.w_bf16, c, w);
 #pragma unroll
         for (int e = 0; e < kVec; ++e) {
-          y[k][e] = to_f(s[k].v[e]) * rstd * w[e];
-          top[k] = fmaxf(top[k], fabsf(y[k][e]));
+          top[k] = fmaxf(top[k], fabsf(to_f(s[k].v[e]) * rstd * w[e]));
         }
       }
       row_top = fmaxf(row_top, top[k]);
@@ -234,14 +248,24 @@ __global__ void __launch_bounds__(norm_threads<kTpr>()) norm_fwd_kernel(const No
       largest = fmaxf(largest, kScaleFloor);
       const float scale = __fdiv_rn(largest, kE4m3Max);
       if (c == g * kNormGroup) p.scales[row * n_groups + g] = scale;
+      // y / scale to half a unit in the last place, so that ties fall as they should: a product by the reciprocal in
+      // two parts
+      const float inv = __fdiv_rn(1.f, scale), rest = fmaf(-scale, inv, 1.f) * inv;
       Pack<uint8_t, kVec> code;
-      const float inv = __fdiv_rn(1.f, scale);
+      float y[kVec];
+      load_weight<kVec>(p.w, p.w_bf16, c, y);
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) {
-        // y / scale to the last bit but one: a product by the reciprocal, and
-        // one correction by its remainder, so that ties fall as they should
-        const float q = y[k][e] * inv;
-        code.v[e] = to_e4m3(fmaf(fmaf(-q, scale, y[k][e]), inv, q));
+      for (int e = 0; e < kVec; ++e) y[e] *= to_f(s[k].v[e]) * rstd;
+      if (kVec == 1) {
+        code.v[0] = to_e4m3(fmaf(y[0], inv, y[0] * rest));
+      } else {
+#pragma unroll
+        for (int e = 0; e < kVec; e += 2) {
+          const float2 q = make_float2(fmaf(y[e], inv, y[e] * rest), fmaf(y[e + 1], inv, y[e + 1] * rest));
+          const uint16_t two = __nv_cvt_float2_to_fp8x2(q, __NV_SATFINITE, __NV_E4M3);
+          code.v[e] = static_cast<uint8_t>(two);
+          code.v[e + 1] = static_cast<uint8_t>(two >> 8);
+        }
       }
       *reinterpret_cast<Pack<uint8_t, kVec>*>(static_cast<uint8_t*>(p.y) + row * p.width + c) = code;
     }
@@ -249,9 +273,10 @@ __global__ void __launch_bounds__(norm_threads<kTpr>()) norm_fwd_kernel(const No
 }
 
 template <typename T, int kVec, int kPacks, int kTpr>
-__global__ void __launch_bounds__(norm_threads<kTpr>()) norm_bwd_kernel(const NormParams p) {
+__global__ void __launch_bounds__(norm_threads<kTpr>(), (norm_bwd_resident<kTpr>()))
+    norm_bwd_kernel(const NormParams p) {
   constexpr int kThreads = norm_threads<kTpr>(), kRows = kThreads / kTpr;
-  __shared__ float red[32];
+  __shared__ float red[64];
   __shared__ float columns[kRows > 1 ? kThreads * kVec : 1];
   const int t = threadIdx.x % kTpr, slot = threadIdx.x / kTpr;
   const float inv_width = 1.f / static_cast<float>(p.width);
@@ -268,7 +293,7 @@ __global__ void __launch_bounds__(norm_threads<kTpr>()) norm_bwd_kernel(const No
     const T* x = static_cast<const T*>(p.x) + row * p.xs;
     const T* dy = static_cast<const T*>(p.dy) + row * p.dys;
     const T* dsum = static_cast<const T*>(p.dsum) + row * p.dss;
-    Pack<T, kVec> s[kPacks], g[kPacks];
+    Pack<T, kVec> s[kPacks], g[kPacks], a[kPacks];
     const float rstd = active ? p.rstd[row] : 0.f;
 #pragma unroll
     for (int k = 0; k < kPacks; ++k) {
@@ -276,6 +301,7 @@ __global__ void __launch_bounds__(norm_threads<kTpr>()) norm_bwd_kernel(const No
       if (active && c < p.width) {
         s[k] = *reinterpret_cast<const Pack<T, kVec>*>(x + c);
         g[k] = *reinterpret_cast<const Pack<T, kVec>*>(dy + c);
+        if (p.dsum) a[k] = *reinterpret_cast<const Pack<T, kVec>*>(dsum + c);
       }
     }
     float dot = 0.f;
@@ -300,17 +326,15 @@ __global__ void __launch_bounds__(norm_threads<kTpr>()) norm_bwd_kernel(const No
       if (active && c < p.width) {
         float w[kVec];
         load_weight<kVec>(p.w, p.w_bf16, c, w);
-        Pack<T, kVec> a;
-        if (p.dsum) a = *reinterpret_cast<const Pack<T, kVec>*>(dsum + c);
 #pragma unroll
         for (int e = 0; e < kVec; ++e) {
           const float u = to_f(s[k].v[e]) * rstd;
           const float dn = to_f(g[k].v[e]) * w[e];
           float d = rstd * (p.width > 1 ? fmaf(-u, dot, dn) : dn * (p.eps * rstd * rstd));
-          if (p.dsum) d += to_f(a.v[e]);
-          a.v[e] = from_f<T>(d);
+          if (p.dsum) d += to_f(a[k].v[e]);
+          a[k].v[e] = from_f<T>(d);
         }
-        *reinterpret_cast<Pack<T, kVec>*>(static_cast<T*>(p.dx) + row * p.width + c) = a;
+        *reinterpret_cast<Pack<T, kVec>*>(static_cast<T*>(p.dx) + row * p.width + c) = a[k];
       }
     }
   }
@@ -337,23 +361,25 @@ __global__ void __launch_bounds__(norm_threads<kTpr>()) norm_bwd_kernel(const No
   }
 }
 
-// Sum of the partial rows: 32 columns a CTA, its 8 warps each over every
-// eighth row, then the warps in order.
-__global__ void __launch_bounds__(256) norm_dweight_kernel(const float* __restrict__ partial, int n, int width,
-                                                           void* dw, int bf16) {
-  __shared__ float part[8][32];
+// Sum of the partial rows: 32 columns a CTA, its 32 warps each over every
+// 32nd row, then the warps in order.
+constexpr int kDwWarps = 32;
+
+__global__ void __launch_bounds__(32 * kDwWarps) norm_dweight_kernel(const float* __restrict__ partial, int n,
+                                                                     int width, void* dw, int bf16) {
+  __shared__ float part[kDwWarps][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + lane;
   float sum = 0.f;
   if (c < width) {
 #pragma unroll 8
-    for (int i = warp; i < n; i += 8) sum += partial[static_cast<long long>(i) * width + c];
+    for (int i = warp; i < n; i += kDwWarps) sum += partial[static_cast<long long>(i) * width + c];
   }
   part[warp][lane] = sum;
   __syncthreads();
   if (warp == 0 && c < width) {
 #pragma unroll
-    for (int i = 1; i < 8; ++i) sum += part[i][lane];
+    for (int i = 1; i < kDwWarps; ++i) sum += part[i][lane];
     if (bf16) {
       static_cast<__nv_bfloat16*>(dw)[c] = __float2bfloat16_rn(sum);
     } else {
@@ -371,22 +397,17 @@ int norm_grid(long long rows, int rows_per_cta, int resident) {
   return static_cast<int>(wanted < most ? wanted : most);
 }
 
-template <typename T, int kVec, int kPacks, int kTpr>
+template <typename T, int kVec, int kPacks, int kTpr, bool kCodes>
 int norm_fwd_launch(const NormParams& p, cudaStream_t s) {
   constexpr int kThreads = norm_threads<kTpr>();
-  const int grid = norm_grid(p.rows, kThreads / kTpr, 2048 / kThreads);
-  if (p.scales) {
-    norm_fwd_kernel<T, kVec, kPacks, kTpr, true><<<grid, kThreads, 0, s>>>(p);
-  } else {
-    norm_fwd_kernel<T, kVec, kPacks, kTpr, false><<<grid, kThreads, 0, s>>>(p);
-  }
+  const int grid = norm_grid(p.rows, kThreads / kTpr, norm_fwd_resident<kTpr>());
+  norm_fwd_kernel<T, kVec, kPacks, kTpr, kCodes><<<grid, kThreads, 0, s>>>(p);
   return check_launch("norm_fwd");
 }
 
 template <int kTpr>
 int norm_bwd_grid(long long rows) {
-  constexpr int kThreads = norm_threads<kTpr>();
-  return norm_grid(rows, kThreads / kTpr, 1024 / kThreads);
+  return norm_grid(rows, norm_threads<kTpr>() / kTpr, norm_bwd_resident<kTpr>());
 }
 
 template <typename T, int kVec, int kPacks, int kTpr>
@@ -394,20 +415,21 @@ int norm_bwd_launch(const NormParams& p, void* dweight, cudaStream_t s) {
   const int grid = norm_bwd_grid<kTpr>(p.rows);
   norm_bwd_kernel<T, kVec, kPacks, kTpr><<<grid, norm_threads<kTpr>(), 0, s>>>(p);
   if (const int rc = check_launch("norm_bwd")) return rc;
-  norm_dweight_kernel<<<ceil_div(p.width, 32), 256, 0, s>>>(p.partial, grid, p.width, dweight, p.w_bf16);
+  norm_dweight_kernel<<<ceil_div(p.width, 32), 32 * kDwWarps, 0, s>>>(p.partial, grid, p.width, dweight, p.w_bf16);
   return check_launch("norm_dweight");
 }
 
-// Threads per row: 16 values of a stream to a thread, up to 512 threads; above 8192 columns 32 values.
+// Threads per row: F::kEach values of a stream to a thread; twice as many in the widest rows.
 template <typename T, int kVec, class F>
 int norm_by_width(int width, F f) {
-  constexpr int kPacks = 16 / kVec;
-  if (width <= 32 * 16) return f.template operator()<T, kVec, kPacks, 32>();
-  if (width <= 64 * 16) return f.template operator()<T, kVec, kPacks, 64>();
-  if (width <= 128 * 16) return f.template operator()<T, kVec, kPacks, 128>();
-  if (width <= 256 * 16) return f.template operator()<T, kVec, kPacks, 256>();
-  if (width <= 512 * 16) return f.template operator()<T, kVec, kPacks, 512>();
-  return f.template operator()<T, kVec, 2 * kPacks, 512>();
+  constexpr int kEach = F::kEach, kPacks = kEach / kVec, kMost = 8192 / kEach;
+  if (width <= 32 * kEach) return f.template operator()<T, kVec, kPacks, 32>();
+  if (width <= 64 * kEach) return f.template operator()<T, kVec, kPacks, 64>();
+  if (width <= 128 * kEach) return f.template operator()<T, kVec, kPacks, 128>();
+  if (width <= 256 * kEach) return f.template operator()<T, kVec, kPacks, 256>();
+  if (kMost > 512 && width <= 512 * kEach) return f.template operator()<T, kVec, kPacks, (kMost > 512 ? 512 : kMost)>();
+  if (width <= kMost * kEach) return f.template operator()<T, kVec, kPacks, kMost>();
+  return f.template operator()<T, kVec, 2 * kPacks, kMost>();
 }
 
 template <class F>
@@ -417,13 +439,16 @@ int norm_dispatch(int dtype, bool vector, int width, F f) {
   return vector ? norm_by_width<float, 4>(width, f) : norm_by_width<float, 1>(width, f);
 }
 
+template <bool kCodes>
 struct NormFwd {
+  static constexpr int kEach = 16;
   const NormParams& p;
   cudaStream_t s;
   template <typename T, int kVec, int kPacks, int kTpr>
-  int operator()() const { return norm_fwd_launch<T, kVec, kPacks, kTpr>(p, s); }
+  int operator()() const { return norm_fwd_launch<T, kVec, kPacks, kTpr, kCodes>(p, s); }
 };
 struct NormBwd {
+  static constexpr int kEach = 8;
   const NormParams& p;
   void* dweight;
   cudaStream_t s;
@@ -431,6 +456,7 @@ struct NormBwd {
   int operator()() const { return norm_bwd_launch<T, kVec, kPacks, kTpr>(p, dweight, s); }
 };
 struct NormBwdGrid {
+  static constexpr int kEach = NormBwd::kEach;
   long long rows;
   template <typename T, int kVec, int kPacks, int kTpr>
   int operator()() const { return norm_bwd_grid<kTpr>(rows); }
@@ -492,7 +518,9 @@ int ts_b200_norm_fwd(const ts_norm_args* a, ts_stream_t stream) {
   if (a->residual && !a->sum) return ts::set_error(TS_ERR_VALUE, "norm_fwd: a residual needs the sum's output");
   if (a->group && !a->scales) return ts::set_error(TS_ERR_VALUE, "norm_fwd: a group needs scales");
   const ts::NormParams p = ts::norm_params(a);
-  return ts::norm_dispatch(a->dtype, ts::norm_vector(a), a->width, ts::NormFwd{p, stream});
+  const bool vector = ts::norm_vector(a);
+  return a->scales ? ts::norm_dispatch(a->dtype, vector, a->width, ts::NormFwd<true>{p, stream})
+                   : ts::norm_dispatch(a->dtype, vector, a->width, ts::NormFwd<false>{p, stream});
 }
 
 size_t ts_b200_norm_bwd_workspace_bytes(const ts_norm_args* a) {

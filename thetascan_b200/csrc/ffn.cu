@@ -47,6 +47,7 @@
 
 #include "capi_internal.h"
 #include "common.cuh"
+#include "ffn.cuh"
 #include "tma.cuh"
 
 namespace ts {
@@ -228,28 +229,6 @@ __device__ __forceinline__ void tie(uint32_t (&r)[kN]) {
   for (int i = 0; i < kN; i += 8)
     asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]),
                  "+r"(r[i + 6]), "+r"(r[i + 7]));
-}
-
-// ---- activations: value and slope
-
-constexpr int kSilu = TS_FFN_SILU, kGelu = TS_FFN_GELU, kRelu2 = TS_FFN_RELU2;
-
-template <int kAct>
-__device__ __forceinline__ float ffn_act(float g, float& slope) {
-  if (kAct == kSilu) {
-    const float s = __fdividef(1.f, 1.f + __expf(-g));
-    slope = s * fmaf(g, 1.f - s, 1.f);
-    return g * s;
-  }
-  if (kAct == kGelu) {
-    // by erfc: 1 + erf would cancel where g is negative
-    const float s = 0.5f * erfcf(g * -0.70710678118654752f);
-    slope = fmaf(g * 0.39894228040143268f, __expf(-0.5f * g * g), s);
-    return g * s;
-  }
-  const float s = fmaxf(g, 0.f);
-  slope = 2.f * s;
-  return s * s;
 }
 
 // ---- g and u between the passes
@@ -489,7 +468,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
         if (p.splits > 1) {
           float* mine = sums + static_cast<size_t>(u.split) * 65536;
 #pragma unroll 1
-          for (int c = 0; c < 64; c += 32) {
+          for (int c = 0; c < 64 && row0 < p.rows; c += 32) {
             uint32_t v[32];
             tmem_ld(acc + c, v);
             tmem_wait();
@@ -507,6 +486,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
           if (!last) continue;
           __threadfence();
         }
+        if (p.splits > 1 && row0 >= p.rows) continue;
 #pragma unroll 1
         for (int c = 0; c < 64; c += 32) {
           const uint32_t block = next_block();
@@ -711,9 +691,9 @@ int ffn_launch(FfnParams<kCount>& q, cudaStream_t s, const char* what) {
 
 template <int kMode>
 int ffn_launch_gate(FfnParams<1>& q, int activation, cudaStream_t s, const char* what) {
-  if (activation == kSilu) return ffn_launch<kMode, kSilu>(q, s, what);
-  if (activation == kGelu) return ffn_launch<kMode, kGelu>(q, s, what);
-  return ffn_launch<kMode, kRelu2>(q, s, what);
+  if (activation == TS_FFN_SILU) return ffn_launch<kMode, TS_FFN_SILU>(q, s, what);
+  if (activation == TS_FFN_GELU) return ffn_launch<kMode, TS_FFN_GELU>(q, s, what);
+  return ffn_launch<kMode, TS_FFN_RELU2>(q, s, what);
 }
 
 size_t ffn_align(size_t x) { return (x + 1023) & ~static_cast<size_t>(1023); }
@@ -724,7 +704,7 @@ int ffn_check(const ts_ffn_args* a) {
   for (int d : {a->width, a->hidden, a->width_out})
     if (d < 8 || d % 8 || d > (1 << 20))
       return set_error(TS_ERR_NOT_IMPLEMENTED, "ffn: width %d must be a multiple of 8 in 8..2^20", d);
-  if (a->activation < kSilu || a->activation > kRelu2)
+  if (a->activation < TS_FFN_SILU || a->activation > TS_FFN_RELU2)
     return set_error(TS_ERR_VALUE, "ffn: unknown activation %d", a->activation);
   // tiles of the largest product, split or not, count in 32 bits
   if (ffn_tiles(a->rows, 256) * ffn_tiles(a->hidden, 128) > (1 << 28) ||
@@ -819,6 +799,15 @@ int ts_b200_ffn_fwd(const ts_ffn_args* a, ts_stream_t stream) {
   if (!ffn_bind_context()) return set_error(TS_ERR_CUDA, "ffn_fwd: no context on the current device");
   uint8_t* ws = static_cast<uint8_t*>(a->workspace);
   void* h = a->h ? a->h : ws;
+  if (a->rows <= kRowsMost && !a->kept) {
+    const auto bad = [](const void* base, long long stride) {
+      return (reinterpret_cast<uintptr_t>(base) & 15) || stride % 8;
+    };
+    if (bad(a->x, a->x_stride) || bad(a->w_gate, a->w_gate_stride) || bad(a->w_up, a->w_up_stride) ||
+        bad(a->w_down, a->w_down_stride) || bad(a->y, 0) || bad(ws, 0))
+      return set_error(TS_ERR_VALUE, kFfnLayout);
+    return ffn_rows_fwd(a, h, stream);
+  }
   FfnParams<1> gate = ffn_gate(a, 128, a->width);
   FfnProblem& p = gate.p[0];
   FfnParams<1> down = {};

@@ -89,6 +89,8 @@ struct FfnParams {
   FfnProblem p[kCount];
   int count;
   int units;
+  int* clear;        // counters of the launch after this one, set to zero (or null)
+  int clear_count;
 };
 
 // ---- pair-of-CTAs forms of the tensor-core instructions
@@ -353,6 +355,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
     fence_mbar_init();
   }
   if (warp == 2) tmem_alloc_pair(&tmem_slot, 512);
+  if (warp == 3 && blockIdx.x == 0)
+    for (int i = lane; i < q.clear_count; i += 32) q.clear[i] = 0;
   tc_fence_before();
   __syncthreads();
   cluster_sync();
@@ -768,12 +772,6 @@ FfnParams<1> ffn_gate(const ts_ffn_args* a, int tile, int inner) {
   return q;
 }
 
-int ffn_clear(int* counters, size_t n, cudaStream_t s) {
-  if (n == 0) return TS_OK;
-  const cudaError_t e = cudaMemsetAsync(counters, 0, n * sizeof(int), s);
-  return e == cudaSuccess ? TS_OK : set_error(TS_ERR_CUDA, "ffn: %s", cudaGetErrorString(e));
-}
-
 }  // namespace
 
 }  // namespace ts
@@ -796,7 +794,6 @@ int ts_b200_ffn_fwd(const ts_ffn_args* a, ts_stream_t stream) {
   if (!a->kept != !a->h) return set_error(TS_ERR_VALUE, "ffn_fwd: h and kept belong together");
   FfnForward f = ffn_forward(a);
   if (!a->workspace || a->workspace_bytes < f.total) return set_error(TS_ERR_VALUE, "ffn_fwd: workspace too small");
-  if (!ffn_bind_context()) return set_error(TS_ERR_CUDA, "ffn_fwd: no context on the current device");
   uint8_t* ws = static_cast<uint8_t*>(a->workspace);
   void* h = a->h ? a->h : ws;
   if (a->rows <= kRowsMost && !a->kept) {
@@ -808,6 +805,7 @@ int ts_b200_ffn_fwd(const ts_ffn_args* a, ts_stream_t stream) {
       return set_error(TS_ERR_VALUE, kFfnLayout);
     return ffn_rows_fwd(a, h, stream);
   }
+  if (!ffn_bind_context()) return set_error(TS_ERR_CUDA, "ffn_fwd: no context on the current device");
   FfnParams<1> gate = ffn_gate(a, 128, a->width);
   FfnProblem& p = gate.p[0];
   FfnParams<1> down = {};
@@ -816,7 +814,8 @@ int ts_b200_ffn_fwd(const ts_ffn_args* a, ts_stream_t stream) {
   d = f.down;
   float* partial = reinterpret_cast<float*>(ws + f.partial);
   int* counters = reinterpret_cast<int*>(ws + f.counters);
-  if (const int rc = ffn_clear(counters, f.space.counters, stream)) return rc;
+  gate.clear = counters;
+  gate.clear_count = static_cast<int>(f.space.counters);
   ffn_place(&d, partial, counters);
   if (!ffn_map(&p.a[0], a->x, a->rows, a->width, a->x_stride, 128) ||
       !ffn_map(&p.b[0], a->w_gate, a->hidden, a->width, a->w_gate_stride, 128) ||
@@ -853,7 +852,8 @@ int ts_b200_ffn_bwd(const ts_ffn_args* a, const ts_ffn_grad_args* g, ts_stream_t
   FfnParams<4> grads = {};
   float* partial = reinterpret_cast<float*>(ws + b.partial);
   int* counters = reinterpret_cast<int*>(ws + b.counters);
-  if (const int rc = ffn_clear(counters, b.space.counters, stream)) return rc;
+  gate.clear = counters;
+  gate.clear_count = static_cast<int>(b.space.counters);
   // dWg = dg^T x, dWu = du^T x, dWd = dy^T h: the inner dimension is the tokens, outside in every operand
   auto weight = [&](FfnProblem& w, const void* left, int left_cols, long long left_stride, const void* right,
                     int right_cols, long long right_stride, void* out) {

@@ -355,13 +355,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
     fence_mbar_init();
   }
   if (warp == 2) tmem_alloc_pair(&tmem_slot, 512);
-  if (warp == 3 && blockIdx.x == 0)
-    for (int i = lane; i < q.clear_count; i += 32) q.clear[i] = 0;
+  if (warp == 3 && lane < q.count) {
+    const FfnProblem& p = q.p[lane];
+    tma_prefetch_map(&p.a[0]);
+    tma_prefetch_map(&p.b[0]);
+    tma_prefetch_map(&p.out[0]);
+  }
   tc_fence_before();
   __syncthreads();
   cluster_sync();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
+  // up to here nothing of the launch before is read or written: this much overlaps its end
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (warp == 3 && blockIdx.x == 0)
+    for (int i = lane; i < q.clear_count; i += 32) q.clear[i] = 0;
 
   if (warp == 0 && lane == 0) {
     // ---- loads
@@ -689,7 +698,18 @@ int ffn_launch(FfnParams<kCount>& q, cudaStream_t s, const char* what) {
                                                cudaFuncAttributeMaxDynamicSharedMemorySize, kFfnSmem);
   if (set != cudaSuccess) return set_error(TS_ERR_CUDA, "%s: %s", what, cudaGetErrorString(set));
   const int pairs = q.units < kPairs ? q.units : kPairs;
-  ffn_kernel<kMode, kAct, kCount><<<2 * pairs, kFfnThreads, kFfnSmem, s>>>(q);
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(static_cast<unsigned>(2 * pairs));
+  config.blockDim = dim3(kFfnThreads);
+  config.dynamicSmemBytes = kFfnSmem;
+  config.stream = s;
+  config.attrs = &attr;
+  config.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&config, ffn_kernel<kMode, kAct, kCount>, q);
+  if (e != cudaSuccess) return set_error(TS_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
   return check_launch(what);
 }
 

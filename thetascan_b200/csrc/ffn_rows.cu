@@ -18,6 +18,8 @@
 // product, to the CTAs of a cluster; sums meet in shared memory in a fixed
 // order.  The down product is launched to overlap the gate (programmatic
 // dependent launch): its first weights are on their way before it waits for h.
+// The gate is launched in full order, so that weights which the launch before
+// it wrote are there for both.
 #include <cuda_bf16.h>
 
 #include "capi_internal.h"

@@ -652,7 +652,8 @@ bool ffn_out_map(CUtensorMap* map, const void* base, long long rows, int cols) {
 }
 
 // Splits of a product's inner length: enough units for every pair of SMs where
-// the tiles alone leave some without work, each at least kMinSplitSteps long.
+// the launch's `tiles` alone leave some without work, each at least
+// kMinSplitSteps long.
 int ffn_splits(long long tiles, int steps) {
   if (tiles >= kPairs) return 1;
   long long s = kPairs / tiles;
@@ -664,20 +665,26 @@ struct FfnSpace {
   size_t partial = 0, counters = 0;   // floats, ints
 };
 
-// Shape part of a product (no pointers): its tiles, steps and splits; its needs are added to `space`.
-void ffn_product(FfnProblem* p, long long rows, int cols, long long k0, long long k1, FfnSpace* space) {
-  p->rows = static_cast<int>(rows);
-  p->cols = cols;
-  p->tiles_n = static_cast<int>(ffn_tiles(cols, 256));
-  p->steps[0] = ffn_steps(k0);
-  p->steps[1] = k1 ? ffn_steps(k1) : 0;
-  const long long tiles = ffn_tiles(rows, 256) * p->tiles_n;
+// Shape part of a product (no pointers).
+FfnProblem ffn_product(long long rows, int cols, long long k0, long long k1) {
+  FfnProblem p = {};
+  p.rows = static_cast<int>(rows);
+  p.cols = cols;
+  p.tiles_n = static_cast<int>(ffn_tiles(cols, 256));
+  p.steps[0] = ffn_steps(k0);
+  p.steps[1] = k1 ? ffn_steps(k1) : 0;
+  p.units = static_cast<int>(ffn_tiles(rows, 256) * p.tiles_n);
+  p.splits = 1;
+  return p;
+}
+
+// Splits it as one of `tiles` of its launch; what it needs is added to `space`.
+void ffn_split(FfnProblem* p, long long tiles, FfnSpace* space) {
   p->splits = ffn_splits(tiles, p->steps[0] + p->steps[1]);
-  p->units = static_cast<int>(tiles * p->splits);
-  if (p->splits > 1) {
-    space->partial += static_cast<size_t>(p->units) * 65536;
-    space->counters += static_cast<size_t>(tiles) * 2;
-  }
+  if (p->splits == 1) return;
+  space->counters += static_cast<size_t>(p->units) * 2;
+  p->units *= p->splits;
+  space->partial += static_cast<size_t>(p->units) * 65536;
 }
 
 void ffn_place(FfnProblem* p, float*& partial, int*& counters) {
@@ -750,7 +757,8 @@ struct FfnForward {
 
 FfnForward ffn_forward(const ts_ffn_args* a) {
   FfnForward f;
-  ffn_product(&f.down, a->rows, a->width_out, a->hidden, 0, &f.space);
+  f.down = ffn_product(a->rows, a->width_out, a->hidden, 0);
+  ffn_split(&f.down, f.down.units, &f.space);
   f.partial = ffn_align(ffn_hidden_bytes(a));
   f.counters = f.partial + ffn_align(f.space.partial * 4);
   f.total = f.counters + ffn_align(f.space.counters * 4);
@@ -765,10 +773,14 @@ struct FfnBackward {
 
 FfnBackward ffn_backward(const ts_ffn_args* a) {
   FfnBackward b;
-  ffn_product(&b.p[0], a->hidden, a->width, a->rows, 0, &b.space);
-  ffn_product(&b.p[1], a->hidden, a->width, a->rows, 0, &b.space);
-  ffn_product(&b.p[2], a->width_out, a->hidden, a->rows, 0, &b.space);
-  ffn_product(&b.p[3], a->rows, a->width, a->hidden, a->hidden, &b.space);
+  b.p[0] = ffn_product(a->hidden, a->width, a->rows, 0);
+  b.p[1] = ffn_product(a->hidden, a->width, a->rows, 0);
+  b.p[2] = ffn_product(a->width_out, a->hidden, a->rows, 0);
+  b.p[3] = ffn_product(a->rows, a->width, a->hidden, a->hidden);
+  // the weights' gradients, whose inner length is the tokens, come first and are split as one; dx takes what they leave
+  const long long tiles = static_cast<long long>(b.p[0].units) + b.p[1].units + b.p[2].units;
+  for (int i = 0; i < 3; ++i) ffn_split(&b.p[i], tiles, &b.space);
+  ffn_split(&b.p[3], static_cast<long long>(b.p[0].units) + b.p[1].units + b.p[2].units + b.p[3].units, &b.space);
   const size_t one = ffn_align(ffn_hidden_bytes(a));
   b.du = one;
   b.partial = 2 * one;

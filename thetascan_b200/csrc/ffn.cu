@@ -41,7 +41,12 @@
 // A product of few tiles and a long inner length (the weight gradients: the
 // inner length is the number of tokens) is split along it; partial tiles go to
 // a workspace in f32 and the CTA that finishes a tile last adds them in the
-// order of the splits, so the result does not depend on timing.
+// order of the splits, so the result does not depend on timing.  That takes
+// some 10 us, which the launch of the gradients has other tiles to spend on.
+// The down product of few rows has not: there the pairs that share a tile are
+// one cluster, and each sends its sums of the columns that another pair
+// finishes into that pair's shared memory (24 tiles of 44 steps: 19 us with the
+// workspace).
 #include <cmath>
 #include <cstring>
 
@@ -63,7 +68,8 @@ constexpr uint32_t kFfnSmem = kStages * kStageBytes + kEpiWarps * 2 * kOutBlock 
 constexpr int kPairs = 74;
 constexpr int kMinSplitSteps = 8;
 
-enum FfnMode { kGateFwd = 0, kGateGrad = 1, kProduct = 2 };
+// kProductCluster: a product whose few tiles are each split among the pairs of a cluster.
+enum FfnMode { kGateFwd = 0, kGateGrad = 1, kProduct = 2, kProductCluster = 3 };
 
 // How an operand lies in memory: inner dimension contiguous; or M (N)
 // contiguous, loaded as two boxes of 64 columns or as one of 2 x 64.
@@ -103,10 +109,10 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// Cluster address of `bar` in the pair's leading CTA.
-__device__ __forceinline__ uint32_t leader_addr(const void* bar) {
+// Cluster address of `at` (a shared address of this CTA) in the CTA of that rank.
+__device__ __forceinline__ uint32_t cluster_addr(uint32_t at, uint32_t rank) {
   uint32_t a;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_u32(bar)));
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(at), "r"(rank));
   return a;
 }
 __device__ __forceinline__ void arrive_cluster(uint32_t addr) {
@@ -155,12 +161,12 @@ __device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t b, uin
       "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// Arrive on `bar` (the same offset) in both CTAs when the instructions issued so far are done.
-__device__ __forceinline__ void mma_commit_pair(uint64_t* bar) {
+// Arrive on `bar` (the same offset) in both CTAs of the pair led by `lead` when the instructions issued so far are done.
+__device__ __forceinline__ void mma_commit_pair(uint64_t* bar, uint32_t lead) {
   asm volatile(
       "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
           smem_u32(bar)),
-      "h"(static_cast<uint16_t>(3))
+      "h"(static_cast<uint16_t>(3u << lead))
       : "memory");
 }
 // Load a box into this CTA's shared memory, its bytes counted on the leading CTA's barrier.
@@ -333,7 +339,7 @@ __device__ __forceinline__ void stage8(uint32_t block, int lane, int chunk, uint
 }
 
 template <int kMode, int kAct, int kCount>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
+__global__ void __launch_bounds__(kFfnThreads, 1)
     ffn_kernel(const __grid_constant__ FfnParams<kCount> q) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ alignas(8) uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2];
@@ -341,7 +347,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
   __shared__ int is_last;
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = cluster_rank();
+  // the CTA's place in its pair, and the rank in the cluster of the pair's leading CTA
+  const uint32_t rank = cluster_rank() & 1, lead = cluster_rank() & ~1u;
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
@@ -384,7 +391,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
         const int s = it % kStages;
         if (!(ok = wait_cluster(&empty[s], ((it / kStages) & 1) ^ 1, kErrMmaTimeout))) break;
         const uint32_t a = base + s * kStageBytes, b = a + 16384;
-        const uint32_t bar = leader_addr(&full[s]);
+        const uint32_t bar = cluster_addr(smem_u32(&full[s]), lead);
         if (rank == 0) mbar_expect_tx(&full[s], 2 * kStageBytes);
         if (kMode == kGateFwd) {
           ffn_load(a, &p.a[0], kInner, row, k, bar);
@@ -425,9 +432,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
         for (int j = 0; j < 4; ++j)
           mma_pair(acc, smem_desc_sw128(a + a_step * j, a_lbo, 1024), smem_desc_sw128(b + b_step * j, b_lbo, 1024), id,
                    k > u.begin || j > 0);
-        mma_commit_pair(&empty[s]);
+        mma_commit_pair(&empty[s], lead);
       }
-      if (ok) mma_commit_pair(&acc_full[buf]);
+      if (ok) mma_commit_pair(&acc_full[buf], lead);
     }
   } else if (warp >= 4) {
     // ---- accumulators out: a warp takes the 32 rows of its quarter of tensor memory (warp % 4) and a quarter of
@@ -459,7 +466,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
       auto release = [&]() {
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) arrive_cluster(leader_addr(&acc_empty[buf]));
+        if (lane == 0) arrive_cluster(cluster_addr(smem_u32(&acc_empty[buf]), lead));
       };
       const int row0 = u.m + 128 * static_cast<int>(rank) + 32 * quad;
       KeptHalf kept;
@@ -474,6 +481,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
       if (kMode == kProduct) ok = epilogue_all(ok);
       if (!ok) break;
       tc_fence_after();
+      if (kMode == kProductCluster) break;   // its one tile goes on below
       if (kMode == kProduct) {
         const uint32_t acc = tmem + 256u * buf + lanes + 64 * part;
         float* sums = p.partial + (static_cast<size_t>(u.tile) * p.splits * 2 + rank) * 32768 + 64 * part * 128 +
@@ -598,6 +606,79 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFfnThreads, 1)
     }
     if (lane == 0) tma_store_read_wait<0>();
   }
+  if (kMode == kProductCluster) {
+    // The pairs of the cluster hold sums of the same tile over their parts of the inner length.  Quarter p of its
+    // columns is finished by pair p splits / 4; the others send it theirs: [sender][column][row], in the stages'
+    // memory, which no instruction reads any more after the first barrier.
+    const FfnUnit u = ffn_unit<kMode>(q, pair);
+    const FfnProblem& p = *u.p;
+    const int quad = warp & 3, part = (warp - 4) >> 2, owner = part * p.splits / 4;
+    const uint32_t acc = tmem + (static_cast<uint32_t>(quad * 32) << 16) + 64 * part;
+    const int row0 = u.m + 128 * static_cast<int>(rank) + 32 * quad;
+    const bool inside = warp >= 4 && row0 < p.rows;
+    // quarters of the owner before this one, and all of them
+    const int first = (4 * owner + p.splits - 1) / p.splits, mine = (4 * (owner + 1) + p.splits - 1) / p.splits - first;
+    auto slot = [&](int sender) {   // this thread's word of column 0
+      const int place = sender < owner ? sender : sender - 1;
+      return base + 4 * (((place * mine + part - first) * 64) * 128 + 32 * quad + lane);
+    };
+    __syncwarp();
+    tc_fence_before();
+    cluster_sync();
+    tc_fence_after();
+    if (inside && owner != u.split) {
+      const uint32_t to = cluster_addr(slot(u.split), 2 * owner + rank);
+#pragma unroll 1
+      for (int c = 0; c < 64; c += 32) {
+        uint32_t v[32];
+        tmem_ld(acc + c, v);
+        tmem_wait();
+        tie(v);
+#pragma unroll
+        for (int e = 0; e < 32; ++e)
+          asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(to + 512 * (c + e)), "r"(v[e]) : "memory");
+      }
+    }
+    __syncwarp();
+    cluster_sync();
+    if (inside && owner == u.split) {
+      const uint32_t stage = base + kStages * kStageBytes + (warp - 4) * 2 * kOutBlock;
+#pragma unroll 1
+      for (int c = 0; c < 64; c += 32) {
+        uint32_t own[32];
+        tmem_ld(acc + c, own);
+        tmem_wait();
+        tie(own);
+        float v[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) v[e] = 0.f;
+        for (int i = 0; i < p.splits; ++i) {   // in the order of the splits
+          if (i == u.split) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] += __uint_as_float(own[e]);
+          } else {
+            const uint32_t from = slot(i) + 512 * c;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              float x;
+              asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(from + 512 * e));
+              v[e] += x;
+            }
+          }
+        }
+        const uint32_t block = stage + (c >> 5) * kOutBlock;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) stage8(block, lane, i, pack8(v + 8 * i));
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0 && u.n + 64 * part + c < p.cols) tma_store_2d(&p.out[0], u.n + 64 * part + c, row0, block);
+      }
+      if (lane == 0) {
+        tma_store_commit();
+        tma_store_read_wait<0>();
+      }
+    }
+  }
   // both CTAs stay until neither's memory is needed
   __syncwarp();
   tc_fence_before();
@@ -704,17 +785,20 @@ int ffn_launch(FfnParams<kCount>& q, cudaStream_t s, const char* what) {
   const cudaError_t set = cudaFuncSetAttribute(ffn_kernel<kMode, kAct, kCount>,
                                                cudaFuncAttributeMaxDynamicSharedMemorySize, kFfnSmem);
   if (set != cudaSuccess) return set_error(TS_ERR_CUDA, "%s: %s", what, cudaGetErrorString(set));
-  const int pairs = q.units < kPairs ? q.units : kPairs;
-  cudaLaunchAttribute attr = {};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
+  const int pairs = kMode == kProductCluster || q.units < kPairs ? q.units : kPairs;
+  cudaLaunchAttribute attr[2] = {};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(kMode == kProductCluster ? 2 * q.p[0].splits : 2);
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(static_cast<unsigned>(2 * pairs));
   config.blockDim = dim3(kFfnThreads);
   config.dynamicSmemBytes = kFfnSmem;
   config.stream = s;
-  config.attrs = &attr;
-  config.numAttrs = 1;
+  config.attrs = attr;
+  config.numAttrs = 2;
   const cudaError_t e = cudaLaunchKernelEx(&config, ffn_kernel<kMode, kAct, kCount>, q);
   if (e != cudaSuccess) return set_error(TS_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
   return check_launch(what);
@@ -749,20 +833,14 @@ const char* const kFfnLayout = "ffn: every matrix needs a 16-byte aligned base a
 
 size_t ffn_hidden_bytes(const ts_ffn_args* a) { return static_cast<size_t>(a->rows) * a->hidden * 2; }
 
-struct FfnForward {
-  FfnProblem down = {};
-  FfnSpace space;
-  size_t partial = 0, counters = 0, total = 0;   // offsets; h is at 0 where the caller keeps none
-};
-
-FfnForward ffn_forward(const ts_ffn_args* a) {
-  FfnForward f;
-  f.down = ffn_product(a->rows, a->width_out, a->hidden, 0);
-  ffn_split(&f.down, f.down.units, &f.space);
-  f.partial = ffn_align(ffn_hidden_bytes(a));
-  f.counters = f.partial + ffn_align(f.space.partial * 4);
-  f.total = f.counters + ffn_align(f.space.counters * 4);
-  return f;
+// Pairs of a cluster that share each of a product's tiles: as many as leave all
+// clusters resident at once (33, 22 and 15 clusters of 2, 3 and 4 pairs on a
+// B200), each with kMinSplitSteps steps at least.
+int ffn_cluster_splits(int tiles, int steps) {
+  constexpr int kResident[] = {kPairs, 33, 22, 15};
+  int s = 1;
+  while (s < 4 && tiles <= kResident[s] && steps >= (s + 1) * kMinSplitSteps) ++s;
+  return s;
 }
 
 struct FfnBackward {
@@ -816,7 +894,7 @@ size_t ts_b200_ffn_kept_bytes(const ts_ffn_args* a) {
 }
 
 size_t ts_b200_ffn_fwd_workspace_bytes(const ts_ffn_args* a) {
-  return ts::ffn_check(a) ? 0 : ts::ffn_forward(a).total;
+  return ts::ffn_check(a) ? 0 : ts::ffn_align(ts::ffn_hidden_bytes(a));   // h, where the caller keeps none
 }
 
 int ts_b200_ffn_fwd(const ts_ffn_args* a, ts_stream_t stream) {
@@ -824,8 +902,8 @@ int ts_b200_ffn_fwd(const ts_ffn_args* a, ts_stream_t stream) {
   if (const int rc = ffn_check(a)) return rc;
   if (!a->x || !a->w_gate || !a->w_up || !a->w_down || !a->y) return set_error(TS_ERR_VALUE, "ffn_fwd: null pointer");
   if (!a->kept != !a->h) return set_error(TS_ERR_VALUE, "ffn_fwd: h and kept belong together");
-  FfnForward f = ffn_forward(a);
-  if (!a->workspace || a->workspace_bytes < f.total) return set_error(TS_ERR_VALUE, "ffn_fwd: workspace too small");
+  if (!a->workspace || a->workspace_bytes < ts_b200_ffn_fwd_workspace_bytes(a))
+    return set_error(TS_ERR_VALUE, "ffn_fwd: workspace too small");
   uint8_t* ws = static_cast<uint8_t*>(a->workspace);
   void* h = a->h ? a->h : ws;
   if (a->rows <= kRowsMost && !a->kept) {
@@ -843,12 +921,9 @@ int ts_b200_ffn_fwd(const ts_ffn_args* a, ts_stream_t stream) {
   FfnParams<1> down = {};
   down.count = 1;
   FfnProblem& d = down.p[0];
-  d = f.down;
-  float* partial = reinterpret_cast<float*>(ws + f.partial);
-  int* counters = reinterpret_cast<int*>(ws + f.counters);
-  gate.clear = counters;
-  gate.clear_count = static_cast<int>(f.space.counters);
-  ffn_place(&d, partial, counters);
+  d = ffn_product(a->rows, a->width_out, a->hidden, 0);
+  d.splits = ffn_cluster_splits(d.units, d.steps[0]);
+  d.units *= d.splits;
   if (!ffn_map(&p.a[0], a->x, a->rows, a->width, a->x_stride, 128) ||
       !ffn_map(&p.b[0], a->w_gate, a->hidden, a->width, a->w_gate_stride, 128) ||
       !ffn_map(&p.b[1], a->w_up, a->hidden, a->width, a->w_up_stride, 128) ||
@@ -857,7 +932,8 @@ int ts_b200_ffn_fwd(const ts_ffn_args* a, ts_stream_t stream) {
       !ffn_out_map(&d.out[0], a->y, a->rows, a->width_out))
     return set_error(TS_ERR_VALUE, kFfnLayout);
   if (const int rc = ffn_launch_gate<kGateFwd>(gate, a->activation, stream, "ffn_gate_fwd")) return rc;
-  return ffn_launch<kProduct, 0>(down, stream, "ffn_down");
+  return d.splits > 1 ? ffn_launch<kProductCluster, 0>(down, stream, "ffn_down")
+                      : ffn_launch<kProduct, 0>(down, stream, "ffn_down");
 }
 
 size_t ts_b200_ffn_bwd_workspace_bytes(const ts_ffn_args* a) {

@@ -21,6 +21,15 @@ whole training step:
 
 The mixer's output projection starts at zero, as the reference's adapter
 initialises it (thetascan_benchmark_adapter.py:83).
+
+Options of the same model on this package's block kernels: ``gated`` (the
+feed-forward block is a :class:`GatedFFN` of that activation), ``fused_norms``
+(each norm takes the previous branch's addition to the residual stream with
+it), training by :class:`AdamW` with states in 32 or 8 bits, and
+:meth:`HybridLM.quantize_head` (inference logits from an 8-bit norm and an
+8-bit vocabulary projection).  ``python -m thetascan_b200.lm`` trains such a
+model on uniform-random tokens for a few steps and reports loss, time and the
+8-bit head's agreement.
 """
 from __future__ import annotations
 
@@ -31,7 +40,9 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .config import GNConfig, RoPEConfig, TemporalConfig, ThetaScanConfig
+from .ffn import GatedFFN
 from .mixer import ThetaScan
+from .norm import add_rms_norm, rms_norm, rms_norm_8bit
 
 
 def gn_mixer_config(d_model: int = 512, n_heads: int = 8, memory_multiplier: int = 2) -> ThetaScanConfig:
@@ -90,15 +101,36 @@ class MLP(nn.Module):
 
 
 class Block(nn.Module):
-    def __init__(self, d_model: int, n_heads: int, mlp_ratio: int, mixer: nn.Module):
+    def __init__(self, d_model: int, n_heads: int, mlp_ratio: int, mixer: nn.Module, gated: str | None = None):
         super().__init__()
         self.norm1, self.norm2 = RMSNorm(d_model), RMSNorm(d_model)
         self.mix = mixer
-        self.mlp = MLP(d_model, mlp_ratio)
+        self.mlp = MLP(d_model, mlp_ratio) if gated is None else GatedFFN(d_model, mlp_ratio * d_model, gated)
 
     def forward(self, x):
         x = x + self.mix(self.norm1(x))
         return x + self.mlp(self.norm2(x))
+
+    def forward_fused(self, branch, stream):
+        """The block on a residual ``stream`` that the previous ``branch``
+        (None: nothing) still has to be added to; returns its own last branch
+        and the stream before that."""
+        y, stream = _add_norm(self.norm1, branch, stream)
+        y, stream = _add_norm(self.norm2, self.mix(y), stream)
+        return self.mlp(y), stream
+
+
+def _add_norm(norm, branch, stream):
+    if branch is None:
+        return rms_norm(stream, norm.weight, norm.eps), stream
+    return add_rms_norm(branch.to(stream.dtype), stream, norm.weight, norm.eps)
+
+
+def _rows_8bit(w):
+    """e4m3 codes and f32 scales of the rows of ``w`` (largest magnitude to 448)."""
+    w = w.detach().float()
+    scale = w.abs().amax(1, keepdim=True).clamp_min(2.0 ** -100) / 448
+    return (w / scale).to(torch.float8_e4m3fn), scale
 
 
 class HybridLM(nn.Module):
@@ -106,10 +138,15 @@ class HybridLM(nn.Module):
 
     def __init__(self, vocab: int = 1024, d_model: int = 512, n_layers: int = 9, n_heads: int = 8,
                  mlp_ratio: int = 2, mixer_layers=(3, 4), mixer_config: ThetaScanConfig | None = None,
-                 mixer_factory=None):
+                 mixer_factory=None, gated: str | None = None, fused_norms: bool = False):
         """``mixer_factory(config)`` builds a mixer module (default: this
-        package's ThetaScan; a test passes the reference's own to compare)."""
+        package's ThetaScan; a test passes the reference's own to compare).
+        ``gated``: the activation of gated feed-forward blocks (default: the
+        plain squared-ReLU MLP).  ``fused_norms``: residual additions within
+        the norms' kernels (CUDA only)."""
         super().__init__()
+        self.fused_norms = fused_norms
+        self.head_8bit = None
         self.embed = nn.Embedding(vocab, d_model)
         nn.init.normal_(self.embed.weight, std=0.02)
         cfg = mixer_config if mixer_config is not None else gn_mixer_config(d_model, n_heads)
@@ -121,7 +158,7 @@ class HybridLM(nn.Module):
                 mixer.zero_output_projection_()
             else:
                 mixer = CausalAttention(d_model, n_heads)
-            blocks.append(Block(d_model, n_heads, mlp_ratio, mixer))
+            blocks.append(Block(d_model, n_heads, mlp_ratio, mixer, gated))
         self.blocks = nn.ModuleList(blocks)
         self.norm = RMSNorm(d_model)
         # residual-branch outputs of the attention and MLP blocks (the mixers
@@ -130,13 +167,77 @@ class HybridLM(nn.Module):
             if name.endswith("mlp.down.weight") or name.endswith("mix.out.weight"):
                 nn.init.normal_(p, std=0.02 / math.sqrt(2 * n_layers))
 
+    def quantize_head(self) -> None:
+        """Keep the vocabulary projection in 8 bits for inference: from now on
+        calls without gradients take the final norm as e4m3 codes with a scale
+        per row and multiply codes by codes (CUDA; the embedding keeps its
+        type).  Call again after the weights change."""
+        self.head_8bit = _rows_8bit(self.embed.weight)
+
+    def _head(self, branch, stream):
+        norm = self.norm
+        if self.head_8bit is not None and not torch.is_grad_enabled():
+            residual = None if branch is None else branch.to(stream.dtype)
+            codes, scales, *_ = rms_norm_8bit(stream, norm.weight, norm.eps, residual=residual)
+            weight, weight_scale = self.head_8bit
+            logits = torch._scaled_mm(codes.reshape(-1, codes.shape[-1]), weight.t(), scales.reshape(-1, 1),
+                                      weight_scale.t(), out_dtype=torch.bfloat16)
+            return logits.view(*codes.shape[:-1], -1)
+        y = norm(stream) if branch is None and not self.fused_norms else _add_norm(norm, branch, stream)[0]
+        return F.linear(y, self.embed.weight)
+
     def forward(self, tokens):
         x = self.embed(tokens)
+        if not self.fused_norms:
+            for block in self.blocks:
+                x = block(x)
+            return self._head(None, x)
+        branch = None
         for block in self.blocks:
-            x = block(x)
-        return F.linear(self.norm(x), self.embed.weight)
+            branch, x = block.forward_fused(branch, x)
+        return self._head(branch, x)
 
     def loss(self, tokens):
         """Next-token cross entropy of ``tokens [B,T]`` (predicting 1..T-1)."""
         logits = self(tokens[:, :-1])
         return F.cross_entropy(logits.float().reshape(-1, logits.shape[-1]), tokens[:, 1:].reshape(-1))
+
+
+def main() -> None:
+    """Train a gated hybrid model on random tokens with this package's norms, feed-forward blocks and optimizer."""
+    import argparse
+    import time
+
+    from .optim import AdamW
+
+    ap = argparse.ArgumentParser(description=main.__doc__)
+    ap.add_argument("--steps", type=int, default=20)
+    ap.add_argument("--batch", type=int, default=8)
+    ap.add_argument("--tokens", type=int, default=1024)
+    ap.add_argument("--gated", default="silu", choices=("silu", "gelu", "relu2"))
+    ap.add_argument("--state-bits", type=int, default=8, choices=(8, 32))
+    a = ap.parse_args()
+    torch.manual_seed(0)
+    model = HybridLM(gated=a.gated, fused_norms=True).cuda()
+    optimizer = AdamW(model.parameters(), lr=3e-4, betas=(0.9, 0.95), weight_decay=0.1, state_bits=a.state_bits)
+    data = torch.randint(0, model.embed.num_embeddings, (a.batch, a.tokens + 1), device="cuda")
+    for step in range(a.steps):
+        torch.cuda.synchronize()
+        start = time.perf_counter()
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            loss = model.loss(data)
+        loss.backward()
+        optimizer.step()
+        optimizer.zero_grad()
+        torch.cuda.synchronize()
+        print(f"step {step + 1}: loss {loss.detach().item():.4f}, {(time.perf_counter() - start) * 1e3:.1f} ms")
+    with torch.no_grad(), torch.autocast("cuda", dtype=torch.bfloat16):
+        want = model(data[:, :-1]).float()
+        model.quantize_head()
+        got = model(data[:, :-1]).float()
+    print(f"8-bit head: logits within {float((got - want).norm() / want.norm()):.3f} of the bf16 head's, "
+          f"{float((got.argmax(-1) == want.argmax(-1)).float().mean()) * 100:.1f} % of the tokens the same")
+
+
+if __name__ == "__main__":
+    main()

@@ -120,7 +120,7 @@ __device__ __forceinline__ float row_reduce(float v, float* red, int& turn) {
 }
 
 template <int kTpr>
-constexpr int norm_threads() { return kTpr < 256 ? 256 : kTpr; }
+constexpr int norm_threads() { return kTpr < 128 ? 128 : kTpr; }
 
 // CTAs of a kernel that an SM holds at once: threads that fit beside `regs`
 // registers each.  The kernels are compiled to it and the grids made for it
@@ -245,12 +245,12 @@ __global__ void __launch_bounds__(norm_threads<kTpr>(), (norm_fwd_resident<kTpr>
       if (!active || c >= p.width) continue;
       const int g = p.group ? c / kNormGroup : 0;
       float largest = p.group ? (kVec == 1 ? __int_as_float(gmax[g]) : top[k]) : row_top;
-      largest = fmaxf(largest, kScaleFloor);
-      const float scale = __fdiv_rn(largest, kE4m3Max);
+      // the scale, its reciprocal in two parts, and y / scale to half a unit in the last place, so that ties fall as
+      // they should
+      const float scale = fmaxf(largest, kScaleFloor) * (1.f / kE4m3Max);
       if (c == g * kNormGroup) p.scales[row * n_groups + g] = scale;
-      // y / scale to half a unit in the last place, so that ties fall as they should: a product by the reciprocal in
-      // two parts
-      const float inv = __fdiv_rn(1.f, scale), rest = fmaf(-scale, inv, 1.f) * inv;
+      const float r = __fdividef(1.f, scale), inv = fmaf(fmaf(-scale, r, 1.f), r, r);
+      const float rest = fmaf(-scale, inv, 1.f) * inv;
       Pack<uint8_t, kVec> code;
       float y[kVec];
       load_weight<kVec>(p.w, p.w_bf16, c, y);

@@ -254,6 +254,21 @@ def test_optimizer_groups_follow_torch(optim):
 
 
 @gpu
+def test_step_is_refused_in_a_graph_and_seen_by_autograd(optim):
+    p = torch.ones(64, device="cuda", requires_grad=True)
+    args = [[torch.zeros(64, device="cuda")] for _ in range(3)]
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="captured"):
+        with torch.cuda.graph(graph):
+            torch.zeros(1, device="cuda")
+            optim.adamw_step([p], *args, step=1, **HYPER)
+    loss = (p * p).sum()
+    optim.adamw_step([p], *args, step=1, **HYPER)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
+@gpu
 def test_refusals(optim):
     p, g, m, v = ([torch.ones(300, device="cuda")] for _ in range(4))
     ok = dict(step=1, **HYPER)

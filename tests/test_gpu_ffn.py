@@ -252,6 +252,18 @@ def test_refusals(ffn):
         ffn.gated_ffn(x, wg.cpu(), wu, wd)
 
 
+@gpu
+def test_custom_op_refuses_what_does_not_fit(ffn):
+    x, wg, wu, wd, dy = _make(40, 64, 128, 64)
+    _, h, kept = ffn.gated_ffn_fwd(x, wg, wu, wd, "silu", True)
+    all_ = [True] * 4
+    assert len(ffn.gated_ffn_bwd(dy, x, wg, wu, wd, h, kept, "silu", all_)) == 4
+    for bad in ((dy[:3], x, wg, wu, wd, h, kept), (dy, x[:8], wg, wu, wd, h, kept), (dy, x, wg, wu, wd, h[:8], kept),
+                (dy, x, wg, wu, wd, h, kept[:-1]), (dy.float(), x, wg, wu, wd, h, kept)):
+        with pytest.raises(ValueError):
+            ffn.gated_ffn_bwd(*bad, "silu", all_)
+
+
 def test_refuses_cpu_tensors_and_widths():
     from thetascan_b200 import GatedFFN, gated_ffn
     with pytest.raises(RuntimeError):

@@ -246,6 +246,22 @@ def test_refusals(norm):
         norm.rms_norm(x.detach(), w.cpu())
 
 
+@gpu
+def test_custom_op_refuses_what_does_not_fit(norm):
+    x, w, rstd = torch.zeros(4, 64, device="cuda"), torch.ones(64, device="cuda"), torch.ones(4, device="cuda")
+    for bad in ((x[:2], None, x, w, rstd), (x, x[:2], x, w, rstd), (x, None, x, w[:32], rstd), (x, None, x, w, rstd[:3]),
+                (x.bfloat16(), None, x, w, rstd)):
+        with pytest.raises(ValueError):
+            norm.norm_bwd(*bad, EPS)
+
+
+@gpu
+def test_second_gradient_is_refused(norm):
+    x, w = torch.ones(2, 8, device="cuda", requires_grad=True), torch.ones(8, device="cuda")
+    with pytest.raises(RuntimeError, match="no gradient"):
+        torch.autograd.grad(norm.rms_norm(x, w).sum(), x, create_graph=True)
+
+
 def test_refuses_cpu_tensors():
     from thetascan_b200 import rms_norm
     with pytest.raises(RuntimeError):

@@ -138,6 +138,12 @@ NormOut norm_run(const Tensor& x, const OptTensor& residual, const Tensor& weigh
 // (dx, dweight): dx is the gradient of x and of the residual; `sum` is the stored sum (x without a residual).
 std::pair<Tensor, Tensor> norm_grads(const Tensor& dy, const Tensor& dsum, const Tensor& sum, const Tensor& weight,
                                      const Tensor& rstd, double eps) {
+  norm_check(sum, OptTensor(dy), weight, eps);
+  if (dsum.defined()) norm_check(sum, OptTensor(dsum), weight, eps);
+  require_cuda("rstd", rstd, sum);
+  TORCH_CHECK_VALUE(rstd.scalar_type() == at::kFloat && rstd.is_contiguous() &&
+                        rstd.numel() * sum.size(-1) == sum.numel(),
+                    "rstd must be contiguous float32, one value for each row of ", sum.sizes());
   const c10::cuda::CUDAGuard guard(sum.device());
   Tensor dx = at::empty(sum.sizes(), sum.options()), dweight = at::empty(weight.sizes(), weight.options());
   if (sum.numel() == 0) return {dx, dweight.zero_()};
@@ -260,6 +266,10 @@ struct FfnOut {
   Tensor y, h, kept;
 };
 
+int64_t kept_bytes(int64_t rows, int64_t hidden) {
+  return (rows + 31) / 32 * ((hidden + 31) / 32) * TS_FFN_KEPT_BLOCK;
+}
+
 FfnOut ffn_run(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& wd, int activation, bool keep) {
   const c10::cuda::CUDAGuard guard(x.device());
   FfnOut o;
@@ -269,7 +279,7 @@ FfnOut ffn_run(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor
   const int64_t rows = x.numel() / x.size(-1), hidden = wg.size(0);
   if (keep) {
     o.h = at::empty({rows, hidden}, x.options());
-    o.kept = at::empty({(rows + 31) / 32 * ((hidden + 31) / 32) * TS_FFN_KEPT_BLOCK}, x.options().dtype(at::kByte));
+    o.kept = at::empty({kept_bytes(rows, hidden)}, x.options().dtype(at::kByte));
   }
   if (x.numel() == 0) return o;
   FfnCall c(x, wg, wu, wd, activation);
@@ -286,6 +296,17 @@ FfnOut ffn_run(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor
 // Gradients of x, w_gate, w_up, w_down; undefined where not wanted.
 std::vector<Tensor> ffn_grads(const Tensor& dy, const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& wd,
                               const Tensor& h, const Tensor& kept, int activation, const std::vector<bool>& wanted) {
+  ffn_check(x, wg, wu, wd);
+  const int64_t rows = x.numel() / x.size(-1), hidden = wg.size(0);
+  for (const auto& [name, t] : {std::pair<const char*, const Tensor*>{"dy", &dy}, {"h", &h}, {"kept", &kept}})
+    require_cuda(name, *t, x);
+  TORCH_CHECK_VALUE(dy.scalar_type() == at::kBFloat16 && dy.dim() == x.dim() && dy.size(-1) == wd.size(0) &&
+                        dy.numel() == rows * wd.size(0),
+                    "dy must be bfloat16 and of the output's shape, got ", dy.scalar_type(), " ", dy.sizes());
+  TORCH_CHECK_VALUE(h.scalar_type() == at::kBFloat16 && h.is_contiguous() && h.numel() == rows * hidden &&
+                        kept.scalar_type() == at::kByte && kept.is_contiguous() &&
+                        kept.numel() == kept_bytes(rows, hidden),
+                    "h and kept must be what the forward of these inputs kept");
   const c10::cuda::CUDAGuard guard(x.device());
   const Tensor* inputs[] = {&x, &wg, &wu, &wd};
   std::vector<Tensor> out(4);
@@ -433,6 +454,9 @@ struct AdamW {
       kinds[2 * (params[i].scalar_type() == at::kBFloat16) + (grads[i].scalar_type() == at::kBFloat16)].push_back(i);
     for (const auto& k : kinds)
       if (!k.empty()) run(k);
+    // the parameters changed under autograd's eyes
+    for (const Tensor& p : params)
+      if (!p.is_inference()) p.unsafeGetTensorImpl()->bump_version();
   }
 };
 

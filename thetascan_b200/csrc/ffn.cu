@@ -30,13 +30,20 @@
 // sixteen more warps take accumulators out of tensor memory while the next
 // tile's are formed in the other half of it.
 //
-// What bounds it: with loads left out the instructions alone take 246 us of
-// the 290 of kGateFwd at 8192 x 2048 x 5632 (1.53 PFLOP/s), the loads alone
-// 174 us (63 bytes a cycle into each SM).  An operand whose tile is 64 rows of
-// the inner dimension comes as one copy of two column blocks (a map of three
-// dimensions) where its columns are a multiple of 64, else as two copies: the
-// loads of the weight gradients alone take 571 us one way and 648 the other
-// at that size.
+// What bounds it.  At 8192 x 2048 x 5632 a forward and backward pass takes
+// 1460 us, 1.17 PFLOP/s, where cuBLAS holds 1.37 in a loop of a large product
+// under the power limit; kGateFwd takes 350 us there (290 without keeping g and
+// u), its instructions alone, loads left out, 248, its loads alone 174 (63
+// bytes a cycle into each SM): both near their limits at once.  At 65536 x 512
+// x 1024 (630 us) the inner length is eight steps, and the traffic of what is
+// kept and exchanged counts: kGateFwd 153 us (134 with the instructions left
+// out), kGateGrad 139 (737 MB), the gradients 262, the down product 73.
+// An operand whose tile is 64 rows of the inner dimension comes as one copy of
+// two column blocks (a map of three dimensions) where its columns are a
+// multiple of 64, else as two copies: at 8192 x 2048 x 5632 the loads of the
+// weight gradients alone take 571 us one way and 648 the other.  Two groups of
+// epilogue warps on alternate tiles, a sixth stage and other orders of the
+// tiles measured no faster.
 //
 // A product of few tiles and a long inner length (the weight gradients: the
 // inner length is the number of tokens) is split along it; partial tiles go to

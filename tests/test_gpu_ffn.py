@@ -83,6 +83,8 @@ SHAPES = [
     (1, 8, 8, 8), (1, 512, 1024, 512), (2, 64, 128, 64), (5, 264, 136, 72), (8, 1024, 2056, 1024), (9, 128, 512, 128),
     (16, 520, 1032, 520), (17, 72, 264, 8), (31, 256, 256, 256), (33, 256, 256, 256), (64, 512, 512, 512), (65, 192, 320, 448),
     (127, 64, 128, 256), (128, 64, 256, 264), (129, 136, 120, 64), (255, 256, 384, 256), (256, 512, 1024, 512), (257, 256, 256, 512),
+    # few rows past wide weights, with a ragged end of each
+    (12, 136, 2376, 600), (30, 264, 2440, 1192),
     # a long inner length and few tiles: split products, forward and backward
     (100, 64, 4096, 64), (5000, 64, 72, 64), (3001, 128, 384, 320),
     # several tiles for each pair of SMs

@@ -8,8 +8,9 @@ namespace ts {
 
 // Rows up to which an inference call streams the weights past the rows
 // (ffn_rows.cu) instead of forming tiles of 256 rows (ffn.cu).
-// At 1024 x 4096 and 1 / 16 / 32 rows this takes 8.2 / 10.9 / 12.7 us, the
-// tiles 40; at 2048 x 5632 and 32 / 48 / 64 rows 36 / 69 / 73 us, the tiles 49.
+// At 1024 x 4096 and 1 / 16 / 32 rows this takes 7.8 / 10.2 / 11.9 us, the
+// tiles 26; at 2048 x 5632 and 32 rows 31 us, the tiles 34, and at 48 and 64
+// rows 69 and 73 with the tiles still at 34.
 constexpr int kRowsMost = 32;
 
 // The forward for few rows; arguments checked, h holds [rows, hidden].

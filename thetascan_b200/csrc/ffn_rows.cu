@@ -56,47 +56,54 @@ __device__ __forceinline__ uint4 load_weights(const __nv_bfloat16* p) {
   return v;
 }
 
-// One warp's sums over its blocks of the inner dimension: rows `a` and `b` of
-// the weights (null: zeros) by the rows of `x`, 8 kTiles of them.  `blocks`,
-// `first` and `stride` count blocks of 32.  ready() is called between the first
-// weights' loads and the first of x.
-template <int kTiles, class F>
-__device__ __forceinline__ void rows_product(float (&c)[kTiles][4], const __nv_bfloat16* a, const __nv_bfloat16* b,
-                                             const __nv_bfloat16* x, long long xs, int rows, int inner, int first,
-                                             int stride, F ready) {
+// One warp's sums over its blocks of the inner dimension: kSets sets of 16 rows
+// of the weights, `a[i]` and `b[i]` this lane's two of each (null: zeros), by the
+// rows of `x`, 8 kTiles of them.  `first` and `stride` count blocks of 32.
+// ready() is called between the first weights' loads and the first of x.
+template <int kSets, int kTiles, class F>
+__device__ __forceinline__ void rows_product(float (&c)[kSets * kTiles][4], const __nv_bfloat16* const (&a)[kSets],
+                                             const __nv_bfloat16* const (&b)[kSets], const __nv_bfloat16* x,
+                                             long long xs, int rows, int inner, int first, int stride, F ready) {
+  constexpr int kBatch = kRowsBatch / kSets;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const uint4 zero = make_uint4(0, 0, 0, 0);
 #pragma unroll
-  for (int i = 0; i < kTiles; ++i) c[i][0] = c[i][1] = c[i][2] = c[i][3] = 0.f;
+  for (int i = 0; i < kSets * kTiles; ++i) c[i][0] = c[i][1] = c[i][2] = c[i][3] = 0.f;
   const int blocks = (inner + 31) / 32;
   bool waited = false;
-  for (int base = first; base < blocks || !waited; base += stride * kRowsBatch) {
-    uint4 wa[kRowsBatch], wb[kRowsBatch];
+  for (int base = first; base < blocks || !waited; base += stride * kBatch) {
+    uint4 wa[kBatch][kSets], wb[kBatch][kSets];
 #pragma unroll
-    for (int i = 0; i < kRowsBatch; ++i) {
+    for (int i = 0; i < kBatch; ++i) {
       const int k = (base + i * stride) * 32 + 8 * t;
-      wa[i] = a && k < inner ? load_weights(a + k) : zero;
-      wb[i] = b && k < inner ? load_weights(b + k) : zero;
+#pragma unroll
+      for (int m = 0; m < kSets; ++m) {
+        wa[i][m] = a[m] && k < inner ? load_weights(a[m] + k) : zero;
+        wb[i][m] = b[m] && k < inner ? load_weights(b[m] + k) : zero;
+      }
     }
     if (!waited) {
       ready();
       waited = true;
     }
 #pragma unroll
-    for (int i = 0; i < kRowsBatch; ++i) {
+    for (int i = 0; i < kBatch; ++i) {
       const int k = (base + i * stride) * 32 + 8 * t;
 #pragma unroll
       for (int n = 0; n < kTiles; ++n) {
         const int row = 8 * n + g;
         const uint4 v = row < rows && k < inner ? *reinterpret_cast<const uint4*>(x + row * xs + k) : zero;
-        mma_16x8x16(c[n], wa[i].x, wb[i].x, wa[i].y, wb[i].y, v.x, v.y);
-        mma_16x8x16(c[n], wa[i].z, wb[i].z, wa[i].w, wb[i].w, v.z, v.w);
+#pragma unroll
+        for (int m = 0; m < kSets; ++m) {
+          mma_16x8x16(c[m * kTiles + n], wa[i][m].x, wb[i][m].x, wa[i][m].y, wb[i][m].y, v.x, v.y);
+          mma_16x8x16(c[m * kTiles + n], wa[i][m].z, wb[i][m].z, wa[i][m].w, wb[i][m].w, v.z, v.w);
+        }
       }
     }
   }
 }
 
-// Sum of the CTA's warps, in their order, by the first 32 kTiles threads: thread 32 n + lane gets tile n's four values.
+// Sum of the CTA's warps, in their order, by the first 32 kTiles threads: thread 32 n + lane gets sum n's four values.
 template <int kTiles>
 __device__ __forceinline__ float4 rows_sum(const float (&c)[kTiles][4], float4* part) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -117,18 +124,26 @@ __device__ __forceinline__ float4 rows_sum(const float (&c)[kTiles][4], float4* 
   return sum;
 }
 
-template <int kTiles, int kAct>
+template <int kSets, int kTiles, int kAct>
 __global__ void __launch_bounds__(32 * kRowsWarps) ffn_rows_gate_kernel(const FfnRowsParams p) {
-  __shared__ float4 part[kRowsWarps * kTiles * 32];
+  constexpr int kAll = kSets * kTiles;
+  __shared__ float4 part[kRowsWarps * kAll * 32];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int j = blockIdx.x * 8 + g;   // hidden is a multiple of 8
-  float c[kTiles][4];
-  rows_product<kTiles>(c, p.wg + j * p.wgs, p.wu + j * p.wus, p.x, p.xs, p.rows, p.width, threadIdx.x >> 5, kRowsWarps,
-                       [] {});
-  const float4 s = rows_sum<kTiles>(c, part);
-  if (threadIdx.x < 32 * kTiles) {
-    const int row = 8 * (threadIdx.x >> 5) + 2 * t;
+  const __nv_bfloat16 *wg[kSets], *wu[kSets];
+#pragma unroll
+  for (int m = 0; m < kSets; ++m) {
+    const int j = (blockIdx.x * kSets + m) * 8 + g;   // hidden is a multiple of 8: a set of 8 columns is in it or not
+    wg[m] = j < p.hidden ? p.wg + j * p.wgs : nullptr;
+    wu[m] = j < p.hidden ? p.wu + j * p.wus : nullptr;
+  }
+  float c[kAll][4];
+  rows_product<kSets, kTiles>(c, wg, wu, p.x, p.xs, p.rows, p.width, threadIdx.x >> 5, kRowsWarps, [] {});
+  const float4 s = rows_sum<kAll>(c, part);
+  const int m = (threadIdx.x >> 5) / kTiles, n = (threadIdx.x >> 5) % kTiles;
+  const int j = (blockIdx.x * kSets + m) * 8 + g;
+  if (threadIdx.x < 32 * kAll && j < p.hidden) {
+    const int row = 8 * n + 2 * t;
     float slope;
     if (row < p.rows)
       p.h[static_cast<long long>(row) * p.hidden + j] = __float2bfloat16_rn(ffn_act<kAct>(s.x, slope) * s.z);
@@ -137,68 +152,81 @@ __global__ void __launch_bounds__(32 * kRowsWarps) ffn_rows_gate_kernel(const Ff
   }
 }
 
-constexpr int kRowsRanks = 8;   // CTAs that share a down tile's inner length, at most
+// CTAs that share a down tile's inner length: at most 8, and 4 where their sums would outgrow static shared memory.
+constexpr int rows_ranks(int all) { return all > 4 ? 4 : 8; }
 
-template <int kTiles>
+template <int kSets, int kTiles>
 __global__ void __launch_bounds__(32 * kRowsWarps) ffn_rows_down_kernel(const FfnRowsParams p) {
-  __shared__ float4 part[kRowsWarps * kTiles * 32];
-  __shared__ float4 sums[kRowsRanks * kTiles * 32];   // the cluster's, in its first CTA
+  constexpr int kAll = kSets * kTiles;
+  __shared__ float4 part[kRowsWarps * kAll * 32];
+  __shared__ float4 sums[rows_ranks(kAll) * kAll * 32];   // the cluster's, in its first CTA
   asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");   // this CTA runs: its memory may be written
   uint32_t rank, ranks;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int o = blockIdx.x / ranks * 16 + g;   // out is a multiple of 8: rows g and g + 8 are whole groups
-  float c[kTiles][4];
-  rows_product<kTiles>(c, p.wd + o * p.wds, o + 8 < p.out ? p.wd + (o + 8) * p.wds : nullptr, p.h, p.hidden, p.rows,
-                       p.hidden, static_cast<int>(rank) * kRowsWarps + (threadIdx.x >> 5),
-                       static_cast<int>(ranks) * kRowsWarps,
-                       [] { asm volatile("griddepcontrol.wait;" ::: "memory"); });
-  float4 s = rows_sum<kTiles>(c, part);
+  const int first = blockIdx.x / ranks * 16 * kSets;
+  const __nv_bfloat16 *wa[kSets], *wb[kSets];
+#pragma unroll
+  for (int m = 0; m < kSets; ++m) {
+    const int o = first + 16 * m + g;   // out is a multiple of 8: rows o and o + 8 are whole groups
+    wa[m] = o < p.out ? p.wd + o * p.wds : nullptr;
+    wb[m] = o + 8 < p.out ? p.wd + (o + 8) * p.wds : nullptr;
+  }
+  float c[kAll][4];
+  rows_product<kSets, kTiles>(c, wa, wb, p.h, p.hidden, p.rows, p.hidden,
+                              static_cast<int>(rank) * kRowsWarps + (threadIdx.x >> 5),
+                              static_cast<int>(ranks) * kRowsWarps,
+                              [] { asm volatile("griddepcontrol.wait;" ::: "memory"); });
+  float4 s = rows_sum<kAll>(c, part);
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-  if (threadIdx.x < 32 * kTiles) {
+  if (threadIdx.x < 32 * kAll) {
     uint32_t at;
     asm volatile("mapa.shared::cluster.u32 %0, %1, 0;"
                  : "=r"(at)
-                 : "r"(smem_u32(&sums[rank * kTiles * 32 + threadIdx.x])));
+                 : "r"(smem_u32(&sums[rank * kAll * 32 + threadIdx.x])));
     asm volatile("st.shared::cluster.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(at), "f"(s.x), "f"(s.y), "f"(s.z), "f"(s.w)
                  : "memory");
   }
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-  if (rank != 0 || threadIdx.x >= 32 * kTiles) return;
+  if (rank != 0 || threadIdx.x >= 32 * kAll) return;
   s = sums[threadIdx.x];
   for (uint32_t i = 1; i < ranks; ++i) {
-    const float4 v = sums[i * kTiles * 32 + threadIdx.x];
+    const float4 v = sums[i * kAll * 32 + threadIdx.x];
     s.x += v.x;
     s.y += v.y;
     s.z += v.z;
     s.w += v.w;
   }
-  const int row = 8 * (threadIdx.x >> 5) + 2 * t;
+  const int o = first + 16 * ((threadIdx.x >> 5) / kTiles) + g, row = 8 * ((threadIdx.x >> 5) % kTiles) + 2 * t;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    if (row + i >= p.rows) continue;
+    if (row + i >= p.rows || o >= p.out) continue;
     __nv_bfloat16* y = p.y + static_cast<long long>(row + i) * p.out + o;
     y[0] = __float2bfloat16_rn(i ? s.y : s.x);
     if (o + 8 < p.out) y[8] = __float2bfloat16_rn(i ? s.w : s.z);
   }
 }
 
-template <int kTiles>
-int ffn_rows_launch(const FfnRowsParams& p, int activation, cudaStream_t s) {
-  const int gate = p.hidden / 8, threads = 32 * kRowsWarps;
+template <int kSets, int kTiles>
+int ffn_rows_gate(const FfnRowsParams& p, int activation, cudaStream_t s) {
+  const int grid = (p.hidden + 8 * kSets - 1) / (8 * kSets), threads = 32 * kRowsWarps;
   if (activation == TS_FFN_SILU) {
-    ffn_rows_gate_kernel<kTiles, TS_FFN_SILU><<<gate, threads, 0, s>>>(p);
+    ffn_rows_gate_kernel<kSets, kTiles, TS_FFN_SILU><<<grid, threads, 0, s>>>(p);
   } else if (activation == TS_FFN_GELU) {
-    ffn_rows_gate_kernel<kTiles, TS_FFN_GELU><<<gate, threads, 0, s>>>(p);
+    ffn_rows_gate_kernel<kSets, kTiles, TS_FFN_GELU><<<grid, threads, 0, s>>>(p);
   } else {
-    ffn_rows_gate_kernel<kTiles, TS_FFN_RELU2><<<gate, threads, 0, s>>>(p);
+    ffn_rows_gate_kernel<kSets, kTiles, TS_FFN_RELU2><<<grid, threads, 0, s>>>(p);
   }
-  if (const int rc = check_launch("ffn_rows_gate")) return rc;
+  return check_launch("ffn_rows_gate");
+}
+
+template <int kSets, int kTiles>
+int ffn_rows_down(const FfnRowsParams& p, cudaStream_t s) {
   // CTAs of a cluster share a tile's inner length: until two CTAs are there for each SM, or a warp has one batch
-  const int tiles = (p.out + 15) / 16, blocks = (p.hidden + 31) / 32;
+  const int tiles = (p.out + 16 * kSets - 1) / (16 * kSets), blocks = (p.hidden + 31) / 32;
   int ranks = 1;
-  while (ranks < kRowsRanks && tiles * ranks < 2 * 148 && blocks > ranks * kRowsWarps * kRowsBatch) ranks *= 2;
+  while (ranks < rows_ranks(kSets * kTiles) && tiles * ranks < 2 * 148 && blocks > ranks * kRowsWarps * kRowsBatch / kSets) ranks *= 2;
   cudaLaunchAttribute attr[2] = {};
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = static_cast<unsigned>(ranks);
@@ -207,13 +235,28 @@ int ffn_rows_launch(const FfnRowsParams& p, int activation, cudaStream_t s) {
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(static_cast<unsigned>(tiles * ranks));
-  config.blockDim = dim3(static_cast<unsigned>(threads));
+  config.blockDim = dim3(32 * kRowsWarps);
   config.stream = s;
   config.attrs = attr;
   config.numAttrs = 2;
-  const cudaError_t e = cudaLaunchKernelEx(&config, ffn_rows_down_kernel<kTiles>, p);
+  const cudaError_t e = cudaLaunchKernelEx(&config, ffn_rows_down_kernel<kSets, kTiles>, p);
   if (e != cudaSuccess) return set_error(TS_ERR_CUDA, "ffn_rows_down: %s", cudaGetErrorString(e));
   return check_launch("ffn_rows_down");
+}
+
+// Two sets of weight rows to a warp read x half as often, one set has twice the
+// CTAs: two where there are several tiles of rows and CTAs enough all the same
+// (2048 x 5632, 16 / 32 rows: 22.5 / 31 us with two, 24.8 / 36 with one).
+constexpr int kRowsCtas = 148;
+
+template <int kTiles>
+int ffn_rows_launch(const FfnRowsParams& p, int activation, cudaStream_t s) {
+  constexpr int kSets = kTiles > 1 ? 2 : 1;
+  const int rc = p.hidden / (8 * kSets) >= kRowsCtas ? ffn_rows_gate<kSets, kTiles>(p, activation, s)
+                                                     : ffn_rows_gate<1, kTiles>(p, activation, s);
+  if (rc) return rc;
+  return p.out / (16 * kSets) * rows_ranks(kSets * kTiles) >= kRowsCtas ? ffn_rows_down<kSets, kTiles>(p, s)
+                                                        : ffn_rows_down<1, kTiles>(p, s);
 }
 
 }  // namespace

@@ -636,7 +636,7 @@ typedef struct ts_ffn_args {
   long long x_stride, w_gate_stride, w_up_stride, w_down_stride;  /* elements between rows */
   void* y;                  /* [rows,width_out] (forward) */
   void* h;                  /* bf16 [rows,hidden], with kept; both NULL in inference */
-  void* kept;
+  void* kept;               /* 16-byte aligned */
   void* workspace;
   size_t workspace_bytes;
 } ts_ffn_args;

@@ -264,6 +264,9 @@ def test_custom_op_refuses_what_does_not_fit(ffn):
                 (dy, x, wg, wu, wd, h, kept[:-1]), (dy.float(), x, wg, wu, wd, h, kept)):
         with pytest.raises(ValueError):
             ffn.gated_ffn_bwd(*bad, "silu", all_)
+    moved = torch.empty(kept.numel() + 4, dtype=torch.uint8, device="cuda")[4:]
+    with pytest.raises(ValueError, match="aligned"):
+        ffn.gated_ffn_bwd(dy, x, wg, wu, wd, h, moved, "silu", all_)
 
 
 def test_refuses_cpu_tensors_and_widths():

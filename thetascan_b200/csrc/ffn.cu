@@ -909,6 +909,7 @@ int ts_b200_ffn_fwd(const ts_ffn_args* a, ts_stream_t stream) {
   if (const int rc = ffn_check(a)) return rc;
   if (!a->x || !a->w_gate || !a->w_up || !a->w_down || !a->y) return set_error(TS_ERR_VALUE, "ffn_fwd: null pointer");
   if (!a->kept != !a->h) return set_error(TS_ERR_VALUE, "ffn_fwd: h and kept belong together");
+  if (reinterpret_cast<uintptr_t>(a->kept) & 15) return set_error(TS_ERR_VALUE, "ffn_fwd: kept must be 16-byte aligned");
   if (!a->workspace || a->workspace_bytes < ts_b200_ffn_fwd_workspace_bytes(a))
     return set_error(TS_ERR_VALUE, "ffn_fwd: workspace too small");
   uint8_t* ws = static_cast<uint8_t*>(a->workspace);
@@ -952,6 +953,7 @@ int ts_b200_ffn_bwd(const ts_ffn_args* a, const ts_ffn_grad_args* g, ts_stream_t
   if (const int rc = ffn_check(a)) return rc;
   if (!g || !a->x || !a->w_gate || !a->w_up || !a->w_down || !a->h || !a->kept || !g->dy)
     return set_error(TS_ERR_VALUE, "ffn_bwd: null pointer");
+  if (reinterpret_cast<uintptr_t>(a->kept) & 15) return set_error(TS_ERR_VALUE, "ffn_bwd: kept must be 16-byte aligned");
   FfnBackward b = ffn_backward(a);
   if (!a->workspace || a->workspace_bytes < b.total) return set_error(TS_ERR_VALUE, "ffn_bwd: workspace too small");
   if (!ffn_bind_context()) return set_error(TS_ERR_CUDA, "ffn_bwd: no context on the current device");

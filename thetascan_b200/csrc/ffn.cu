@@ -901,7 +901,9 @@ size_t ts_b200_ffn_kept_bytes(const ts_ffn_args* a) {
 }
 
 size_t ts_b200_ffn_fwd_workspace_bytes(const ts_ffn_args* a) {
-  return ts::ffn_check(a) ? 0 : ts::ffn_align(ts::ffn_hidden_bytes(a));   // h, where the caller keeps none
+  if (ts::ffn_check(a)) return 0;
+  // h, where the caller keeps none; for few rows in two parts
+  return ts::ffn_align(ts::ffn_hidden_bytes(a) * (a->rows <= ts::kRowsMost ? 2 : 1));
 }
 
 int ts_b200_ffn_fwd(const ts_ffn_args* a, ts_stream_t stream) {

@@ -8,12 +8,12 @@ namespace ts {
 
 // Rows up to which an inference call streams the weights past the rows
 // (ffn_rows.cu) instead of forming tiles of 256 rows (ffn.cu).
-// At 1024 x 4096 and 1 / 16 / 32 rows this takes 7.8 / 10.2 / 11.9 us, the
-// tiles 26; at 2048 x 5632 and 32 rows 31 us, the tiles 34, and at 48 and 64
+// At 1024 x 4096 and 1 / 16 / 32 rows this takes 8.8 / 11.2 / 13.8 us, the
+// tiles 26; at 2048 x 5632 and 32 rows 32 us, the tiles 34, and at 48 and 64
 // rows 69 and 73 with the tiles still at 34.
 constexpr int kRowsMost = 32;
 
-// The forward for few rows; arguments checked, h holds [rows, hidden].
+// The forward for few rows; arguments checked, h holds [2, rows, hidden].
 int ffn_rows_fwd(const ts_ffn_args* a, void* h, cudaStream_t s);
 
 // The activations: value and slope.

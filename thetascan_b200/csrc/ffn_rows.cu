@@ -11,6 +11,11 @@
 //         that a thread ends with g and u of the same place: h = act(g) u
 //   down: A = 16 rows of Wd
 //
+// h passes between the two as two bf16 values, its rounding and the rest's
+// (2^-17 together): the result then carries its own rounding alone (1.66e-3 of
+// its norm, with h in bf16 2.35e-3), for a second load and instruction beside
+// the weights' traffic (1024 x 4096, one row: 7.8 -> 8.8 us).
+//
 // The order of the inner dimension is free as long as A and B agree, so a lane
 // takes 8 neighbouring elements (16 bytes) of its row for two steps of
 // m16n8k16.  The inner dimension is dealt in blocks of 32 to the CTA's eight
@@ -36,7 +41,7 @@ constexpr int kRowsBatch = 4;        // blocks of 32 a warp has in flight
 struct FfnRowsParams {
   const __nv_bfloat16 *x, *wg, *wu, *wd;
   long long xs, wgs, wus, wds;
-  __nv_bfloat16 *h, *y;
+  __nv_bfloat16 *h, *y;      // h: [2][rows][hidden]
   int rows, width, hidden, out;
 };
 
@@ -58,9 +63,9 @@ __device__ __forceinline__ uint4 load_weights(const __nv_bfloat16* p) {
 
 // One warp's sums over its blocks of the inner dimension: kSets sets of 16 rows
 // of the weights, `a[i]` and `b[i]` this lane's two of each (null: zeros), by the
-// rows of `x`, 8 kTiles of them.  `first` and `stride` count blocks of 32.
-// ready() is called between the first weights' loads and the first of x.
-template <int kSets, int kTiles, class F>
+// rows of `x`, 8 kTiles of them (kTwo: and by those of a second matrix behind
+// it).  `first` and `stride` count blocks of 32.  ready() is called between the first weights' loads and the first of x.
+template <int kSets, int kTiles, bool kTwo, class F>
 __device__ __forceinline__ void rows_product(float (&c)[kSets * kTiles][4], const __nv_bfloat16* const (&a)[kSets],
                                              const __nv_bfloat16* const (&b)[kSets], const __nv_bfloat16* x,
                                              long long xs, int rows, int inner, int first, int stride, F ready) {
@@ -92,12 +97,18 @@ __device__ __forceinline__ void rows_product(float (&c)[kSets * kTiles][4], cons
 #pragma unroll
       for (int n = 0; n < kTiles; ++n) {
         const int row = 8 * n + g;
-        const uint4 v = row < rows && k < inner ? *reinterpret_cast<const uint4*>(x + row * xs + k) : zero;
+        const bool there = row < rows && k < inner;
+        uint4 v[kTwo ? 2 : 1];
 #pragma unroll
-        for (int m = 0; m < kSets; ++m) {
-          mma_16x8x16(c[m * kTiles + n], wa[i][m].x, wb[i][m].x, wa[i][m].y, wb[i][m].y, v.x, v.y);
-          mma_16x8x16(c[m * kTiles + n], wa[i][m].z, wb[i][m].z, wa[i][m].w, wb[i][m].w, v.z, v.w);
-        }
+        for (int h = 0; h < (kTwo ? 2 : 1); ++h)
+          v[h] = there ? *reinterpret_cast<const uint4*>(x + (static_cast<long long>(h) * rows + row) * xs + k) : zero;
+#pragma unroll
+        for (int h = 0; h < (kTwo ? 2 : 1); ++h)
+#pragma unroll
+          for (int m = 0; m < kSets; ++m) {
+            mma_16x8x16(c[m * kTiles + n], wa[i][m].x, wb[i][m].x, wa[i][m].y, wb[i][m].y, v[h].x, v[h].y);
+            mma_16x8x16(c[m * kTiles + n], wa[i][m].z, wb[i][m].z, wa[i][m].w, wb[i][m].w, v[h].z, v[h].w);
+          }
       }
     }
   }
@@ -138,17 +149,24 @@ __global__ void __launch_bounds__(32 * kRowsWarps) ffn_rows_gate_kernel(const Ff
     wu[m] = j < p.hidden ? p.wu + j * p.wus : nullptr;
   }
   float c[kAll][4];
-  rows_product<kSets, kTiles>(c, wg, wu, p.x, p.xs, p.rows, p.width, threadIdx.x >> 5, kRowsWarps, [] {});
+  rows_product<kSets, kTiles, false>(c, wg, wu, p.x, p.xs, p.rows, p.width, threadIdx.x >> 5, kRowsWarps, [] {});
   const float4 s = rows_sum<kAll>(c, part);
   const int m = (threadIdx.x >> 5) / kTiles, n = (threadIdx.x >> 5) % kTiles;
   const int j = (blockIdx.x * kSets + m) * 8 + g;
   if (threadIdx.x < 32 * kAll && j < p.hidden) {
     const int row = 8 * n + 2 * t;
     float slope;
-    if (row < p.rows)
-      p.h[static_cast<long long>(row) * p.hidden + j] = __float2bfloat16_rn(ffn_act<kAct>(s.x, slope) * s.z);
-    if (row + 1 < p.rows)
-      p.h[static_cast<long long>(row + 1) * p.hidden + j] = __float2bfloat16_rn(ffn_act<kAct>(s.y, slope) * s.w);
+    const float h[2] = {ffn_act<kAct>(s.x, slope) * s.z, ffn_act<kAct>(s.y, slope) * s.w};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (row + i >= p.rows) continue;
+      const __nv_bfloat16 high = __float2bfloat16_rn(h[i]);
+      // nothing is left of an infinity or a NaN
+      const float rest = isfinite(h[i]) && isfinite(__bfloat162float(high)) ? h[i] - __bfloat162float(high) : 0.f;
+      __nv_bfloat16* to = p.h + static_cast<long long>(row + i) * p.hidden + j;
+      *to = high;
+      to[static_cast<long long>(p.rows) * p.hidden] = __float2bfloat16_rn(rest);
+    }
   }
 }
 
@@ -174,10 +192,10 @@ __global__ void __launch_bounds__(32 * kRowsWarps) ffn_rows_down_kernel(const Ff
     wb[m] = o + 8 < p.out ? p.wd + (o + 8) * p.wds : nullptr;
   }
   float c[kAll][4];
-  rows_product<kSets, kTiles>(c, wa, wb, p.h, p.hidden, p.rows, p.hidden,
-                              static_cast<int>(rank) * kRowsWarps + (threadIdx.x >> 5),
-                              static_cast<int>(ranks) * kRowsWarps,
-                              [] { asm volatile("griddepcontrol.wait;" ::: "memory"); });
+  rows_product<kSets, kTiles, true>(c, wa, wb, p.h, p.hidden, p.rows, p.hidden,
+                                    static_cast<int>(rank) * kRowsWarps + (threadIdx.x >> 5),
+                                    static_cast<int>(ranks) * kRowsWarps,
+                                    [] { asm volatile("griddepcontrol.wait;" ::: "memory"); });
   float4 s = rows_sum<kAll>(c, part);
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   if (threadIdx.x < 32 * kAll) {
@@ -246,7 +264,8 @@ int ffn_rows_down(const FfnRowsParams& p, cudaStream_t s) {
 
 // Two sets of weight rows to a warp read x half as often, one set has twice the
 // CTAs: two where there are several tiles of rows and CTAs enough all the same
-// (2048 x 5632, 16 / 32 rows: 22.5 / 31 us with two, 24.8 / 36 with one).
+// (2048 x 5632, 16 / 32 rows: 22.5 / 31 us with two, 24.8 / 36 with one, before
+// h had two parts).
 constexpr int kRowsCtas = 148;
 
 template <int kTiles>

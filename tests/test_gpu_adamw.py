@@ -189,6 +189,35 @@ def test_8bit_step_at_extreme_magnitudes(optim, size):
 
 
 @gpu
+@pytest.mark.parametrize("pdtype,gdtype,master", [(F32, F32, False), (BF16, BF16, False), (BF16, F32, True)])
+@pytest.mark.parametrize("size", [2e14, 3e14, 1e16, 1e19, 1e25, 1e37])
+def test_8bit_step_of_large_finite_gradients(optim, size, pdtype, gdtype, master):
+    # the first step moves by lr (with eps = 0) whatever the gradient's size, in the blocks with one large gradient, the
+    # whole one and the ragged last one, as in those without.  f32: a few roundings and an approximate quotient, 1e-5;
+    # the gradient's own rounding cancels.  A block's small values keep their step, and the least code.
+    gen = torch.Generator().manual_seed(6)
+    g = torch.rand(700, generator=gen) + 1
+    g[:256] *= size
+    g[256:] *= 1e-3
+    g[600] = size
+    g = g.to(gdtype).cuda()
+    m, r = (torch.zeros(700, device="cuda", dtype=E4M3) for _ in range(2))
+    ms, rs = (torch.zeros(3, device="cuda") for _ in range(2))
+    p, p32 = torch.zeros(700, device="cuda", dtype=pdtype), torch.zeros(700, device="cuda")
+    optim.adamw_step([p], [g], [m], [r], step=1, lr=1.0, betas=(0.9, 0.95), eps=0.0, weight_decay=0.0, exp_avg_scales=[ms],
+                     exp_avg_sq_scales=[rs], masters=[p32] if master else None)
+    for value in (p, p32) if master else (p,):
+        _within_ulp(value, torch.full((700,), -1.0, device="cuda", dtype=torch.float64), value.dtype, 1e-5)
+    for codes, scale, c in ((m, ms, 0.1), (r, rs, math.sqrt(0.05))):
+        want = c * g.double()
+        top = torch.stack([b.max() for b in want.split(256)])
+        assert ((scale.double() * 448 - top).abs() <= 1e-6 * top).all()
+        each = scale.double().repeat_interleave(256)[:700]
+        assert ((_decode(codes, scale) - want).abs() <= (want / 8).maximum(each * 2.0 ** -9) * 1.0001).all()
+    assert (r.float() > 0).all()
+
+
+@gpu
 def test_8bit_infinite_value_makes_its_block_non_finite(optim):
     g = torch.ones(600, device="cuda")
     g[10] = float("inf")

@@ -218,6 +218,48 @@ def test_8bit_step_of_large_finite_gradients(optim, size, pdtype, gdtype, master
 
 
 @gpu
+@pytest.mark.parametrize("pdtype,gdtype,master", [(F32, F32, False), (BF16, BF16, False), (BF16, F32, True)])
+@pytest.mark.parametrize("size", [1e-18, 1e-20, 1e-21, 1e-22, 1e-24, 1e-27])
+def test_8bit_step_of_tiny_gradients(optim, size, pdtype, gdtype, master):
+    # as above: steps of lr whatever the gradient's size, next to zeros (whose step is 0 / 0 with eps = 0: left out) and
+    # next to ordinary values
+    gen = torch.Generator().manual_seed(7)
+    g = (torch.rand(700, generator=gen) + 1) * size
+    g[256:400] = 1e-3
+    g[3] = g[650] = 0
+    g = g.to(gdtype).cuda()
+    m, r = (torch.zeros(700, device="cuda", dtype=E4M3) for _ in range(2))
+    ms, rs = (torch.zeros(3, device="cuda") for _ in range(2))
+    p, p32 = torch.zeros(700, device="cuda", dtype=pdtype), torch.zeros(700, device="cuda")
+    optim.adamw_step([p], [g], [m], [r], step=1, lr=1.0, betas=(0.9, 0.95), eps=0.0, weight_decay=0.0, exp_avg_scales=[ms],
+                     exp_avg_sq_scales=[rs], masters=[p32] if master else None)
+    there = g != 0
+    for value in (p, p32) if master else (p,):
+        _within_ulp(value[there], torch.full((698,), -1.0, device="cuda", dtype=torch.float64), value.dtype, 1e-5)
+    for codes, scale, c in ((m, ms, 0.1), (r, rs, math.sqrt(0.05))):
+        want = c * g.double()
+        top = torch.stack([b.max() for b in want.split(256)])
+        assert ((scale.double() * 448 - top).abs() <= 1e-6 * top).all()
+        each = scale.double().repeat_interleave(256)[:700]
+        assert ((_decode(codes, scale) - want).abs() <= (want / 8).maximum(each * 2.0 ** -9) * 1.0001).all()
+    assert torch.equal(r.float() > 0, there)
+
+
+@gpu
+def test_8bit_roots_without_gradients_fade_evenly(optim):
+    # no gradient and no first moment: the root shrinks by sqrt(b2) a step at every size down to the least scale
+    sizes = torch.tensor([1e-15, 1e-18, 1e-21, 1e-24, 1e-27], dtype=torch.float64)
+    n = 256 * len(sizes)
+    m, r = torch.zeros(n, device="cuda", dtype=E4M3), torch.full((n,), 448.0, device="cuda").to(E4M3)
+    ms, rs = torch.zeros(len(sizes), device="cuda"), (sizes / 448).float().cuda()
+    start, g = rs.double(), torch.zeros(n, device="cuda")
+    p = torch.ones(n, device="cuda")
+    optim.adamw_step([p], [g], [m], [r], step=9, **HYPER, exp_avg_scales=[ms], exp_avg_sq_scales=[rs])
+    assert ((rs.double() / start - math.sqrt(0.95)).abs() <= 1e-6).all()
+    assert ((p.double() - (1 - HYPER["lr"] * HYPER["weight_decay"])).abs() <= 1e-6).all()
+
+
+@gpu
 def test_8bit_infinite_value_makes_its_block_non_finite(optim):
     g = torch.ones(600, device="cuda")
     g[10] = float("inf")

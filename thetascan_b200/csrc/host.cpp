@@ -10,10 +10,12 @@
 // device of its tensors and returns without waiting.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/object_ptr.h>
 
@@ -45,7 +47,14 @@ ts_stream_t current_stream(const Tensor& t) {
   return c10::cuda::getCurrentCUDAStream(t.get_device()).stream();
 }
 
+// Forward-mode derivatives are not formed here: the result would have none, which reads as zero.
+void refuse_tangent(const char* name, const Tensor& t) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined() || !c10::AutogradState::get_tls_state().get_fw_grad_mode(),
+                              name, " carries a forward-mode derivative, which is not supported");
+}
+
 void require_cuda(const char* name, const Tensor& t, const Tensor& first) {
+  refuse_tangent(name, t);
   TORCH_CHECK(t.is_cuda(), "b200 backend requires CUDA tensors (", name, " is on ", t.device(), ")");
   TORCH_CHECK_VALUE(t.device() == first.device(), name, " is on ", t.device(), ", x on ", first.device());
 }
@@ -69,7 +78,7 @@ Tensor rows_of(const Tensor& t) {
 // ------------------------------------------------------------------ norm
 
 void norm_check(const Tensor& x, const OptTensor& residual, const Tensor& weight, double eps) {
-  TORCH_CHECK(x.is_cuda(), "b200 backend requires CUDA tensors (x is on ", x.device(), ")");
+  require_cuda("x", x, x);
   require_cuda("weight", weight, x);
   dtype_code("x", x);
   dtype_code("weight", weight);
@@ -426,6 +435,10 @@ struct AdamW {
       dtype_code("gradients", grads[i]);
       TORCH_CHECK_VALUE(grads[i].numel() == params[i].numel() && grads[i].device() == params[0].device(),
                         "adamw: gradient ", i, " does not match its parameter");
+    }
+    if (torch::autograd::ForwardADLevel::try_get_by_idx(0)) {
+      for (const auto& list : {std::make_pair("a parameter", &params), std::make_pair("a gradient", &grads)})
+        for (const Tensor& t : *list.second) refuse_tangent(list.first, t);
     }
     const c10::cuda::CUDAGuard guard(params[0].device());
     TORCH_CHECK(at::cuda::currentStreamCaptureStatusMayInitCtx() == at::cuda::CaptureStatus::None,

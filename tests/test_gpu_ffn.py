@@ -240,6 +240,30 @@ def test_compiles_into_one_graph(ffn):
 
 
 @gpu
+@pytest.mark.parametrize("rows", [1, 32, 300])
+def test_compiled_inference_runs_what_eager_inference_runs(ffn, rows):
+    # bit for bit, also where only the mode or only the inputs say that no gradient is wanted; the op keeps nothing
+    torch._dynamo.reset()   # the modes and sizes below are each a compilation of the same function
+    x, wg, wu, wd, _ = _make(rows, 128, 512, 128)
+    f = lambda *t: ffn.gated_ffn(*t, "gelu")  # noqa: E731
+    want = f(x, wg, wu, wd)
+    compiled = torch.compile(f, fullgraph=True, backend="aot_eager")
+    assert torch.equal(compiled(x, wg, wu, wd), want)
+    with torch.no_grad():
+        assert torch.equal(compiled(x, wg.clone().requires_grad_(True), wu, wd), want)
+    with torch.inference_mode():
+        assert torch.equal(compiled(x, wg, wu, wd), want)
+    y = compiled(x, wg.clone().requires_grad_(True), wu, wd)
+    assert y.requires_grad and torch.equal(y.detach(), f(x, wg.clone().requires_grad_(True), wu, wd).detach())
+    base = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    with torch.no_grad():
+        y = compiled(x, wg, wu, wd)
+    assert torch.cuda.max_memory_allocated() - base < rows * (512 * 4 + 128 * 2) + 8192   # h and y, not g and u
+    assert torch.equal(y, want)
+
+
+@gpu
 def test_refusals(ffn):
     x, wg, wu, wd, _ = _make(4, 64, 128, 64)
     for bad in ((x.float(), wg, wu, wd), (x, wg.half(), wu, wd), (x, wg[:64], wu, wd), (x, wg, wu, wd[:, :64]), (x[:, :32], wg, wu, wd),

@@ -84,7 +84,9 @@ def gated_ffn(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, activatio
     ``w_down`` is ``[width_out, hidden]``, all bf16.  ``activation`` is
     ``"silu"``, ``"gelu"`` (exact) or ``"relu2"`` (``max(g, 0)^2``)."""
     if torch.compiler.is_compiling():
-        return _TracedFFN.apply(x, w_gate, w_up, w_down, activation)
+        if torch.is_grad_enabled() and any(t.requires_grad for t in (x, w_gate, w_up, w_down)):
+            return _TracedFFN.apply(x, w_gate, w_up, w_down, activation)
+        return gated_ffn_fwd(x, w_gate, w_up, w_down, activation, False)[0]
     return _lib.host().gated_ffn(x, w_gate, w_up, w_down, activation)
 
 

@@ -227,6 +227,35 @@ def test_compiles_into_one_graph(norm):
 
 
 @gpu
+@pytest.mark.parametrize("residual", [False, True])
+def test_compiled_inference_runs_what_eager_inference_runs(norm, residual, monkeypatch):
+    # bit for bit, and with nothing kept for a backward pass unless one is wanted
+    torch._dynamo.reset()
+    x, r, w = _make((40, 256), BF16, F32, residual=residual)
+    f = norm.add_rms_norm if residual else norm.rms_norm
+    args = (x, r, w) if residual else (x, w)
+    outputs = lambda y: y if residual else (y,)  # noqa: E731
+    kept, host = [], norm._lib.host()
+
+    class Host:
+        def __getattr__(self, name):
+            if name != "norm_fwd":
+                return getattr(host, name)
+            return lambda *a: kept.append(a[-1]) or host.norm_fwd(*a)
+
+    want = outputs(f(*args))
+    compiled = torch.compile(lambda *t: f(*t), fullgraph=True, backend="aot_eager")
+    monkeypatch.setattr(norm._lib, "host", lambda: Host())
+    assert all(torch.equal(a, b) for a, b in zip(outputs(compiled(*args)), want))
+    with torch.no_grad():
+        got = outputs(compiled(*args[:-1], w.clone().requires_grad_(True)))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert kept == [False, False]
+    got = outputs(compiled(*args[:-1], w.clone().requires_grad_(True)))
+    assert got[0].requires_grad and torch.equal(got[0].detach(), want[0]) and kept[2:] == [True]
+
+
+@gpu
 def test_refusals(norm):
     x, w = torch.zeros(2, 64, device="cuda"), torch.ones(64, device="cuda")
     for bad in (dict(x=x.half()), dict(w=w.half()), dict(w=w[:32]), dict(eps=-1.0), dict(w=w[None])):

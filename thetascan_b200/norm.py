@@ -74,7 +74,10 @@ class _TracedNorm(torch.autograd.Function):
 
 def _norm(x, residual, weight, eps):
     if torch.compiler.is_compiling():
-        return _TracedNorm.apply(x, residual, weight, float(eps))
+        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, weight)):
+            return _TracedNorm.apply(x, residual, weight, float(eps))
+        y, total, _ = norm_fwd(x, residual, weight, float(eps), False)
+        return y if residual is None else (y, total)
     return _lib.host().rms_norm(x, residual, weight, eps)
 
 

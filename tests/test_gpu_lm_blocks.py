@@ -92,6 +92,22 @@ def test_trains_with_a_mixer_and_quantizes_its_head(bits):
     assert model(tokens[:, :-1]).requires_grad   # with gradients: the exact head
 
 
+@gpu
+def test_quantized_model_compiles_into_one_graph():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a CUDA device")
+    torch._dynamo.reset()
+    model, _ = _pair("silu")
+    model.quantize_head()
+    tokens = torch.randint(0, 256, (3, 20), generator=torch.Generator().manual_seed(7)).cuda()
+    with torch.no_grad(), torch.autocast("cuda", dtype=torch.bfloat16):
+        want = model(tokens)
+        got = torch.compile(model, fullgraph=True, backend="aot_eager")(tokens)
+    # the same kernels; a stream that rounds elsewhere may move a code by a step, 2^-4 of one of 128 terms
+    assert got.dtype == want.dtype and got.shape == want.shape
+    assert float((got.float() - want.float()).norm()) <= 0.02 * float(want.float().norm())
+
+
 def test_default_model_is_unchanged_on_the_cpu():
     # the options off: the modules, their order and their initial values are what they were
     from thetascan_b200.lm import HybridLM

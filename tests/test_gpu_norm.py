@@ -256,6 +256,26 @@ def test_compiled_inference_runs_what_eager_inference_runs(norm, residual, monke
 
 
 @gpu
+@pytest.mark.parametrize("group", [None, 128])
+@pytest.mark.parametrize("residual", [False, True])
+def test_8bit_compiles_into_one_graph(norm, residual, group):
+    torch._dynamo.reset()
+    x, r, w = _make((3, 20, 200), BF16, F32, residual=residual)
+    f = lambda x, w: norm.rms_norm_8bit(x, w, residual=r, group=group)  # noqa: E731
+    want = f(x, w)
+    compiled = torch.compile(f, fullgraph=True, backend="aot_eager")
+    got = compiled(x, w)
+    assert len(got) == len(want) == (3 if residual else 2)
+    for a, b in zip(got, want):
+        assert a.dtype == b.dtype and a.shape == b.shape and torch.equal(a.float(), b.float())
+    w.requires_grad_(True)
+    with torch.no_grad():
+        assert torch.equal(compiled(x, w)[1], want[1])
+    with pytest.raises(Exception, match="no gradient"):
+        compiled(x, w)
+
+
+@gpu
 def test_refusals(norm):
     x, w = torch.zeros(2, 64, device="cuda"), torch.ones(64, device="cuda")
     for bad in (dict(x=x.half()), dict(w=w.half()), dict(w=w[:32]), dict(eps=-1.0), dict(w=w[None])):

@@ -52,6 +52,21 @@ def _(dy, dsum, total, weight, rstd, eps):
     return total.new_empty(total.shape), weight.new_empty(weight.shape)
 
 
+@torch.library.custom_op(f"{LIB}::norm_8bit", mutates_args=())
+def norm_8bit(x: Tensor, residual: Optional[Tensor], weight: Tensor, eps: float,
+              group: Optional[int]) -> tuple[Tensor, Tensor, Tensor]:
+    """The norm's codes and scales, and the stored sum (empty without a residual)."""
+    codes, scales, *total = _lib.host().rms_norm_8bit(x, residual, weight, eps, group)
+    return codes, scales, *(total or [x.new_empty(0)])
+
+
+@norm_8bit.register_fake
+def _(x, residual, weight, eps, group):
+    n = 1 if group is None else -(-x.shape[-1] // group)
+    return (x.new_empty(x.shape, dtype=torch.float8_e4m3fn), x.new_empty((*x.shape[:-1], n), dtype=torch.float32),
+            x.new_empty(x.shape if residual is not None else (0,)))
+
+
 class _TracedNorm(torch.autograd.Function):
     """The autograd node as a tracing compiler sees it; eager calls have theirs in ``csrc/host.cpp``."""
 
@@ -72,9 +87,13 @@ class _TracedNorm(torch.autograd.Function):
         return dx, dx if ctx.added else None, dweight, None
 
 
+def _wants_grad(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
 def _norm(x, residual, weight, eps):
     if torch.compiler.is_compiling():
-        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, weight)):
+        if _wants_grad(x, residual, weight):
             return _TracedNorm.apply(x, residual, weight, float(eps))
         y, total, _ = norm_fwd(x, residual, weight, float(eps), False)
         return y if residual is None else (y, total)
@@ -99,4 +118,9 @@ def rms_norm_8bit(x: Tensor, weight: Tensor, eps: float = 1e-6, *, residual: Opt
     magnitude that it covers to 448, the type's largest value; the norm is
     rounded once, from f32 to the code.  Returns ``(codes, scales)``, and the
     stored sum too where there is a residual.  For inference: no gradient."""
+    if torch.compiler.is_compiling():
+        if _wants_grad(x, residual, weight):
+            raise RuntimeError("rms_norm_8bit has no gradient: call it under torch.no_grad()")
+        codes, scales, total = norm_8bit(x, residual, weight, float(eps), group)
+        return (codes, scales) if residual is None else (codes, scales, total)
     return _lib.host().rms_norm_8bit(x, residual, weight, eps, group)

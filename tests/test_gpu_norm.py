@@ -154,6 +154,33 @@ def test_rows_of_zeros_and_non_finite_rows(norm):
 
 
 @gpu
+@pytest.mark.parametrize("group", [None, 128])
+@pytest.mark.parametrize("width", [200, 203, 1000, 8200])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_8bit_of_non_finite_rows(norm, dtype, width, group):
+    # a scale is the largest magnitude's: NaN where one of its values is (an infinity's row is 0 * inf there), and so are
+    # its codes; the other groups and rows are what they are without it
+    x, _, w = _make((6, width), dtype, F32, seed=width)
+    clean = norm.rms_norm_8bit(x, w, EPS, group=group)
+    bad = x.clone()
+    bad[1, 5], bad[2, width - 1], bad[3, 130] = float("nan"), float("inf"), float("-inf")
+    codes, scales = norm.rms_norm_8bit(bad, w, EPS, group=group)
+    y = norm.rms_norm(bad.float(), w, EPS)
+    nan = torch.stack([p.isnan().any(-1) for p in y.split(group or width, -1)], -1)
+    assert nan[1].all() and nan[2, -1] and nan[3].any() and not nan[[0, 4, 5]].any()
+    assert torch.equal(scales.isnan(), nan)
+    assert torch.equal(codes.float().isnan(), nan.repeat_interleave(group or width, -1)[:, :width])
+    for row in (0, 4, 5):
+        assert torch.equal(scales[row], clean[1][row]) and torch.equal(codes[row].float(), clean[0][row].float())
+    spoilt = w.clone()
+    spoilt[150] = float("nan")
+    codes, scales = norm.rms_norm_8bit(x, spoilt, EPS, group=group)
+    hit = torch.arange(scales.shape[1], device="cuda") == (150 // group if group else 0)
+    assert torch.equal(scales.isnan(), hit.expand(6, -1))
+    assert torch.equal(scales[:, ~hit], clean[1][:, ~hit])
+
+
+@gpu
 def test_leading_dimensions_strides_and_alignment(norm):
     g = torch.Generator().manual_seed(1)
     big = torch.randn(3, 5, 2, 72, generator=g).to(BF16).cuda()

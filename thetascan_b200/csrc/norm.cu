@@ -100,6 +100,13 @@ __device__ __forceinline__ void load_weight(const void* w, bool bf16, int c, flo
   }
 }
 
+// The larger of two; NaN where one is (a scale has to show it).
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // Sum (or, kMax, maximum) over the kTpr threads of this thread's row.  `red`
 // holds two buffers of one float per warp; `turn` picks one, so that a
 // reduction needs a single barrier.
@@ -108,7 +115,7 @@ __device__ __forceinline__ float row_reduce(float v, float* red, int& turn) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const float other = __shfl_xor_sync(0xffffffffu, v, o);
-    v = kMax ? fmaxf(v, other) : v + other;
+    v = kMax ? max_nan(v, other) : v + other;
   }
   if (kTpr > 32) {
     float* buf = red + turn * 32;
@@ -120,7 +127,7 @@ __device__ __forceinline__ float row_reduce(float v, float* red, int& turn) {
     const int first = warp / kWarps * kWarps;
     v = buf[first];
 #pragma unroll
-    for (int i = 1; i < kWarps; ++i) v = kMax ? fmaxf(v, buf[first + i]) : v + buf[first + i];
+    for (int i = 1; i < kWarps; ++i) v = kMax ? max_nan(v, buf[first + i]) : v + buf[first + i];
   }
   return v;
 }
@@ -211,7 +218,7 @@ __global__ void __launch_bounds__(norm_threads<kTpr>(), (norm_fwd_resident<kTpr>
     // 8-bit codes.  A pack's columns lie in one group; with packs of 16 bytes a
     // group is 16 (bf16) or 32 (f32) neighbouring lanes, with single values it
     // is 128 / kTpr passes of this row's threads, whose maxima meet in shared
-    // memory (as the bits of non-negative floats, which order like integers).
+    // memory (as the bits of non-negative floats, which order like integers, NaN above all).
     constexpr int kLanes = kNormGroup / kVec < 32 ? kNormGroup / kVec : 32;
     const int n_groups = p.group ? (p.width + kNormGroup - 1) / kNormGroup : 1;
     int* gmax = group_max + slot * (kNormMaxWidth / kNormGroup);
@@ -230,13 +237,13 @@ __global__ void __launch_bounds__(norm_threads<kTpr>(), (norm_fwd_resident<kTpr>
         load_weight<kVec>(p.w, p.w_bf16, c, w);
 #pragma unroll
         for (int e = 0; e < kVec; ++e) {
-          top[k] = fmaxf(top[k], fabsf(to_f(s[k].v[e]) * rstd * w[e]));
+          top[k] = max_nan(top[k], fabsf(to_f(s[k].v[e]) * rstd * w[e]));
         }
       }
-      row_top = fmaxf(row_top, top[k]);
+      row_top = max_nan(row_top, top[k]);
       if (p.group) {
 #pragma unroll
-        for (int o = kLanes / 2; o > 0; o >>= 1) top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], o));
+        for (int o = kLanes / 2; o > 0; o >>= 1) top[k] = max_nan(top[k], __shfl_xor_sync(0xffffffffu, top[k], o));
         if (kVec == 1 && (t & 31) == 0 && c < p.width) atomicMax(&gmax[c / kNormGroup], __float_as_int(top[k]));
       }
     }
@@ -253,7 +260,7 @@ __global__ void __launch_bounds__(norm_threads<kTpr>(), (norm_fwd_resident<kTpr>
       float largest = p.group ? (kVec == 1 ? __int_as_float(gmax[g]) : top[k]) : row_top;
       // the scale, its reciprocal in two parts, and y / scale to half a unit in the last place, so that ties fall as
       // they should
-      const float scale = fmaxf(largest, kScaleFloor) * (1.f / kE4m3Max);
+      const float scale = max_nan(largest, kScaleFloor) * (1.f / kE4m3Max);
       if (c == g * kNormGroup) p.scales[row * n_groups + g] = scale;
       const float r = __fdividef(1.f, scale), inv = fmaf(fmaf(-scale, r, 1.f), r, r);
       const float rest = fmaf(-scale, inv, 1.f) * inv;

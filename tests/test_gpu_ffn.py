@@ -165,6 +165,36 @@ def test_rows_are_independent(ffn):
 
 
 @gpu
+@pytest.mark.parametrize("kind", ["silu", "gelu", "relu2"])
+@pytest.mark.parametrize("rows", [4, 70])
+def test_non_finite_weights_show(ffn, rows, kind):
+    # one hidden value is NaN, plus or minus infinity by its gate alone: outputs and gradients are finite, infinite or
+    # NaN where the formula's are
+    x, wg, wu, wd, dy = _make(rows, 64, 128, 64, seed=1)
+    x = x.abs() + 0.5
+    x[rows // 2] = 0.25
+    for value in (float("nan"), float("inf"), -float("inf")):
+        gate = wg.clone()
+        gate[77] = value
+        leaves = [t.clone().requires_grad_(True) for t in (x, gate, wu, wd)]
+        wide = [t.detach().double().requires_grad_(True) for t in leaves]
+        g = wide[0] @ wide[1].T
+        want = (_act(g, kind)[0] * (wide[0] @ wide[2].T)) @ wide[3].T
+        y = ffn.gated_ffn(*leaves, kind)
+        with torch.no_grad():
+            results = [(y, want), (ffn.gated_ffn(*leaves, kind), want)]
+        # the gradients' formula, as NaN-free subexpressions differ between ways to write a derivative
+        dh = dy.double() @ wide[3]
+        slope = _act(g, kind)[1]
+        dg, du = dh * (wide[0] @ wide[2].T) * slope, dh * _act(g, kind)[0]
+        grads = torch.autograd.grad(y, leaves, dy)
+        results += [(grads[1], dg.T @ wide[0]), (grads[2], du.T @ wide[0]), (grads[0], dg @ wide[1] + du @ wide[2])]
+        for got, ref in results:
+            assert torch.equal(got.isnan(), ref.isnan()), (value, kind)
+            assert torch.equal(got.isinf(), ref.isinf()), (value, kind)
+
+
+@gpu
 @pytest.mark.parametrize("rows", [3, 70])
 def test_strides_leading_dimensions_and_alignment(ffn, rows):
     g = torch.Generator().manual_seed(3)

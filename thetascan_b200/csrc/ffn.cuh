@@ -45,7 +45,8 @@ __device__ __forceinline__ float ffn_act(float g, float& slope) {
     slope = fmaf(g * 0.39894228040143268f, __expf(-zz), s);
     return g * s;
   }
-  const float s = fmaxf(g, 0.f);
+  float s;   // max(g, 0), and NaN for a NaN
+  asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(s) : "f"(g));
   slope = 2.f * s;
   return s * s;
 }

@@ -370,6 +370,39 @@ def test_refusals(optim):
         optim.adamw_step([torch.ones(3)], [torch.ones(3)], [torch.ones(3)], [torch.ones(3)], **ok)
 
 
+def test_a_refused_step_does_not_count():
+    # on the CPU every step is refused; the bias corrections of the next one must not move
+    from thetascan_b200 import AdamW
+    p = torch.ones(8, requires_grad=True)
+    opt = AdamW([p])
+    p.grad = torch.ones(8)
+    for _ in range(2):
+        with pytest.raises(RuntimeError):
+            opt.step()
+    assert opt.state[p]["step"] == 0
+    p.grad = torch.sparse_coo_tensor([[1]], [1.0], (8,))
+    with pytest.raises(RuntimeError, match="sparse"):
+        opt.step()
+    assert opt.state[p]["step"] == 0 and (p == 1).all()
+
+
+@gpu
+def test_steps_after_a_refused_one(optim):
+    a, b = (torch.ones(300, device="cuda", requires_grad=True) for _ in range(2))
+    x, y = optim.AdamW([a]), optim.AdamW([b])
+    for i in range(3):
+        a.grad = torch.full((300,), 0.5 + i, device="cuda")
+        b.grad = a.grad.clone()
+        if i == 1:
+            x.param_groups[0]["betas"] = (2.0, 0.9)
+            with pytest.raises(ValueError):
+                x.step()
+            x.param_groups[0]["betas"] = (0.9, 0.999)
+        x.step()
+        y.step()
+    assert torch.equal(a, b) and x.state[a]["step"] == 3
+
+
 def test_c_entry_refuses_bad_arguments():
     import ctypes
     from thetascan_b200 import _lib

@@ -108,9 +108,9 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        ordinal = 0
+        calls, ordinal = [], 0
         for group in self.param_groups:
-            calls = {}
+            together = {}
             for p in group["params"]:
                 ordinal += 1
                 if p.grad is None:
@@ -120,19 +120,19 @@ class AdamW(torch.optim.Optimizer):
                 state = self.state[p]
                 if not state:
                     state.update(self._new_state(p, group))
-                state["step"] += 1
                 # tensors of one step count and device go together, those with a master apart
                 master = "master" in state
-                key = (state["step"], p.device, master, (p.dtype, p.grad.dtype) if master else None)
-                calls.setdefault(key, []).append((ordinal - 1, p, state))
-            for (count, _, master, _), entries in calls.items():
-                ordinals, params, states = zip(*entries)
-                eight = group["state_bits"] == 8
-                adamw_step(params, [p.grad for p in params], [s["exp_avg"] for s in states],
-                           [s["exp_avg_sq"] for s in states], step=count, lr=float(group["lr"]), betas=group["betas"],
-                           eps=group["eps"], weight_decay=group["weight_decay"],
-                           masters=[s["master"] for s in states] if master else None,
-                           exp_avg_scales=[s["exp_avg_scale"] for s in states] if eight else None,
-                           exp_avg_sq_scales=[s["exp_avg_sq_scale"] for s in states] if eight else None,
-                           seed=group["seed"], ordinals=ordinals)
+                key = (state["step"] + 1, p.device, master, (p.dtype, p.grad.dtype) if master else None)
+                together.setdefault(key, []).append((ordinal - 1, p, state))
+            calls += [(group, count, master, *zip(*entries)) for (count, _, master, _), entries in together.items()]
+        for group, count, master, ordinals, params, states in calls:
+            eight = group["state_bits"] == 8
+            adamw_step(params, [p.grad for p in params], [s["exp_avg"] for s in states], [s["exp_avg_sq"] for s in states],
+                       step=count, lr=float(group["lr"]), betas=group["betas"], eps=group["eps"],
+                       weight_decay=group["weight_decay"], masters=[s["master"] for s in states] if master else None,
+                       exp_avg_scales=[s["exp_avg_scale"] for s in states] if eight else None,
+                       exp_avg_sq_scales=[s["exp_avg_sq_scale"] for s in states] if eight else None,
+                       seed=group["seed"], ordinals=ordinals)
+            for state in states:   # a refused step does not count
+                state["step"] = count
         return loss

@@ -403,6 +403,22 @@ def test_steps_after_a_refused_one(optim):
     assert torch.equal(a, b) and x.state[a]["step"] == 3
 
 
+def test_options_of_a_group_are_checked_as_the_defaults_are():
+    from thetascan_b200 import AdamW
+    p, q = torch.ones(8, requires_grad=True), torch.ones(8, requires_grad=True)
+    opt = AdamW([p])
+    for bad in (dict(state_bits=16), dict(lr=-1.0), dict(betas=(0.9, 1.0)), dict(eps=-1e-8), dict(weight_decay=-0.1)):
+        with pytest.raises(ValueError):
+            AdamW([dict(params=[q], **bad)])
+        with pytest.raises(ValueError):
+            AdamW([q], **bad)
+        with pytest.raises(ValueError):
+            opt.add_param_group(dict(params=[q], **bad))
+        assert len(opt.param_groups) == 1
+    opt.add_param_group(dict(params=[q], state_bits=8, lr=0.5))
+    assert opt.param_groups[1]["state_bits"] == 8
+
+
 def test_c_entry_refuses_bad_arguments():
     import ctypes
     from thetascan_b200 import _lib

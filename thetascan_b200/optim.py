@@ -35,6 +35,11 @@ def _require(ok, message):
         raise ValueError(f"adamw: {message}")
 
 
+def _require_options(lr, betas, eps, weight_decay):
+    _require(all(0 <= b < 1 for b in betas), f"betas must lie in [0, 1), got {betas}")
+    _require(lr >= 0 and eps >= 0 and weight_decay >= 0, "lr, eps and weight_decay must be >= 0")
+
+
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step: int, lr: float, betas=(0.9, 0.999), eps: float = 1e-8,
                weight_decay: float = 1e-2, masters=None, exp_avg_scales=None, exp_avg_sq_scales=None,
                seed: int = 0, ordinals=None) -> None:
@@ -48,9 +53,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step: int, lr: float, be
     the tensors' places in the whole step (default 0, 1, ...), which key the
     stochastic rounding of 8-bit states with ``seed``."""
     _require(isinstance(step, int) and step >= 1, f"step must be an integer >= 1, got {step!r}")
+    _require_options(lr, betas, eps, weight_decay)
     b1, b2 = betas
-    _require(0 <= b1 < 1 and 0 <= b2 < 1, f"betas must lie in [0, 1), got {betas}")
-    _require(lr >= 0 and eps >= 0 and weight_decay >= 0, "lr, eps and weight_decay must be >= 0")
     _lib.host().adamw(params, grads, exp_avgs, exp_avg_sqs, masters, exp_avg_scales, exp_avg_sq_scales, ordinals, step, lr,
                       b1, b2, eps, weight_decay, seed)
 
@@ -65,18 +69,21 @@ class AdamW(torch.optim.Optimizer):
 
     def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, *,
                  state_bits: int = 32, master_weights: bool = False, seed: int = 0):
-        if state_bits not in (8, 32):
-            raise ValueError(f"adamw: state_bits must be 8 or 32, got {state_bits}")
-        _require(lr >= 0 and eps >= 0 and weight_decay >= 0, "lr, eps and weight_decay must be >= 0")
-        _require(0 <= betas[0] < 1 and 0 <= betas[1] < 1, f"betas must lie in [0, 1), got {betas}")
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay,
                                       state_bits=state_bits, master_weights=master_weights, seed=seed))
 
     def add_param_group(self, param_group):
         super().add_param_group(param_group)
-        for p in self.param_groups[-1]["params"]:
-            _require(p.dtype in _DTYPES, f"parameters must be float32 or bfloat16, got {p.dtype}")
-            _require(p.is_contiguous(), "parameters must be contiguous")
+        group = self.param_groups[-1]
+        try:
+            _require(group["state_bits"] in (8, 32), f"state_bits must be 8 or 32, got {group['state_bits']}")
+            _require_options(group["lr"], group["betas"], group["eps"], group["weight_decay"])
+            for p in group["params"]:
+                _require(p.dtype in _DTYPES, f"parameters must be float32 or bfloat16, got {p.dtype}")
+                _require(p.is_contiguous(), "parameters must be contiguous")
+        except ValueError:
+            self.param_groups.pop()
+            raise
 
     def _new_state(self, p, group):
         state = {"step": 0}

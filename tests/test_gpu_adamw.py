@@ -419,6 +419,22 @@ def test_options_of_a_group_are_checked_as_the_defaults_are():
     assert opt.param_groups[1]["state_bits"] == 8
 
 
+@gpu
+def test_lists_are_of_the_parameters_shapes_or_flat(optim):
+    make = lambda *shape: torch.rand(shape, generator=torch.Generator().manual_seed(1)).cuda()  # noqa: E731
+    args = [make(4, 6) for _ in range(5)]
+    args[0] = args[0].bfloat16()
+    for i in range(1, 5):
+        for shape in ((6, 4), (4, 3, 2)):
+            bad = [t.reshape(shape) if j == i else t for j, t in enumerate(args)]
+            with pytest.raises(ValueError):
+                optim.adamw_step(*([t] for t in bad[:4]), step=1, **HYPER, masters=[bad[4]])
+    flat = [t.clone().reshape(-1) if i else t.clone() for i, t in enumerate(args)]
+    for lists in (args, flat):
+        optim.adamw_step(*([t] for t in lists[:4]), step=1, **HYPER, masters=[lists[4]])
+    assert all(torch.equal(a, b.view(4, 6)) for a, b in zip(args, flat))
+
+
 def test_c_entry_refuses_bad_arguments():
     import ctypes
     from thetascan_b200 import _lib

@@ -377,7 +377,13 @@ std::vector<Tensor> tensors_of(PyObject* object, const char* what) {
   return out;
 }
 
-// Contiguous tensors of one dtype on the parameters' device, with the sizes of `like` (their block counts: `blocks`).
+// Whether the elements of t are those of `like` in their order: of its shape, or one of the two flat.
+bool in_order(const Tensor& t, const Tensor& like) {
+  return t.sizes() == like.sizes() || ((t.dim() == 1 || like.dim() == 1) && t.numel() == like.numel());
+}
+
+// Contiguous tensors of one dtype on the parameters' device, with the shapes of `like` or flat (`blocks`: a scale for
+// each block).
 void same(const std::vector<Tensor>& list, const std::vector<Tensor>& like, at::ScalarType type, bool blocks,
           const char* what) {
   TORCH_CHECK_VALUE(list.size() == like.size(), "adamw: ", like.size(), " parameters but ", list.size(), " ", what);
@@ -386,6 +392,8 @@ void same(const std::vector<Tensor>& list, const std::vector<Tensor>& like, at::
     const int64_t n = blocks ? (like[i].numel() + kStateBlock - 1) / kStateBlock : like[i].numel();
     TORCH_CHECK_VALUE(t.scalar_type() == type, "adamw: ", what, " must be ", type, ", got ", t.scalar_type());
     TORCH_CHECK_VALUE(t.numel() == n, "adamw: ", what, " ", i, " has ", t.numel(), " elements, not ", n);
+    TORCH_CHECK_VALUE(blocks || in_order(t, like[i]), "adamw: ", what, " ", i, " is ", t.sizes(), ", its parameter ",
+                      like[i].sizes());
     TORCH_CHECK_VALUE(t.device() == like[0].device(), "adamw: ", what, " must be on the parameters' device");
     TORCH_CHECK_VALUE(t.is_contiguous(), "adamw: ", what, " must be contiguous");
   }
@@ -433,7 +441,7 @@ struct AdamW {
     for (size_t i = 0; i < n; ++i) {
       TORCH_CHECK_VALUE(!grads[i].is_sparse(), "adamw: sparse gradients are not supported");
       dtype_code("gradients", grads[i]);
-      TORCH_CHECK_VALUE(grads[i].numel() == params[i].numel() && grads[i].device() == params[0].device(),
+      TORCH_CHECK_VALUE(in_order(grads[i], params[i]) && grads[i].device() == params[0].device(),
                         "adamw: gradient ", i, " does not match its parameter");
     }
     if (torch::autograd::ForwardADLevel::try_get_by_idx(0)) {

@@ -46,8 +46,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step: int, lr: float, be
     """One AdamW step, in place, on lists of CUDA tensors of one device.
 
     ``params`` are f32 or bf16 and contiguous, ``grads`` f32 or bf16 of the
-    same shapes.  ``masters`` (f32) belong to bf16 parameters and carry their
-    values.  States are f32 tensors, or ``float8_e4m3fn`` codes (of the first
+    same shapes (or flat, as the other lists).  ``masters`` (f32) belong to
+    bf16 parameters and carry their values.  States are f32 tensors, or ``float8_e4m3fn`` codes (of the first
     moment, and of the root of the second) with f32 scales of
     ``state_scales(numel)`` entries.  ``step`` counts from 1; ``ordinals`` are
     the tensors' places in the whole step (default 0, 1, ...), which key the

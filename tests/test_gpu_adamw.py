@@ -154,6 +154,59 @@ def test_many_tensors_mixed_kinds_and_alignment(optim):
         assert ((v.double() - wv).abs() <= 2.0 ** -21 * wv).all()
 
 
+def _mix32(x):
+    x = ((x ^ (x >> 16)) * 0x7FEB352D) & 0xFFFFFFFF
+    x = ((x ^ (x >> 15)) * 0x846CA68B) & 0xFFFFFFFF
+    return x ^ (x >> 16)
+
+
+@gpu
+def test_8bit_states_are_the_formulas_to_the_bit(optim):
+    # each sum, product, root and quotient rounded to f32 by itself (the CPU's are), the code's random rounding in float64
+    # (exact).  The kernel's root is the next value in one case of a million: of 4000 blocks' scales at most one may be
+    # off, and in the other blocks a code where its value is within 2^-20 of a step's end, at most ten in a million.
+    n, seed = 4000 * 256, 17
+    b1, b2 = HYPER["betas"]
+    f = lambda v: torch.tensor(v, dtype=F32)  # noqa: E731
+    gen = torch.Generator().manual_seed(12)
+    m, r = (torch.zeros(n, device="cuda", dtype=E4M3) for _ in range(2))
+    ms, rs = (torch.zeros(n // 256, device="cuda") for _ in range(2))
+    p = torch.zeros(n, device="cuda")
+    for step in (1, 2, 3):
+        g = torch.randn(n, generator=gen) * torch.exp(2 * torch.randn(n, generator=gen) - 7)
+        state = [(c.cpu().float().view(-1, 256) * s.cpu()[:, None]).view(-1) for c, s in ((m, ms), (r, rs))]
+        optim.adamw_step([p], [g.cuda()], [m], [r], step=step, **HYPER, exp_avg_scales=[ms], exp_avg_sq_scales=[rs], seed=seed)
+        first = f(b1) * state[0] + f(1 - b1) * g
+        root = (f(b2) * (state[1] * state[1]) + f(1 - b2) * (g * g)).double().sqrt().float()   # the CPU's f32 root is not rounded correctly
+        word = _mix32(torch.arange(n) ^ _mix32(torch.tensor(_mix32((seed + 0x9E3779B9 * step) & 0xFFFFFFFF))))
+        for x, codes, scales, u in ((first, m, ms, word & 0xFFFF), (root, r, rs, word >> 16)):
+            blocks = x.view(-1, 256)
+            want = blocks.abs().amax(1) * f(1 / 448)
+            same = scales.cpu() == want
+            assert int((~same).sum()) <= 1
+            a = (blocks.abs() / want[:, None]).double()
+            size = torch.exp2(torch.floor(torch.log2(a.clamp_min(2.0 ** -6))) - 3)
+            code = (torch.floor(a / size + u.view(-1, 256) / 65536) * size).clamp_max(448.0)
+            if codes is r:
+                code = torch.where(blocks > 0, code.clamp_min(2.0 ** -9), code)
+            got = codes.cpu().double().view(-1, 256)
+            assert int(((got != code * blocks.sign().double()) & same[:, None]).sum()) <= 10
+
+
+@gpu
+def test_step_inside_a_compiled_function(optim):
+    # the step is not traced: the graph breaks around it and goes on with what it wrote
+    def f(p, g, m, v):
+        optim.adamw_step([p], [g * 2], [m], [v], step=1, **HYPER)
+        return p * 2 + m
+
+    torch._dynamo.reset()
+    make = lambda: [torch.rand(300, generator=torch.Generator().manual_seed(i)).cuda() for i in range(4)]  # noqa: E731
+    a, b = make(), make()
+    want, got = f(*a), torch.compile(f, backend="aot_eager")(*b)
+    assert torch.equal(want, got) and all(torch.equal(x, y) for x, y in zip(a, b))
+
+
 @gpu
 def test_8bit_special_values(optim):
     n = 1024

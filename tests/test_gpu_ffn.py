@@ -107,6 +107,64 @@ def test_block_is_the_formulas(ffn, rows, width, hidden, out, kind):
         _close(g.detach(), w, b, name)
 
 
+# The down product split among clusters of three pairs (one tile, ragged ones, twenty), and the few rows' wide kernels at
+# both ends of their rows and where their width begins.
+MORE_SHAPES = [
+    (40, 128, 1536, 256), (33, 72, 1480, 8), (300, 136, 1672, 264), (1000, 64, 2560, 1280),
+    (9, 64, 2568, 640), (12, 136, 2376, 616), (16, 1024, 4096, 1024), (32, 256, 256, 256), (32, 512, 2376, 1192),
+]
+
+
+@gpu
+@pytest.mark.parametrize("rows,width,hidden,out", MORE_SHAPES)
+@pytest.mark.parametrize("kind", ["silu", "gelu", "relu2"])
+def test_block_is_the_formulas_where_the_split_changes(ffn, rows, width, hidden, out, kind):
+    test_block_is_the_formulas(ffn, rows, width, hidden, out, kind)
+
+
+@gpu
+@pytest.mark.parametrize("rows,width,hidden,out", [(1, 1024, 4096, 4096), (7, 520, 1032, 1024), (12, 136, 2376, 616),
+                                                   (16, 520, 1032, 520), (31, 256, 256, 256), (32, 512, 2376, 1192)])
+@pytest.mark.parametrize("kind", ["silu", "gelu", "relu2"])
+def test_few_rows_carry_their_results_rounding_alone(ffn, rows, width, hidden, out, kind):
+    # h goes to the product in two bf16 parts, within 2^-17 of it, which the 4e-5 covers: what is left is the result's
+    # rounding, U at most and uniform, so U / sqrt 12 = 1.13e-3 of a value at an even mantissa and up to sqrt 3 of that
+    # near a power of two; 1.9e-3 of the norm is over both, and under the 2.35e-3 of h in one part
+    *inputs, dy = _make(rows, width, hidden, out, seed=rows + 1)
+    want, bound = _formula(*inputs, dy, kind)
+    x, wg, wu, wd = (t.double() for t in inputs)
+    h = _act(x @ wg.T, kind)[0] * (x @ wu.T)
+    alone = bound[0] - U * (h.abs() @ wd.abs().T)
+    with torch.no_grad():
+        y = ffn.gated_ffn(*inputs, kind)
+    off = (y.double() - want[0]).abs()
+    assert (off <= alone + U * want[0].abs()).all()
+    assert float(off.norm()) <= 1.9e-3 * float(want[0].norm())
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["silu", "gelu", "relu2"])
+def test_activation_over_its_range(ffn, kind):
+    # one row, w_up = 1, and for each gate value a second hidden value that takes act(g) rounded to bf16 away again
+    # (act(64) is 64 to the last bit, or 4096 for relu2): what comes out is act(g) less that, so an error of act(g) shows
+    # at 2^-17 of it.  Allowed: 2^-17 for the two parts of h, 2^-17 for the result's own rounding, and the activation's
+    # 2e-5 (far out in gelu's and silu's tails; exponentials of large arguments).
+    g = torch.linspace(-12, 12, 512).to(BF16)
+    exact = g.double() * torch.erfc(-g.double() / math.sqrt(2)) / 2 if kind == "gelu" else _act(g.double(), kind)[0]
+    near = exact.to(BF16)
+    back = 4096.0 if kind == "relu2" else 64.0
+    wg, wu = torch.zeros(1024, 8, dtype=BF16), torch.zeros(1024, 8, dtype=BF16)
+    wg[:512, 0], wg[512:, 0] = g, 64.0
+    wu[:512, 0], wu[512:, 0] = 1.0, near / back
+    eye = torch.eye(512, dtype=BF16)
+    x = torch.zeros(1, 8, dtype=BF16)
+    x[0, 0] = 1
+    with torch.no_grad():
+        y = ffn.gated_ffn(x.cuda(), wg.cuda(), wu.cuda(), torch.cat([eye, -eye], 1).cuda(), kind)[0].double().cpu()
+    off = (y - (exact - near.double())).abs()
+    assert (off <= (2 * 2.0 ** -17 + 2e-5) * exact.abs()).all(), float((off / exact.abs().clamp_min(1e-300)).max())
+
+
 @gpu
 def test_gradient_is_the_difference_of_the_forward(ffn):
     # along the gradient, a step of 5 % of x: the difference of two forwards of N rounded outputs is off by at most

@@ -545,7 +545,7 @@ int ts_b200_gn_prep_bwd(const ts_gn_prep_args* args, ts_stream_t stream);
  * Rows have contiguous channels and any row stride; outputs are contiguous.
  * With `scales`, y receives e4m3 codes of y / scale, scale = max(max|y|,
  * 2^-100) / 448 over the row (group 0) or over each 128 columns (group 128,
- * scales [rows, ceil(width/128)]).  The backward reads as x the STORED sum. */
+ * scales [rows, ceil(width/128)]); NaN over a NaN.  The backward reads as x the STORED sum. */
 typedef struct ts_norm_args {
   long long rows;
   int width;                /* 1..16384 */

@@ -9,7 +9,7 @@
 //
 //   kGateFwd   both projections, the activation and the product: h; for a
 //              backward pass also g and u, in 24 bits (the f32 without its last
-//              byte, within 2^-16: a bf16 copy would double the error of dg
+//              byte, within 2^-15: a bf16 copy would double the error of dg
 //              and du, an f32 copy costs a third more traffic)
 //   kProduct   y = h Wd^T
 //   kGateGrad  dh = dy Wd and, from g and u, dg and du
@@ -31,11 +31,11 @@
 // tile's are formed in the other half of it.
 //
 // What bounds it.  At 8192 x 2048 x 5632 a forward and backward pass takes
-// 1460 us, 1.17 PFLOP/s, where cuBLAS holds 1.37 in a loop of a large product
-// under the power limit; kGateFwd takes 350 us there (290 without keeping g and
+// 1460 to 1590 us from box to box, 1.17 to 1.07 PFLOP/s, where cuBLAS holds 1.37
+// in a loop of a large product under the power limit; kGateFwd takes 350 us there (290 without keeping g and
 // u), its instructions alone, loads left out, 248, its loads alone 174 (63
 // bytes a cycle into each SM): both near their limits at once.  At 65536 x 512
-// x 1024 (630 us) the inner length is eight steps, and the traffic of what is
+// x 1024 (630 to 740 us) the inner length is eight steps, and the traffic of what is
 // kept and exchanged counts: kGateFwd 153 us (134 with the instructions left
 // out), kGateGrad 139 (737 MB), the gradients 262, the down product 73.
 // An operand whose tile is 64 rows of the inner dimension comes as one copy of
@@ -287,7 +287,8 @@ struct KeptHalf {
     }
   }
   // The word again, with its third byte in the place of the lost fourth too:
-  // nearer to the middle of what was cut off than zero.
+  // nearer to the middle of what was cut off than zero on average (255 units of
+  // 2^-23 at most), and zero and infinity stay what they are.
   __device__ __forceinline__ float value(int i, int e) const {
     const uint32_t byte = 4 + (e & 3), half = e & 1 ? 0x3200 : 0x1000;
     return __uint_as_float(__byte_perm(high[i][e >> 1], low[i][e >> 2], half | byte << 4 | byte));

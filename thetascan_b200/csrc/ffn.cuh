@@ -8,9 +8,9 @@ namespace ts {
 
 // Rows up to which an inference call streams the weights past the rows
 // (ffn_rows.cu) instead of forming tiles of 256 rows (ffn.cu).
-// At 1024 x 4096 and 1 / 16 / 32 rows this takes 8.8 / 11.2 / 13.8 us, the
-// tiles 26; at 2048 x 5632 and 32 rows 32 us, the tiles 34, and at 48 and 64
-// rows 69 and 73 with the tiles still at 34.
+// At 1024 x 4096 and 1 / 16 / 32 rows this takes 8.8 / 13.0 / 13.9 us, the
+// tiles 26 / 25 / 25; at 2048 x 5632 21.7 / 25.9 / 31.7 us, the tiles 39 / 35 /
+// 34, and 34 still at 48 and 64 rows, where this would read x and h once more.
 constexpr int kRowsMost = 32;
 
 // The forward for few rows; arguments checked, h holds [2, rows, hidden].
@@ -27,10 +27,12 @@ __device__ __forceinline__ float ffn_act(float g, float& slope) {
   if (kAct == TS_FFN_GELU) {
     // The normal distribution's share below -|g| is erfc(z) / 2, z = |g| / sqrt 2
     // (1 + erf would cancel there).  With t = 1 / (1 + z / 2), erfc(z) = t exp(f(t)
-    // - z^2) and f is smooth on (0, 1]: a least-squares polynomial of degree 7 on
-    // the Chebyshev points of log(exp(z^2) erfc(z) / t) is within 3e-6, and f32
-    // keeps the whole within 4e-6 of the value.  CUDA's erfcf took a forward pass
-    // of 1531 x 1024 x 2816 5 us more.
+    // - z^2) (the form of erfc in Numerical Recipes, Press et al.) and f is smooth
+    // on (0, 1]: a least-squares polynomial of degree 7 on 64 Chebyshev points of
+    // (0, 1], fitted here to log(exp(z^2) erfc(z) / t), is within 3e-6.  f32 keeps
+    // gelu within 4e-6 of itself for g >= -5; below, the rounding of z^2 counts:
+    // 8e-6 to -9 and 2.3e-5 to -13, where gelu is under 1e-17 itself.  CUDA's erfcf
+    // took a forward pass of 1531 x 1024 x 2816 5 us more.
     const float z = fabsf(g) * 0.70710678118654752f, zz = z * z;
     const float t = __fdividef(1.f, fmaf(0.5f, z, 1.f));
     float f = fmaf(-0.16612210869789124f, t, 0.668515145778656f);

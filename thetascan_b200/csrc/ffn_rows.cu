@@ -14,7 +14,8 @@
 // h passes between the two as two bf16 values, its rounding and the rest's
 // (2^-17 together): the result then carries its own rounding alone (1.66e-3 of
 // its norm, with h in bf16 2.35e-3), for a second load and instruction beside
-// the weights' traffic (1024 x 4096, one row: 7.8 -> 8.8 us).
+// the weights' traffic (one row of 1024 x 4096: 7.8 -> 8.8 us, of 2048 x 5632:
+// 16.6 -> 21.7 us).
 //
 // The order of the inner dimension is free as long as A and B agree, so a lane
 // takes 8 neighbouring elements (16 bytes) of its row for two steps of
@@ -264,8 +265,8 @@ int ffn_rows_down(const FfnRowsParams& p, cudaStream_t s) {
 
 // Two sets of weight rows to a warp read x half as often, one set has twice the
 // CTAs: two where there are several tiles of rows and CTAs enough all the same
-// (2048 x 5632, 16 / 32 rows: 22.5 / 31 us with two, 24.8 / 36 with one, before
-// h had two parts).
+// (2048 x 5632, 9 / 16 / 32 rows: 25.8 / 25.9 / 31.7 us with two, 27.4 / 29.7 /
+// 37.5 with one; 1024 x 4096: 12.7 / 12.9 / 13.9 and 12.1 / 12.9 / 17.9).
 constexpr int kRowsCtas = 148;
 
 template <int kTiles>

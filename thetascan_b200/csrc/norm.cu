@@ -4,7 +4,8 @@
 //   s = round(x + r)                    the residual stream, as it is stored
 //   y = s * rstd * w,  rstd = (mean_c s_c^2 + eps)^(-1/2)
 //   8-bit output: scale = max(max|y|, 2^-100) / 448 over the row or over each
-//   128 columns, code = e4m3(y / scale), y in f32 (no rounding in between)
+//   128 columns, code = e4m3(y / scale), y in f32 (no rounding in between); a
+//   NaN makes its scale NaN, and with it the codes of that row or those columns
 //   backward, u = s rstd:  dx = rstd (w dy - u mean_c(w dy u)) + dsum,
 //                          dw = sum_rows dy u
 //   (1 - mean u^2 = eps rstd^2, so that in a row of one column the difference

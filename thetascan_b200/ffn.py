@@ -6,9 +6,16 @@
 The kernels (``csrc/ffn.cu``) form both projections, the activation and the
 product in one launch and the down projection in a second.  For a backward
 pass the block keeps its input and 8 bytes per hidden value: ``h`` in bf16 and
-both projections in 24 bits.  bf16 operands with f32 accumulators and one
-rounding for every stored value.  Any number of rows; widths that are
-multiples of 8.
+both projections in 24 bits.  bf16 operands, f32 accumulators.  Any number of
+rows; widths that are multiples of 8.
+
+What is rounded on the way: ``h`` to bf16 between the two launches, and ``dg``
+and ``du`` in the backward, as operands of the next product.  A result's error
+is then 2.35e-3 of its norm, where its own rounding to bf16 alone is 1.66e-3.
+Inference with up to 32 rows is bound by the weights' traffic and passes ``h``
+in two bf16 parts, which leaves the result's own rounding alone; so the same
+row comes out the same within that rounding, not to the bit, from a call with
+more rows or with gradients.  A compiled call computes what the eager one does.
 """
 from __future__ import annotations
 

@@ -117,7 +117,8 @@ def rms_norm_8bit(x: Tensor, weight: Tensor, eps: float = 1e-6, *, residual: Opt
     (``group=128``), shape ``[..., n_scales]``.  Each scale maps the largest
     magnitude that it covers to 448, the type's largest value; the norm is
     rounded once, from f32 to the code.  Returns ``(codes, scales)``, and the
-    stored sum too where there is a residual.  For inference: no gradient."""
+    stored sum too where there is a residual.  A NaN makes its scale NaN and
+    with it all codes under that scale.  For inference: no gradient."""
     if torch.compiler.is_compiling():
         if _wants_grad(x, residual, weight):
             raise RuntimeError("rms_norm_8bit has no gradient: call it under torch.no_grad()")

@@ -13,7 +13,7 @@ stochastically, because a moving average moves by less than half a code per
 step and rounding to nearest would hold it in place.  The random words are a
 hash of ``(seed, step, place of the tensor, element)``: a step is a function of
 its arguments.  A NaN stays in its element; an infinite value makes its block
-of 256 non-finite.
+of 256 non-finite.  Finite gradients up to 1e37 do neither.
 """
 from __future__ import annotations
 
@@ -63,9 +63,12 @@ class AdamW(torch.optim.Optimizer):
     """AdamW with decoupled weight decay over :func:`adamw_step`.
 
     ``state_bits=8`` keeps the moments in 8 bits; ``master_weights=True`` keeps
-    an f32 value behind every bf16 parameter.  Parameters are contiguous CUDA
-    tensors in f32 or bf16; gradients may be either type.  ``seed`` keys the
-    rounding of 8-bit states."""
+    an f32 value behind every bf16 parameter, which carries it from its first
+    step on: a parameter that is written otherwise afterwards (weights loaded
+    into the model) needs its ``state["master"]`` written too, or the optimizer
+    made anew.  Parameters are contiguous CUDA tensors in f32 or bf16; gradients
+    may be either type.  ``seed`` keys the rounding of 8-bit states.  A step
+    that is refused with an error does not count."""
 
     def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, *,
                  state_bits: int = 32, master_weights: bool = False, seed: int = 0):

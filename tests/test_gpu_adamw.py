@@ -313,6 +313,28 @@ def test_8bit_roots_without_gradients_fade_evenly(optim):
 
 
 @gpu
+@pytest.mark.parametrize("size", [1e-24, 1e-3, 1e16, 1e30])
+def test_8bit_steps_go_on_at_any_magnitude_and_alignment(optim, size):
+    # five steps on views that start at odd elements: the decoded states follow the average of what went in, whose codes
+    # are within 1/16 of a step (2^-3 of the value at most) each time, and the parameter moves by lr within the sum of
+    # both moments' errors (5 * 2^-3 in the worst order)
+    n = 1000
+    gen = torch.Generator().manual_seed(9)
+    hold = lambda dtype: torch.zeros(n + 3, device="cuda", dtype=dtype)[3:]  # noqa: E731
+    m, r, p, g = hold(E4M3), hold(E4M3), hold(F32), hold(F32)
+    ms, rs = torch.zeros(4, device="cuda"), torch.zeros(4, device="cuda")
+    g.copy_((1 + 0.1 * torch.rand(n, generator=gen)) * size)
+    for step in range(1, 6):
+        before = p.clone()
+        optim.adamw_step([p], [g], [m], [r], step=step, lr=1.0, betas=(0.9, 0.95), eps=0.0, weight_decay=0.0,
+                         exp_avg_scales=[ms], exp_avg_sq_scales=[rs], seed=3)
+        assert ((p - before + 1).abs() <= 5 * 2.0 ** -3).all()
+        assert ((p - before).mean() + 1).abs() <= 0.02
+        for codes, scale, c in ((m, ms, 1 - 0.9 ** step), (r, rs, math.sqrt(1 - 0.95 ** step))):
+            assert ((_decode(codes, scale) / (c * g.double()) - 1).abs() <= 5 * 2.0 ** -3).all()
+
+
+@gpu
 def test_8bit_infinite_value_makes_its_block_non_finite(optim):
     g = torch.ones(600, device="cuda")
     g[10] = float("inf")

@@ -115,3 +115,45 @@ def test_saved_tensors_pass_through_their_hooks(ts):
         assert len(count) >= 3, name
         got = torch.autograd.grad(y.float().sum(), leaves)
         assert all(torch.equal(a, b) for a, b in zip(got, want)), name
+
+
+@gpu
+def test_one_tensor_as_both_terms_of_the_sum(ts):
+    # its gradient is the sum of both terms'
+    x, *_, w = _inputs()
+    a, b = x.clone().requires_grad_(True), x.clone().requires_grad_(True)
+    y, s = ts.add_rms_norm(a, a, w)
+    (y.float().sum() + 3 * s.float().sum()).backward()
+    c = x.clone().requires_grad_(True)
+    y2, s2 = ts.add_rms_norm(b, c, w)
+    (y2.float().sum() + 3 * s2.float().sum()).backward()
+    assert torch.equal(y, y2) and torch.equal(a.grad, b.grad + c.grad) and torch.equal(b.grad, c.grad)
+
+
+@gpu
+@pytest.mark.parametrize("rows", [8, 300])
+def test_forward_and_backward_in_a_graph(ts, rows):
+    x, wg, wu, wd, w = _inputs(rows)
+    leaves = [t.requires_grad_(True) for t in (x, wg, wu, wd, w)]
+
+    def step():
+        y, s = ts.add_rms_norm(x, x.detach(), w)
+        z = ts.gated_ffn(y, wg, wu, wd)
+        return [z.detach(), *torch.autograd.grad((z, s), leaves, (torch.ones_like(z), torch.ones_like(s)))]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    with torch.no_grad():
+        for t in leaves:
+            t.mul_(1.25)
+    want = step()
+    for _ in range(2):
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -127,7 +127,7 @@ def test_block_is_the_formulas_where_the_split_changes(ffn, rows, width, hidden,
                                                    (16, 520, 1032, 520), (31, 256, 256, 256), (32, 512, 2376, 1192)])
 @pytest.mark.parametrize("kind", ["silu", "gelu", "relu2"])
 def test_few_rows_carry_their_results_rounding_alone(ffn, rows, width, hidden, out, kind):
-    # h goes to the product in two bf16 parts, within 2^-17 of it, which the 4e-5 covers: what is left is the result's
+    # h goes to the product in two bf16 parts, within 2^-16 of it, which the 4e-5 covers: what is left is the result's
     # rounding, U at most and uniform, so U / sqrt 12 = 1.13e-3 of a value at an even mantissa and up to sqrt 3 of that
     # near a power of two; 1.9e-3 of the norm is over both, and under the 2.35e-3 of h in one part
     *inputs, dy = _make(rows, width, hidden, out, seed=rows + 1)
@@ -147,8 +147,8 @@ def test_few_rows_carry_their_results_rounding_alone(ffn, rows, width, hidden, o
 def test_activation_over_its_range(ffn, kind):
     # one row, w_up = 1, and for each gate value a second hidden value that takes act(g) rounded to bf16 away again
     # (act(64) is 64 to the last bit, or 4096 for relu2): what comes out is act(g) less that, so an error of act(g) shows
-    # at 2^-17 of it.  Allowed: 2^-17 for the two parts of h, 2^-17 for the result's own rounding, and the activation's
-    # 2e-5 (far out in gelu's and silu's tails; exponentials of large arguments).
+    # at 2^-17 of it.  Allowed: 3.5e-5, of which 2^-16 are for the two parts of h and the result's own rounding, and 2e-5
+    # for the activation (far out in gelu's and silu's tails; exponentials of large arguments).
     g = torch.linspace(-12, 12, 512).to(BF16)
     exact = g.double() * torch.erfc(-g.double() / math.sqrt(2)) / 2 if kind == "gelu" else _act(g.double(), kind)[0]
     near = exact.to(BF16)
@@ -250,6 +250,26 @@ def test_non_finite_weights_show(ffn, rows, kind):
         for got, ref in results:
             assert torch.equal(got.isnan(), ref.isnan()), (value, kind)
             assert torch.equal(got.isinf(), ref.isinf()), (value, kind)
+
+
+@gpu
+@pytest.mark.parametrize("rows", [1, 4, 32, 70])
+def test_infinite_down_weights_show(ffn, rows):
+    # h times an infinity is infinite with h's sign, whatever is left of h's rounding: also for an h of few bits (the last
+    # rows' x is 0.5 in one place, and its weights are powers of two), and NaN for an h of zero
+    x, wg, wu, wd, _ = _make(rows, 64, 128, 64, seed=2)
+    wg[5], wu[5] = 2.0, 4.0
+    x[rows - 1] = 0
+    if rows > 1:
+        x[rows - 2] = 0
+        x[rows - 2, 7] = 0.5
+    wd = wd.clone()
+    wd[9, 5], wd[11, 5] = float("inf"), -float("inf")
+    with torch.no_grad():
+        y = ffn.gated_ffn(x, wg, wu, wd, "relu2")
+    want = (_act(x.double() @ wg.double().T, "relu2")[0] * (x.double() @ wu.double().T)) @ wd.double().T
+    assert torch.equal(y.isnan(), want.isnan()) and torch.equal(y.isinf(), want.isinf())
+    assert torch.equal(y[y.isinf()].double(), want[want.isinf()])
 
 
 @gpu

@@ -16,6 +16,17 @@ constexpr int kRowsMost = 32;
 // The forward for few rows; arguments checked, h holds [2, rows, hidden].
 int ffn_rows_fwd(const ts_ffn_args* a, void* h, cudaStream_t s);
 
+// A value in two bf16 parts, within 2^-16 of it: its upper half, and what is
+// left.  Cut off and not rounded, so that both parts have the value's sign, and
+// the second is never zero beside a first that is not: a product with an
+// infinity is then infinite in both, where the difference of two infinities, or
+// 0 inf, would be NaN.  (2^-126 is nothing beside values over 2^-100.)
+__device__ __forceinline__ float ffn_high(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
+__device__ __forceinline__ float ffn_rest(float x) {
+  const float rest = x - ffn_high(x);   // NaN of an infinity
+  return fabsf(x) > 7.8886090522101181e-31f && !(fabsf(rest) > 0.f) ? copysignf(1.1754943508222875e-38f, x) : rest;
+}
+
 // The activations: value and slope.
 template <int kAct>
 __device__ __forceinline__ float ffn_act(float g, float& slope) {

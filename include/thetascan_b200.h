@@ -624,6 +624,8 @@ enum { TS_FFN_SILU = 0, TS_FFN_GELU = 1 /* exact, by erf */, TS_FFN_RELU2 = 2 /*
 
 /* Bytes of `kept` for each 32 rows x 32 hidden columns (both rounded up). */
 #define TS_FFN_KEPT_BLOCK 6144
+/* Rows up to which h is kept in two bf16 parts, its upper half and the rest. */
+#define TS_FFN_TWO_PART_ROWS 32
 
 typedef struct ts_ffn_args {
   long long rows;
@@ -635,7 +637,8 @@ typedef struct ts_ffn_args {
   const void* w_down;
   long long x_stride, w_gate_stride, w_up_stride, w_down_stride;  /* elements between rows */
   void* y;                  /* [rows,width_out] (forward) */
-  void* h;                  /* bf16 [rows,hidden], with kept; both NULL in inference */
+  void* h;                  /* bf16 [rows,hidden] ([2,rows,hidden] up to TS_FFN_TWO_PART_ROWS), with kept; both
+                               NULL in inference */
   void* kept;               /* 16-byte aligned */
   void* workspace;
   size_t workspace_bytes;

@@ -143,6 +143,35 @@ def test_few_rows_carry_their_results_rounding_alone(ffn, rows, width, hidden, o
 
 
 @gpu
+@pytest.mark.parametrize("rows,width,hidden,out", [(1, 1024, 512, 4096), (2, 680, 512, 680), (3, 1296, 488, 1296), (8, 520, 1032, 600),
+                                                   (16, 72, 136, 264), (17, 264, 392, 264), (32, 512, 1336, 512)])
+@pytest.mark.parametrize("kind", ["silu", "gelu", "relu2"])
+def test_few_rows_carry_their_gradients_rounding_alone(ffn, rows, width, hidden, out, kind):
+    # as above for the results of a call with gradients: h, dg and du in two parts each, g and u within 2^-15 (which is
+    # 6.1e-5 of the sums of magnitudes for the two of them: 1e-4 is allowed)
+    *inputs, dy = _make(rows, width, hidden, out, seed=rows + 2)
+    want, _ = _formula(*inputs, dy, kind)
+    x, wg, wu, wd = (t.double() for t in inputs)
+    g, u, dh = x @ wg.T, x @ wu.T, dy.double() @ wd
+    a, slope = _act(g, kind)
+    at_x, at_g, at_u = x.abs(), x.abs() @ wg.abs().T, x.abs() @ wu.abs().T
+    terms = dy.double().abs() @ wd.abs()
+    du = terms * a.abs() + dh.abs() * slope.abs() * at_g
+    dg = terms * (u * slope).abs() + dh.abs() * slope.abs() * at_u + 2 * (dh * u).abs() * at_g
+    h = a.abs() * at_u + slope.abs() * u.abs() * at_g
+    sums = (h @ wd.abs().T, dg @ wg.abs() + du @ wu.abs(), dg.T @ at_x, du.T @ at_x, dy.double().abs().T @ h)
+    with torch.no_grad():
+        alone = ffn.gated_ffn(*inputs, kind)
+    leaves = [t.requires_grad_(True) for t in inputs]
+    y = ffn.gated_ffn(*leaves, kind)
+    assert torch.equal(y.detach(), alone)   # the forward with gradients is the one without
+    for name, got, ref, magnitude in zip(NAMES, (y.detach(), *torch.autograd.grad(y, leaves, dy)), want, sums):
+        off = (got.double() - ref).abs()
+        assert (off <= 1e-4 * magnitude + U * ref.abs()).all(), name
+        assert float(off.norm()) <= 1.9e-3 * float(ref.norm()), name
+
+
+@gpu
 @pytest.mark.parametrize("kind", ["silu", "gelu", "relu2"])
 def test_activation_over_its_range(ffn, kind):
     # one row, w_up = 1, and for each gate value a second hidden value that takes act(g) rounded to bf16 away again

@@ -15,6 +15,11 @@
 //   kGateGrad  dh = dy Wd and, from g and u, dg and du
 //   kProduct   dx, dWg, dWu and dWd: one launch over all their tiles
 //
+// Up to kRowsMost rows the forward is ffn_rows.cu's, with gradients too, and h,
+// dg and du pass in two bf16 parts each (kGateGradTwo, and products over twice
+// the segments): with few rows the errors of a few large hidden values do not
+// average out (2.6e-3 of dx's norm now and then, 1.66e-3 so).
+//
 // Forming g and u again in the backward instead of keeping them was built
 // first and measured slower: dh, g and u then share a tile of 128 hidden
 // columns, and the N = 128 instructions of dh run at half the rate of N = 256
@@ -76,19 +81,20 @@ constexpr int kPairs = 74;
 constexpr int kMinSplitSteps = 8;
 
 // kProductCluster: a product whose few tiles are each split among the pairs of a cluster.
-enum FfnMode { kGateFwd = 0, kGateGrad = 1, kProduct = 2, kProductCluster = 3 };
+// kGateGradTwo: kGateGrad with dg and du in two parts; kProductTwo: kProduct over such parts.
+enum FfnMode { kGateFwd = 0, kGateGrad = 1, kProduct = 2, kProductCluster = 3, kGateGradTwo = 4, kProductTwo = 5 };
+// Maps of each kind that a problem has: the launches of the two-part forms alone have to carry more than 4 KB.
+constexpr int ffn_maps(int mode) { return mode == kGateGradTwo || mode == kProductTwo ? 4 : 2; }
 
 // How an operand lies in memory: inner dimension contiguous; or M (N)
 // contiguous, loaded as two boxes of 64 columns or as one of 2 x 64.
 enum FfnLayout { kInner = 0, kOuter = 1, kOuterBlocks = 2 };
 
-// One product of a launch: C[M, N] = sum over segments A_i B_i^T.
-struct FfnProblem {
-  CUtensorMap a[2], b[2];    // per segment; kGateFwd: a[0] = x, b = {Wg, Wu}
-  CUtensorMap out[2];        // {C}; kGateGrad: {dg, du}
+// One product of a launch: C[M, N] = sum over segments A_i B_i^T, all of one inner length.
+struct FfnSizes {
   int rows, cols;            // of C
   int tiles_n;
-  int steps[2];              // 64-wide inner steps of each segment
+  int segments, steps;       // 64-wide inner steps of each segment
   int splits;
   int units;                 // tiles * splits
   int a_layout, b_layout;
@@ -97,9 +103,16 @@ struct FfnProblem {
   uint8_t* kept;             // g and u (see keep_at), or null
 };
 
-template <int kCount>
+template <int kMaps>
+struct FfnProblemOf : FfnSizes {
+  CUtensorMap a[kMaps], b[kMaps];   // per segment; kGateFwd: a[0] = x, b = {Wg, Wu}
+  CUtensorMap out[kMaps];           // {C}; kGateGrad: {dg, du}; kGateGradTwo: and the rests of both
+};
+using FfnProblem = FfnProblemOf<4>;
+
+template <int kCount, int kMaps = 4>
 struct FfnParams {
-  FfnProblem p[kCount];
+  FfnProblemOf<kMaps> p[kCount];
   int count;
   int units;
   int* clear;        // counters of the launch after this one, set to zero (or null)
@@ -246,17 +259,7 @@ __device__ __forceinline__ void tie(uint32_t (&r)[kN]) {
                  "+r"(r[i + 6]), "+r"(r[i + 7]));
 }
 
-// ---- g and u between the passes
-//
-// Blocks of 32 rows x 32 columns, a lane's row as twelve 16-byte vectors
-// [vector][lane] (a warp's access is 512 contiguous bytes); for each half of
-// 16 columns: the upper halves of g's words, two vectors, their third bytes,
-// one vector, and the same of u.
-
-__device__ __forceinline__ uint8_t* keep_at(uint8_t* base, int cols, int row, int col, int lane) {
-  const size_t blocks = static_cast<size_t>((cols + 31) >> 5);
-  return base + ((row >> 5) * blocks + (col >> 5)) * TS_FFN_KEPT_BLOCK + 16 * lane;
-}
+// ---- g and u between the passes (keep_at)
 
 // 16 values from r[c] on, as three vectors.
 __device__ __forceinline__ void keep16(uint8_t* to, const uint32_t (&r)[32], int c) {
@@ -299,28 +302,29 @@ struct KeptHalf {
 
 // ---- one unit of work
 
+template <int kMaps>
 struct FfnUnit {
-  const FfnProblem* p;
+  const FfnProblemOf<kMaps>* p;
   int m, n;             // first row and column of the pair's tile
   int begin, end;       // inner steps
   int split, tile;
 };
 
-template <int kMode, int kCount>
-__device__ __forceinline__ FfnUnit ffn_unit(const FfnParams<kCount>& q, int unit) {
+template <int kMode, int kCount, int kMaps>
+__device__ __forceinline__ FfnUnit<kMaps> ffn_unit(const FfnParams<kCount, kMaps>& q, int unit) {
   int i = 0;
   while (i + 1 < q.count && unit >= q.p[i].units) {
     unit -= q.p[i].units;
     ++i;
   }
-  FfnUnit u;
+  FfnUnit<kMaps> u;
   u.p = &q.p[i];
   const int splits = u.p->splits;
   u.tile = unit / splits;
   u.split = unit - u.tile * splits;
   u.m = u.tile / u.p->tiles_n * 256;
   u.n = u.tile % u.p->tiles_n * (kMode == kGateFwd ? 128 : 256);
-  const int steps = u.p->steps[0] + u.p->steps[1];
+  const int steps = u.p->segments * u.p->steps;
   u.begin = static_cast<int>(static_cast<long long>(steps) * u.split / splits);
   u.end = static_cast<int>(static_cast<long long>(steps) * (u.split + 1) / splits);
   return u;
@@ -348,7 +352,10 @@ __device__ __forceinline__ void stage8(uint32_t block, int lane, int chunk, uint
 
 template <int kMode, int kAct, int kCount>
 __global__ void __launch_bounds__(kFfnThreads, 1)
-    ffn_kernel(const __grid_constant__ FfnParams<kCount> q) {
+    ffn_kernel(const __grid_constant__ FfnParams<kCount, ffn_maps(kMode)> q) {
+  constexpr bool kGrad = kMode == kGateGrad || kMode == kGateGradTwo;
+  constexpr bool kJoin = kMode == kProduct || kMode == kProductTwo;
+  constexpr int kPasses = kMode == kGateGradTwo ? 2 : 1;
   extern __shared__ uint8_t smem_raw[];
   __shared__ alignas(8) uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2];
   __shared__ uint32_t tmem_slot;
@@ -371,7 +378,7 @@ __global__ void __launch_bounds__(kFfnThreads, 1)
   }
   if (warp == 2) tmem_alloc_pair(&tmem_slot, 512);
   if (warp == 3 && lane < q.count) {
-    const FfnProblem& p = q.p[lane];
+    const auto& p = q.p[lane];
     tma_prefetch_map(&p.a[0]);
     tma_prefetch_map(&p.b[0]);
     tma_prefetch_map(&p.out[0]);
@@ -392,8 +399,8 @@ __global__ void __launch_bounds__(kFfnThreads, 1)
     int it = 0;
     bool ok = true;
     for (int w = pair; w < q.units && ok; w += pairs) {
-      const FfnUnit u = ffn_unit<kMode>(q, w);
-      const FfnProblem& p = *u.p;
+      const auto u = ffn_unit<kMode>(q, w);
+      const auto& p = *u.p;
       const int row = u.m + 128 * static_cast<int>(rank);
       for (int k = u.begin; k < u.end; ++k, ++it) {
         const int s = it % kStages;
@@ -405,8 +412,9 @@ __global__ void __launch_bounds__(kFfnThreads, 1)
           ffn_load(a, &p.a[0], kInner, row, k, bar);
           ffn_load(b, &p.b[rank], kInner, u.n, k, bar);
         } else {
-          const int seg = k < p.steps[0] ? 0 : 1;
-          const int step = k - (seg ? p.steps[0] : 0);
+          // two segments at most, but for the products over two parts
+          const int seg = kMode == kProductTwo ? k / p.steps : (k < p.steps ? 0 : 1);
+          const int step = k - seg * p.steps;
           ffn_load(a, &p.a[seg], p.a_layout, row, step, bar);
           ffn_load(b, &p.b[seg], p.b_layout, u.n + 128 * static_cast<int>(rank), step, bar);
         }
@@ -423,8 +431,8 @@ __global__ void __launch_bounds__(kFfnThreads, 1)
     int it = 0, n_unit = 0;
     bool ok = true;
     for (int w = pair; w < q.units && ok; w += pairs, ++n_unit) {
-      const FfnUnit u = ffn_unit<kMode>(q, w);
-      const FfnProblem& p = *u.p;
+      const auto u = ffn_unit<kMode>(q, w);
+      const auto& p = *u.p;
       const bool a_mn = p.a_layout != kInner, b_mn = p.b_layout != kInner;
       const int buf = n_unit & 1;
       const uint32_t acc = tmem + 256u * buf, id = idesc_bf16(256, 256, a_mn, b_mn);
@@ -458,7 +466,7 @@ __global__ void __launch_bounds__(kFfnThreads, 1)
       __syncwarp();
       return stage + (turn++ & 1) * kOutBlock;
     };
-    auto store_block = [&](const CUtensorMap* map, uint32_t block, int x, int y, const FfnProblem& p) {
+    auto store_block = [&](const CUtensorMap* map, uint32_t block, int x, int y, const FfnSizes& p) {
       fence_async_smem();
       __syncwarp();
       if (lane == 0) {
@@ -468,8 +476,8 @@ __global__ void __launch_bounds__(kFfnThreads, 1)
       }
     };
     for (int w = pair; w < q.units; w += pairs, ++n_unit) {
-      const FfnUnit u = ffn_unit<kMode>(q, w);
-      const FfnProblem& p = *u.p;
+      const auto u = ffn_unit<kMode>(q, w);
+      const auto& p = *u.p;
       const int buf = n_unit & 1;
       auto release = [&]() {
         tc_fence_before();
@@ -479,18 +487,18 @@ __global__ void __launch_bounds__(kFfnThreads, 1)
       const int row0 = u.m + 128 * static_cast<int>(rank) + 32 * quad;
       KeptHalf kept;
       const uint8_t* from = nullptr;
-      if (kMode == kGateGrad) {
+      if (kGrad) {
         // 64 columns of g and u: two blocks, the first half-block ahead of the wait
         from = keep_at(p.kept, p.cols, row0, u.n + 64 * part, lane);
         if (row0 < p.rows && u.n + 64 * part < p.cols) kept.load(from);
       }
       bool ok = wait_cluster(&acc_full[buf], (n_unit >> 1) & 1, kErrMmaTimeout);
       // the warps of a product meet in barriers below: they go on, or give up, together
-      if (kMode == kProduct) ok = epilogue_all(ok);
+      if (kJoin) ok = epilogue_all(ok);
       if (!ok) break;
       tc_fence_after();
       if (kMode == kProductCluster) break;   // its one tile goes on below
-      if (kMode == kProduct) {
+      if (kJoin) {
         const uint32_t acc = tmem + 256u * buf + lanes + 64 * part;
         float* sums = p.partial + (static_cast<size_t>(u.tile) * p.splits * 2 + rank) * 32768 + 64 * part * 128 +
                       32 * quad + lane;   // [split][rank][column][row]
@@ -574,9 +582,11 @@ __global__ void __launch_bounds__(kFfnThreads, 1)
         store_block(&p.out[0], block, col, row0, p);
       } else {
         const uint32_t acc = tmem + 256u * buf + lanes + 64 * part;
-        // blocks of 32 columns, in halves of 16; the next half's g and u are on their way meanwhile
+        // blocks of 32 columns, in halves of 16; the next half's g and u are on their way meanwhile.  The second pass,
+        // where there is one, stores what the first left.
 #pragma unroll 1
-        for (int c = 0; c < 64; c += 32) {
+        for (int turn_c = 0; turn_c < 64 * kPasses; turn_c += 32) {
+          const int c = turn_c & 63, pass = kPasses > 1 ? turn_c >> 6 : 0;
           const int col = u.n + 64 * part + c;
           if (lane == 0) tma_store_read_wait<0>();
           __syncwarp();
@@ -586,9 +596,10 @@ __global__ void __launch_bounds__(kFfnThreads, 1)
             tmem_ld(acc + c + o, d);
             tmem_wait();
             tie(d);
-            if (c + o == 48) release();
+            if (turn_c + o == 64 * kPasses - 16) release();
             KeptHalf next;
-            const int ahead = c + o + 16;   // the columns after this half, where they are this tile's and inside
+            // the columns after this half (or the first again), where they are this tile's and inside
+            const int ahead = kPasses > 1 ? (c + o + 16) & 63 : c + o + 16;
             if (ahead < 64 && row0 < p.rows && u.n + 64 * part + (ahead & 32) < p.cols)
               next.load(from + (ahead >> 5) * TS_FFN_KEPT_BLOCK + ((ahead >> 4) & 1) * (6 * 512));
 #pragma unroll
@@ -601,14 +612,18 @@ __global__ void __launch_bounds__(kFfnThreads, 1)
                 const float act = ffn_act<kAct>(kept.gate(8 * i + e), slope);
                 x[e] = dh * kept.up(8 * i + e) * slope;
                 y[e] = dh * act;
+                if (kPasses > 1) {
+                  x[e] = pass ? ffn_rest(x[e]) : ffn_high(x[e]);
+                  y[e] = pass ? ffn_rest(y[e]) : ffn_high(y[e]);
+                }
               }
               stage8(stage, lane, o / 8 + i, pack8(x));
               stage8(stage + kOutBlock, lane, o / 8 + i, pack8(y));
             }
             kept = next;
           }
-          store_block(&p.out[0], stage, col, row0, p);
-          store_block(&p.out[1], stage + kOutBlock, col, row0, p);
+          store_block(&p.out[2 * pass], stage, col, row0, p);
+          store_block(&p.out[2 * pass + 1], stage + kOutBlock, col, row0, p);
         }
       }
     }
@@ -618,8 +633,8 @@ __global__ void __launch_bounds__(kFfnThreads, 1)
     // The pairs of the cluster hold sums of the same tile over their parts of the inner length.  Quarter p of its
     // columns is finished by pair p splits / 4; the others send it theirs: [sender][column][row], in the stages'
     // memory, which no instruction reads any more after the first barrier.
-    const FfnUnit u = ffn_unit<kMode>(q, pair);
-    const FfnProblem& p = *u.p;
+    const auto u = ffn_unit<kMode>(q, pair);
+    const auto& p = *u.p;
     const int quad = warp & 3, part = (warp - 4) >> 2, owner = part * p.splits / 4;
     const uint32_t acc = tmem + (static_cast<uint32_t>(quad * 32) << 16) + 64 * part;
     const int row0 = u.m + 128 * static_cast<int>(rank) + 32 * quad;
@@ -755,13 +770,13 @@ struct FfnSpace {
 };
 
 // Shape part of a product (no pointers).
-FfnProblem ffn_product(long long rows, int cols, long long k0, long long k1) {
+FfnProblem ffn_product(long long rows, int cols, long long inner, int segments) {
   FfnProblem p = {};
   p.rows = static_cast<int>(rows);
   p.cols = cols;
   p.tiles_n = static_cast<int>(ffn_tiles(cols, 256));
-  p.steps[0] = ffn_steps(k0);
-  p.steps[1] = k1 ? ffn_steps(k1) : 0;
+  p.segments = segments;
+  p.steps = ffn_steps(inner);
   p.units = static_cast<int>(ffn_tiles(rows, 256) * p.tiles_n);
   p.splits = 1;
   return p;
@@ -769,7 +784,7 @@ FfnProblem ffn_product(long long rows, int cols, long long k0, long long k1) {
 
 // Splits it as one of `tiles` of its launch; what it needs is added to `space`.
 void ffn_split(FfnProblem* p, long long tiles, FfnSpace* space) {
-  p->splits = ffn_splits(tiles, p->steps[0] + p->steps[1]);
+  p->splits = ffn_splits(tiles, p->segments * p->steps);
   if (p->splits == 1) return;
   space->counters += static_cast<size_t>(p->units) * 2;
   p->units *= p->splits;
@@ -793,6 +808,17 @@ int ffn_launch(FfnParams<kCount>& q, cudaStream_t s, const char* what) {
   const cudaError_t set = cudaFuncSetAttribute(ffn_kernel<kMode, kAct, kCount>,
                                                cudaFuncAttributeMaxDynamicSharedMemorySize, kFfnSmem);
   if (set != cudaSuccess) return set_error(TS_ERR_CUDA, "%s: %s", what, cudaGetErrorString(set));
+  FfnParams<kCount, ffn_maps(kMode)> r;
+  for (int i = 0; i < q.count; ++i) {
+    static_cast<FfnSizes&>(r.p[i]) = q.p[i];
+    std::memcpy(r.p[i].a, q.p[i].a, sizeof(r.p[i].a));
+    std::memcpy(r.p[i].b, q.p[i].b, sizeof(r.p[i].b));
+    std::memcpy(r.p[i].out, q.p[i].out, sizeof(r.p[i].out));
+  }
+  r.count = q.count;
+  r.units = q.units;
+  r.clear = q.clear;
+  r.clear_count = q.clear_count;
   const int pairs = kMode == kProductCluster || q.units < kPairs ? q.units : kPairs;
   cudaLaunchAttribute attr[2] = {};
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -807,7 +833,7 @@ int ffn_launch(FfnParams<kCount>& q, cudaStream_t s, const char* what) {
   config.stream = s;
   config.attrs = attr;
   config.numAttrs = 2;
-  const cudaError_t e = cudaLaunchKernelEx(&config, ffn_kernel<kMode, kAct, kCount>, q);
+  const cudaError_t e = cudaLaunchKernelEx(&config, ffn_kernel<kMode, kAct, kCount>, r);
   if (e != cudaSuccess) return set_error(TS_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
   return check_launch(what);
 }
@@ -859,15 +885,19 @@ struct FfnBackward {
 
 FfnBackward ffn_backward(const ts_ffn_args* a) {
   FfnBackward b;
-  b.p[0] = ffn_product(a->hidden, a->width, a->rows, 0);
-  b.p[1] = ffn_product(a->hidden, a->width, a->rows, 0);
-  b.p[2] = ffn_product(a->width_out, a->hidden, a->rows, 0);
-  b.p[3] = ffn_product(a->rows, a->width, a->hidden, a->hidden);
-  // the weights' gradients, whose inner length is the tokens, come first and are split as one; dx takes what they leave
+  const int parts = ffn_parts(a->rows);   // of h, dg and du
+  b.p[0] = ffn_product(a->hidden, a->width, a->rows, parts);
+  b.p[1] = ffn_product(a->hidden, a->width, a->rows, parts);
+  b.p[2] = ffn_product(a->width_out, a->hidden, a->rows, parts);
+  b.p[3] = ffn_product(a->rows, a->width, a->hidden, 2 * parts);
+  // the weights' gradients, whose inner length is the tokens, come first and are split as one; dx takes what they
+  // leave, but for few rows is split as if alone: its few tiles, each the whole length of both parts, would end long
+  // after the others' (one row of 2048 x 5632, forward and backward: 196 us, split 106)
   const long long tiles = static_cast<long long>(b.p[0].units) + b.p[1].units + b.p[2].units;
   for (int i = 0; i < 3; ++i) ffn_split(&b.p[i], tiles, &b.space);
-  ffn_split(&b.p[3], static_cast<long long>(b.p[0].units) + b.p[1].units + b.p[2].units + b.p[3].units, &b.space);
-  const size_t one = ffn_align(ffn_hidden_bytes(a));
+  const long long before = static_cast<long long>(b.p[0].units) + b.p[1].units + b.p[2].units;
+  ffn_split(&b.p[3], (parts > 1 ? 0 : before) + b.p[3].units, &b.space);
+  const size_t one = ffn_align(ffn_hidden_bytes(a) * parts);
   b.du = one;
   b.partial = 2 * one;
   b.counters = b.partial + ffn_align(b.space.partial * 4);
@@ -883,7 +913,8 @@ FfnParams<1> ffn_gate(const ts_ffn_args* a, int tile, int inner) {
   p.rows = static_cast<int>(a->rows);
   p.cols = a->hidden;
   p.tiles_n = static_cast<int>(ffn_tiles(a->hidden, tile));
-  p.steps[0] = ffn_steps(inner);
+  p.segments = 1;
+  p.steps = ffn_steps(inner);
   p.splits = 1;
   p.units = static_cast<int>(ffn_tiles(a->rows, 256)) * p.tiles_n;
   p.kept = static_cast<uint8_t*>(a->kept);
@@ -904,7 +935,7 @@ size_t ts_b200_ffn_kept_bytes(const ts_ffn_args* a) {
 size_t ts_b200_ffn_fwd_workspace_bytes(const ts_ffn_args* a) {
   if (ts::ffn_check(a)) return 0;
   // h, where the caller keeps none; for few rows in two parts
-  return ts::ffn_align(ts::ffn_hidden_bytes(a) * (a->rows <= ts::kRowsMost ? 2 : 1));
+  return ts::ffn_align(ts::ffn_hidden_bytes(a) * ts::ffn_parts(a->rows));
 }
 
 int ts_b200_ffn_fwd(const ts_ffn_args* a, ts_stream_t stream) {
@@ -917,12 +948,12 @@ int ts_b200_ffn_fwd(const ts_ffn_args* a, ts_stream_t stream) {
     return set_error(TS_ERR_VALUE, "ffn_fwd: workspace too small");
   uint8_t* ws = static_cast<uint8_t*>(a->workspace);
   void* h = a->h ? a->h : ws;
-  if (a->rows <= kRowsMost && !a->kept) {
+  if (a->rows <= kRowsMost) {
     const auto bad = [](const void* base, long long stride) {
       return (reinterpret_cast<uintptr_t>(base) & 15) || stride % 8;
     };
     if (bad(a->x, a->x_stride) || bad(a->w_gate, a->w_gate_stride) || bad(a->w_up, a->w_up_stride) ||
-        bad(a->w_down, a->w_down_stride) || bad(a->y, 0) || bad(ws, 0))
+        bad(a->w_down, a->w_down_stride) || bad(a->y, 0) || bad(h, 0))
       return set_error(TS_ERR_VALUE, kFfnLayout);
     return ffn_rows_fwd(a, h, stream);
   }
@@ -932,8 +963,8 @@ int ts_b200_ffn_fwd(const ts_ffn_args* a, ts_stream_t stream) {
   FfnParams<1> down = {};
   down.count = 1;
   FfnProblem& d = down.p[0];
-  d = ffn_product(a->rows, a->width_out, a->hidden, 0);
-  d.splits = ffn_cluster_splits(d.units, d.steps[0]);
+  d = ffn_product(a->rows, a->width_out, a->hidden, 1);
+  d.splits = ffn_cluster_splits(d.units, d.steps);
   d.units *= d.splits;
   if (!ffn_map(&p.a[0], a->x, a->rows, a->width, a->x_stride, 128) ||
       !ffn_map(&p.b[0], a->w_gate, a->hidden, a->width, a->w_gate_stride, 128) ||
@@ -966,40 +997,53 @@ int ts_b200_ffn_bwd(const ts_ffn_args* a, const ts_ffn_grad_args* g, ts_stream_t
   const int D = a->width, H = a->hidden, O = a->width_out;
   FfnParams<1> gate = ffn_gate(a, 256, O);
   FfnProblem& p = gate.p[0];
+  const int parts = ffn_parts(M);
+  // a part of a [parts, rows, hidden] matrix
+  auto part_of = [&](const void* base, int part) {
+    return static_cast<const uint8_t*>(base) + part * ffn_hidden_bytes(a);
+  };
   bool ok = ffn_map(&p.a[0], g->dy, M, O, g->dy_stride, 128) &&
-            ffn_outer_map(&p.b[0], &p.b_layout, a->w_down, O, H, a->w_down_stride) &&
-            ffn_out_map(&p.out[0], dg, M, H) && ffn_out_map(&p.out[1], du, M, H);
+            ffn_outer_map(&p.b[0], &p.b_layout, a->w_down, O, H, a->w_down_stride);
+  for (int i = 0; i < parts && ok; ++i)
+    ok = ffn_out_map(&p.out[2 * i], part_of(dg, i), M, H) && ffn_out_map(&p.out[2 * i + 1], part_of(du, i), M, H);
   FfnParams<4> grads = {};
   float* partial = reinterpret_cast<float*>(ws + b.partial);
   int* counters = reinterpret_cast<int*>(ws + b.counters);
   gate.clear = counters;
   gate.clear_count = static_cast<int>(b.space.counters);
   // dWg = dg^T x, dWu = du^T x, dWd = dy^T h: the inner dimension is the tokens, outside in every operand
-  auto weight = [&](FfnProblem& w, const void* left, int left_cols, long long left_stride, const void* right,
-                    int right_cols, long long right_stride, void* out) {
+  // (`two_left`, `two_right`: the operand that is in parts)
+  auto weight = [&](FfnProblem& w, const void* left, int left_cols, long long left_stride, bool two_left,
+                    const void* right, int right_cols, long long right_stride, bool two_right, void* out) {
     if (!out) return true;
     ffn_place(&w, partial, counters);
-    const bool mapped = ffn_outer_map(&w.a[0], &w.a_layout, left, M, left_cols, left_stride) &&
-                        ffn_outer_map(&w.b[0], &w.b_layout, right, M, right_cols, right_stride) &&
-                        ffn_out_map(&w.out[0], out, left_cols, right_cols);
+    bool mapped = ffn_out_map(&w.out[0], out, left_cols, right_cols);
+    for (int i = 0; i < parts && mapped; ++i)
+      mapped = ffn_outer_map(&w.a[i], &w.a_layout, two_left ? part_of(left, i) : left, M, left_cols, left_stride) &&
+               ffn_outer_map(&w.b[i], &w.b_layout, two_right ? part_of(right, i) : right, M, right_cols, right_stride);
     grads.p[grads.count++] = w;
     return mapped;
   };
-  ok = ok && weight(b.p[0], dg, H, H, a->x, D, a->x_stride, g->dw_gate) &&
-       weight(b.p[1], du, H, H, a->x, D, a->x_stride, g->dw_up) &&
-       weight(b.p[2], g->dy, O, g->dy_stride, a->h, H, H, g->dw_down);
+  ok = ok && weight(b.p[0], dg, H, H, true, a->x, D, a->x_stride, false, g->dw_gate) &&
+       weight(b.p[1], du, H, H, true, a->x, D, a->x_stride, false, g->dw_up) &&
+       weight(b.p[2], g->dy, O, g->dy_stride, false, a->h, H, H, true, g->dw_down);
   if (ok && g->dx) {
     FfnProblem& x = b.p[3];
     ffn_place(&x, partial, counters);
-    ok = ffn_map(&x.a[0], dg, M, H, H, 128) && ffn_map(&x.a[1], du, M, H, H, 128) &&
-         ffn_outer_map(&x.b[0], &x.b_layout, a->w_gate, H, D, a->w_gate_stride) &&
-         ffn_outer_map(&x.b[1], &x.b_layout, a->w_up, H, D, a->w_up_stride) && ffn_out_map(&x.out[0], g->dx, M, D);
+    ok = ffn_out_map(&x.out[0], g->dx, M, D);
+    for (int i = 0; i < parts && ok; ++i)
+      ok = ffn_map(&x.a[2 * i], part_of(dg, i), M, H, H, 128) && ffn_map(&x.a[2 * i + 1], part_of(du, i), M, H, H, 128) &&
+           ffn_outer_map(&x.b[2 * i], &x.b_layout, a->w_gate, H, D, a->w_gate_stride) &&
+           ffn_outer_map(&x.b[2 * i + 1], &x.b_layout, a->w_up, H, D, a->w_up_stride);
     grads.p[grads.count++] = x;
   }
   if (!ok) return set_error(TS_ERR_VALUE, kFfnLayout);
   if (grads.count == 0) return TS_OK;
-  if (const int rc = ffn_launch_gate<kGateGrad>(gate, a->activation, stream, "ffn_gate_grad")) return rc;
-  return ffn_launch<kProduct, 0>(grads, stream, "ffn_grads");
+  if (const int rc = parts > 1 ? ffn_launch_gate<kGateGradTwo>(gate, a->activation, stream, "ffn_gate_grad")
+                               : ffn_launch_gate<kGateGrad>(gate, a->activation, stream, "ffn_gate_grad"))
+    return rc;
+  return parts > 1 ? ffn_launch<kProductTwo, 0>(grads, stream, "ffn_grads")
+                   : ffn_launch<kProduct, 0>(grads, stream, "ffn_grads");
 }
 
 }  // extern "C"

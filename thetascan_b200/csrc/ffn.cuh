@@ -11,10 +11,34 @@ namespace ts {
 // At 1024 x 4096 and 1 / 16 / 32 rows this takes 8.8 / 13.0 / 13.9 us, the
 // tiles 26 / 25 / 25; at 2048 x 5632 21.7 / 25.9 / 31.7 us, the tiles 39 / 35 /
 // 34, and 34 still at 48 and 64 rows, where this would read x and h once more.
-constexpr int kRowsMost = 32;
+constexpr int kRowsMost = TS_FFN_TWO_PART_ROWS;
+
+// bf16 parts of h, dg and du of a call (ffn_high, ffn_rest).
+constexpr int ffn_parts(long long rows) { return rows <= kRowsMost ? 2 : 1; }
 
 // The forward for few rows; arguments checked, h holds [2, rows, hidden].
 int ffn_rows_fwd(const ts_ffn_args* a, void* h, cudaStream_t s);
+
+// g and u kept for a backward pass: blocks of 32 rows x 32 columns, a lane's
+// row as twelve 16-byte vectors [vector][lane] (a warp's access is 512
+// contiguous bytes); for each half of 16 columns: the upper halves of g's words,
+// two vectors, their third bytes, one vector, and the same of u.
+__device__ __forceinline__ uint8_t* keep_at(uint8_t* base, int cols, int row, int col, int lane) {
+  const size_t blocks = static_cast<size_t>((cols + 31) >> 5);
+  return base + ((row >> 5) * blocks + (col >> 5)) * TS_FFN_KEPT_BLOCK + 16 * lane;
+}
+// One place of them.
+__device__ __forceinline__ void keep_one(uint8_t* base, int cols, int row, int col, float g, float u) {
+  uint8_t* half = keep_at(base, cols, row, col, row & 31) + ((col >> 4) & 1) * (6 * 512);
+  const int c = col & 15;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t word = __float_as_uint(i ? u : g);
+    uint8_t* to = half + 3 * 512 * i;
+    reinterpret_cast<uint16_t*>(to + 512 * (c >> 3))[c & 7] = static_cast<uint16_t>(word >> 16);
+    to[2 * 512 + c] = static_cast<uint8_t>(word >> 8);
+  }
+}
 
 // A value in two bf16 parts, within 2^-16 of it: its upper half, and what is
 // left.  Cut off and not rounded, so that both parts have the value's sign, and

@@ -1,4 +1,5 @@
-// The gated feed-forward block for few rows (decoding steps), forward only.
+// The gated feed-forward block for few rows (decoding steps): the forward,
+// which keeps g and u where a backward pass follows (ffn.cu).
 //
 // With up to kRowsMost rows the weights are read once for almost no
 // arithmetic (6 D H bytes against 6 M D H operations), so what counts is to
@@ -43,6 +44,7 @@ struct FfnRowsParams {
   const __nv_bfloat16 *x, *wg, *wu, *wd;
   long long xs, wgs, wus, wds;
   __nv_bfloat16 *h, *y;      // h: [2][rows][hidden]
+  uint8_t* kept;             // g and u (keep_at), or null
   int rows, width, hidden, out;
 };
 
@@ -164,6 +166,7 @@ __global__ void __launch_bounds__(32 * kRowsWarps) ffn_rows_gate_kernel(const Ff
       __nv_bfloat16* to = p.h + static_cast<long long>(row + i) * p.hidden + j;
       *to = __float2bfloat16_rn(ffn_high(h[i]));
       to[static_cast<long long>(p.rows) * p.hidden] = __float2bfloat16_rn(ffn_rest(h[i]));
+      if (p.kept) keep_one(p.kept, p.hidden, row + i, j, i ? s.y : s.x, i ? s.w : s.z);
     }
   }
 }
@@ -290,6 +293,7 @@ int ffn_rows_fwd(const ts_ffn_args* a, void* h, cudaStream_t s) {
   p.wds = a->w_down_stride;
   p.h = static_cast<__nv_bfloat16*>(h);
   p.y = static_cast<__nv_bfloat16*>(a->y);
+  p.kept = static_cast<uint8_t*>(a->kept);
   p.rows = static_cast<int>(a->rows);
   p.width = a->width;
   p.hidden = a->hidden;

@@ -275,6 +275,9 @@ struct FfnOut {
   Tensor y, h, kept;
 };
 
+// bf16 parts that h is kept in.
+int64_t h_parts(int64_t rows) { return rows <= TS_FFN_TWO_PART_ROWS ? 2 : 1; }
+
 int64_t kept_bytes(int64_t rows, int64_t hidden) {
   return (rows + 31) / 32 * ((hidden + 31) / 32) * TS_FFN_KEPT_BLOCK;
 }
@@ -287,7 +290,7 @@ FfnOut ffn_run(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor
   o.y = at::empty(shape, x.options());
   const int64_t rows = x.numel() / x.size(-1), hidden = wg.size(0);
   if (keep) {
-    o.h = at::empty({rows, hidden}, x.options());
+    o.h = at::empty({h_parts(rows) * rows, hidden}, x.options());
     o.kept = at::empty({kept_bytes(rows, hidden)}, x.options().dtype(at::kByte));
   }
   if (x.numel() == 0) return o;
@@ -312,7 +315,7 @@ std::vector<Tensor> ffn_grads(const Tensor& dy, const Tensor& x, const Tensor& w
   TORCH_CHECK_VALUE(dy.scalar_type() == at::kBFloat16 && dy.dim() == x.dim() && dy.size(-1) == wd.size(0) &&
                         dy.numel() == rows * wd.size(0),
                     "dy must be bfloat16 and of the output's shape, got ", dy.scalar_type(), " ", dy.sizes());
-  TORCH_CHECK_VALUE(h.scalar_type() == at::kBFloat16 && h.is_contiguous() && h.numel() == rows * hidden &&
+  TORCH_CHECK_VALUE(h.scalar_type() == at::kBFloat16 && h.is_contiguous() && h.numel() == h_parts(rows) * rows * hidden &&
                         kept.scalar_type() == at::kByte && kept.is_contiguous() &&
                         kept.numel() == kept_bytes(rows, hidden),
                     "h and kept must be what the forward of these inputs kept");

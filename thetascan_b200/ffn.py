@@ -5,17 +5,18 @@
 
 The kernels (``csrc/ffn.cu``) form both projections, the activation and the
 product in one launch and the down projection in a second.  For a backward
-pass the block keeps its input and 8 bytes per hidden value: ``h`` in bf16 and
-both projections in 24 bits.  bf16 operands, f32 accumulators.  Any number of
+pass the block keeps its input and 8 bytes per hidden value (10 with up to 32
+rows): ``h`` in bf16 and both projections in 24 bits.  bf16 operands, f32 accumulators.  Any number of
 rows; widths that are multiples of 8.
 
 What is rounded on the way: ``h`` to bf16 between the two launches, and ``dg``
 and ``du`` in the backward, as operands of the next product.  A result's error
 is then 2.35e-3 of its norm, where its own rounding to bf16 alone is 1.66e-3.
-Inference with up to 32 rows is bound by the weights' traffic and passes ``h``
-in two bf16 parts, which leaves the result's own rounding alone; so the same
-row comes out the same within that rounding, not to the bit, from a call with
-more rows or with gradients.  A compiled call computes what the eager one does.
+With up to 32 rows, where a few large hidden values may carry a result, each of
+the three passes in two bf16 parts, which leaves the result's own rounding
+alone; so the same row comes out the same within that rounding, not to the bit,
+from a call with more rows.  The output does not depend on whether gradients are
+wanted, and a compiled call computes what the eager one does.
 """
 from __future__ import annotations
 
@@ -30,6 +31,7 @@ from . import _lib
 LIB = "thetascan_b200"
 ACTIVATIONS = ("gelu", "relu2", "silu")
 KEPT_BLOCK = 6144   # bytes kept for each 32 rows x 32 hidden columns
+TWO_PART_ROWS = 32  # rows up to which h is kept in two parts
 
 
 def _kept_bytes(rows, hidden):
@@ -51,7 +53,8 @@ def gated_ffn_fwd(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, activ
 @gated_ffn_fwd.register_fake
 def _(x, w_gate, w_up, w_down, activation, keep):
     rows, hidden = x.numel() // x.shape[-1], w_gate.shape[0]
-    return (x.new_empty(*x.shape[:-1], w_down.shape[0]), x.new_empty((rows, hidden) if keep else (0,)),
+    parts = 2 if rows <= TWO_PART_ROWS else 1
+    return (x.new_empty(*x.shape[:-1], w_down.shape[0]), x.new_empty((parts * rows, hidden) if keep else (0,)),
             x.new_empty(_kept_bytes(rows, hidden) if keep else 0, dtype=torch.uint8))
 
 

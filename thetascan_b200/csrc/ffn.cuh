@@ -8,7 +8,7 @@ namespace ts {
 
 // Rows up to which an inference call streams the weights past the rows
 // (ffn_rows.cu) instead of forming tiles of 256 rows (ffn.cu).
-// At 1024 x 4096 and 1 / 16 / 32 rows this takes 8.8 / 13.0 / 13.9 us, the
+// At 1024 x 4096 and 1 / 16 / 32 rows this takes 8.8 / 13.3 / 13.9 us, the
 // tiles 26 / 25 / 25; at 2048 x 5632 21.7 / 25.9 / 31.7 us, the tiles 39 / 35 /
 // 34, and 34 still at 48 and 64 rows, where this would read x and h once more.
 constexpr int kRowsMost = TS_FFN_TWO_PART_ROWS;

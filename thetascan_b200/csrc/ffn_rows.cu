@@ -138,7 +138,9 @@ __device__ __forceinline__ float4 rows_sum(const float (&c)[kTiles][4], float4* 
   return sum;
 }
 
-template <int kSets, int kTiles, int kAct>
+// kKeep: g and u are kept.  An instance of its own: with both in one the compiler holds fewer loads in flight (86
+// registers for 108; 2048 x 5632, 32 rows: 49 us for 32).
+template <int kSets, int kTiles, int kAct, bool kKeep>
 __global__ void __launch_bounds__(32 * kRowsWarps) ffn_rows_gate_kernel(const FfnRowsParams p) {
   constexpr int kAll = kSets * kTiles;
   __shared__ float4 part[kRowsWarps * kAll * 32];
@@ -166,7 +168,7 @@ __global__ void __launch_bounds__(32 * kRowsWarps) ffn_rows_gate_kernel(const Ff
       __nv_bfloat16* to = p.h + static_cast<long long>(row + i) * p.hidden + j;
       *to = __float2bfloat16_rn(ffn_high(h[i]));
       to[static_cast<long long>(p.rows) * p.hidden] = __float2bfloat16_rn(ffn_rest(h[i]));
-      if (p.kept) keep_one(p.kept, p.hidden, row + i, j, i ? s.y : s.x, i ? s.w : s.z);
+      if (kKeep) keep_one(p.kept, p.hidden, row + i, j, i ? s.y : s.x, i ? s.w : s.z);
     }
   }
 }
@@ -227,15 +229,15 @@ __global__ void __launch_bounds__(32 * kRowsWarps) ffn_rows_down_kernel(const Ff
   }
 }
 
-template <int kSets, int kTiles>
+template <int kSets, int kTiles, bool kKeep>
 int ffn_rows_gate(const FfnRowsParams& p, int activation, cudaStream_t s) {
   const int grid = (p.hidden + 8 * kSets - 1) / (8 * kSets), threads = 32 * kRowsWarps;
   if (activation == TS_FFN_SILU) {
-    ffn_rows_gate_kernel<kSets, kTiles, TS_FFN_SILU><<<grid, threads, 0, s>>>(p);
+    ffn_rows_gate_kernel<kSets, kTiles, TS_FFN_SILU, kKeep><<<grid, threads, 0, s>>>(p);
   } else if (activation == TS_FFN_GELU) {
-    ffn_rows_gate_kernel<kSets, kTiles, TS_FFN_GELU><<<grid, threads, 0, s>>>(p);
+    ffn_rows_gate_kernel<kSets, kTiles, TS_FFN_GELU, kKeep><<<grid, threads, 0, s>>>(p);
   } else {
-    ffn_rows_gate_kernel<kSets, kTiles, TS_FFN_RELU2><<<grid, threads, 0, s>>>(p);
+    ffn_rows_gate_kernel<kSets, kTiles, TS_FFN_RELU2, kKeep><<<grid, threads, 0, s>>>(p);
   }
   return check_launch("ffn_rows_gate");
 }
@@ -265,15 +267,18 @@ int ffn_rows_down(const FfnRowsParams& p, cudaStream_t s) {
 
 // Two sets of weight rows to a warp read x half as often, one set has twice the
 // CTAs: two where there are several tiles of rows and CTAs enough all the same
-// (2048 x 5632, 9 / 16 / 32 rows: 25.8 / 25.9 / 31.7 us with two, 27.4 / 29.7 /
-// 37.5 with one; 1024 x 4096: 12.7 / 12.9 / 13.9 and 12.1 / 12.9 / 17.9).
+// (2048 x 5632, 9 / 16 / 32 rows: 25.9 / 25.9 / 31.7 us with two, 27.3 / 29.7 /
+// 37.6 with one; 1024 x 4096: 13.1 / 13.3 / 13.9 and 12.1 / 12.9 / 17.8).
 constexpr int kRowsCtas = 148;
 
 template <int kTiles>
 int ffn_rows_launch(const FfnRowsParams& p, int activation, cudaStream_t s) {
   constexpr int kSets = kTiles > 1 ? 2 : 1;
-  const int rc = p.hidden / (8 * kSets) >= kRowsCtas ? ffn_rows_gate<kSets, kTiles>(p, activation, s)
-                                                     : ffn_rows_gate<1, kTiles>(p, activation, s);
+  const bool wide = p.hidden / (8 * kSets) >= kRowsCtas;
+  const int rc = p.kept ? (wide ? ffn_rows_gate<kSets, kTiles, true>(p, activation, s)
+                                : ffn_rows_gate<1, kTiles, true>(p, activation, s))
+                        : (wide ? ffn_rows_gate<kSets, kTiles, false>(p, activation, s)
+                                : ffn_rows_gate<1, kTiles, false>(p, activation, s));
   if (rc) return rc;
   return p.out / (16 * kSets) * rows_ranks(kSets * kTiles) >= kRowsCtas ? ffn_rows_down<kSets, kTiles>(p, s)
                                                         : ffn_rows_down<1, kTiles>(p, s);

@@ -36,7 +36,9 @@ def _require(ok, message):
 
 
 def _require_options(lr, betas, eps, weight_decay):
-    _require(all(0 <= b < 1 for b in betas), f"betas must lie in [0, 1), got {betas}")
+    b1, b2 = betas
+    if not (0 <= b1 < 1 and 0 <= b2 < 1):
+        raise ValueError(f"adamw: betas must lie in [0, 1), got {betas}")
     _require(lr >= 0 and eps >= 0 and weight_decay >= 0, "lr, eps and weight_decay must be >= 0")
 
 
@@ -52,7 +54,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step: int, lr: float, be
     ``state_scales(numel)`` entries.  ``step`` counts from 1; ``ordinals`` are
     the tensors' places in the whole step (default 0, 1, ...), which key the
     stochastic rounding of 8-bit states with ``seed``."""
-    _require(isinstance(step, int) and step >= 1, f"step must be an integer >= 1, got {step!r}")
+    if not (isinstance(step, int) and step >= 1):
+        raise ValueError(f"adamw: step must be an integer >= 1, got {step!r}")
     _require_options(lr, betas, eps, weight_decay)
     b1, b2 = betas
     _lib.host().adamw(params, grads, exp_avgs, exp_avg_sqs, masters, exp_avg_scales, exp_avg_sq_scales, ordinals, step, lr,

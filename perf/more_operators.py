@@ -205,13 +205,12 @@ def _own_attention(s):
     with torch.no_grad():
         if case["mode"] == "token":
             y = window_attention_step(s["q"], s["k"], s["v"], s["keys"], s["values"], s["lengths"], sinks)
-            return y, s["keys"], s["values"], s["lengths"]
+            return y, s["keys"], s["values"]
         y = window_attention(s["q"], s["k"], s["v"], window, sinks, lengths=s["lengths"])
         if case["mode"] == "piece":
             return y
-        s["filled"].zero_()
         window_cache_extend(s["k"], s["v"], s["keys"], s["values"], s["filled"], sinks, new=s["lengths"])
-        return y, s["keys"], s["values"], s["filled"]
+        return y, s["keys"], s["values"]
 
 
 def _plain_window(q, k, v, window, sinks, lengths):
@@ -255,7 +254,6 @@ def _plain_extend(k, v, keys, values, filled, sinks, new):
     index = source.clamp(0, n - 1)[:, None, :, None].expand(b, k.shape[1], slots, k.shape[3])
     keys.copy_(torch.where(fresh, k.gather(2, index), keys))
     values.copy_(torch.where(fresh, v.gather(2, index), values))
-    filled.copy_(after)
 
 
 def _plain_attention(s):
@@ -270,20 +268,18 @@ def _plain_attention(s):
         row = torch.arange(b, device=q.device)
         slot = torch.where(lengths < sinks, lengths, sinks + (lengths - sinks) % window).long()
         keys[row, :, slot], values[row, :, slot] = s["k"][:, :, 0], s["v"][:, :, 0]
-        lengths += 1
-        seen = (torch.arange(keys.shape[2], device=q.device) < lengths[:, None])[:, None, None]
+        seen = (torch.arange(keys.shape[2], device=q.device) <= lengths[:, None])[:, None, None]
         scores = q.float().reshape(b, keys.shape[1], -1, d) @ keys.float().transpose(-1, -2) * (1 / math.sqrt(d))
         scores = scores.masked_fill(~seen, -math.inf)
         p = torch.exp(scores - scores.amax(-1, keepdim=True))
         y = p @ values.float() / p.sum(-1, keepdim=True)
-        return y.reshape(b, h, 1, d).to(q.dtype), keys, values, lengths
+        return y.reshape(b, h, 1, d).to(q.dtype), keys, values
     with torch.no_grad():
         y = _plain_window(s["q"], s["k"], s["v"], window, sinks, s["lengths"])
     if case["mode"] == "piece":
         return y
-    s["filled"].zero_()
     _plain_extend(s["k"], s["v"], s["keys"], s["values"], s["filled"], sinks, s["lengths"])
-    return y, s["keys"], s["values"], s["filled"]
+    return y, s["keys"], s["values"]
 
 
 def _own_scan(s):
@@ -429,7 +425,7 @@ def _exact_attention(s):
             buffer[i, :, :min(sinks, length)] = new[i, :, :min(sinks, length)].double()
             kept = torch.arange(max(sinks, length - window), max(sinks, length), device=q.device)
             buffer[i, :, sinks + (kept - sinks) % window] = new[i, :, kept].double()
-    return y, keys, values, torch.tensor(lengths, dtype=torch.int32, device=q.device)
+    return y, keys, values
 
 
 def _exact_token(s):
@@ -439,13 +435,12 @@ def _exact_token(s):
     for i, n in enumerate(lengths):
         slot = n if n < sinks else sinks + (n - sinks) % window
         keys[i, :, slot], values[i, :, slot] = s["k"][i, :, 0], s["v"][i, :, 0]
-        lengths[i] = n + 1
         seen = min(n + 1, sinks + window)
         for head in range(case["kv_heads"]):
             heads = slice(head * share, (head + 1) * share)
             logits = torch.einsum("hd,kd->hk", s["q"][i, heads, 0].double(), keys[i, head, :seen].double()) / case["dim"] ** 0.5
             y[i, heads, 0] = torch.einsum("hk,kd->hd", torch.softmax(logits, -1), values[i, head, :seen].double())
-    return y, keys.double(), values.double(), torch.tensor(lengths, dtype=torch.int32, device=y.device)
+    return y, keys.double(), values.double()
 
 
 def _exact_scan(s):

@@ -24,12 +24,23 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   return fn;
 }
 
+// The encoder wants the device's context current in the calling thread, which a thread that has made no runtime call
+// yet (a backward pass's first operator) has not.
+bool context_here() {
+  thread_local int ready = -1;
+  int device = -1;
+  if (cudaGetDevice(&device) != cudaSuccess) return false;
+  if (device != ready && cudaSetDevice(device) != cudaSuccess) return false;
+  ready = device;
+  return true;
+}
+
 }  // namespace
 
 bool make_tmap_bf16(CUtensorMap* map, const void* base, int rank, const uint64_t* dims, const int64_t* strides,
                     const uint32_t* box, CUtensorMapSwizzle swizzle) {
   const PFN_cuTensorMapEncodeTiled_v12000 encode = encode_fn();
-  if (encode == nullptr || rank < 2 || rank > 5) return false;
+  if (encode == nullptr || rank < 2 || rank > 5 || !context_here()) return false;
   if (reinterpret_cast<uintptr_t>(base) % 16 != 0) return false;
   cuuint64_t gdim[5], gstride[4];
   cuuint32_t bdim[5], estride[5];

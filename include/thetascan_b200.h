@@ -659,6 +659,135 @@ int ts_b200_ffn_fwd(const ts_ffn_args* args, ts_stream_t stream);
 size_t ts_b200_ffn_bwd_workspace_bytes(const ts_ffn_args* args);
 int ts_b200_ffn_bwd(const ts_ffn_args* args, const ts_ffn_grad_args* grads, ts_stream_t stream);
 
+/* ---------------------------------------------------------------- window
+ * Causal attention over a sliding window with first tokens that stay visible:
+ *   y_i = sum_j softmax_j(scale q_i.k_j) v_j
+ * over the keys j <= i with i - j < window or j < sinks, i and j below the
+ * sequence's length; rows that see nothing are zero.  The queries are the last
+ * q_tokens of kv_tokens positions.  heads / kv_heads query heads share a key
+ * head.  bf16 [batch, heads, tokens, dim] with any strides that are multiples
+ * of 8 elements, contiguous channels and 16-byte aligned bases; dim a multiple
+ * of 8 up to 128.  No reference counterpart (its host model's attention). */
+typedef struct ts_window_args {
+  int batch, heads, kv_heads, dim;
+  int q_tokens, kv_tokens;
+  int window, sinks;
+  float scale;              /* > 0 */
+  const void* q;
+  const void* k;
+  const void* v;
+  long long q_strides[3], k_strides[3], v_strides[3];   /* batch, head, token; elements */
+  const int* lengths;       /* [batch] on the device, or NULL: kv_tokens each */
+  void* y;
+  long long y_strides[3];
+  float* lse;               /* [batch, heads, q_tokens rounded up to 128]: written by the forward (NULL in inference),
+                             * read by the backward */
+} ts_window_args;
+
+typedef struct ts_window_grad_args {
+  const void* dy;
+  long long dy_strides[3];
+  void* dq;                 /* all three are written, zeros where nothing is seen; channels contiguous */
+  void* dk;
+  void* dv;
+  long long dq_strides[3], dk_strides[3], dv_strides[3];
+  void* workspace;          /* 16-byte aligned */
+  size_t workspace_bytes;
+} ts_window_grad_args;
+
+int ts_b200_window_fwd(const ts_window_args* args, ts_stream_t stream);
+size_t ts_b200_window_bwd_workspace_bytes(const ts_window_args* args);
+int ts_b200_window_bwd(const ts_window_args* args, const ts_window_grad_args* grads, ts_stream_t stream);
+
+/* The same attention for one new token of each sequence, over a ring cache of
+ * sinks + window slots: position j lies in slot j below sinks, in slot
+ * sinks + (j - sinks) mod window above.  `lengths` counts the tokens before the
+ * new one (negative: no sequence; nothing is written and y is zero) and is not
+ * changed: the layers of a model share it.  window_extend copies new tokens (the
+ * first fresh[b] of each row, or all) into the cache behind those lengths. */
+typedef struct ts_window_cache {
+  int batch, kv_heads, dim;
+  int window, sinks;
+  void* keys;               /* bf16 [batch, kv_heads, sinks + window, dim], strides multiples of 8, bases of 16 bytes */
+  void* values;
+  long long keys_strides[3], values_strides[3];   /* batch, head, slot */
+  const int* lengths;       /* [batch] on the device */
+} ts_window_cache;
+
+typedef struct ts_window_step_args {
+  ts_window_cache cache;
+  int heads;
+  float scale;
+  const void* q;            /* bf16 [batch, heads, dim], k and v [batch, kv_heads, dim] */
+  const void* k;
+  const void* v;
+  long long q_strides[2], k_strides[2], v_strides[2];   /* batch, head */
+  void* y;                  /* [batch, heads, dim] contiguous */
+} ts_window_step_args;
+
+typedef struct ts_window_extend_args {
+  ts_window_cache cache;
+  int tokens;
+  const void* k;            /* bf16 [batch, kv_heads, tokens, dim] */
+  const void* v;
+  long long k_strides[3], v_strides[3];   /* batch, head, token */
+  const int* fresh;         /* [batch] on the device, or NULL */
+} ts_window_extend_args;
+
+int ts_b200_window_step(const ts_window_step_args* args, ts_stream_t stream);
+int ts_b200_window_extend(const ts_window_extend_args* args, ts_stream_t stream);
+
+/* The scan for one new token of each sequence, its state updated in place:
+ * S <- exp(log_alpha) S + k^T [v | 1], out = q S, for each retention.  The state
+ * is what ts_b200_scan_fwd leaves as final_state. */
+typedef struct ts_scan_step_args {
+  int batch, heads;
+  int dk, dv;               /* 1..256; dv counts the appended unit column */
+  int v_append_unit;        /* 0 or 1 */
+  int dtype;                /* of q, k, v, out */
+  const void* q;            /* [batch, heads, dk] */
+  const void* k;
+  const void* v;            /* [batch, heads, dv - v_append_unit] */
+  long long q_strides[2], k_strides[2], v_strides[2];   /* batch, head; channels contiguous */
+  int n_retentions;
+  const float* log_alpha[TS_MAX_RETENTIONS];            /* [heads] of each sequence, or NULL: the plain sum */
+  long long log_alpha_batch[TS_MAX_RETENTIONS];         /* elements between sequences, 0: one for all */
+  float* state;             /* [batch, heads, n_retentions, dk, dv] contiguous */
+  void* out;                /* [n_retentions, batch, heads, dv] contiguous */
+} ts_scan_step_args;
+
+int ts_b200_scan_step(const ts_scan_step_args* args, ts_stream_t stream);
+
+/* ---------------------------------------------------------------- sample
+ * A token for each row of logits: softmax(logits / temperature), the top_k
+ * tokens (lower index first among equals), of these the shortest prefix with
+ * top_p of their mass, of these the ones with min_p times the largest
+ * probability; then the first token, by index, at which the running mass exceeds
+ * uniform times its total.  Settings are one value for all rows, or a device
+ * array with one for each.  A temperature that is not above 0 takes the largest
+ * logit.  NaN and minus infinity are masked tokens; a row of nothing else gives
+ * -1.  logprobs: log softmax(logits / temperature) of the token, before the
+ * filters (at temperature 1 for a greedy row). */
+typedef struct ts_sample_args {
+  int rows, vocab;
+  int dtype;                /* of the logits */
+  const void* logits;       /* [rows, vocab], contiguous tokens */
+  long long row_stride;     /* elements */
+  const float* uniform;     /* [rows], in [0, 1) */
+  const float* temperature; /* [rows], or NULL: temperature_value */
+  double temperature_value;
+  const int* top_k;         /* [rows], or NULL: top_k_value; 0 or less: off */
+  int top_k_value;
+  const float* top_p;       /* 1 or more: off; 0 or less: the first token */
+  double top_p_value;
+  const float* min_p;       /* 0 or less: off */
+  double min_p_value;
+  long long* tokens;        /* [rows] */
+  float* logprobs;          /* [rows], or NULL */
+} ts_sample_args;
+
+int ts_b200_sample(const ts_sample_args* args, ts_stream_t stream);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif

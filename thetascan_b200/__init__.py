@@ -9,6 +9,9 @@ Public surface (mirrors the reference package ``thetascan``):
 * ``rms_norm`` / ``add_rms_norm`` / ``rms_norm_8bit``: the norms around it;
 * ``gated_ffn`` / ``GatedFFN``: the gated feed-forward block;
 * ``AdamW`` / ``adamw_step``: the optimizer step over many tensors;
+* ``window_attention`` / ``window_attention_step`` / ``window_cache_extend`` /
+  ``WindowCache``: attention over a sliding window, and its ring cache;
+* ``sample_tokens``: the choice of a token from logits;
 * ``integration.install()``: register ``backend="b200"`` in an installed
   reference package.
 
@@ -22,10 +25,13 @@ from .ffn import GatedFFN, gated_ffn
 from .mixer import ThetaScan
 from .norm import add_rms_norm, rms_norm, rms_norm_8bit
 from .optim import AdamW, adamw_step
+from .sample import sample_tokens
+from .window import WindowCache, window_attention, window_attention_step, window_cache_extend
 
 __version__ = "0.1.0"
 BACKEND_NAME = "b200"
 
 __all__ = ["GNConfig", "KernelConfig", "RegularizationConfig", "RoPEConfig", "RuntimeConfig",
            "TemporalConfig", "ThetaScan", "ThetaScanConfig", "BACKEND_NAME",
-           "AdamW", "GatedFFN", "adamw_step", "add_rms_norm", "gated_ffn", "rms_norm", "rms_norm_8bit"]
+           "AdamW", "GatedFFN", "WindowCache", "adamw_step", "add_rms_norm", "gated_ffn", "rms_norm", "rms_norm_8bit",
+           "sample_tokens", "window_attention", "window_attention_step", "window_cache_extend"]

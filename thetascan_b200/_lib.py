@@ -267,6 +267,90 @@ _host = None
 class ThetaScanB200Error(RuntimeError):
     """A CUDA-side failure reported by the library."""
 
+c_longlong_2, c_longlong_3 = ctypes.c_longlong * 2, ctypes.c_longlong * 3
+
+
+class WindowArgs(ctypes.Structure):
+    _fields_ = [
+        *((n, ctypes.c_int) for n in ("batch", "heads", "kv_heads", "dim", "q_tokens", "kv_tokens", "window", "sinks")),
+        ("scale", ctypes.c_float),
+        ("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+        ("q_strides", c_longlong_3), ("k_strides", c_longlong_3), ("v_strides", c_longlong_3),
+        ("lengths", ctypes.c_void_p),
+        ("y", ctypes.c_void_p), ("y_strides", c_longlong_3),
+        ("lse", ctypes.c_void_p),
+    ]
+
+
+class WindowGradArgs(ctypes.Structure):
+    _fields_ = [
+        ("dy", ctypes.c_void_p), ("dy_strides", c_longlong_3),
+        ("dq", ctypes.c_void_p), ("dk", ctypes.c_void_p), ("dv", ctypes.c_void_p),
+        ("dq_strides", c_longlong_3), ("dk_strides", c_longlong_3), ("dv_strides", c_longlong_3),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class WindowCacheArgs(ctypes.Structure):
+    _fields_ = [
+        *((n, ctypes.c_int) for n in ("batch", "kv_heads", "dim", "window", "sinks")),
+        ("keys", ctypes.c_void_p), ("values", ctypes.c_void_p),
+        ("keys_strides", c_longlong_3), ("values_strides", c_longlong_3),
+        ("lengths", ctypes.c_void_p),
+    ]
+
+
+class WindowStepArgs(ctypes.Structure):
+    _fields_ = [
+        ("cache", WindowCacheArgs), ("heads", ctypes.c_int), ("scale", ctypes.c_float),
+        ("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+        ("q_strides", c_longlong_2), ("k_strides", c_longlong_2), ("v_strides", c_longlong_2),
+        ("y", ctypes.c_void_p),
+    ]
+
+
+class WindowExtendArgs(ctypes.Structure):
+    _fields_ = [
+        ("cache", WindowCacheArgs), ("tokens", ctypes.c_int),
+        ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+        ("k_strides", c_longlong_3), ("v_strides", c_longlong_3),
+        ("fresh", ctypes.c_void_p),
+    ]
+
+
+class ScanStepArgs(ctypes.Structure):
+    _fields_ = [
+        *((n, ctypes.c_int) for n in ("batch", "heads", "dk", "dv", "v_append_unit", "dtype")),
+        ("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+        ("q_strides", c_longlong_2), ("k_strides", c_longlong_2), ("v_strides", c_longlong_2),
+        ("n_retentions", ctypes.c_int),
+        ("log_alpha", c_ptr4), ("log_alpha_batch", ctypes.c_longlong * MAX_RETENTIONS),
+        ("state", ctypes.c_void_p), ("out", ctypes.c_void_p),
+    ]
+
+
+class SampleArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", ctypes.c_int), ("vocab", ctypes.c_int), ("dtype", ctypes.c_int),
+        ("logits", ctypes.c_void_p), ("row_stride", ctypes.c_longlong), ("uniform", ctypes.c_void_p),
+        ("temperature", ctypes.c_void_p), ("temperature_value", ctypes.c_double),
+        ("top_k", ctypes.c_void_p), ("top_k_value", ctypes.c_int),
+        ("top_p", ctypes.c_void_p), ("top_p_value", ctypes.c_double),
+        ("min_p", ctypes.c_void_p), ("min_p_value", ctypes.c_double),
+        ("tokens", ctypes.c_void_p), ("logprobs", ctypes.c_void_p),
+    ]
+
+
+SIGNATURES |= {
+    "ts_b200_window_fwd": (ctypes.c_int, [ctypes.POINTER(WindowArgs), ctypes.c_void_p]),
+    "ts_b200_window_bwd_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(WindowArgs)]),
+    "ts_b200_window_bwd": (ctypes.c_int, [ctypes.POINTER(WindowArgs), ctypes.POINTER(WindowGradArgs), ctypes.c_void_p]),
+    "ts_b200_window_step": (ctypes.c_int, [ctypes.POINTER(WindowStepArgs), ctypes.c_void_p]),
+    "ts_b200_window_extend": (ctypes.c_int, [ctypes.POINTER(WindowExtendArgs), ctypes.c_void_p]),
+    "ts_b200_scan_step": (ctypes.c_int, [ctypes.POINTER(ScanStepArgs), ctypes.c_void_p]),
+    "ts_b200_sample": (ctypes.c_int, [ctypes.POINTER(SampleArgs), ctypes.c_void_p]),
+}
+
 
 def load():
     """Load the shared library (once) and bind every declared symbol."""

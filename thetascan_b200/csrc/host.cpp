@@ -1,5 +1,6 @@
-// Host side of the norm, the gated feed-forward block and the AdamW step: a
-// Python extension over the C ABI (include/thetascan_b200.h).
+// Host side of the norm, the gated feed-forward block, the AdamW step, windowed
+// attention, the scan's token step and the choice of tokens: a Python extension
+// over the C ABI (include/thetascan_b200.h).
 //
 // These operators are called with few rows (a decoding step) or many small
 // tensors (an optimizer step), where the host's share of a call exceeds the
@@ -19,6 +20,8 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/object_ptr.h>
 
+#include <climits>
+#include <cmath>
 #include <optional>
 #include <string>
 #include <vector>
@@ -484,6 +487,394 @@ struct AdamW {
   }
 };
 
+// ---------------------------------------------------------------- window
+
+// t [batch, heads, tokens, dim] as the kernels read it: a view where its channels are contiguous and its base and
+// strides are multiples of 16 bytes, else a copy.
+Tensor streams_of(const Tensor& t) {
+  bool fits = reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && t.stride(3) == 1;
+  for (int i = 0; i < 3 && fits; ++i) {
+    const int64_t s = t.stride(i);
+    fits = t.size(i) == 1 || (s > 0 && s % 8 == 0 && s < (int64_t{1} << 38));
+  }
+  return fits ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+void set_strides(long long (&to)[3], const Tensor& t) {
+  // a dimension of one has no stride of its own
+  for (int i = 0; i < 3; ++i) to[i] = t.size(i) > 1 ? t.stride(i) : (t.size(3) + 7) / 8 * 8;
+}
+
+void lengths_check(const char* name, const Tensor& lengths, int64_t batch, const Tensor& first) {
+  require_cuda(name, lengths, first);
+  TORCH_CHECK_VALUE(lengths.scalar_type() == at::kInt && lengths.is_contiguous() && lengths.dim() == 1 &&
+                        lengths.size(0) == batch,
+                    name, " must be contiguous int32 [", batch, "], got ", lengths.scalar_type(), " ", lengths.sizes());
+}
+
+void bf16_4d(const char* name, const Tensor& t, const Tensor& first) {
+  require_cuda(name, t, first);
+  TORCH_CHECK_VALUE(t.scalar_type() == at::kBFloat16, name, " must be bfloat16, got ", t.scalar_type());
+  TORCH_CHECK_VALUE(t.dim() == 4, name, " must be [batch, heads, tokens, head width], got ", t.sizes());
+}
+
+void window_check(const Tensor& q, const Tensor& k, const Tensor& v, int64_t window, int64_t sinks, double scale,
+                  const OptTensor& lengths) {
+  bf16_4d("q", q, q);
+  bf16_4d("k", k, q);
+  bf16_4d("v", v, q);
+  TORCH_CHECK_VALUE(k.sizes() == v.sizes() && k.size(0) == q.size(0) && k.size(3) == q.size(3) && k.size(2) >= q.size(2),
+                    "k ", k.sizes(), " and v ", v.sizes(), " do not go with q ", q.sizes());
+  TORCH_CHECK_VALUE(k.size(1) > 0 && q.size(1) % k.size(1) == 0, "the ", q.size(1), " heads of q do not share the ",
+                    k.size(1), " of k");
+  TORCH_CHECK_NOT_IMPLEMENTED(q.size(3) >= 8 && q.size(3) <= 128 && q.size(3) % 8 == 0,
+                              "window_attention: the head width must be a multiple of 8 up to 128, got ", q.size(3));
+  TORCH_CHECK_VALUE(window >= 1 && sinks >= 0, "window must be >= 1 and sinks >= 0, got ", window, " and ", sinks);
+  TORCH_CHECK_VALUE(std::isfinite(static_cast<float>(scale)) && static_cast<float>(scale) > 0,
+                    "scale must be positive and finite, got ", scale);
+  TORCH_CHECK_NOT_IMPLEMENTED(k.size(2) <= (1 << 30), "window_attention: more than 2^30 tokens");
+  if (lengths) lengths_check("lengths", *lengths, q.size(0), q);
+}
+
+int clipped(int64_t n) { return static_cast<int>(n > (1 << 30) ? 1 << 30 : n); }
+
+struct WindowCall {
+  Tensor q, k, v;
+  ts_window_args a = {};
+  WindowCall(const Tensor& q_, const Tensor& k_, const Tensor& v_, int64_t window, int64_t sinks, double scale,
+             const OptTensor& lengths)
+      : q(streams_of(q_)), k(streams_of(k_)), v(streams_of(v_)) {
+    a.batch = clipped(q.size(0));
+    a.heads = clipped(q.size(1));
+    a.kv_heads = clipped(k.size(1));
+    a.dim = static_cast<int>(q.size(3));
+    a.q_tokens = static_cast<int>(q.size(2));
+    a.kv_tokens = static_cast<int>(k.size(2));
+    a.window = clipped(window);
+    a.sinks = clipped(sinks);
+    a.scale = static_cast<float>(scale);
+    a.q = q.data_ptr();
+    a.k = k.data_ptr();
+    a.v = v.data_ptr();
+    set_strides(a.q_strides, q);
+    set_strides(a.k_strides, k);
+    set_strides(a.v_strides, v);
+    a.lengths = lengths ? lengths->data_ptr<int>() : nullptr;
+  }
+};
+
+// [batch, heads, tokens, dim] whose memory is [batch, tokens, heads, dim]: the heads of a token lie together, as the
+// projections around an attention have them.
+Tensor token_major(const Tensor& like) {
+  return at::empty({like.size(0), like.size(2), like.size(1), like.size(3)}, like.options()).transpose(1, 2);
+}
+
+std::pair<Tensor, Tensor> window_run(const Tensor& q, const Tensor& k, const Tensor& v, int64_t window, int64_t sinks,
+                                     double scale, const OptTensor& lengths, bool keep) {
+  const c10::cuda::CUDAGuard guard(q.device());
+  const Tensor y = token_major(q);
+  Tensor lse;
+  if (keep) lse = at::empty({q.size(0), q.size(1), (q.size(2) + 127) / 128 * 128}, q.options().dtype(at::kFloat));
+  if (q.numel() == 0) return {y, lse};
+  WindowCall c(q, k, v, window, sinks, scale, lengths);
+  c.a.y = y.data_ptr();
+  set_strides(c.a.y_strides, y);
+  if (keep) c.a.lse = lse.data_ptr<float>();
+  check(ts_b200_window_fwd(&c.a, current_stream(q)));
+  return {y, lse};
+}
+
+std::vector<Tensor> window_grads(const Tensor& dy_, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& y,
+                                 const Tensor& lse, int64_t window, int64_t sinks, double scale, const OptTensor& lengths) {
+  window_check(q, k, v, window, sinks, scale, lengths);
+  bf16_4d("dy", dy_, q);
+  bf16_4d("y", y, q);
+  require_cuda("lse", lse, q);
+  TORCH_CHECK_VALUE(dy_.sizes() == q.sizes() && y.sizes() == q.sizes(), "dy ", dy_.sizes(), " and y ", y.sizes(),
+                    " must have the shape of q ", q.sizes());
+  TORCH_CHECK_VALUE(lse.scalar_type() == at::kFloat && lse.is_contiguous() &&
+                        lse.numel() == q.size(0) * q.size(1) * ((q.size(2) + 127) / 128 * 128),
+                    "lse must be what the forward of these inputs kept");
+  const c10::cuda::CUDAGuard guard(q.device());
+  const Tensor dq = token_major(q), dk = token_major(k), dv = token_major(v);
+  if (q.numel() == 0) {
+    dk.zero_();
+    dv.zero_();
+    return {dq, dk, dv};
+  }
+  WindowCall c(q, k, v, window, sinks, scale, lengths);
+  const Tensor dy = streams_of(dy_), yy = streams_of(y);
+  c.a.y = yy.data_ptr();
+  set_strides(c.a.y_strides, yy);
+  c.a.lse = lse.data_ptr<float>();
+  ts_window_grad_args g = {};
+  g.dy = dy.data_ptr();
+  set_strides(g.dy_strides, dy);
+  g.dq = dq.data_ptr();
+  g.dk = dk.data_ptr();
+  g.dv = dv.data_ptr();
+  set_strides(g.dq_strides, dq);
+  set_strides(g.dk_strides, dk);
+  set_strides(g.dv_strides, dv);
+  g.workspace_bytes = ts_b200_window_bwd_workspace_bytes(&c.a);
+  if (g.workspace_bytes == 0) {   // the size query refused the arguments
+    char text[512];
+    check(ts_b200_last_error(text, sizeof(text)));
+  }
+  const Tensor ws = at::empty({static_cast<int64_t>(g.workspace_bytes)}, q.options().dtype(at::kByte));
+  g.workspace = ws.data_ptr();
+  check(ts_b200_window_bwd(&c.a, &g, current_stream(q)));
+  return {dq, dk, dv};
+}
+
+struct WindowNode : torch::autograd::Function<WindowNode> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, int64_t window,
+                        int64_t sinks, double scale, const OptTensor& lengths) {
+    const auto [y, lse] = window_run(q, k, v, window, sinks, scale, lengths, true);
+    ctx->saved_data["window"] = window;
+    ctx->saved_data["sinks"] = sinks;
+    ctx->saved_data["scale"] = scale;
+    ctx->save_for_backward({q, k, v, y, lse, lengths ? *lengths : Tensor()});
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    refuse_double_backward("window_attention");
+    const variable_list s = ctx->get_saved_variables();
+    const variable_list g = window_grads(grads[0], s[0], s[1], s[2], s[3], s[4], ctx->saved_data["window"].toInt(),
+                                         ctx->saved_data["sinks"].toInt(), ctx->saved_data["scale"].toDouble(),
+                                         s[5].defined() ? OptTensor(s[5]) : OptTensor());
+    return {g[0], g[1], g[2], Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+// What a kernel writes in place: its autograd version moves on.
+void changed(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+void in_place_check(const char* name, const Tensor& t) {
+  TORCH_CHECK(!(at::GradMode::is_enabled() && t.requires_grad()), name, " is written in place and must not require a gradient");
+  for (int64_t i = 0; i < t.dim(); ++i)
+    TORCH_CHECK_VALUE(t.size(i) < 2 || t.stride(i) > 0, name, " is written in place and must not be an expanded view");
+}
+
+// The cache's part of the arguments; `k` and `v` are the new tokens.
+ts_window_cache window_cache(const Tensor& k, const Tensor& v, const Tensor& keys, const Tensor& values,
+                             const Tensor& lengths, int64_t sinks) {
+  bf16_4d("k", k, k);
+  bf16_4d("v", v, k);
+  bf16_4d("keys", keys, k);
+  bf16_4d("values", values, k);
+  TORCH_CHECK_VALUE(k.sizes() == v.sizes(), "k ", k.sizes(), " and v ", v.sizes(), " must have one shape");
+  TORCH_CHECK_VALUE(keys.sizes() == values.sizes() && keys.size(0) == k.size(0) && keys.size(1) == k.size(1) &&
+                        keys.size(3) == k.size(3),
+                    "a cache of ", keys.sizes(), " and ", values.sizes(), " does not go with k ", k.sizes());
+  TORCH_CHECK_VALUE(sinks >= 0 && sinks < keys.size(2), "of the cache's ", keys.size(2), " slots, sinks must leave one, got ", sinks);
+  TORCH_CHECK_NOT_IMPLEMENTED(k.size(3) >= 8 && k.size(3) <= 128 && k.size(3) % 8 == 0,
+                              "window attention: the head width must be a multiple of 8 up to 128, got ", k.size(3));
+  lengths_check("lengths", lengths, k.size(0), k);
+  ts_window_cache c = {};
+  for (const auto& [name, t] : {std::pair<const char*, const Tensor*>{"keys", &keys}, {"values", &values}}) {
+    in_place_check(name, *t);
+    bool fits = reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0 && t->stride(3) == 1;
+    for (int i = 0; i < 3; ++i) fits = fits && (t->size(i) == 1 || t->stride(i) % 8 == 0);
+    TORCH_CHECK_VALUE(fits, name, " must have contiguous channels, and a base and strides that are multiples of 16 bytes");
+  }
+  c.batch = clipped(k.size(0));
+  c.kv_heads = clipped(k.size(1));
+  c.dim = static_cast<int>(k.size(3));
+  c.sinks = clipped(sinks);
+  c.window = clipped(keys.size(2) - sinks);
+  TORCH_CHECK_NOT_IMPLEMENTED(keys.size(2) <= (1 << 30), "window attention: more than 2^30 slots");
+  c.keys = keys.data_ptr();
+  c.values = values.data_ptr();
+  set_strides(c.keys_strides, keys);
+  set_strides(c.values_strides, values);
+  c.lengths = lengths.data_ptr<int>();
+  return c;
+}
+
+Tensor window_step_run(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& keys, const Tensor& values,
+                       const Tensor& lengths, int64_t sinks, double scale) {
+  bf16_4d("q", q, k);
+  TORCH_CHECK_VALUE(q.size(2) == 1 && k.size(2) == 1, "window_attention_step takes one token, got q ", q.sizes(), " and k ", k.sizes());
+  TORCH_CHECK_VALUE(q.size(0) == k.size(0) && q.size(3) == k.size(3) && k.size(1) > 0 && q.size(1) % k.size(1) == 0, "q ",
+                    q.sizes(), " does not go with k ", k.sizes());
+  TORCH_CHECK_VALUE(std::isfinite(static_cast<float>(scale)) && static_cast<float>(scale) > 0,
+                    "scale must be positive and finite, got ", scale);
+  ts_window_step_args a = {};
+  a.cache = window_cache(k, v, keys, values, lengths, sinks);
+  const c10::cuda::CUDAGuard guard(k.device());
+  Tensor y = at::empty(q.sizes(), q.options());
+  if (q.numel() == 0) return y;
+  const Tensor q4 = streams_of(q), k4 = streams_of(k), v4 = streams_of(v);
+  a.heads = clipped(q.size(1));
+  a.scale = static_cast<float>(scale);
+  a.q = q4.data_ptr();
+  a.k = k4.data_ptr();
+  a.v = v4.data_ptr();
+  for (const auto& [to, t] : {std::pair<long long*, const Tensor*>{a.q_strides, &q4}, {a.k_strides, &k4}, {a.v_strides, &v4}}) {
+    long long s[3];
+    set_strides(s, *t);
+    to[0] = s[0];
+    to[1] = s[1];
+  }
+  a.y = y.data_ptr();
+  check(ts_b200_window_step(&a, current_stream(k)));
+  changed(keys);
+  changed(values);
+  return y;
+}
+
+void window_extend_run(const Tensor& k, const Tensor& v, const Tensor& keys, const Tensor& values, const Tensor& lengths,
+                       int64_t sinks, const OptTensor& fresh) {
+  ts_window_extend_args a = {};
+  a.cache = window_cache(k, v, keys, values, lengths, sinks);
+  if (fresh) lengths_check("new", *fresh, k.size(0), k);
+  TORCH_CHECK_NOT_IMPLEMENTED(k.size(2) <= (1 << 30), "window_cache_extend: more than 2^30 tokens");
+  if (k.numel() == 0) return;
+  const c10::cuda::CUDAGuard guard(k.device());
+  const Tensor k4 = streams_of(k), v4 = streams_of(v);
+  a.tokens = static_cast<int>(k.size(2));
+  a.k = k4.data_ptr();
+  a.v = v4.data_ptr();
+  set_strides(a.k_strides, k4);
+  set_strides(a.v_strides, v4);
+  a.fresh = fresh ? fresh->data_ptr<int>() : nullptr;
+  check(ts_b200_window_extend(&a, current_stream(k)));
+  changed(keys);
+  changed(values);
+}
+
+// ------------------------------------------------------------- scan step
+
+// Reads [views, batch, heads, 1, width]; the state changes in place.
+Tensor scan_step_run(const Tensor& q, const Tensor& k, const Tensor& v, const std::vector<OptTensor>& retentions, bool unit,
+                     const Tensor& state) {
+  const std::pair<const char*, const Tensor*> all[] = {{"q", &q}, {"k", &k}, {"v", &v}, {"state", &state}};
+  for (const auto& [name, t] : all) require_cuda(name, *t, q);
+  TORCH_CHECK_NOT_IMPLEMENTED(q.scalar_type() == k.scalar_type() && q.scalar_type() == v.scalar_type() &&
+                                  (q.scalar_type() == at::kFloat || q.scalar_type() == at::kBFloat16),
+                              "b200 scan step: q, k and v must all be bf16 or all float32, got ", q.scalar_type(), ", ",
+                              k.scalar_type(), ", ", v.scalar_type());
+  TORCH_CHECK_VALUE(q.dim() == 4 && q.size(2) == 1 && k.sizes() == q.sizes() && v.dim() == 4 && v.size(0) == q.size(0) &&
+                        v.size(1) == q.size(1) && v.size(2) == 1,
+                    "b200 scan step: q and k must be [B,H,1,Dk] and v [B,H,1,Dv], got ", q.sizes(), ", ", k.sizes(), " and ",
+                    v.sizes());
+  const int64_t B = q.size(0), H = q.size(1), width = v.size(3) + unit, R = static_cast<int64_t>(retentions.size());
+  TORCH_CHECK_NOT_IMPLEMENTED(R <= TS_MAX_RETENTIONS, "b200 scan step: at most ", TS_MAX_RETENTIONS, " retentions per call");
+  TORCH_CHECK_NOT_IMPLEMENTED(q.size(3) >= 1 && q.size(3) <= 256 && width <= 256 && width > unit,
+                              "b200 scan step: key and payload widths up to 256, got ", q.size(3), " and ", width);
+  TORCH_CHECK_VALUE(state.scalar_type() == at::kFloat && state.is_contiguous() &&
+                        state.sizes() == at::IntArrayRef({B, H, R, q.size(3), width}),
+                    "b200 scan step: state must be contiguous f32 [", B, ",", H, ",", R, ",", q.size(3), ",", width, "], got ",
+                    state.scalar_type(), " ", state.sizes());
+  in_place_check("state", state);
+  const c10::cuda::CUDAGuard guard(q.device());
+  Tensor out = at::empty({R, B, H, 1, width}, q.options());
+  std::vector<Tensor> las;
+  ts_scan_step_args a = {};
+  for (int64_t i = 0; i < R; ++i) {
+    if (!retentions[i]) continue;
+    const Tensor& r = *retentions[i];
+    require_cuda("retention", r, q);
+    const bool gate = r.dim() == 4;
+    TORCH_CHECK_VALUE(gate ? r.sizes() == at::IntArrayRef({B, H, 1, 1}) : r.numel() == H,
+                      "b200 scan step: a retention is None, one entry per head or [B,H,1,1], got ", r.sizes());
+    las.push_back(r.detach().reshape({-1}).to(at::kFloat).contiguous());
+    a.log_alpha[i] = las.back().data_ptr<float>();
+    a.log_alpha_batch[i] = gate ? H : 0;
+  }
+  if (out.numel() == 0) return out;
+  auto rows = [](const Tensor& t) { return t.stride(3) == 1 || t.size(3) == 1 ? t : t.contiguous(); };
+  const Tensor q4 = rows(q), k4 = rows(k), v4 = rows(v);
+  a.batch = clipped(B);
+  a.heads = clipped(H);
+  a.dk = static_cast<int>(q.size(3));
+  a.dv = static_cast<int>(width);
+  a.v_append_unit = unit;
+  a.dtype = dtype_code("q", q);
+  a.q = q4.data_ptr();
+  a.k = k4.data_ptr();
+  a.v = v4.data_ptr();
+  for (int i = 0; i < 2; ++i) {
+    a.q_strides[i] = q4.stride(i);
+    a.k_strides[i] = k4.stride(i);
+    a.v_strides[i] = v4.stride(i);
+  }
+  a.n_retentions = static_cast<int>(R);
+  a.state = state.data_ptr<float>();
+  a.out = out.data_ptr();
+  check(ts_b200_scan_step(&a, current_stream(q)));
+  changed(state);
+  return out;
+}
+
+// ---------------------------------------------------------------- sample
+
+// A setting of the choice: a number for all rows, or a tensor with one for each.
+struct Setting {
+  Tensor rows;
+  double value;
+  Setting(const OptTensor& t, double value_, at::ScalarType type, const char* name, int64_t count, const Tensor& logits)
+      : value(value_) {
+    if (!t) return;
+    require_cuda(name, *t, logits);
+    TORCH_CHECK_VALUE(type == at::kInt ? at::isIntegralType(t->scalar_type(), false) : t->scalar_type() == type, name,
+                      " must be a number or a tensor of ", type, ", got ", t->scalar_type());
+    TORCH_CHECK_VALUE(t->numel() == count, name, " must have one value for each of the ", count, " rows, got ", t->sizes());
+    rows = t->scalar_type() == type ? t->contiguous()
+                                    : t->clamp(INT_MIN, INT_MAX).to(type).contiguous();   // of 64-bit integers
+  }
+};
+
+std::pair<Tensor, Tensor> sample_run(const Tensor& logits, const Tensor& uniform, const OptTensor& temperature,
+                                     double temperature_value, const OptTensor& top_k, int64_t top_k_value,
+                                     const OptTensor& top_p, double top_p_value, const OptTensor& min_p, double min_p_value,
+                                     bool logprobs) {
+  require_cuda("logits", logits, logits);
+  require_cuda("uniform", uniform, logits);
+  dtype_code("logits", logits);
+  TORCH_CHECK_VALUE(logits.dim() >= 1 && logits.size(-1) >= 1, "logits must be [..., vocabulary], got ", logits.sizes());
+  const int64_t vocab = logits.size(-1), rows = logits.numel() / vocab;
+  TORCH_CHECK_VALUE(uniform.scalar_type() == at::kFloat && uniform.sizes() == logits.sizes().slice(0, logits.dim() - 1),
+                    "uniform must be float32 ", logits.sizes().slice(0, logits.dim() - 1), ", got ", uniform.scalar_type(), " ",
+                    uniform.sizes());
+  TORCH_CHECK_NOT_IMPLEMENTED(vocab <= (1 << 22) && rows <= (1 << 27), "sample_tokens: more than 2^22 tokens or 2^27 rows");
+  TORCH_CHECK_VALUE(temperature || (temperature_value >= 0 && std::isfinite(temperature_value)),
+                    "temperature must be >= 0 and finite, got ", temperature_value);
+  TORCH_CHECK_VALUE(top_k || top_k_value >= 0, "top_k must be >= 1, got ", top_k_value);
+  TORCH_CHECK_VALUE(top_p || (top_p_value > 0 && top_p_value <= 1), "top_p must be in (0, 1], got ", top_p_value);
+  TORCH_CHECK_VALUE(min_p || (min_p_value >= 0 && min_p_value <= 1), "min_p must be in [0, 1], got ", min_p_value);
+  const c10::cuda::CUDAGuard guard(logits.device());
+  const Setting t(temperature, temperature_value, at::kFloat, "temperature", rows, logits),
+      k(top_k, 0, at::kInt, "top_k", rows, logits), pp(top_p, top_p_value, at::kFloat, "top_p", rows, logits),
+      mp(min_p, min_p_value, at::kFloat, "min_p", rows, logits);
+  Tensor tokens = at::empty(uniform.sizes(), logits.options().dtype(at::kLong)), chances;
+  if (logprobs) chances = at::empty(uniform.sizes(), logits.options().dtype(at::kFloat));
+  if (rows == 0) return {tokens, chances};
+  const Tensor x = rows_of(logits.detach()), u = uniform.contiguous();
+  ts_sample_args a = {};
+  a.rows = static_cast<int>(rows);
+  a.vocab = static_cast<int>(vocab);
+  a.dtype = dtype_code("logits", x);
+  a.logits = x.data_ptr();
+  a.row_stride = x.stride(0);
+  a.uniform = u.data_ptr<float>();
+  a.temperature = t.rows.defined() ? t.rows.data_ptr<float>() : nullptr;
+  a.temperature_value = t.value;
+  a.top_k = k.rows.defined() ? k.rows.data_ptr<int>() : nullptr;
+  a.top_k_value = clipped(top_k_value);
+  a.top_p = pp.rows.defined() ? pp.rows.data_ptr<float>() : nullptr;
+  a.top_p_value = pp.value;
+  a.min_p = mp.rows.defined() ? mp.rows.data_ptr<float>() : nullptr;
+  a.min_p_value = mp.value;
+  a.tokens = reinterpret_cast<long long*>(tokens.data_ptr<int64_t>());
+  a.logprobs = logprobs ? chances.data_ptr<float>() : nullptr;
+  check(ts_b200_sample(&a, current_stream(logits)));
+  return {tokens, chances};
+}
+
 // ---------------------------------------------------------------- Python
 
 const Tensor& tensor_arg(PyObject* o, const char* name) {
@@ -673,13 +1064,122 @@ PyObject* py_adamw(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+double scale_arg(PyObject* o, const Tensor& q) {
+  return o == Py_None ? 1.0 / std::sqrt(static_cast<double>(q.dim() > 0 ? std::max<int64_t>(q.size(-1), 1) : 1)) : double_arg(o);
+}
+
+// window_attention(q, k, v, window, sinks, scale or None, lengths or None) -> y; with gradients
+PyObject* py_window_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  count_args(n, 7);
+  const Tensor &q = tensor_arg(args[0], "q"), &k = tensor_arg(args[1], "k"), &v = tensor_arg(args[2], "v");
+  const int64_t window = int_arg(args[3]), sinks = int_arg(args[4]);
+  const double scale = scale_arg(args[5], q);
+  const OptTensor lengths = optional_arg(args[6], "lengths");
+  window_check(q, k, v, window, sinks, scale, lengths);
+  if (needs_grad({&q, &k, &v})) return wrap(WindowNode::apply(q, k, v, window, sinks, scale, lengths));
+  return wrap(window_run(q, k, v, window, sinks, scale, lengths, false).first);
+  END_HANDLE_TH_ERRORS
+}
+
+// window_fwd(q, k, v, window, sinks, scale, lengths or None, keep) -> (y, lse or None); no gradients
+PyObject* py_window_fwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  count_args(n, 8);
+  const Tensor &q = tensor_arg(args[0], "q"), &k = tensor_arg(args[1], "k"), &v = tensor_arg(args[2], "v");
+  const int64_t window = int_arg(args[3]), sinks = int_arg(args[4]);
+  const double scale = scale_arg(args[5], q);
+  const OptTensor lengths = optional_arg(args[6], "lengths");
+  window_check(q, k, v, window, sinks, scale, lengths);
+  const auto [y, lse] = window_run(q, k, v, window, sinks, scale, lengths, args[7] == Py_True);
+  return wrap_all({&y, &lse});
+  END_HANDLE_TH_ERRORS
+}
+
+// window_bwd(dy, q, k, v, y, lse, window, sinks, scale, lengths or None) -> (dq, dk, dv)
+PyObject* py_window_bwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  count_args(n, 10);
+  const Tensor& q = tensor_arg(args[1], "q");
+  const std::vector<Tensor> g =
+      window_grads(tensor_arg(args[0], "dy"), q, tensor_arg(args[2], "k"), tensor_arg(args[3], "v"), tensor_arg(args[4], "y"),
+                   tensor_arg(args[5], "lse"), int_arg(args[6]), int_arg(args[7]), scale_arg(args[8], q),
+                   optional_arg(args[9], "lengths"));
+  return wrap_all({&g[0], &g[1], &g[2]});
+  END_HANDLE_TH_ERRORS
+}
+
+// window_step(q, k, v, keys, values, lengths, sinks, scale or None) -> y; keys and values change in place
+PyObject* py_window_step(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  count_args(n, 8);
+  const Tensor &q = tensor_arg(args[0], "q"), &k = tensor_arg(args[1], "k"), &v = tensor_arg(args[2], "v");
+  TORCH_CHECK(!needs_grad({&q, &k, &v}), "window_attention_step has no gradient: call it under torch.no_grad()");
+  return wrap(window_step_run(q, k, v, tensor_arg(args[3], "keys"), tensor_arg(args[4], "values"),
+                              tensor_arg(args[5], "lengths"), int_arg(args[6]), scale_arg(args[7], q)));
+  END_HANDLE_TH_ERRORS
+}
+
+// window_extend(k, v, keys, values, lengths, sinks, new or None); keys and values change in place
+PyObject* py_window_extend(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  count_args(n, 7);
+  const Tensor &k = tensor_arg(args[0], "k"), &v = tensor_arg(args[1], "v");
+  TORCH_CHECK(!needs_grad({&k, &v}), "window_cache_extend has no gradient: call it under torch.no_grad()");
+  window_extend_run(k, v, tensor_arg(args[2], "keys"), tensor_arg(args[3], "values"), tensor_arg(args[4], "lengths"),
+                    int_arg(args[5]), optional_arg(args[6], "new"));
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
+// scan_step(q, k, v, retentions, append_unit, state) -> reads [views, B, H, 1, width]; the state changes in place
+PyObject* py_scan_step(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  count_args(n, 6);
+  const Tensor &q = tensor_arg(args[0], "q"), &k = tensor_arg(args[1], "k"), &v = tensor_arg(args[2], "v");
+  THPObjectPtr list(PySequence_Fast(args[3], "retentions"));
+  if (!list) throw python_error();
+  std::vector<OptTensor> retentions;
+  for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(list.get()); ++i) {
+    retentions.push_back(optional_arg(PySequence_Fast_GET_ITEM(list.get(), i), "a retention"));
+    if (retentions.back())
+      TORCH_CHECK(!needs_grad({&*retentions.back()}), "linattn_views_step has no gradient: call it under torch.no_grad()");
+  }
+  TORCH_CHECK(!needs_grad({&q, &k, &v}), "linattn_views_step has no gradient: call it under torch.no_grad()");
+  TORCH_CHECK_VALUE(!retentions.empty(), "b200 scan step: no retentions");
+  return wrap(scan_step_run(q, k, v, retentions, PyObject_IsTrue(args[4]) == 1, tensor_arg(args[5], "state")));
+  END_HANDLE_TH_ERRORS
+}
+
+// sample(logits, uniform, temperature, top_k or None, top_p or None, min_p or None, logprobs) -> tokens, or (tokens, logprobs)
+PyObject* py_sample(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  count_args(n, 7);
+  const Tensor& logits = tensor_arg(args[0], "logits");
+  const bool logprobs = args[6] == Py_True;
+  TORCH_CHECK(!logprobs || !needs_grad({&logits}), "sample_tokens: the log-probabilities have no gradient: call it under torch.no_grad()");
+  auto tensor = [](PyObject* o, const char* name) { return THPVariable_Check(o) ? OptTensor(tensor_arg(o, name)) : OptTensor(); };
+  auto number = [](PyObject* o, double off) { return o == Py_None || THPVariable_Check(o) ? off : double_arg(o); };
+  const bool k_number = args[3] != Py_None && !THPVariable_Check(args[3]);
+  const int64_t top_k = k_number ? int_arg(args[3]) : 0;
+  TORCH_CHECK_VALUE(!k_number || top_k >= 1, "top_k must be >= 1, got ", top_k);
+  const auto [tokens, chances] =
+      sample_run(logits, tensor_arg(args[1], "uniform"), tensor(args[2], "temperature"), number(args[2], 1.0),
+                 tensor(args[3], "top_k"), top_k, tensor(args[4], "top_p"), number(args[4], 1.0), tensor(args[5], "min_p"),
+                 number(args[5], 0.0), logprobs);
+  return logprobs ? wrap_all({&tokens, &chances}) : wrap(tokens);
+  END_HANDLE_TH_ERRORS
+}
+
 #define TS_METHOD(name) \
   { #name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_##name)), METH_FASTCALL, nullptr }
 PyMethodDef methods[] = {TS_METHOD(rms_norm),  TS_METHOD(norm_fwd), TS_METHOD(norm_bwd), TS_METHOD(rms_norm_8bit),
                          TS_METHOD(gated_ffn), TS_METHOD(ffn_fwd),  TS_METHOD(ffn_bwd),  TS_METHOD(adamw),
+                         TS_METHOD(window_attention), TS_METHOD(window_fwd), TS_METHOD(window_bwd), TS_METHOD(window_step),
+                         TS_METHOD(window_extend), TS_METHOD(scan_step), TS_METHOD(sample),
                          {nullptr, nullptr, 0, nullptr}};
 
-PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "Host side of the norm, the gated block and the AdamW step.", -1,
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "Host side of the operators whose calls are short.", -1,
                       methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -1,0 +1,119 @@
+// What the kernels of the windowed attention share: sizes, the tensor-memory
+// operand form of the matrix instruction, masks of a row's columns.
+//
+// The query at position i sees the key at position j when j <= i and
+// i - j < window or j < sinks, both below the sequence's length.  Queries are the
+// last q_tokens of kv_tokens positions.  Tiles are 128 queries and 128 keys; the
+// grid of the window's key tiles starts at the first query, so that a window that
+// is a multiple of 128 is covered by window / 128 + 1 tiles whatever comes before.
+#pragma once
+
+#include "../../include/thetascan_b200.h"
+#include "common.cuh"
+#include "tma.cuh"
+
+namespace ts {
+
+constexpr int kWinWarps = 12;                  // 0-7: two groups of row warps, 8: loads, 9: instructions, 10: tensor memory
+constexpr int kWinThreads = 32 * kWinWarps;
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct WinSizes {
+  int batch, heads, kv_heads, share;   // share: query heads to a key head
+  int dim;
+  int q_tokens, kv_tokens, past;       // past: kv_tokens - q_tokens
+  int window, sinks;                   // both at most kv_tokens
+  int q_tiles;
+  float scale;
+  const int* lengths;                  // or null
+};
+
+__device__ __forceinline__ int win_length(const WinSizes& w, int b) {
+  return w.lengths ? max(0, min(__ldg(w.lengths + b), w.kv_tokens)) : w.kv_tokens;
+}
+
+// D (+)= A B with A [128 x 16 per step] in tensor memory (bf16, two to a column) and B in shared memory.
+__device__ __forceinline__ void mma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// 32 columns of this lane's row (visible after tmem_store_wait()).
+__device__ __forceinline__ void tmem_st(uint32_t addr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,"
+      "%30,%31,%32};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st(uint32_t addr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+          addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Bits [low, high] of a word (either may lie outside it; none where low > high).
+__device__ __forceinline__ uint32_t bit_range(int low, int high) {
+  if (high < 0 || low > 31 || low > high) return 0;
+  const uint32_t up = high >= 31 ? 0xffffffffu : (2u << high) - 1;
+  return low <= 0 ? up : up & ~((1u << low) - 1);
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// The K-major operand (rows = M or N) and the MN-major one (rows = inner) of a 128-byte-swizzled tile of 128 rows
+// in 64-column boxes, at inner step s of 16.
+__device__ __forceinline__ uint64_t win_rows(uint32_t tile, int s) {
+  return smem_desc_sw128(tile + (s >> 2) * kSwBox + (s & 3) * 32, 16, 1024);
+}
+__device__ __forceinline__ uint64_t win_inner(uint32_t tile, int s) {
+  return smem_desc_sw128(tile + 2048 * s, kSwBox, 1024);
+}
+
+// The two operands again, from the descriptor of step 0: the address field counts 16 bytes and has room for all of
+// shared memory, so that a step is an addition.
+__device__ __forceinline__ uint64_t win_rows_step(uint64_t first, int s) {
+  return first + ((s >> 2) * (kSwBox >> 4) + (s & 3) * 2);
+}
+__device__ __forceinline__ uint64_t win_inner_step(uint64_t first, int s) { return first + 128 * s; }
+
+// One lane of a converged warp.  The warps that feed the tensor cores run with all lanes and let one issue, so that
+// addresses stay in uniform registers (a single lane's loop took 120 cycles for each instruction of 64).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+  return one != 0;
+}
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, int code) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, code));
+}
+
+// Host: a [batch, heads, tokens, dim] tensor as boxes of 64 columns x `rows` tokens.
+bool win_map(CUtensorMap* map, const void* base, const long long* strides, int batch, int heads, int tokens, int dim,
+             int rows);
+// Checked arguments as sizes, or an error code.
+int win_sizes(const ts_window_args* a, WinSizes* w, const char* what);
+
+}  // namespace ts

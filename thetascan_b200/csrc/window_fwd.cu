@@ -1,0 +1,535 @@
+// Causal attention over a sliding window with first tokens that stay visible:
+// the forward pass over many queries.
+//
+//   y_i = sum_j p_ij v_j / sum_j p_ij, p_ij = exp(scale q_i.k_j - m_i), j visible to i
+//
+// One pass over the keys with a running reference m_i and sum.  A CTA takes two
+// tiles of 128 queries at a time, A and B: of two heads that share a key head, or
+// neighbours of one head, so that both read the same keys.  Warp 8 feeds a ring of
+// key and value tiles by TMA, a thread of warp 9 issues the matrix instructions,
+// warps 0-3 and 4-7 each own the rows of one query tile, a row to a thread.
+// S = Q K^T lies in tensor memory, 128 columns for each of A and B; P replaces it
+// there in bf16 and is the operand of O += P V from where it lies.  While one
+// group forms its P the tensor cores work for the other.
+//
+// A row's reference moves only when a score exceeds it by 2^8 (P is then at most
+// 256, and bf16 keeps its relative error): O is seldom rescaled, and the row's own
+// thread does that, before it hands P over.
+//
+// First tokens are tiles of their own, as narrow as 16 columns, so that four sinks
+// cost a sixteenth of a tile; the window's tiles leave those keys out.
+#include <cmath>
+#include <cstring>
+
+#include "capi_internal.h"
+#include "window.cuh"
+
+namespace ts {
+
+namespace {
+
+template <int kD>
+struct WinFwdLayout {
+  static constexpr int kBoxes = kD / 64;
+  static constexpr uint32_t kTileBytes = kBoxes * kSwBox;
+  static constexpr int kSlots = kD == 64 ? 8 : 4;
+  static constexpr uint32_t kOutBytes = 4096;          // a warp's 32 rows x 64 columns
+  static constexpr uint32_t kQ = 0, kRing = 2 * kTileBytes, kOut = kRing + kSlots * kTileBytes;
+  static constexpr uint32_t kSmem = kOut + 8 * kOutBytes + 1024;
+};
+
+struct WinFwdParams {
+  CUtensorMap q, k, v, k_sink, v_sink, y;
+  WinSizes w;
+  int pairs, units;
+  int sink_rows;         // rows of a sink box
+  float* lse;            // or null
+};
+
+// One of the two query tiles of a unit.
+struct WinFwdTile {
+  int tile, head;
+  bool exists, live;    // a tile of the tensor; a tile with rows below the length
+  int low, last;        // its first window tile; its last index in the list of tiles
+};
+
+// What a CTA works on: two query tiles of one key head, and the key tiles that either sees.
+struct WinFwdUnit {
+  int b, kv_head, length;
+  WinFwdTile a, z;
+  int sinks;                 // keys below this come in sink tiles, not in the window's
+  int sink_tiles, first;     // window tiles run from `first` (in tiles from the first query)
+  int count;                 // tiles to go over
+
+  __device__ __forceinline__ WinFwdTile place(const WinSizes& w, int at) const {
+    WinFwdTile t;
+    t.tile = at / w.share;
+    t.head = kv_head * w.share + at - t.tile * w.share;
+    t.exists = t.tile < w.q_tiles;
+    t.live = t.exists && w.past + 128 * t.tile < length;
+    return t;
+  }
+  __device__ __forceinline__ WinFwdUnit(const WinFwdParams& p, int unit) {
+    const WinSizes& w = p.w;
+    const int row = unit / p.pairs, pair = unit - row * p.pairs;
+    b = row / w.kv_heads;
+    kv_head = row - b * w.kv_heads;
+    length = win_length(w, b);
+    a = place(w, 2 * pair);
+    z = place(w, 2 * pair + 1);
+    const int top = z.live ? z.tile : a.live ? a.tile : -1;
+    const int end = min(w.past + 128 * top + 127, length - 1);   // the last position
+    // rows that all see everything before them need no sinks
+    sinks = end < w.window ? 0 : min(w.sinks, end + 1);
+    sink_tiles = (sinks + 127) >> 7;
+    const int reach = (w.window + 126) >> 7, least = (sinks - w.past) >> 7;
+    first = a.low = max(a.tile - reach, least);
+    z.low = max(z.tile - reach, least);
+    a.last = sink_tiles - 1 + (a.tile >= a.low ? a.tile - first + 1 : 0);
+    z.last = sink_tiles - 1 + (z.tile >= z.low ? z.tile - first + 1 : 0);
+    count = top < 0 ? 0 : sink_tiles + top - first + 1;
+  }
+  __device__ __forceinline__ WinFwdTile of(int x) const {
+    WinFwdTile t;
+    t.tile = x ? z.tile : a.tile;
+    t.head = x ? z.head : a.head;
+    t.exists = x ? z.exists : a.exists;
+    t.live = x ? z.live : a.live;
+    t.low = x ? z.low : a.low;
+    t.last = x ? z.last : a.last;
+    return t;
+  }
+  __device__ __forceinline__ bool active(const WinFwdTile& x, int n) const {
+    const int t = first + n - sink_tiles;
+    return x.live && n < count && (n < sink_tiles || (t >= x.low && t <= x.tile));
+  }
+  __device__ __forceinline__ int columns(int n) const {
+    return n < sink_tiles ? min(128, (sinks - 128 * n + 15) & ~15) : 128;
+  }
+  __device__ __forceinline__ int key(const WinSizes& w, int n) const {
+    return n < sink_tiles ? 128 * n : w.past + 128 * (first + n - sink_tiles);
+  }
+};
+
+// The row's scores are read twice, 32 columns at a time: 128 of them in registers spill, and what spills beside this
+// much shared memory goes to L2 (16 heads x 16384, width 128, window 2048: 560 us).  Tiles that are masked or narrow go
+// by a loop over their columns, the others without one.
+struct RowColumns {
+  int cols, from, until;   // the tile's, and this row's first and last visible one
+  bool masked;
+  __device__ __forceinline__ void hide(uint32_t (&s)[32], int c) const {
+    const uint32_t bits = bit_range(from - c, until - c);
+#pragma unroll
+    for (int e = 0; e < 32; ++e)
+      if (!(bits >> e & 1)) s[e] = 0xff800000u;
+  }
+};
+
+__device__ __forceinline__ void row_top(const uint32_t (&s)[32], float (&top)[2]) {
+#pragma unroll
+  for (int e = 0; e < 32; e += 4) {
+    top[0] = max3(top[0], __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
+    top[1] = max3(top[1], __uint_as_float(s[e + 2]), __uint_as_float(s[e + 3]));
+  }
+}
+
+// The largest visible score of the row that starts at `at` in tensor memory.
+__device__ __forceinline__ float row_max(uint32_t at, const RowColumns& r) {
+  float top[2] = {-INFINITY, -INFINITY};
+  if (r.masked) {
+#pragma unroll 1
+    for (int c = 0; c < r.cols; c += 32) {
+      uint32_t s[32];
+      tmem_ld(at + c, s);
+      tmem_wait();
+      tie(s);
+      r.hide(s, c);
+      row_top(s, top);
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < 128; c += 64) {
+      uint32_t s[32], t[32];
+      tmem_ld(at + c, s);
+      tmem_ld(at + c + 32, t);
+      tmem_wait();
+      tie(s);
+      tie(t);
+      row_top(s, top);
+      row_top(t, top);
+    }
+  }
+  return fmaxf(top[0], top[1]);
+}
+
+__device__ __forceinline__ void row_exp(const uint32_t (&s)[32], uint32_t at, float scale2, float origin,
+                                        float (&part)[4]) {
+  uint32_t packed[16];
+#pragma unroll
+  for (int e = 0; e < 32; e += 2) {
+    const float a = exp2_fast(fmaf(__uint_as_float(s[e]), scale2, -origin));
+    const float b = exp2_fast(fmaf(__uint_as_float(s[e + 1]), scale2, -origin));
+    part[e & 2] += a;
+    part[(e & 2) + 1] += b;
+    packed[e / 2] = pack_bf16(a, b);
+  }
+  tmem_st(at, packed);
+}
+
+// Scores to weights in their place, in bf16; returns the sum of the weights (before their rounding).
+__device__ __forceinline__ float row_weights(uint32_t at, const RowColumns& r, float scale2, float origin) {
+  float part[4] = {0.f, 0.f, 0.f, 0.f};
+  if (r.masked) {
+#pragma unroll 1
+    for (int c = 0; c < r.cols; c += 32) {
+      uint32_t s[32];
+      tmem_ld(at + c, s);
+      tmem_wait();
+      tie(s);
+      r.hide(s, c);
+      row_exp(s, at + c / 2, scale2, origin, part);
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < 128; c += 64) {
+      uint32_t s[32], t[32];
+      tmem_ld(at + c, s);
+      tmem_ld(at + c + 32, t);
+      tmem_wait();
+      tie(s);
+      tie(t);
+      row_exp(s, at + c / 2, scale2, origin, part);
+      row_exp(t, at + c / 2 + 16, scale2, origin, part);
+    }
+  }
+  return (part[0] + part[2]) + (part[1] + part[3]);
+}
+
+template <int kD>
+__global__ void __launch_bounds__(kWinThreads, 1) window_fwd_kernel(const __grid_constant__ WinFwdParams p) {
+  using L = WinFwdLayout<kD>;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ alignas(8) uint64_t full[L::kSlots], empty[L::kSlots], q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2];
+  __shared__ uint32_t tmem_slot;
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const WinSizes& w = p.w;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < L::kSlots; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&q_empty[i], 1);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&o_full[i], 1);
+    }
+    fence_mbar_init();
+  }
+  if (warp == 10) tmem_alloc(&tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  // all of tensor memory: its addresses start at 0.  Columns: S of A and B, then O of A and B
+  constexpr uint32_t kScores = 128, kO = 256;
+
+  if (warp >= 8) {
+    if (warp == 8) {
+      // ---- loads
+      uint32_t it = 0, q_turn[2] = {0, 0};
+      bool ok = true;
+      auto load = [&](const CUtensorMap* map, const CUtensorMap* sink_map, const WinFwdUnit& u, int n) {
+        const uint32_t s = it % L::kSlots;
+        if (!(ok = ok && mbar_wait_warp(&empty[s], ((it / L::kSlots) & 1) ^ 1, kErrMmaTimeout))) return;
+        const bool sink = n < u.sink_tiles;
+        const uint32_t rows = sink ? p.sink_rows : 128, to = base + L::kRing + s * L::kTileBytes;
+        if (elect_one()) {
+          mbar_expect_tx(&full[s], L::kBoxes * rows * 128);
+#pragma unroll
+          for (int c = 0; c < L::kBoxes; ++c)
+            tma_load_4d(to + c * kSwBox, sink ? sink_map : map, 64 * c, u.key(w, n), u.kv_head, u.b, &full[s]);
+        }
+        ++it;
+      };
+      for (int unit = blockIdx.x; unit < p.units && ok; unit += gridDim.x) {
+        const WinFwdUnit u(p, unit);
+        for (int n = 0; n < u.count && ok; ++n) {
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            if (!u.of(x).live || n > 0) continue;
+            if (!(ok = ok && mbar_wait_warp(&q_empty[x], (q_turn[x]++ & 1) ^ 1, kErrMmaTimeout))) break;
+            if (elect_one()) {
+              mbar_expect_tx(&q_full[x], L::kTileBytes);
+#pragma unroll
+              for (int c = 0; c < L::kBoxes; ++c)
+                tma_load_4d(base + L::kQ + x * L::kTileBytes + c * kSwBox, &p.q, 64 * c, 128 * u.of(x).tile, u.of(x).head, u.b,
+                            &q_full[x]);
+            }
+          }
+          load(&p.k, &p.k_sink, u, n);
+          load(&p.v, &p.v_sink, u, n);
+        }
+      }
+      if (!ok) {
+        // given up: let the copies in flight land before the memory goes (for a bounded time too)
+        for (uint32_t i = it > L::kSlots ? it - L::kSlots : 0; i < it; ++i)
+          for (int poll = 0; poll < (1 << 16) && !mbar_try_wait(&full[i % L::kSlots], (i / L::kSlots) & 1); ++poll) {
+          }
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          for (int poll = 0; poll < (1 << 16) && q_turn[x] > 0 && !mbar_try_wait(&q_full[x], (q_turn[x] - 1) & 1); ++poll) {
+          }
+      }
+    } else if (warp == 9) {
+      // ---- instructions
+      uint32_t it = 0, q_turn[2] = {0, 0}, p_turn[2] = {0, 0};
+      bool ok = true;
+      constexpr uint32_t id_o = idesc_bf16(128, kD, false, true);
+      auto landed = [&](uint32_t item) {
+        ok = ok && mbar_wait_warp(&full[item % L::kSlots], (item / L::kSlots) & 1, kErrCopyTimeout);
+        tc_fence_after();
+        return ok;
+      };
+      for (int unit = blockIdx.x; unit < p.units && ok; unit += gridDim.x) {
+        const WinFwdUnit u(p, unit);
+        bool begun[2] = {false, false}, summed[2] = {false, false};
+        // S of query tile x against key tile n, which lies in ring item `item`
+        auto scores = [&](int x, int n, uint32_t item) {
+          if (!begun[x]) {
+            if (!(ok = ok && mbar_wait_warp(&q_full[x], q_turn[x]++ & 1, kErrCopyTimeout))) return;
+            begun[x] = true;
+            tc_fence_after();
+          }
+          const uint32_t id = idesc_bf16(128, u.columns(n), false, false);
+          const uint64_t a = win_rows(base + L::kQ + x * L::kTileBytes, 0);
+          const uint64_t k = win_rows(base + L::kRing + item % L::kSlots * L::kTileBytes, 0);
+          if (elect_one()) {
+#pragma unroll
+            for (int s = 0; s < kD / 16; ++s)
+              mma_bf16(kScores * x, win_rows_step(a, s), win_rows_step(k, s), id, s > 0);
+            mma_commit(&s_full[x]);
+            if (n == u.of(x).last) mma_commit(&q_empty[x]);
+          }
+        };
+        if (u.count > 0) {
+          if (!landed(it)) break;
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+            if (u.active(u.of(x), 0)) scores(x, 0, it);
+          if (ok && elect_one()) mma_commit(&empty[it % L::kSlots]);
+        }
+        for (int n = 0; n < u.count && ok; ++n, it += 2) {
+          const uint32_t item = it + 1;
+          if (!landed(item)) break;
+          const uint64_t v = win_inner(base + L::kRing + item % L::kSlots * L::kTileBytes, 0);
+          const bool more = n + 1 < u.count;
+          const int steps = u.columns(n) >> 4;
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            if (ok && u.active(u.of(x), n)) {
+              if (!(ok = mbar_wait_warp(&p_full[x], p_turn[x]++ & 1, kErrMmaTimeout))) break;
+              tc_fence_after();
+              if (elect_one()) {
+#pragma unroll
+                for (int s = 0; s < 8; ++s)
+                  if (s < steps)
+                    mma_bf16_ts(kO + kD * x, kScores * x + 8 * s, win_inner_step(v, s), id_o, summed[x] || s > 0);
+                if (n == u.of(x).last) mma_commit(&o_full[x]);
+              }
+              summed[x] = true;
+            }
+            if (ok && more && u.active(u.of(x), n + 1)) {
+              if (!landed(it + 2)) break;
+              scores(x, n + 1, it + 2);
+            }
+          }
+          if (!ok) break;
+          if (elect_one()) {
+            mma_commit(&empty[item % L::kSlots]);
+            if (more) mma_commit(&empty[(it + 2) % L::kSlots]);
+          }
+        }
+      }
+    }
+  } else {
+    // ---- rows: thread t of group x owns row t of tile x
+    const int x = warp >> 2, quad = warp & 3, row = 32 * quad + lane;
+    const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
+    const uint32_t s_at = kScores * x + lanes, o_at = kO + kD * x + lanes;
+    const uint32_t stage = base + L::kOut + warp * L::kOutBytes;
+    const float scale2 = w.scale * kLog2e;
+    uint32_t s_turn = 0, o_turn = 0;
+    bool ok = true;
+    for (int unit = blockIdx.x; unit < p.units && ok; unit += gridDim.x) {
+      const WinFwdUnit u(p, unit);
+      const WinFwdTile mine = u.of(x);
+      if (!mine.exists) continue;
+      const int q_row = 128 * mine.tile + row, at = w.past + q_row;
+      const int near = max(at - w.window + 1, u.sinks), to = at < u.length ? at : -1;   // visible: first ones, near..to
+      float ref = -INFINITY, sum = 0.f;
+      bool first = true;
+      for (int n = 0; n < u.count; ++n) {
+        if (!u.active(mine, n)) continue;
+        const int cols = u.columns(n), key = u.key(w, n);
+        const bool sink = n < u.sink_tiles;
+        if (!(ok = mbar_wait(&s_full[x], s_turn++ & 1, kErrMmaTimeout))) break;
+        tc_fence_after();
+        // this row's first and last visible column; a tile within reach of all rows is not masked
+        const int from = sink ? 0 : near - key, until = min(to, sink ? u.sinks - 1 : to) - key;
+        const RowColumns r{cols, from, until, !__all_sync(0xffffffffu, from <= 0 && until >= 127)};
+        const float best = row_max(s_at, r) * scale2;
+        if (first) {
+          ref = best;
+          first = false;
+        } else if (__any_sync(0xffffffffu, best > ref + 8.f)) {
+          const float next = best > ref + 8.f ? best : ref;
+          const float factor = next == ref ? 1.f : exp2_fast(ref - next);
+          ref = next;
+          sum *= factor;
+#pragma unroll 1
+          for (int c = 0; c < kD; c += 32) {
+            uint32_t o[32];
+            tmem_ld(o_at + c, o);
+            tmem_wait();
+            tie(o);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
+            tmem_st(o_at + c, o);
+          }
+        }
+        const float origin = ref == -INFINITY ? 0.f : ref;
+        sum += row_weights(s_at, r, scale2, origin);
+        tmem_store_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[x]);
+      }
+      if (!ok) break;
+      if (mine.live && !(ok = mbar_wait(&o_full[x], o_turn++ & 1, kErrMmaTimeout))) break;
+      tc_fence_after();
+      // a row that sees nothing has no sum: zero
+      const float inverse = sum != 0.f ? 1.f / sum : 0.f;
+#pragma unroll 1
+      for (int c = 0; c < w.dim; c += 64) {
+        if (lane == 0) tma_store_read_wait<0>();
+        __syncwarp();
+#pragma unroll
+        for (int h = 0; h < 64; h += 32) {
+          uint32_t o[32];
+          tmem_ld(o_at + c + h, o);
+          tmem_wait();
+          tie(o);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float f[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = inverse != 0.f ? __uint_as_float(o[8 * i + e]) * inverse : 0.f;
+            st_shared_v4(stage + sw128_offset(lane, h / 8 + i), pack8(f));
+          }
+        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          const int to_row = 128 * mine.tile + 32 * quad;
+          if (to_row < w.q_tokens) tma_store_4d(&p.y, c, to_row, mine.head, u.b, stage);
+          tma_store_commit();
+        }
+      }
+      tc_fence_before();
+      if (p.lse) {
+        // of the scores in units of log 2; +infinity, which makes every weight zero, for a row that sees nothing
+        const float l = sum != 0.f ? (ref == -INFINITY ? 0.f : ref) + log2f(sum) : INFINITY;
+        p.lse[(static_cast<size_t>(u.b) * w.heads + mine.head) * (128 * static_cast<size_t>(w.q_tiles)) + q_row] = l;
+      }
+    }
+    if (lane == 0) tma_store_read_wait<0>();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 10) {
+    tc_fence_after();
+    tmem_dealloc(tmem_slot, 512);
+  }
+}
+
+template <int kD>
+int window_fwd_launch(const WinFwdParams& p, cudaStream_t s) {
+  constexpr int smem = WinFwdLayout<kD>::kSmem;
+  const cudaError_t set = cudaFuncSetAttribute(window_fwd_kernel<kD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (set != cudaSuccess) return set_error(TS_ERR_CUDA, "window_fwd: %s", cudaGetErrorString(set));
+  window_fwd_kernel<kD><<<p.units < 148 ? p.units : 148, kWinThreads, smem, s>>>(p);
+  return check_launch("window_fwd");
+}
+
+}  // namespace
+
+bool win_map(CUtensorMap* map, const void* base, const long long* strides, int batch, int heads, int tokens, int dim,
+             int rows) {
+  const uint64_t dims[4] = {static_cast<uint64_t>(dim), static_cast<uint64_t>(tokens), static_cast<uint64_t>(heads),
+                            static_cast<uint64_t>(batch)};
+  // a dimension of one has no stride of its own
+  const int64_t any = (static_cast<int64_t>(dim) + 7) & ~7;
+  const int64_t steps[3] = {tokens > 1 ? strides[2] : any, heads > 1 ? strides[1] : any, batch > 1 ? strides[0] : any};
+  const uint32_t box[4] = {64, static_cast<uint32_t>(rows), 1, 1};
+  return make_tmap_bf16_sw128(map, base, 4, dims, steps, box);
+}
+
+int win_sizes(const ts_window_args* a, WinSizes* w, const char* what) {
+  if (!a) return set_error(TS_ERR_VALUE, "%s: null arguments", what);
+  if (a->batch < 1 || a->heads < 1 || a->kv_heads < 1 || a->q_tokens < 1 || a->kv_tokens < a->q_tokens)
+    return set_error(TS_ERR_VALUE, "%s: sizes must be positive and kv_tokens at least q_tokens", what);
+  if (a->heads % a->kv_heads) return set_error(TS_ERR_VALUE, "%s: %d heads do not share %d key heads", what, a->heads, a->kv_heads);
+  if (a->dim < 8 || a->dim > 128 || a->dim % 8)
+    return set_error(TS_ERR_NOT_IMPLEMENTED, "%s: head width %d is not a multiple of 8 up to 128", what, a->dim);
+  if (a->kv_tokens > (1 << 30) || a->batch > 65535 || a->heads > 65535)
+    return set_error(TS_ERR_NOT_IMPLEMENTED, "%s: more than 2^30 tokens, 65535 sequences or 65535 heads", what);
+  if (a->window < 1 || a->sinks < 0) return set_error(TS_ERR_VALUE, "%s: window must be >= 1 and sinks >= 0", what);
+  if (!(a->scale > 0.f) || !std::isfinite(a->scale)) return set_error(TS_ERR_VALUE, "%s: scale must be positive and finite", what);
+  if (!a->q || !a->k || !a->v) return set_error(TS_ERR_VALUE, "%s: null tensor", what);
+  w->batch = a->batch;
+  w->heads = a->heads;
+  w->kv_heads = a->kv_heads;
+  w->share = a->heads / a->kv_heads;
+  w->dim = a->dim;
+  w->q_tokens = a->q_tokens;
+  w->kv_tokens = a->kv_tokens;
+  w->past = a->kv_tokens - a->q_tokens;
+  w->window = a->window < a->kv_tokens ? a->window : a->kv_tokens;
+  w->sinks = a->sinks < a->kv_tokens ? a->sinks : a->kv_tokens;
+  w->q_tiles = ceil_div(a->q_tokens, 128);
+  w->scale = a->scale;
+  w->lengths = a->lengths;
+  const long long units = static_cast<long long>(w->batch) * w->heads * (w->q_tiles + 1);
+  if (units > 0x3fffffffll) return set_error(TS_ERR_NOT_IMPLEMENTED, "%s: too many query tiles", what);
+  return TS_OK;
+}
+
+}  // namespace ts
+
+using namespace ts;
+
+extern "C" {
+
+int ts_b200_window_fwd(const ts_window_args* a, ts_stream_t stream) {
+  WinFwdParams p = {};
+  if (const int rc = win_sizes(a, &p.w, "window_fwd")) return rc;
+  if (!a->y) return set_error(TS_ERR_VALUE, "window_fwd: null output");
+  const WinSizes& w = p.w;
+  p.pairs = (w.q_tiles * w.share + 1) / 2;
+  p.units = w.batch * w.kv_heads * p.pairs;
+  p.sink_rows = w.sinks >= 128 ? 128 : round_up(w.sinks > 0 ? w.sinks : 1, 16);
+  p.lse = a->lse;
+  const bool ok = win_map(&p.q, a->q, a->q_strides, w.batch, w.heads, w.q_tokens, w.dim, 128) &&
+                  win_map(&p.k, a->k, a->k_strides, w.batch, w.kv_heads, w.kv_tokens, w.dim, 128) &&
+                  win_map(&p.v, a->v, a->v_strides, w.batch, w.kv_heads, w.kv_tokens, w.dim, 128) &&
+                  win_map(&p.k_sink, a->k, a->k_strides, w.batch, w.kv_heads, w.kv_tokens, w.dim, p.sink_rows) &&
+                  win_map(&p.v_sink, a->v, a->v_strides, w.batch, w.kv_heads, w.kv_tokens, w.dim, p.sink_rows) &&
+                  win_map(&p.y, a->y, a->y_strides, w.batch, w.heads, w.q_tokens, w.dim, 32);
+  if (!ok) return set_error(TS_ERR_VALUE, "window_fwd: bases and strides must be multiples of 16 bytes");
+  const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  return w.dim <= 64 ? window_fwd_launch<64>(p, s) : window_fwd_launch<128>(p, s);
+}
+
+}  // extern "C"

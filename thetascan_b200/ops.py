@@ -463,6 +463,21 @@ def _stream_backward(ctx, douts, dstate, dws):
 torch.library.register_autograd(f"{LIB}::scan_views_stream_fwd", _stream_backward, setup_context=_stream_setup)
 
 
+@torch.library.custom_op(f"{LIB}::scan_views_step", mutates_args=("state",))
+def scan_views_step(q: Tensor, k: Tensor, v: Tensor, log_alphas: list[Tensor], present: list[bool], append_unit: bool,
+                    state: Tensor) -> Tensor:
+    """One token of each sequence: reads ``[R,B,H,1,Dv(+unit)]`` in the type of
+    the streams; ``state`` moves on in place."""
+    _require_cuda(q, k, v, state, *log_alphas)
+    return _lib.host().scan_step(q, k, v, _retentions(log_alphas, present), append_unit, state)
+
+
+@scan_views_step.register_fake
+def _(q, k, v, log_alphas, present, append_unit, state):
+    B, H = q.shape[:2]
+    return q.new_empty(len(present), B, H, 1, v.shape[-1] + int(append_unit))
+
+
 # --------------------------------------------------------------------------- GN core
 
 @torch.library.custom_op(f"{LIB}::gn_core_fwd", mutates_args=())

@@ -342,3 +342,25 @@ def linattn_views_stream(q, k, v, retentions, state=None, *, append_unit: bool =
         q, k, v, [r for r in retentions if r is not None], [r is not None for r in retentions], int(append_unit),
         state)
     return tuple(o.to(q.dtype) for o in outs_all.unbind(0)), new_state
+
+
+def linattn_views_step(q, k, v, retentions, state, *, append_unit: bool = False):
+    """The scan for one new token of each sequence: ``state`` f32
+    ``[B,H,R,Dk,Dv(+1)]`` (contiguous, as :func:`linattn_views_stream` returns it)
+    becomes ``exp(retention) state + k^T [v | 1]`` in place, and the reads ``q
+    state`` of every retention are returned, ``[B,H,1,Dv(+1)]`` in the type of the
+    streams.
+
+    ``q``, ``k`` ``[B,H,1,Dk]`` and ``v`` ``[B,H,1,Dv]`` are bf16 or float32, the
+    arithmetic is float32 for either.  A retention is ``None`` (the plain sum),
+    one log-retention per head, or this token's own, ``[B,H,1,1]``.  One kernel
+    that reads and writes the state once (``csrc/scan_step.cu``).  For inference:
+    no gradient."""
+    if not retentions:
+        return ()
+    if torch.compiler.is_compiling():
+        from . import ops  # noqa: F401  (registers the operators)
+        return torch.ops.thetascan_b200.scan_views_step(
+            q, k, v, [r for r in retentions if r is not None], [r is not None for r in retentions], bool(append_unit),
+            state).unbind(0)
+    return tuple(_lib.host().scan_step(q, k, v, retentions, append_unit, state).unbind(0))

@@ -100,7 +100,7 @@ def test_scan_step_refuses(over, code):
 
 
 @pytest.mark.parametrize("over,code", [
-    (dict(rows=0), BAD), (dict(vocab=0), BAD), (dict(vocab=(1 << 22) + 1), NOT_BUILT), (dict(logits=None), BAD),
+    (dict(rows=0), BAD), (dict(vocab=0), BAD), (dict(vocab=(1 << 21) + 1), NOT_BUILT), (dict(logits=None), BAD),
     (dict(uniform=None), BAD), (dict(tokens=None), BAD), (dict(dtype=9), BAD)])
 def test_sample_refuses(over, code):
     a = _lib.SampleArgs(rows=1, vocab=8, dtype=0, logits=THERE, row_stride=8, uniform=THERE, temperature_value=1.0,

@@ -840,7 +840,7 @@ std::pair<Tensor, Tensor> sample_run(const Tensor& logits, const Tensor& uniform
   TORCH_CHECK_VALUE(uniform.scalar_type() == at::kFloat && uniform.sizes() == logits.sizes().slice(0, logits.dim() - 1),
                     "uniform must be float32 ", logits.sizes().slice(0, logits.dim() - 1), ", got ", uniform.scalar_type(), " ",
                     uniform.sizes());
-  TORCH_CHECK_NOT_IMPLEMENTED(vocab <= (1 << 22) && rows <= (1 << 27), "sample_tokens: more than 2^22 tokens or 2^27 rows");
+  TORCH_CHECK_NOT_IMPLEMENTED(vocab <= (1 << 21) && rows <= (1 << 27), "sample_tokens: more than 2^21 tokens or 2^27 rows");
   TORCH_CHECK_VALUE(temperature || (temperature_value >= 0 && std::isfinite(temperature_value)),
                     "temperature must be >= 0 and finite, got ", temperature_value);
   TORCH_CHECK_VALUE(top_k || top_k_value >= 0, "top_k must be >= 1, got ", top_k_value);

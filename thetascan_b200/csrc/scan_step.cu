@@ -92,6 +92,8 @@ __global__ void __launch_bounds__(kScanStepThreads) scan_step_kernel(const __gri
 
 }  // namespace ts
 
+using namespace ts;
+
 extern "C" int ts_b200_scan_step(const ts_scan_step_args* a, ts_stream_t stream) {
   if (!a) return set_error(TS_ERR_VALUE, "scan_step: null arguments");
   if (a->batch < 1 || a->heads < 1) return set_error(TS_ERR_VALUE, "scan_step: batch and heads must be >= 1");

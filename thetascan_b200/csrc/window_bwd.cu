@@ -771,6 +771,8 @@ int window_bwd_launch(WinBwdParams& p, cudaStream_t s) {
 
 }  // namespace ts
 
+using namespace ts;
+
 extern "C" {
 
 size_t ts_b200_window_bwd_workspace_bytes(const ts_window_args* a) {

@@ -295,6 +295,8 @@ int window_step_launch(const WinStepParams& p, int cluster, cudaStream_t s) {
 
 }  // namespace ts
 
+using namespace ts;
+
 extern "C" {
 
 int ts_b200_window_step(const ts_window_step_args* a, ts_stream_t stream) {

@@ -18,12 +18,54 @@ constexpr int kWinWarps = 12;                  // 0-7: two groups of row warps, 
 constexpr int kWinThreads = 32 * kWinWarps;
 constexpr float kLog2e = 1.4426950408889634f;
 
+// A division by a constant of the launch.
+struct Divisor {
+  unsigned by, factor;   // factor: 2^32 / by, rounded up
+  static Divisor of(int by) {
+    return Divisor{static_cast<unsigned>(by), by > 1 ? static_cast<unsigned>(((1ull << 32) + by - 1) / by) : 0u};
+  }
+  // n below 2^31: the product is the quotient, or one more
+  __device__ __forceinline__ int operator()(int n) const {
+    if (by == 1) return n;
+    const unsigned q = __umulhi(static_cast<unsigned>(n), factor);
+    return static_cast<int>(q * by > static_cast<unsigned>(n) ? q - 1 : q);
+  }
+};
+
+// The K-major operand (rows = M or N) and the MN-major one (rows = inner) of a 128-byte-swizzled tile of 128 rows
+// in 64-column boxes, at inner step s of 16.
+__device__ __forceinline__ uint64_t win_rows(uint32_t tile, int s) {
+  return smem_desc_sw128(tile + (s >> 2) * kSwBox + (s & 3) * 32, 16, 1024);
+}
+__device__ __forceinline__ uint64_t win_inner(uint32_t tile, int s) {
+  return smem_desc_sw128(tile + 2048 * s, kSwBox, 1024);
+}
+
+// The two operands again, from the descriptor of step 0: the address field counts 16 bytes and has room for all of
+// shared memory, so that a step is an addition.
+__device__ __forceinline__ uint64_t win_rows_step(uint64_t first, int s) {
+  return first + ((s >> 2) * (kSwBox >> 4) + (s & 3) * 2);
+}
+__device__ __forceinline__ uint64_t win_inner_step(uint64_t first, int s) { return first + 128 * s; }
+
+// One lane of a converged warp.  The warps that feed the tensor cores run with all lanes and let one issue, so that
+// addresses stay in uniform registers (a single lane's loop took 120 cycles for each instruction of 64).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+  return one != 0;
+}
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, int code) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, code));
+}
+
 struct WinSizes {
   int batch, heads, kv_heads, share;   // share: query heads to a key head
   int dim;
   int q_tokens, kv_tokens, past;       // past: kv_tokens - q_tokens
   int window, sinks;                   // both at most kv_tokens
   int q_tiles;
+  Divisor by_share, by_kv_heads;
   float scale;
   const int* lengths;                  // or null
 };
@@ -77,38 +119,71 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// (Of numbers; a NaN is left out.)
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
 
-// The K-major operand (rows = M or N) and the MN-major one (rows = inner) of a 128-byte-swizzled tile of 128 rows
-// in 64-column boxes, at inner step s of 16.
-__device__ __forceinline__ uint64_t win_rows(uint32_t tile, int s) {
-  return smem_desc_sw128(tile + (s >> 2) * kSwBox + (s & 3) * 32, 16, 1024);
+// Two f32 side by side: one instruction for both.
+struct Pair {
+  uint64_t v;
+  __device__ __forceinline__ Pair() {}
+  __device__ __forceinline__ Pair(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+  __device__ __forceinline__ explicit Pair(float a) : Pair(a, a) {}
+  __device__ __forceinline__ void get(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+};
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return d;
 }
-__device__ __forceinline__ uint64_t win_inner(uint32_t tile, int s) {
-  return smem_desc_sw128(tile + 2048 * s, kSwBox, 1024);
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+  Pair d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+  return d;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+  Pair d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+  return d;
 }
 
-// The two operands again, from the descriptor of step 0: the address field counts 16 bytes and has room for all of
-// shared memory, so that a step is an addition.
-__device__ __forceinline__ uint64_t win_rows_step(uint64_t first, int s) {
-  return first + ((s >> 2) * (kSwBox >> 4) + (s & 3) * 2);
+// 2^x of two, without the special function unit (16 a cycle, which bounds a softmax): the nearest integer from the low
+// bits of a sum with 1.5 2^23, the rest by a polynomial of degree 3 on [-1/2, 1/2], fitted here (relative error 1.0e-4,
+// 2.3e-5 on average; 1 at 0): the weight is rounded to bf16 next, by up to 3.9e-3.  Exactly 0 from -127 down; a NaN stays
+// one.
+__device__ __forceinline__ void exp2_poly(Pair x, float& a, float& b) {
+  float u, v;
+  x.get(u, v);
+  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(u));
+  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(v));
+  const Pair t(u, v), near = add2(t, Pair(12582912.f)), whole = add2(near, Pair(-12582912.f));
+  const Pair f = fma2(whole, Pair(-1.f), t);
+  Pair e = fma2(f, Pair(0.05500892177224159f), Pair(0.2422109693288803f));
+  e = fma2(e, f, Pair(0.6932829022407532f));
+  e = fma2(e, f, Pair(1.f));
+  float nu, nv;
+  near.get(nu, nv);
+  mul2(e, Pair(__int_as_float((__float_as_int(nu) << 23) + 0x3f800000), __int_as_float((__float_as_int(nv) << 23) + 0x3f800000)))
+      .get(a, b);
 }
-__device__ __forceinline__ uint64_t win_inner_step(uint64_t first, int s) { return first + 128 * s; }
 
-// One lane of a converged warp.  The warps that feed the tensor cores run with all lanes and let one issue, so that
-// addresses stay in uniform registers (a single lane's loop took 120 cycles for each instruction of 64).
-__device__ __forceinline__ bool elect_one() {
-  uint32_t one;
-  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
-  return one != 0;
+// A division by a constant of the launch.
+
+// Give up registers of a warpgroup, or take more.
+template <int kRegs>
+__device__ __forceinline__ void win_fewer_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
 }
-__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, int code) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, code));
+template <int kRegs>
+__device__ __forceinline__ void win_more_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
 }
+// Of the 64512 registers that 384 threads of 168 are launched with: 8 row warps of 200 and 4 others of 96 take 63488.
+constexpr int kWinRowRegs = 200, kWinOtherRegs = 96;
+static_assert(32 * (8 * kWinRowRegs + 4 * kWinOtherRegs) <= kWinThreads * 168, "registers");
 
 // Host: a [batch, heads, tokens, dim] tensor as boxes of 64 columns x `rows` tokens.
 bool win_map(CUtensorMap* map, const void* base, const long long* strides, int batch, int heads, int tokens, int dim,

@@ -6,8 +6,7 @@
 // One pass over the keys with a running reference m_i and sum.  A CTA takes two
 // tiles of 128 queries at a time, A and B: of two heads that share a key head, or
 // neighbours of one head, so that both read the same keys.  Warp 8 feeds a ring of
-// key and value tiles by TMA, a thread of warp 9 issues the matrix instructions,
-// warps 0-3 and 4-7 each own the rows of one query tile, a row to a thread.
+// key and value tiles by TMA, warps 9 and 11 issue the matrix instructions, warps 0-3 and 4-7 each own the rows of one query tile, a row to a thread.
 // S = Q K^T lies in tensor memory, 128 columns for each of A and B; P replaces it
 // there in bf16 and is the operand of O += P V from where it lies.  While one
 // group forms its P the tensor cores work for the other.
@@ -42,6 +41,7 @@ struct WinFwdParams {
   CUtensorMap q, k, v, k_sink, v_sink, y;
   WinSizes w;
   int pairs, units;
+  Divisor by_pairs;
   int sink_rows;         // rows of a sink box
   float* lse;            // or null
 };
@@ -63,7 +63,7 @@ struct WinFwdUnit {
 
   __device__ __forceinline__ WinFwdTile place(const WinSizes& w, int at) const {
     WinFwdTile t;
-    t.tile = at / w.share;
+    t.tile = w.by_share(at);
     t.head = kv_head * w.share + at - t.tile * w.share;
     t.exists = t.tile < w.q_tiles;
     t.live = t.exists && w.past + 128 * t.tile < length;
@@ -71,8 +71,8 @@ struct WinFwdUnit {
   }
   __device__ __forceinline__ WinFwdUnit(const WinFwdParams& p, int unit) {
     const WinSizes& w = p.w;
-    const int row = unit / p.pairs, pair = unit - row * p.pairs;
-    b = row / w.kv_heads;
+    const int row = p.by_pairs(unit), pair = unit - row * p.pairs;
+    b = w.by_kv_heads(row);
     kv_head = row - b * w.kv_heads;
     length = win_length(w, b);
     a = place(w, 2 * pair);
@@ -111,13 +111,13 @@ struct WinFwdUnit {
   }
 };
 
-// The row's scores are read twice, 32 columns at a time: 128 of them in registers spill, and what spills beside this
-// much shared memory goes to L2 (16 heads x 16384, width 128, window 2048: 560 us).  Tiles that are masked or narrow go
-// by a loop over their columns, the others without one.
 struct RowColumns {
   int cols, from, until;   // the tile's, and this row's first and last visible one
   bool masked;
+  // whether none of the warp's rows sees any of the 32 columns from c on
+  __device__ __forceinline__ bool none(int c) const { return masked && __all_sync(0xffffffffu, until < c || from > c + 31); }
   __device__ __forceinline__ void hide(uint32_t (&s)[32], int c) const {
+    if (__all_sync(0xffffffffu, from <= c && until >= c + 31)) return;
     const uint32_t bits = bit_range(from - c, until - c);
 #pragma unroll
     for (int e = 0; e < 32; ++e)
@@ -125,91 +125,33 @@ struct RowColumns {
   }
 };
 
-__device__ __forceinline__ void row_top(const uint32_t (&s)[32], float (&top)[2]) {
-#pragma unroll
-  for (int e = 0; e < 32; e += 4) {
-    top[0] = max3(top[0], __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
-    top[1] = max3(top[1], __uint_as_float(s[e + 2]), __uint_as_float(s[e + 3]));
-  }
-}
-
-// The largest visible score of the row that starts at `at` in tensor memory.
-__device__ __forceinline__ float row_max(uint32_t at, const RowColumns& r) {
-  float top[2] = {-INFINITY, -INFINITY};
-  if (r.masked) {
-#pragma unroll 1
-    for (int c = 0; c < r.cols; c += 32) {
-      uint32_t s[32];
-      tmem_ld(at + c, s);
-      tmem_wait();
-      tie(s);
-      r.hide(s, c);
-      row_top(s, top);
-    }
-  } else {
-#pragma unroll
-    for (int c = 0; c < 128; c += 64) {
-      uint32_t s[32], t[32];
-      tmem_ld(at + c, s);
-      tmem_ld(at + c + 32, t);
-      tmem_wait();
-      tie(s);
-      tie(t);
-      row_top(s, top);
-      row_top(t, top);
-    }
-  }
-  return fmaxf(top[0], top[1]);
-}
-
-__device__ __forceinline__ void row_exp(const uint32_t (&s)[32], uint32_t at, float scale2, float origin,
-                                        float (&part)[4]) {
+// 32 scores to weights in bf16, their sum to `part`.  Half of the exponentials go by exp2_poly, beside the special
+// function unit.
+__device__ __forceinline__ void row_exp(const uint32_t (&s)[32], uint32_t to, Pair scale2, Pair origin, Pair (&part)[2]) {
   uint32_t packed[16];
 #pragma unroll
   for (int e = 0; e < 32; e += 2) {
-    const float a = exp2_fast(fmaf(__uint_as_float(s[e]), scale2, -origin));
-    const float b = exp2_fast(fmaf(__uint_as_float(s[e + 1]), scale2, -origin));
-    part[e & 2] += a;
-    part[(e & 2) + 1] += b;
+    const Pair x = fma2(Pair(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), scale2, origin);
+    float a, b;
+    if (false && e & 2) {
+      exp2_poly(x, a, b);
+    } else {
+      x.get(a, b);
+      a = exp2_fast(a);
+      b = exp2_fast(b);
+    }
+    part[e >> 1 & 1] = add2(part[e >> 1 & 1], Pair(a, b));
     packed[e / 2] = pack_bf16(a, b);
   }
-  tmem_st(at, packed);
-}
-
-// Scores to weights in their place, in bf16; returns the sum of the weights (before their rounding).
-__device__ __forceinline__ float row_weights(uint32_t at, const RowColumns& r, float scale2, float origin) {
-  float part[4] = {0.f, 0.f, 0.f, 0.f};
-  if (r.masked) {
-#pragma unroll 1
-    for (int c = 0; c < r.cols; c += 32) {
-      uint32_t s[32];
-      tmem_ld(at + c, s);
-      tmem_wait();
-      tie(s);
-      r.hide(s, c);
-      row_exp(s, at + c / 2, scale2, origin, part);
-    }
-  } else {
-#pragma unroll
-    for (int c = 0; c < 128; c += 64) {
-      uint32_t s[32], t[32];
-      tmem_ld(at + c, s);
-      tmem_ld(at + c + 32, t);
-      tmem_wait();
-      tie(s);
-      tie(t);
-      row_exp(s, at + c / 2, scale2, origin, part);
-      row_exp(t, at + c / 2 + 16, scale2, origin, part);
-    }
-  }
-  return (part[0] + part[2]) + (part[1] + part[3]);
+  tmem_st(to, packed);
 }
 
 template <int kD>
 __global__ void __launch_bounds__(kWinThreads, 1) window_fwd_kernel(const __grid_constant__ WinFwdParams p) {
   using L = WinFwdLayout<kD>;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ alignas(8) uint64_t full[L::kSlots], empty[L::kSlots], q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2];
+  __shared__ alignas(8) uint64_t full[L::kSlots], empty[L::kSlots], q_full[2], q_empty[2], s_full[2], s_free[2], p_full[2],
+      p_free[2], o_full[2];
   __shared__ uint32_t tmem_slot;
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -217,13 +159,15 @@ __global__ void __launch_bounds__(kWinThreads, 1) window_fwd_kernel(const __grid
   if (threadIdx.x == 0) {
     for (int i = 0; i < L::kSlots; ++i) {
       mbar_init(&full[i], 1);
-      mbar_init(&empty[i], 1);
+      mbar_init(&empty[i], kD == 64 ? 2 : 1);   // the warps that issue instructions
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_full[i], 1);
       mbar_init(&q_empty[i], 1);
       mbar_init(&s_full[i], 1);
+      mbar_init(&s_free[i], 4);
       mbar_init(&p_full[i], 4);
+      mbar_init(&p_free[i], 1);
       mbar_init(&o_full[i], 1);
     }
     fence_mbar_init();
@@ -232,10 +176,13 @@ __global__ void __launch_bounds__(kWinThreads, 1) window_fwd_kernel(const __grid
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  // all of tensor memory: its addresses start at 0.  Columns: S of A and B, then O of A and B
-  constexpr uint32_t kScores = 128, kO = 256;
+  // all of tensor memory: its addresses start at 0.  Columns: S of A and B, then O of A and B.  P lies in S's place, or,
+  // where O is narrow, behind O: the next S then need not wait for the product with P.
+  constexpr bool kApart = kD == 64;
+  constexpr uint32_t kScores = 128, kO = 256, kP = kApart ? 384 : 0, kPStride = kApart ? 64 : kScores;
 
   if (warp >= 8) {
+    win_fewer_registers<kWinOtherRegs>();
     if (warp == 8) {
       // ---- loads
       uint32_t it = 0, q_turn[2] = {0, 0};
@@ -282,131 +229,294 @@ __global__ void __launch_bounds__(kWinThreads, 1) window_fwd_kernel(const __grid
           for (int poll = 0; poll < (1 << 16) && q_turn[x] > 0 && !mbar_try_wait(&q_full[x], (q_turn[x] - 1) & 1); ++poll) {
           }
       }
-    } else if (warp == 9) {
-      // ---- instructions
-      uint32_t it = 0, q_turn[2] = {0, 0}, p_turn[2] = {0, 0};
+    } else if (!kApart && warp == 9) {
+      // ---- instructions, where P takes S's place: one warp, each tile's products with P and then with the next keys,
+      // in turn, so that a product has the tensor cores to itself.  This warp's own steps come between the tensor
+      // cores': little is worked out here.
+      constexpr uint32_t id_o = idesc_bf16(128, kD, false, true), id_s = idesc_bf16(128, 128, false, false);
+      constexpr uint32_t kSlotStep = L::kTileBytes >> 4;
+      const uint64_t q0 = win_rows(base + L::kQ, 0), k0 = win_rows(base + L::kRing, 0), v0 = win_inner(base + L::kRing, 0);
+      // the ring's next key tile and its next value tile: their slots and parities
+      uint32_t k_slot = 0, k_parity = 0, v_slot = 1, v_parity = 0;
+      uint32_t q_parity[2] = {0, 0}, p_parity[2] = {0, 0};
       bool ok = true;
-      constexpr uint32_t id_o = idesc_bf16(128, kD, false, true);
-      auto landed = [&](uint32_t item) {
-        ok = ok && mbar_wait_warp(&full[item % L::kSlots], (item / L::kSlots) & 1, kErrCopyTimeout);
-        tc_fence_after();
-        return ok;
-      };
       for (int unit = blockIdx.x; unit < p.units && ok; unit += gridDim.x) {
         const WinFwdUnit u(p, unit);
-        bool begun[2] = {false, false}, summed[2] = {false, false};
-        // S of query tile x against key tile n, which lies in ring item `item`
-        auto scores = [&](int x, int n, uint32_t item) {
-          if (!begun[x]) {
-            if (!(ok = ok && mbar_wait_warp(&q_full[x], q_turn[x]++ & 1, kErrCopyTimeout))) return;
-            begun[x] = true;
-            tc_fence_after();
+        // tile x takes part in the first tokens' (n < sink_tiles) and from `low` to `last`
+        const int low[2] = {0, u.sink_tiles + u.z.low - u.first}, last[2] = {u.a.live ? u.a.last : -1, u.z.live ? u.z.last : -1};
+        auto active = [&](int x, int n) { return n <= last[x] && (x == 0 || n < u.sink_tiles || n >= low[x]); };
+        auto keys_landed = [&] { return ok = ok && mbar_wait_warp(&full[k_slot], k_parity, kErrCopyTimeout); };
+        auto keys_done = [&] {
+          if (ok && elect_one()) mma_commit(&empty[k_slot]);
+          k_slot += 2;
+          if (k_slot >= L::kSlots) {
+            k_slot -= L::kSlots;
+            k_parity ^= 1;
           }
-          const uint32_t id = idesc_bf16(128, u.columns(n), false, false);
-          const uint64_t a = win_rows(base + L::kQ + x * L::kTileBytes, 0);
-          const uint64_t k = win_rows(base + L::kRing + item % L::kSlots * L::kTileBytes, 0);
-          if (elect_one()) {
+        };
+        // Q of tile x, before its first product
+        auto queries_landed = [&](int x, int n) {
+          if (n == 0 || (x == 1 && u.sink_tiles == 0 && n == low[1])) {
+            ok = ok && mbar_wait_warp(&q_full[x], q_parity[x], kErrCopyTimeout);
+            q_parity[x] ^= 1;
+          }
+        };
+        // S of query tile x against the next key tile, n in the list; by one lane
+        auto scores = [&](int x, int n) {
+          const uint32_t id = n < u.sink_tiles ? idesc_bf16(128, u.columns(n), false, false) : id_s;
+          const uint64_t q = q0 + x * kSlotStep, k = k0 + k_slot * kSlotStep;
 #pragma unroll
-            for (int s = 0; s < kD / 16; ++s)
-              mma_bf16(kScores * x, win_rows_step(a, s), win_rows_step(k, s), id, s > 0);
-            mma_commit(&s_full[x]);
-            if (n == u.of(x).last) mma_commit(&q_empty[x]);
+          for (int s = 0; s < kD / 16; ++s) mma_bf16(kScores * x, win_rows_step(q, s), win_rows_step(k, s), id, s > 0);
+          mma_commit(&s_full[x]);
+          if (n == last[x]) mma_commit(&q_empty[x]);
+        };
+        // O += P V with the next value tile, and then the next S, without a pause between them
+        auto step = [&](int x, int n, bool more) {
+          const bool now = active(x, n), then = more && active(x, n + 1);
+          if (then) queries_landed(x, n + 1);
+          if (now) {
+            ok = ok && mbar_wait_warp(&p_full[x], p_parity[x], kErrMmaTimeout);
+            p_parity[x] ^= 1;
+          }
+          if (!ok) return;
+          tc_fence_after();
+          const bool summed = x == 0 || u.sink_tiles > 0 ? n > 0 : n > low[1];
+          const uint64_t v = v0 + v_slot * kSlotStep;
+          const int steps = u.columns(n) >> 4;
+          if (elect_one()) {
+            if (now) {
+#pragma unroll
+              for (int s = 0; s < 8; ++s)
+                if (s < steps) mma_bf16_ts(kO + kD * x, kP + kPStride * x + 8 * s, win_inner_step(v, s), id_o, summed || s > 0);
+              if (n == last[x]) mma_commit(&o_full[x]);
+            }
+            if (then) scores(x, n + 1);
           }
         };
         if (u.count > 0) {
-          if (!landed(it)) break;
-#pragma unroll
-          for (int x = 0; x < 2; ++x)
-            if (u.active(u.of(x), 0)) scores(x, 0, it);
-          if (ok && elect_one()) mma_commit(&empty[it % L::kSlots]);
-        }
-        for (int n = 0; n < u.count && ok; ++n, it += 2) {
-          const uint32_t item = it + 1;
-          if (!landed(item)) break;
-          const uint64_t v = win_inner(base + L::kRing + item % L::kSlots * L::kTileBytes, 0);
-          const bool more = n + 1 < u.count;
-          const int steps = u.columns(n) >> 4;
+          if (!keys_landed()) break;
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            if (ok && u.active(u.of(x), n)) {
-              if (!(ok = mbar_wait_warp(&p_full[x], p_turn[x]++ & 1, kErrMmaTimeout))) break;
-              tc_fence_after();
-              if (elect_one()) {
+            if (!active(x, 0)) continue;
+            queries_landed(x, 0);
+            tc_fence_after();
+            if (ok && elect_one()) scores(x, 0);
+          }
+          keys_done();
+        }
+        for (int n = 0; n < u.count && ok; ++n) {
+          const bool more = n + 1 < u.count;
+          if (!(ok = ok && mbar_wait_warp(&full[v_slot], v_parity, kErrCopyTimeout))) break;
+          if (more && !keys_landed()) break;
+          step(0, n, more);
+          step(1, n, more);
+          if (ok && elect_one()) mma_commit(&empty[v_slot]);
+          if (more) keys_done();
+          v_slot += 2;
+          if (v_slot >= L::kSlots) {
+            v_slot -= L::kSlots;
+            v_parity ^= 1;
+          }
+        }
+      }
+    } else if (kApart && warp != 10) {
+      // ---- instructions: warp 9 for tile A, warp 11 for B, so that neither waits for the other's rows.  These warps' own
+      // steps come between the tensor cores': little is worked out here.
+      const int x = warp == 9 ? 0 : 1;
+      constexpr uint32_t id_o = idesc_bf16(128, kD, false, true), id_s = idesc_bf16(128, 128, false, false);
+      constexpr uint32_t kSlotStep = L::kTileBytes >> 4;
+      const uint64_t q0 = win_rows(base + L::kQ, 0) + x * kSlotStep;
+      const uint64_t k0 = win_rows(base + L::kRing, 0), v0 = win_inner(base + L::kRing, 0);
+      const uint32_t s_to = kScores * x, p_at = kP + kPStride * x, o_to = kO + kD * x;
+      uint64_t* const done_s = &s_full[x];
+      // the ring's next key tile and its next value tile: their slots and parities
+      uint32_t k_slot = 0, k_parity = 0, v_slot = 1, v_parity = 0;
+      uint32_t q_parity = 0, s_parity = 1, p_parity = 0;
+      bool ok = true;
+      for (int unit = blockIdx.x; unit < p.units && ok; unit += gridDim.x) {
+        const WinFwdUnit u(p, unit);
+        const WinFwdTile mine = u.of(x);
+        // this tile takes part in the first tokens' (n < sink_tiles) and from `low` to `last`
+        const int low = u.sink_tiles + mine.low - u.first, last = mine.live ? mine.last : -1;
+        const int begin = u.sink_tiles > 0 ? 0 : low;
+        auto active = [&](int n) { return n <= last && (n < u.sink_tiles || n >= low); };
+        // S against the next key tile, n in the list
+        auto scores = [&](int n) {
+          if (!(ok = ok && mbar_wait_warp(&full[k_slot], k_parity, kErrCopyTimeout))) return;
+          if (active(n)) {
+            if (n == begin) {
+              ok = ok && mbar_wait_warp(&q_full[x], q_parity, kErrCopyTimeout);
+              q_parity ^= 1;
+            }
+            ok = ok && mbar_wait_warp(&s_free[x], s_parity, kErrMmaTimeout);
+            s_parity ^= 1;
+            if (!ok) return;
+            tc_fence_after();
+            const uint32_t id = n < u.sink_tiles ? idesc_bf16(128, u.columns(n), false, false) : id_s;
+            const uint64_t k = k0 + k_slot * kSlotStep;
+            if (elect_one()) {
 #pragma unroll
-                for (int s = 0; s < 8; ++s)
-                  if (s < steps)
-                    mma_bf16_ts(kO + kD * x, kScores * x + 8 * s, win_inner_step(v, s), id_o, summed[x] || s > 0);
-                if (n == u.of(x).last) mma_commit(&o_full[x]);
+              for (int s = 0; s < kD / 16; ++s) mma_bf16(s_to, win_rows_step(q0, s), win_rows_step(k, s), id, s > 0);
+              mma_commit(done_s);
+              mma_commit(&empty[k_slot]);
+              if (n == last) mma_commit(&q_empty[x]);
+            }
+          } else if (elect_one()) {
+            mbar_arrive(&empty[k_slot]);
+          }
+          k_slot += 2;
+          if (k_slot >= L::kSlots) {
+            k_slot -= L::kSlots;
+            k_parity ^= 1;
+          }
+        };
+        // O += P V with the next value tile
+        auto sums = [&](int n) {
+          if (!(ok = ok && mbar_wait_warp(&full[v_slot], v_parity, kErrCopyTimeout))) return;
+          if (active(n)) {
+            ok = mbar_wait_warp(&p_full[x], p_parity, kErrMmaTimeout);
+            p_parity ^= 1;
+            if (!ok) return;
+            tc_fence_after();
+            const uint64_t v = v0 + v_slot * kSlotStep;
+            if (elect_one()) {
+              if (n >= u.sink_tiles) {
+#pragma unroll
+                for (int s = 0; s < 8; ++s) mma_bf16_ts(o_to, p_at + 8 * s, win_inner_step(v, s), id_o, n > begin || s > 0);
+              } else {
+                const int steps = u.columns(n) >> 4;
+                for (int s = 0; s < steps; ++s)
+                  mma_bf16_ts(o_to, p_at + 8 * s, win_inner_step(v, s), id_o, n > begin || s > 0);
               }
-              summed[x] = true;
+              mma_commit(&p_free[x]);
+              mma_commit(&empty[v_slot]);
+              if (n == last) mma_commit(&o_full[x]);
             }
-            if (ok && more && u.active(u.of(x), n + 1)) {
-              if (!landed(it + 2)) break;
-              scores(x, n + 1, it + 2);
-            }
+          } else if (elect_one()) {
+            mbar_arrive(&empty[v_slot]);
           }
-          if (!ok) break;
-          if (elect_one()) {
-            mma_commit(&empty[item % L::kSlots]);
-            if (more) mma_commit(&empty[(it + 2) % L::kSlots]);
+          v_slot += 2;
+          if (v_slot >= L::kSlots) {
+            v_slot -= L::kSlots;
+            v_parity ^= 1;
           }
+        };
+        for (int n = 0; n <= u.count && u.count > 0 && ok; ++n) {
+          if (n < u.count) scores(n);
+          if (n > 0) sums(n - 1);
         }
       }
     }
   } else {
     // ---- rows: thread t of group x owns row t of tile x
+    win_more_registers<kWinRowRegs>();
     const int x = warp >> 2, quad = warp & 3, row = 32 * quad + lane;
     const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
-    const uint32_t s_at = kScores * x + lanes, o_at = kO + kD * x + lanes;
+    const uint32_t s_at = kScores * x + lanes, p_at = kP + kPStride * x + lanes, o_at = kO + kD * x + lanes;
     const uint32_t stage = base + L::kOut + warp * L::kOutBytes;
     const float scale2 = w.scale * kLog2e;
-    uint32_t s_turn = 0, o_turn = 0;
+    uint32_t turn = 0, o_turn = 0;
     bool ok = true;
+    auto signal = [&](uint64_t* bar) {
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar);
+    };
+    WinFwdUnit next(p, blockIdx.x);
     for (int unit = blockIdx.x; unit < p.units && ok; unit += gridDim.x) {
-      const WinFwdUnit u(p, unit);
+      const WinFwdUnit u = next;
       const WinFwdTile mine = u.of(x);
-      if (!mine.exists) continue;
+      if (!mine.exists) {
+        if (unit + gridDim.x < p.units) next = WinFwdUnit(p, unit + gridDim.x);
+        continue;
+      }
       const int q_row = 128 * mine.tile + row, at = w.past + q_row;
       const int near = max(at - w.window + 1, u.sinks), to = at < u.length ? at : -1;   // visible: first ones, near..to
       float ref = -INFINITY, sum = 0.f;
       bool first = true;
-      for (int n = 0; n < u.count; ++n) {
-        if (!u.active(mine, n)) continue;
+      // first tokens, then the window's own
+      for (int n = 0; mine.live && n <= mine.last; ++n, ++turn) {
+        if (n == u.sink_tiles) n += mine.low - u.first;
         const int cols = u.columns(n), key = u.key(w, n);
         const bool sink = n < u.sink_tiles;
-        if (!(ok = mbar_wait(&s_full[x], s_turn++ & 1, kErrMmaTimeout))) break;
-        tc_fence_after();
         // this row's first and last visible column; a tile within reach of all rows is not masked
         const int from = sink ? 0 : near - key, until = min(to, sink ? u.sinks - 1 : to) - key;
         const RowColumns r{cols, from, until, !__all_sync(0xffffffffu, from <= 0 && until >= 127)};
-        const float best = row_max(s_at, r) * scale2;
+        if (!(ok = mbar_wait(&s_full[x], turn & 1, kErrMmaTimeout))) break;
+        tc_fence_after();
+        uint32_t s[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld(s_at + 32 * c, s[c]);
+        tmem_wait();
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tie(s[c]);
+        if (kApart) signal(&s_free[x]);
+        if (r.masked) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) r.hide(s[c], 32 * c);
+        }
+        // eight chains side by side: a warp has its scheduler almost to itself, and each step waits for the one before
+        float top[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top[i] = __uint_as_float(s[i >> 1][16 * (i & 1)]);
+#pragma unroll
+        for (int e = 1; e < 15; e += 2)
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            top[i] = max3(top[i], __uint_as_float(s[i >> 1][16 * (i & 1) + e]), __uint_as_float(s[i >> 1][16 * (i & 1) + e + 1]));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top[i] = fmaxf(top[i], __uint_as_float(s[i >> 1][16 * (i & 1) + 15]));
+        const float best = fmaxf(max3(max3(top[0], top[1], top[2]), top[3], top[4]), max3(top[5], top[6], top[7])) * scale2;
+        if (kApart) {
+          if (!(ok = mbar_wait(&p_free[x], (turn & 1) ^ 1, kErrMmaTimeout))) break;
+          tc_fence_after();
+        }
+        // The row's reference: the largest score of its first tile, and later one that exceeds it by 2^8.  (A NaN is not
+        // at most anything: it becomes the reference, and with it the row.)
         if (first) {
           ref = best;
           first = false;
-        } else if (__any_sync(0xffffffffu, best > ref + 8.f)) {
-          const float next = best > ref + 8.f ? best : ref;
+        } else if (__any_sync(0xffffffffu, !(best <= ref + 8.f))) {
+          const float next = best <= ref + 8.f ? ref : best;
           const float factor = next == ref ? 1.f : exp2_fast(ref - next);
           ref = next;
           sum *= factor;
 #pragma unroll 1
-          for (int c = 0; c < kD; c += 32) {
-            uint32_t o[32];
+          for (int c = 0; c < kD; c += 16) {
+            uint32_t o[16];
             tmem_ld(o_at + c, o);
             tmem_wait();
             tie(o);
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
             tmem_st(o_at + c, o);
           }
         }
-        const float origin = ref == -INFINITY ? 0.f : ref;
-        sum += row_weights(s_at, r, scale2, origin);
+        const Pair scales(scale2), origin(ref == -INFINITY ? 0.f : -ref);
+        Pair part[2] = {Pair(sum, 0.f), Pair(0.f)};
+        if (!kApart && !r.masked) {   // (twice the code is worth it where most tiles have no mask)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) row_exp(s[c], p_at + 16 * c, scales, origin, part);
+        } else {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            if (32 * c >= cols) continue;
+            if (r.none(32 * c)) {
+              const uint32_t zero[16] = {};
+              tmem_st(p_at + 16 * c, zero);
+            } else {
+              row_exp(s[c], p_at + 16 * c, scales, origin, part);
+            }
+          }
+        }
+        float even, odd;
+        add2(part[0], part[1]).get(even, odd);
+        sum = even + odd;
         tmem_store_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[x]);
+        signal(&p_full[x]);
       }
       if (!ok) break;
+      if (unit + gridDim.x < p.units) next = WinFwdUnit(p, unit + gridDim.x);   // while the last product runs
       if (mine.live && !(ok = mbar_wait(&o_full[x], o_turn++ & 1, kErrMmaTimeout))) break;
       tc_fence_after();
       // a row that sees nothing has no sum: zero
@@ -499,6 +609,8 @@ int win_sizes(const ts_window_args* a, WinSizes* w, const char* what) {
   w->window = a->window < a->kv_tokens ? a->window : a->kv_tokens;
   w->sinks = a->sinks < a->kv_tokens ? a->sinks : a->kv_tokens;
   w->q_tiles = ceil_div(a->q_tokens, 128);
+  w->by_share = Divisor::of(w->share);
+  w->by_kv_heads = Divisor::of(w->kv_heads);
   w->scale = a->scale;
   w->lengths = a->lengths;
   const long long units = static_cast<long long>(w->batch) * w->heads * (w->q_tiles + 1);
@@ -518,6 +630,7 @@ int ts_b200_window_fwd(const ts_window_args* a, ts_stream_t stream) {
   if (!a->y) return set_error(TS_ERR_VALUE, "window_fwd: null output");
   const WinSizes& w = p.w;
   p.pairs = (w.q_tiles * w.share + 1) / 2;
+  p.by_pairs = Divisor::of(p.pairs);
   p.units = w.batch * w.kv_heads * p.pairs;
   p.sink_rows = w.sinks >= 128 ? 128 : round_up(w.sinks > 0 ? w.sinks : 1, 16);
   p.lse = a->lse;

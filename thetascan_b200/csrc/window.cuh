@@ -14,8 +14,6 @@
 
 namespace ts {
 
-constexpr int kWinWarps = 12;                  // 0-7: two groups of row warps, 8: loads, 9: instructions, 10: tensor memory
-constexpr int kWinThreads = 32 * kWinWarps;
 constexpr float kLog2e = 1.4426950408889634f;
 
 // A division by a constant of the launch.
@@ -32,33 +30,6 @@ struct Divisor {
   }
 };
 
-// The K-major operand (rows = M or N) and the MN-major one (rows = inner) of a 128-byte-swizzled tile of 128 rows
-// in 64-column boxes, at inner step s of 16.
-__device__ __forceinline__ uint64_t win_rows(uint32_t tile, int s) {
-  return smem_desc_sw128(tile + (s >> 2) * kSwBox + (s & 3) * 32, 16, 1024);
-}
-__device__ __forceinline__ uint64_t win_inner(uint32_t tile, int s) {
-  return smem_desc_sw128(tile + 2048 * s, kSwBox, 1024);
-}
-
-// The two operands again, from the descriptor of step 0: the address field counts 16 bytes and has room for all of
-// shared memory, so that a step is an addition.
-__device__ __forceinline__ uint64_t win_rows_step(uint64_t first, int s) {
-  return first + ((s >> 2) * (kSwBox >> 4) + (s & 3) * 2);
-}
-__device__ __forceinline__ uint64_t win_inner_step(uint64_t first, int s) { return first + 128 * s; }
-
-// One lane of a converged warp.  The warps that feed the tensor cores run with all lanes and let one issue, so that
-// addresses stay in uniform registers (a single lane's loop took 120 cycles for each instruction of 64).
-__device__ __forceinline__ bool elect_one() {
-  uint32_t one;
-  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
-  return one != 0;
-}
-__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, int code) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, code));
-}
-
 struct WinSizes {
   int batch, heads, kv_heads, share;   // share: query heads to a key head
   int dim;
@@ -74,6 +45,8 @@ __device__ __forceinline__ int win_length(const WinSizes& w, int b) {
   return w.lengths ? max(0, min(__ldg(w.lengths + b), w.kv_tokens)) : w.kv_tokens;
 }
 
+// ---- instructions
+
 // D (+)= A B with A [128 x 16 per step] in tensor memory (bf16, two to a column) and B in shared memory.
 __device__ __forceinline__ void mma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
                                             uint32_t accumulate) {
@@ -85,7 +58,7 @@ __device__ __forceinline__ void mma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, ui
       : "memory");
 }
 
-// 32 columns of this lane's row (visible after tmem_store_wait()).
+// 32 (16) columns of this lane's row (visible after tmem_store_wait()).
 __device__ __forceinline__ void tmem_st(uint32_t addr, const uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
@@ -107,11 +80,51 @@ __device__ __forceinline__ void tmem_st(uint32_t addr, const uint32_t (&r)[16]) 
 }
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// The K-major operand (rows = M or N) and the MN-major one (rows = inner) of a 128-byte-swizzled tile of 128 rows
+// in 64-column boxes, at inner step 0, and at step s of 16 from there: the descriptor's address counts 16 bytes and has
+// room for all of shared memory, so that a step is an addition.
+__device__ __forceinline__ uint64_t win_rows(uint32_t tile) { return smem_desc_sw128(tile, 16, 1024); }
+__device__ __forceinline__ uint64_t win_inner(uint32_t tile) { return smem_desc_sw128(tile, kSwBox, 1024); }
+__device__ __forceinline__ uint64_t win_rows_step(uint64_t first, int s) {
+  return first + ((s >> 2) * (kSwBox >> 4) + (s & 3) * 2);
+}
+__device__ __forceinline__ uint64_t win_inner_step(uint64_t first, int s) { return first + 128 * s; }
+
+// One lane of a converged warp.  The warps that feed the tensor cores run with all lanes and let one issue, so that
+// addresses stay in uniform registers (a single lane's loop took 120 cycles for each instruction of 64).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+  return one != 0;
+}
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, int code) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, code));
+}
+
+// Give up registers of a warpgroup, or take more.
+template <int kRegs>
+__device__ __forceinline__ void win_fewer_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
+}
+template <int kRegs>
+__device__ __forceinline__ void win_more_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
+}
+
+// ---- rows
+
 // Bits [low, high] of a word (either may lie outside it; none where low > high).
 __device__ __forceinline__ uint32_t bit_range(int low, int high) {
   if (high < 0 || low > 31 || low > high) return 0;
   const uint32_t up = high >= 31 ? 0xffffffffu : (2u << high) - 1;
   return low <= 0 ? up : up & ~((1u << low) - 1);
+}
+// Scores outside the columns [from, until] become minus infinity.
+__device__ __forceinline__ void hide(uint32_t (&s)[32], int from, int until) {
+  const uint32_t bits = bit_range(from, until);
+#pragma unroll
+  for (int e = 0; e < 32; ++e)
+    if (!(bits >> e & 1)) s[e] = 0xff800000u;
 }
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -119,7 +132,7 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// (Of numbers; a NaN is left out.)
+// Of numbers; a NaN is left out.
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -144,48 +157,10 @@ __device__ __forceinline__ Pair add2(Pair a, Pair b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
   return d;
 }
-__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
-  Pair d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
-  return d;
-}
 
-// 2^x of two, without the special function unit (16 a cycle, which bounds a softmax): the nearest integer from the low
-// bits of a sum with 1.5 2^23, the rest by a polynomial of degree 3 on [-1/2, 1/2], fitted here (relative error 1.0e-4,
-// 2.3e-5 on average; 1 at 0): the weight is rounded to bf16 next, by up to 3.9e-3.  Exactly 0 from -127 down; a NaN stays
-// one.
-__device__ __forceinline__ void exp2_poly(Pair x, float& a, float& b) {
-  float u, v;
-  x.get(u, v);
-  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(u));
-  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(v));
-  const Pair t(u, v), near = add2(t, Pair(12582912.f)), whole = add2(near, Pair(-12582912.f));
-  const Pair f = fma2(whole, Pair(-1.f), t);
-  Pair e = fma2(f, Pair(0.05500892177224159f), Pair(0.2422109693288803f));
-  e = fma2(e, f, Pair(0.6932829022407532f));
-  e = fma2(e, f, Pair(1.f));
-  float nu, nv;
-  near.get(nu, nv);
-  mul2(e, Pair(__int_as_float((__float_as_int(nu) << 23) + 0x3f800000), __int_as_float((__float_as_int(nv) << 23) + 0x3f800000)))
-      .get(a, b);
-}
+// ---- host
 
-// A division by a constant of the launch.
-
-// Give up registers of a warpgroup, or take more.
-template <int kRegs>
-__device__ __forceinline__ void win_fewer_registers() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
-}
-template <int kRegs>
-__device__ __forceinline__ void win_more_registers() {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
-}
-// Of the 64512 registers that 384 threads of 168 are launched with: 8 row warps of 200 and 4 others of 96 take 63488.
-constexpr int kWinRowRegs = 200, kWinOtherRegs = 96;
-static_assert(32 * (8 * kWinRowRegs + 4 * kWinOtherRegs) <= kWinThreads * 168, "registers");
-
-// Host: a [batch, heads, tokens, dim] tensor as boxes of 64 columns x `rows` tokens.
+// A [batch, heads, tokens, dim] tensor as boxes of 64 columns x `rows` tokens.
 bool win_map(CUtensorMap* map, const void* base, const long long* strides, int batch, int heads, int tokens, int dim,
              int rows);
 // Checked arguments as sizes, or an error code.

@@ -23,6 +23,9 @@ namespace ts {
 
 namespace {
 
+// Warps 0-7: rows, 8: loads, 9: instructions, 10: tensor memory.
+constexpr int kBwdThreads = 384;
+
 template <int kD>
 struct WinBwdLayout {
   static constexpr int kBoxes = kD / 64;
@@ -57,13 +60,6 @@ __device__ __forceinline__ void store_row(__nv_bfloat16* row, const uint32_t (&r
     for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(r[8 * i + e]) * scale;
     if (c + 8 * i < dim) *reinterpret_cast<uint4*>(row + c + 8 * i) = pack8(f);
   }
-}
-
-__device__ __forceinline__ void hide(uint32_t (&s)[32], int from, int until) {
-  const uint32_t bits = bit_range(from, until);
-#pragma unroll
-  for (int e = 0; e < 32; ++e)
-    if (!(bits >> e & 1)) s[e] = 0xff800000u;
 }
 
 // ------------------------------------------------------------------ dq
@@ -126,7 +122,7 @@ __device__ __forceinline__ bool rows_all(bool ok) {
 }
 
 template <int kD>
-__global__ void __launch_bounds__(kWinThreads, 1) window_bwd_q_kernel(const __grid_constant__ WinBwdParams p) {
+__global__ void __launch_bounds__(kBwdThreads, 1) window_bwd_q_kernel(const __grid_constant__ WinBwdParams p) {
   using L = WinBwdLayout<kD>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ alignas(8) uint64_t full[L::kSlots], empty[L::kSlots], q_full, q_empty, y_full, y_empty, s_full, dp_full,
@@ -220,7 +216,7 @@ __global__ void __launch_bounds__(kWinThreads, 1) window_bwd_q_kernel(const __gr
     uint32_t it = 0, q_turn = 0, n_s = 0, n_ds = 0;
     bool ok = true;
     constexpr uint32_t id_dq = idesc_bf16(128, kD, false, true);
-    const uint64_t q0 = win_rows(q_at, 0), dy0 = win_rows(dy_at, 0);
+    const uint64_t q0 = win_rows(q_at), dy0 = win_rows(dy_at);
     for (int unit = blockIdx.x; unit < p.units && ok; unit += gridDim.x) {
       const WinQueryUnit u(w, unit);
       if (u.count == 0) continue;
@@ -230,7 +226,7 @@ __global__ void __launch_bounds__(kWinThreads, 1) window_bwd_q_kernel(const __gr
              mbar_wait_warp(&full[item % L::kSlots], (item / L::kSlots) & 1, kErrCopyTimeout);
         if (!ok) return;
         tc_fence_after();
-        const uint64_t b = win_rows(ring + item % L::kSlots * L::kTileBytes, 0);
+        const uint64_t b = win_rows(ring + item % L::kSlots * L::kTileBytes);
         const uint32_t id = idesc_bf16(128, u.columns(n), false, false);
         if (elect_one()) {
 #pragma unroll
@@ -259,7 +255,7 @@ __global__ void __launch_bounds__(kWinThreads, 1) window_bwd_q_kernel(const __gr
         }
         if (!(ok = ok && mbar_wait_warp(&ds_full, n_ds++ & 1, kErrMmaTimeout))) break;
         tc_fence_after();
-        const uint64_t k = win_inner(ring + it % L::kSlots * L::kTileBytes, 0);
+        const uint64_t k = win_inner(ring + it % L::kSlots * L::kTileBytes);
         const int steps = u.columns(n) >> 4;
         if (elect_one()) {
 #pragma unroll
@@ -458,7 +454,7 @@ struct WinKeyUnit {
 };
 
 template <int kD>
-__global__ void __launch_bounds__(kWinThreads, 1) window_bwd_kv_kernel(const __grid_constant__ WinBwdParams p) {
+__global__ void __launch_bounds__(kBwdThreads, 1) window_bwd_kv_kernel(const __grid_constant__ WinBwdParams p) {
   using L = WinBwdLayout<kD>;
   constexpr int kSlots = L::kPairSlots;
   extern __shared__ uint8_t smem_raw[];
@@ -537,10 +533,10 @@ __global__ void __launch_bounds__(kWinThreads, 1) window_bwd_kv_kernel(const __g
     uint32_t it = 0, turn = 0, n_p = 0;
     bool ok = true;
     constexpr uint32_t id_s = idesc_bf16(128, 128, false, false), id_d = idesc_bf16(128, kD, false, true);
-    const uint64_t k0 = win_rows(k_at, 0), v0 = win_rows(v_at, 0);
+    const uint64_t k0 = win_rows(k_at), v0 = win_rows(v_at);
     // S^T or dP^T: rows of K or V with rows of the item's queries or their gradients
     auto product = [&](uint32_t to, uint64_t a, uint32_t tile, uint64_t* finished) {
-      const uint64_t b = win_rows(tile, 0);
+      const uint64_t b = win_rows(tile);
       if (elect_one()) {
 #pragma unroll
         for (int s = 0; s < kD / 16; ++s) mma_bf16(to, win_rows_step(a, s), win_rows_step(b, s), id_s, s > 0);
@@ -549,7 +545,7 @@ __global__ void __launch_bounds__(kWinThreads, 1) window_bwd_kv_kernel(const __g
     };
     // dv or dk: what lies at `a` in tensor memory, 64 queries in each half of 64 columns
     auto sum = [&](uint32_t to, uint32_t a, uint32_t tile, bool more) {
-      const uint64_t b = win_inner(tile, 0);
+      const uint64_t b = win_inner(tile);
       if (elect_one()) {
 #pragma unroll
         for (int s = 0; s < 8; ++s)
@@ -757,10 +753,10 @@ int window_bwd_launch(WinBwdParams& p, cudaStream_t s) {
     set = cudaFuncSetAttribute(window_bwd_kv_kernel<kD>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmemKV);
   if (set != cudaSuccess) return set_error(TS_ERR_CUDA, "window_bwd: %s", cudaGetErrorString(set));
   p.units = w.batch * w.heads * w.q_tiles;
-  window_bwd_q_kernel<kD><<<p.units < 148 ? p.units : 148, kWinThreads, L::kSmemQ, s>>>(p);
+  window_bwd_q_kernel<kD><<<p.units < 148 ? p.units : 148, kBwdThreads, L::kSmemQ, s>>>(p);
   if (const int rc = check_launch("window_bwd_q")) return rc;
   p.units = w.batch * w.kv_heads * (p.sink_tiles * p.chunks + p.key_tiles - p.sink_tiles);
-  window_bwd_kv_kernel<kD><<<p.units < 148 ? p.units : 148, kWinThreads, L::kSmemKV, s>>>(p);
+  window_bwd_kv_kernel<kD><<<p.units < 148 ? p.units : 148, kBwdThreads, L::kSmemKV, s>>>(p);
   if (const int rc = check_launch("window_bwd_kv")) return rc;
   if (p.sink_tiles == 0 || p.chunks < 2) return TS_OK;
   window_bwd_join_kernel<kD><<<dim3(kD / 32 * 2, w.batch * w.kv_heads * p.sink_tiles), 128, 0, s>>>(p);

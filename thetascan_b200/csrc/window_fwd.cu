@@ -27,14 +27,21 @@ namespace ts {
 
 namespace {
 
+// Warps 0-15: rows, 16: loads, 17 and 19: instructions, 18: tensor memory.  Of the 61440 registers that 640 threads of 96
+// are launched with, the row warps take 104 each, the others 64.
+constexpr int kFwdRowWarps = 16;
+constexpr int kFwdThreads = 32 * (kFwdRowWarps + 4);
+constexpr int kFwdRowRegs = 104, kFwdOtherRegs = 64;
+static_assert(32 * (kFwdRowWarps * kFwdRowRegs + 4 * kFwdOtherRegs) <= kFwdThreads * 96, "registers");
+
 template <int kD>
 struct WinFwdLayout {
   static constexpr int kBoxes = kD / 64;
   static constexpr uint32_t kTileBytes = kBoxes * kSwBox;
   static constexpr int kSlots = kD == 64 ? 8 : 4;
-  static constexpr uint32_t kOutBytes = 4096;          // a warp's 32 rows x 64 columns
+  static constexpr uint32_t kOutBytes = 2048;          // a warp's 32 rows x 32 columns
   static constexpr uint32_t kQ = 0, kRing = 2 * kTileBytes, kOut = kRing + kSlots * kTileBytes;
-  static constexpr uint32_t kSmem = kOut + 8 * kOutBytes + 1024;
+  static constexpr uint32_t kSmem = kOut + kFwdRowWarps * kOutBytes + 1024;
 };
 
 struct WinFwdParams {
@@ -111,21 +118,16 @@ struct WinFwdUnit {
   }
 };
 
-struct RowColumns {
-  int cols, from, until;   // the tile's, and this row's first and last visible one
-  bool masked;
-  // whether none of the warp's rows sees any of the 32 columns from c on
-  __device__ __forceinline__ bool none(int c) const { return masked && __all_sync(0xffffffffu, until < c || from > c + 31); }
-  __device__ __forceinline__ void hide(uint32_t (&s)[32], int c) const {
-    if (__all_sync(0xffffffffu, from <= c && until >= c + 31)) return;
-    const uint32_t bits = bit_range(from - c, until - c);
-#pragma unroll
-    for (int e = 0; e < 32; ++e)
-      if (!(bits >> e & 1)) s[e] = 0xff800000u;
-  }
-};
+__device__ __forceinline__ void st_shared_f32(uint32_t at, float v) {
+  asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory");
+}
+__device__ __forceinline__ float ld_shared_f32(uint32_t at) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+  return v;
+}
 
-// 32 scores to weights in bf16, their sum to `part`.  Half of the exponentials go by exp2_poly, beside the special
+// 32 scores to weights in bf16, their sum to `part`.  A quarter of the exponentials goes by exp2_poly, beside the special
 // function unit.
 __device__ __forceinline__ void row_exp(const uint32_t (&s)[32], uint32_t to, Pair scale2, Pair origin, Pair (&part)[2]) {
   uint32_t packed[16];
@@ -133,13 +135,9 @@ __device__ __forceinline__ void row_exp(const uint32_t (&s)[32], uint32_t to, Pa
   for (int e = 0; e < 32; e += 2) {
     const Pair x = fma2(Pair(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), scale2, origin);
     float a, b;
-    if (false && e & 2) {
-      exp2_poly(x, a, b);
-    } else {
-      x.get(a, b);
-      a = exp2_fast(a);
-      b = exp2_fast(b);
-    }
+    x.get(a, b);
+    a = exp2_fast(a);
+    b = exp2_fast(b);
     part[e >> 1 & 1] = add2(part[e >> 1 & 1], Pair(a, b));
     packed[e / 2] = pack_bf16(a, b);
   }
@@ -147,7 +145,7 @@ __device__ __forceinline__ void row_exp(const uint32_t (&s)[32], uint32_t to, Pa
 }
 
 template <int kD>
-__global__ void __launch_bounds__(kWinThreads, 1) window_fwd_kernel(const __grid_constant__ WinFwdParams p) {
+__global__ void __launch_bounds__(kFwdThreads, 1) window_fwd_kernel(const __grid_constant__ WinFwdParams p) {
   using L = WinFwdLayout<kD>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ alignas(8) uint64_t full[L::kSlots], empty[L::kSlots], q_full[2], q_empty[2], s_full[2], s_free[2], p_full[2],
@@ -165,14 +163,14 @@ __global__ void __launch_bounds__(kWinThreads, 1) window_fwd_kernel(const __grid
       mbar_init(&q_full[i], 1);
       mbar_init(&q_empty[i], 1);
       mbar_init(&s_full[i], 1);
-      mbar_init(&s_free[i], 4);
-      mbar_init(&p_full[i], 4);
+      mbar_init(&s_free[i], 8);
+      mbar_init(&p_full[i], 8);
       mbar_init(&p_free[i], 1);
       mbar_init(&o_full[i], 1);
     }
     fence_mbar_init();
   }
-  if (warp == 10) tmem_alloc(&tmem_slot, 512);
+  if (warp == 18) tmem_alloc(&tmem_slot, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -181,9 +179,9 @@ __global__ void __launch_bounds__(kWinThreads, 1) window_fwd_kernel(const __grid
   constexpr bool kApart = kD == 64;
   constexpr uint32_t kScores = 128, kO = 256, kP = kApart ? 384 : 0, kPStride = kApart ? 64 : kScores;
 
-  if (warp >= 8) {
-    win_fewer_registers<kWinOtherRegs>();
-    if (warp == 8) {
+  if (warp >= kFwdRowWarps) {
+    win_fewer_registers<kFwdOtherRegs>();
+    if (warp == 16) {
       // ---- loads
       uint32_t it = 0, q_turn[2] = {0, 0};
       bool ok = true;
@@ -202,21 +200,25 @@ __global__ void __launch_bounds__(kWinThreads, 1) window_fwd_kernel(const __grid
       };
       for (int unit = blockIdx.x; unit < p.units && ok; unit += gridDim.x) {
         const WinFwdUnit u(p, unit);
-        for (int n = 0; n < u.count && ok; ++n) {
+        auto queries = [&](int x) {
+          if (!u.of(x).live || !(ok = ok && mbar_wait_warp(&q_empty[x], (q_turn[x]++ & 1) ^ 1, kErrMmaTimeout))) return;
+          if (elect_one()) {
+            mbar_expect_tx(&q_full[x], L::kTileBytes);
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            if (!u.of(x).live || n > 0) continue;
-            if (!(ok = ok && mbar_wait_warp(&q_empty[x], (q_turn[x]++ & 1) ^ 1, kErrMmaTimeout))) break;
-            if (elect_one()) {
-              mbar_expect_tx(&q_full[x], L::kTileBytes);
-#pragma unroll
-              for (int c = 0; c < L::kBoxes; ++c)
-                tma_load_4d(base + L::kQ + x * L::kTileBytes + c * kSwBox, &p.q, 64 * c, 128 * u.of(x).tile, u.of(x).head, u.b,
-                            &q_full[x]);
-            }
+            for (int c = 0; c < L::kBoxes; ++c)
+              tma_load_4d(base + L::kQ + x * L::kTileBytes + c * kSwBox, &p.q, 64 * c, 128 * u.of(x).tile, u.of(x).head, u.b,
+                          &q_full[x]);
           }
+        };
+        for (int n = 0; n < u.count && ok; ++n) {
+          // (tile B's last product comes after A's: what A needs to begin comes before B's queries)
+          if (n == 0) queries(0);
           load(&p.k, &p.k_sink, u, n);
-          load(&p.v, &p.v_sink, u, n);
+          if (n > 0) load(&p.v, &p.v_sink, u, n);
+          if (n == 0) {
+            queries(1);
+            load(&p.v, &p.v_sink, u, n);
+          }
         }
       }
       if (!ok) {
@@ -229,13 +231,13 @@ __global__ void __launch_bounds__(kWinThreads, 1) window_fwd_kernel(const __grid
           for (int poll = 0; poll < (1 << 16) && q_turn[x] > 0 && !mbar_try_wait(&q_full[x], (q_turn[x] - 1) & 1); ++poll) {
           }
       }
-    } else if (!kApart && warp == 9) {
+    } else if (!kApart && warp == 17) {
       // ---- instructions, where P takes S's place: one warp, each tile's products with P and then with the next keys,
       // in turn, so that a product has the tensor cores to itself.  This warp's own steps come between the tensor
       // cores': little is worked out here.
       constexpr uint32_t id_o = idesc_bf16(128, kD, false, true), id_s = idesc_bf16(128, 128, false, false);
       constexpr uint32_t kSlotStep = L::kTileBytes >> 4;
-      const uint64_t q0 = win_rows(base + L::kQ, 0), k0 = win_rows(base + L::kRing, 0), v0 = win_inner(base + L::kRing, 0);
+      const uint64_t q0 = win_rows(base + L::kQ), k0 = win_rows(base + L::kRing), v0 = win_inner(base + L::kRing);
       // the ring's next key tile and its next value tile: their slots and parities
       uint32_t k_slot = 0, k_parity = 0, v_slot = 1, v_parity = 0;
       uint32_t q_parity[2] = {0, 0}, p_parity[2] = {0, 0};
@@ -287,7 +289,8 @@ __global__ void __launch_bounds__(kWinThreads, 1) window_fwd_kernel(const __grid
             if (now) {
 #pragma unroll
               for (int s = 0; s < 8; ++s)
-                if (s < steps) mma_bf16_ts(kO + kD * x, kP + kPStride * x + 8 * s, win_inner_step(v, s), id_o, summed || s > 0);
+                if (s < steps)   // the columns of each half of the rows' warps lie in that half
+                  mma_bf16_ts(kO + kD * x, kScores * x + 64 * (s >> 2) + 8 * (s & 3), win_inner_step(v, s), id_o, summed || s > 0);
               if (n == last[x]) mma_commit(&o_full[x]);
             }
             if (then) scores(x, n + 1);
@@ -319,14 +322,14 @@ __global__ void __launch_bounds__(kWinThreads, 1) window_fwd_kernel(const __grid
           }
         }
       }
-    } else if (kApart && warp != 10) {
-      // ---- instructions: warp 9 for tile A, warp 11 for B, so that neither waits for the other's rows.  These warps' own
+    } else if (kApart && warp != 18) {
+      // ---- instructions: warp 17 for tile A, warp 19 for B, so that neither waits for the other's rows.  These warps' own
       // steps come between the tensor cores': little is worked out here.
-      const int x = warp == 9 ? 0 : 1;
+      const int x = warp == 17 ? 0 : 1;
       constexpr uint32_t id_o = idesc_bf16(128, kD, false, true), id_s = idesc_bf16(128, 128, false, false);
       constexpr uint32_t kSlotStep = L::kTileBytes >> 4;
-      const uint64_t q0 = win_rows(base + L::kQ, 0) + x * kSlotStep;
-      const uint64_t k0 = win_rows(base + L::kRing, 0), v0 = win_inner(base + L::kRing, 0);
+      const uint64_t q0 = win_rows(base + L::kQ) + x * kSlotStep;
+      const uint64_t k0 = win_rows(base + L::kRing), v0 = win_inner(base + L::kRing);
       const uint32_t s_to = kScores * x, p_at = kP + kPStride * x, o_to = kO + kD * x;
       uint64_t* const done_s = &s_full[x];
       // the ring's next key tile and its next value tile: their slots and parities
@@ -408,28 +411,37 @@ __global__ void __launch_bounds__(kWinThreads, 1) window_fwd_kernel(const __grid
       }
     }
   } else {
-    // ---- rows: thread t of group x owns row t of tile x
-    win_more_registers<kWinRowRegs>();
-    const int x = warp >> 2, quad = warp & 3, row = 32 * quad + lane;
+    // ---- rows: two threads for a row of tile x, each with half of the columns.  (One thread to a row leaves a scheduler
+    // two warps, whose steps wait for one another: 64 x 8 heads x 1024, width 64, window 256 took 135 us.)
+    win_more_registers<kFwdRowRegs>();
+    const int x = warp >> 3, half = warp >> 2 & 1, quad = warp & 3, row = 32 * quad + lane;
     const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
-    const uint32_t s_at = kScores * x + lanes, p_at = kP + kPStride * x + lanes, o_at = kO + kD * x + lanes;
-    const uint32_t stage = base + L::kOut + warp * L::kOutBytes;
+    const uint32_t s_at = kScores * x + lanes + 64 * half, p_at = kP + kPStride * x + lanes + (kApart ? 32 : 64) * half;
+    const uint32_t o_at = kO + kD * x + lanes + kD / 2 * half;
+    const uint32_t stage = base + L::kOut + warp * L::kOutBytes, partner = base + L::kOut + (warp ^ 4) * L::kOutBytes;
     const float scale2 = w.scale * kLog2e;
-    uint32_t turn = 0, o_turn = 0;
+    uint32_t turn = 0, o_turn = 0, exchanges = 0;
     bool ok = true;
     auto signal = [&](uint64_t* bar) {
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar);
     };
+    // the value of the other thread of the row, by two places in turn
+    auto exchange = [&](float v) {
+      const uint32_t slot = exchanges++ & 1;
+      st_shared_f32(stage + 128 * slot + 4 * lane, v);
+      asm volatile("bar.sync %0, 64;" ::"r"(1 + 4 * x + quad) : "memory");
+      return ld_shared_f32(partner + 128 * slot + 4 * lane);
+    };
     WinFwdUnit next(p, blockIdx.x);
-    for (int unit = blockIdx.x; unit < p.units && ok; unit += gridDim.x) {
+    for (int unit = blockIdx.x; unit < p.units; unit += gridDim.x) {
       const WinFwdUnit u = next;
       const WinFwdTile mine = u.of(x);
-      if (!mine.exists) {
-        if (unit + gridDim.x < p.units) next = WinFwdUnit(p, unit + gridDim.x);
-        continue;
-      }
+      if (unit + gridDim.x < p.units) next = WinFwdUnit(p, unit + gridDim.x);
+      if (!mine.exists) continue;
+      if (lane == 0) tma_store_read_wait<0>();   // the last store has read the stage, which carries exchanges now
+      __syncwarp();
       const int q_row = 128 * mine.tile + row, at = w.past + q_row;
       const int near = max(at - w.window + 1, u.sinks), to = at < u.length ? at : -1;   // visible: first ones, near..to
       float ref = -INFINITY, sum = 0.f;
@@ -437,52 +449,60 @@ __global__ void __launch_bounds__(kWinThreads, 1) window_fwd_kernel(const __grid
       // first tokens, then the window's own
       for (int n = 0; mine.live && n <= mine.last; ++n, ++turn) {
         if (n == u.sink_tiles) n += mine.low - u.first;
-        const int cols = u.columns(n), key = u.key(w, n);
+        const int cols = u.columns(n) - 64 * half, key = u.key(w, n) + 64 * half;
         const bool sink = n < u.sink_tiles;
         // this row's first and last visible column; a tile within reach of all rows is not masked
         const int from = sink ? 0 : near - key, until = min(to, sink ? u.sinks - 1 : to) - key;
-        const RowColumns r{cols, from, until, !__all_sync(0xffffffffu, from <= 0 && until >= 127)};
-        if (!(ok = mbar_wait(&s_full[x], turn & 1, kErrMmaTimeout))) break;
+        const bool masked = !__all_sync(0xffffffffu, from <= 0 && until >= 63);
+        ok = ok && mbar_wait(&s_full[x], turn & 1, kErrMmaTimeout);
         tc_fence_after();
-        uint32_t s[4][32];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld(s_at + 32 * c, s[c]);
+        uint32_t s[2][32];
+        tmem_ld(s_at, s[0]);
+        tmem_ld(s_at + 32, s[1]);
         tmem_wait();
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tie(s[c]);
+        tie(s[0]);
+        tie(s[1]);
         if (kApart) signal(&s_free[x]);
-        if (r.masked) {
+        // whether the warp's rows see anything of each 32 columns
+        const bool some[2] = {!masked || __any_sync(0xffffffffu, until >= 0 && from <= 31),
+                              !masked || __any_sync(0xffffffffu, until >= 32 && from <= 63)};
+        if (masked) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) r.hide(s[c], 32 * c);
+          for (int c = 0; c < 2; ++c)
+            if (some[c]) hide(s[c], from - 32 * c, until - 32 * c);
         }
-        // eight chains side by side: a warp has its scheduler almost to itself, and each step waits for the one before
-        float top[8];
+        float best = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) top[i] = __uint_as_float(s[i >> 1][16 * (i & 1)]);
+        for (int c = 0; c < 2; ++c) {
+          if (!some[c]) continue;
+          // chains side by side: each step waits for the one before
+          float top[4];
 #pragma unroll
-        for (int e = 1; e < 15; e += 2)
+          for (int i = 0; i < 4; ++i) top[i] = max3(__uint_as_float(s[c][i]), __uint_as_float(s[c][i + 4]), __uint_as_float(s[c][i + 8]));
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            top[i] = max3(top[i], __uint_as_float(s[i >> 1][16 * (i & 1) + e]), __uint_as_float(s[i >> 1][16 * (i & 1) + e + 1]));
+          for (int e = 12; e < 28; e += 8)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) top[i] = fmaxf(top[i], __uint_as_float(s[i >> 1][16 * (i & 1) + 15]));
-        const float best = fmaxf(max3(max3(top[0], top[1], top[2]), top[3], top[4]), max3(top[5], top[6], top[7])) * scale2;
+            for (int i = 0; i < 4; ++i) top[i] = max3(top[i], __uint_as_float(s[c][e + i]), __uint_as_float(s[c][e + i + 4]));
+          best = max3(best, max3(top[0], top[1], max3(top[2], top[3], __uint_as_float(s[c][28]))),
+                      max3(__uint_as_float(s[c][29]), __uint_as_float(s[c][30]), __uint_as_float(s[c][31])));
+        }
+        best = fmaxf(best, exchange(best)) * scale2;
         if (kApart) {
-          if (!(ok = mbar_wait(&p_free[x], (turn & 1) ^ 1, kErrMmaTimeout))) break;
+          ok = ok && mbar_wait(&p_free[x], (turn & 1) ^ 1, kErrMmaTimeout);
           tc_fence_after();
         }
-        // The row's reference: the largest score of its first tile, and later one that exceeds it by 2^8.  (A NaN is not
-        // at most anything: it becomes the reference, and with it the row.)
+        // The row's reference: the largest score of its first tile, and later one that exceeds it by 2^8.  (A NaN leaves
+        // the reference alone, and reaches the row by its weight.)
         if (first) {
           ref = best;
           first = false;
-        } else if (__any_sync(0xffffffffu, !(best <= ref + 8.f))) {
-          const float next = best <= ref + 8.f ? ref : best;
-          const float factor = next == ref ? 1.f : exp2_fast(ref - next);
-          ref = next;
+        } else if (__any_sync(0xffffffffu, best > ref + 8.f)) {
+          const float moved = best > ref + 8.f ? best : ref;
+          const float factor = moved == ref ? 1.f : exp2_fast(ref - moved);
+          ref = moved;
           sum *= factor;
 #pragma unroll 1
-          for (int c = 0; c < kD; c += 16) {
+          for (int c = 0; c < kD / 2; c += 16) {
             uint32_t o[16];
             tmem_ld(o_at + c, o);
             tmem_wait();
@@ -494,19 +514,13 @@ __global__ void __launch_bounds__(kWinThreads, 1) window_fwd_kernel(const __grid
         }
         const Pair scales(scale2), origin(ref == -INFINITY ? 0.f : -ref);
         Pair part[2] = {Pair(sum, 0.f), Pair(0.f)};
-        if (!kApart && !r.masked) {   // (twice the code is worth it where most tiles have no mask)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) row_exp(s[c], p_at + 16 * c, scales, origin, part);
-        } else {
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            if (32 * c >= cols) continue;
-            if (r.none(32 * c)) {
-              const uint32_t zero[16] = {};
-              tmem_st(p_at + 16 * c, zero);
-            } else {
-              row_exp(s[c], p_at + 16 * c, scales, origin, part);
-            }
+        for (int c = 0; c < 2; ++c) {
+          if (some[c]) {
+            row_exp(s[c], p_at + 16 * c, scales, origin, part);
+          } else if (32 * c < cols) {
+            const uint32_t zero[16] = {};
+            tmem_st(p_at + 16 * c, zero);
           }
         }
         float even, odd;
@@ -515,40 +529,40 @@ __global__ void __launch_bounds__(kWinThreads, 1) window_fwd_kernel(const __grid
         tmem_store_wait();
         signal(&p_full[x]);
       }
+      sum += exchange(sum);
+      ok = ok && (!mine.live || mbar_wait(&o_full[x], o_turn++ & 1, kErrMmaTimeout));
       if (!ok) break;
-      if (unit + gridDim.x < p.units) next = WinFwdUnit(p, unit + gridDim.x);   // while the last product runs
-      if (mine.live && !(ok = mbar_wait(&o_full[x], o_turn++ & 1, kErrMmaTimeout))) break;
       tc_fence_after();
       // a row that sees nothing has no sum: zero
       const float inverse = sum != 0.f ? 1.f / sum : 0.f;
 #pragma unroll 1
-      for (int c = 0; c < w.dim; c += 64) {
+      for (int c = 0; c < kD / 2; c += 32) {
+        const int channel = kD / 2 * half + c;
+        if (channel >= w.dim) break;
+        uint32_t o[32];
+        tmem_ld(o_at + c, o);
+        tmem_wait();
+        tie(o);
         if (lane == 0) tma_store_read_wait<0>();
         __syncwarp();
 #pragma unroll
-        for (int h = 0; h < 64; h += 32) {
-          uint32_t o[32];
-          tmem_ld(o_at + c + h, o);
-          tmem_wait();
-          tie(o);
+        for (int i = 0; i < 4; ++i) {
+          float f[8];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float f[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = inverse != 0.f ? __uint_as_float(o[8 * i + e]) * inverse : 0.f;
-            st_shared_v4(stage + sw128_offset(lane, h / 8 + i), pack8(f));
-          }
+          for (int e = 0; e < 8; ++e) f[e] = inverse != 0.f ? __uint_as_float(o[8 * i + e]) * inverse : 0.f;
+          // 64-byte rows, swizzled as the store expects: the 16-byte piece's index XORed with bits 1-2 of the row
+          st_shared_v4(stage + 64 * lane + ((i ^ (lane >> 1 & 3)) << 4), pack8(f));
         }
         fence_async_smem();
         __syncwarp();
         if (lane == 0) {
           const int to_row = 128 * mine.tile + 32 * quad;
-          if (to_row < w.q_tokens) tma_store_4d(&p.y, c, to_row, mine.head, u.b, stage);
+          if (to_row < w.q_tokens) tma_store_4d(&p.y, channel, to_row, mine.head, u.b, stage);
           tma_store_commit();
         }
       }
       tc_fence_before();
-      if (p.lse) {
+      if (p.lse && half == 0) {
         // of the scores in units of log 2; +infinity, which makes every weight zero, for a row that sees nothing
         const float l = sum != 0.f ? (ref == -INFINITY ? 0.f : ref) + log2f(sum) : INFINITY;
         p.lse[(static_cast<size_t>(u.b) * w.heads + mine.head) * (128 * static_cast<size_t>(w.q_tiles)) + q_row] = l;
@@ -558,7 +572,7 @@ __global__ void __launch_bounds__(kWinThreads, 1) window_fwd_kernel(const __grid
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 10) {
+  if (warp == 18) {
     tc_fence_after();
     tmem_dealloc(tmem_slot, 512);
   }
@@ -569,7 +583,7 @@ int window_fwd_launch(const WinFwdParams& p, cudaStream_t s) {
   constexpr int smem = WinFwdLayout<kD>::kSmem;
   const cudaError_t set = cudaFuncSetAttribute(window_fwd_kernel<kD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (set != cudaSuccess) return set_error(TS_ERR_CUDA, "window_fwd: %s", cudaGetErrorString(set));
-  window_fwd_kernel<kD><<<p.units < 148 ? p.units : 148, kWinThreads, smem, s>>>(p);
+  window_fwd_kernel<kD><<<p.units < 148 ? p.units : 148, kFwdThreads, smem, s>>>(p);
   return check_launch("window_fwd");
 }
 
@@ -584,6 +598,16 @@ bool win_map(CUtensorMap* map, const void* base, const long long* strides, int b
   const int64_t steps[3] = {tokens > 1 ? strides[2] : any, heads > 1 ? strides[1] : any, batch > 1 ? strides[0] : any};
   const uint32_t box[4] = {64, static_cast<uint32_t>(rows), 1, 1};
   return make_tmap_bf16_sw128(map, base, 4, dims, steps, box);
+}
+
+// The output in blocks of 32 rows and columns.
+static bool win_out_map(CUtensorMap* map, const void* base, const long long* strides, const WinSizes& w) {
+  const uint64_t dims[4] = {static_cast<uint64_t>(w.dim), static_cast<uint64_t>(w.q_tokens), static_cast<uint64_t>(w.heads),
+                            static_cast<uint64_t>(w.batch)};
+  const int64_t any = (static_cast<int64_t>(w.dim) + 7) & ~7;
+  const int64_t steps[3] = {w.q_tokens > 1 ? strides[2] : any, w.heads > 1 ? strides[1] : any, w.batch > 1 ? strides[0] : any};
+  const uint32_t box[4] = {32, 32, 1, 1};
+  return make_tmap_bf16(map, base, 4, dims, steps, box, CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
 int win_sizes(const ts_window_args* a, WinSizes* w, const char* what) {
@@ -639,7 +663,7 @@ int ts_b200_window_fwd(const ts_window_args* a, ts_stream_t stream) {
                   win_map(&p.v, a->v, a->v_strides, w.batch, w.kv_heads, w.kv_tokens, w.dim, 128) &&
                   win_map(&p.k_sink, a->k, a->k_strides, w.batch, w.kv_heads, w.kv_tokens, w.dim, p.sink_rows) &&
                   win_map(&p.v_sink, a->v, a->v_strides, w.batch, w.kv_heads, w.kv_tokens, w.dim, p.sink_rows) &&
-                  win_map(&p.y, a->y, a->y_strides, w.batch, w.heads, w.q_tokens, w.dim, 32);
+                  win_out_map(&p.y, a->y, a->y_strides, w);
   if (!ok) return set_error(TS_ERR_VALUE, "window_fwd: bases and strides must be multiples of 16 bytes");
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   return w.dim <= 64 ? window_fwd_launch<64>(p, s) : window_fwd_launch<128>(p, s);

@@ -89,12 +89,12 @@ struct SampleShared {
   int piece_at;
 };
 
-__device__ __forceinline__ u64 warp_max(u64 v) {
+__device__ __forceinline__ u64 warp_max64(u64 v) {
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, d));
   return v;
 }
-__device__ __forceinline__ u64 warp_sum(u64 v) {
+__device__ __forceinline__ u64 warp_sum64(u64 v) {
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
   return v;
@@ -429,8 +429,8 @@ struct Sampler {
           high = max(high, static_cast<u64>(order_key(v)));
         });
       });
-      low = block_join(~warp_max(~low), m.warp_sum, [](u64 a, u64 b) { return min(a, b); });
-      high = block_join(warp_max(high), m.warp_sum_b, [](u64 a, u64 b) { return max(a, b); });
+      low = block_join(~warp_max64(~low), m.warp_sum, [](u64 a, u64 b) { return min(a, b); });
+      high = block_join(warp_max64(high), m.warp_sum_b, [](u64 a, u64 b) { return max(a, b); });
       if (threadIdx.x == 0) {
         m.smallest = low;
         m.largest = high;
@@ -449,7 +449,7 @@ struct Sampler {
         auto one = [&](float v, int) -> u64 { return in_question(v) ? 1 : 0; };
         u64 all = 0;
         each([&](Tokens x, int, int piece) {
-          const u64 s = warp_sum(__popc(which(x, [&](float v, int) { return in_question(v); })));
+          const u64 s = warp_sum64(__popc(which(x, [&](float v, int) { return in_question(v); })));
           if ((threadIdx.x & 31) == 0) m.piece[piece] = s;
           all += s;
         });
@@ -545,7 +545,7 @@ struct Sampler {
         top = fmaxf(top, x[j]);
       }
     }
-    top = key_value(static_cast<uint32_t>(block_join(warp_max(order_key(top)), m.warp_sum, [](u64 a, u64 b) { return max(a, b); })));
+    top = key_value(static_cast<uint32_t>(block_join(warp_max64(order_key(top)), m.warp_sum, [](u64 a, u64 b) { return max(a, b); })));
     if (ranks > 1) {
       if (threadIdx.x == 0) m.top = top;
       cluster_barrier();
@@ -609,7 +609,7 @@ struct Sampler {
         });
       }
       if (want_total) {
-        sum = block_join(warp_sum(sum), m.warp_sum, [](u64 a, u64 b) { return a + b; });
+        sum = block_join(warp_sum64(sum), m.warp_sum, [](u64 a, u64 b) { return a + b; });
         if (threadIdx.x == 0) m.total_b = sum;
       }
       barrier();
@@ -631,7 +631,7 @@ struct Sampler {
             u64 s = 0;
 #pragma unroll
             for (int i = 0; i < kPerThread; ++i) s += b.mass[i];
-            kept = block_join(warp_sum(s), m.warp_sum, [](u64 x, u64 y) { return x + y; });
+            kept = block_join(warp_sum64(s), m.warp_sum, [](u64 x, u64 y) { return x + y; });
           }
         }
         if (by_mass) {
@@ -671,7 +671,7 @@ struct Sampler {
             const u64 w = mass(x[j]);
             sum += bits >> j & 1 ? w : 0;
           }
-          sum = warp_sum(sum);
+          sum = warp_sum64(sum);
           mine += sum;
         }
         if ((threadIdx.x & 31) == 0) m.piece[piece] = sum;
@@ -700,7 +700,7 @@ struct Sampler {
           [&](float, int i) { first = min(first, static_cast<uint32_t>(start + i)); });
     });
     __syncthreads();
-    first = ~static_cast<uint32_t>(block_join(warp_max(~first), m.warp_sum, [](u64 a, u64 b) { return max(a, b); }));
+    first = ~static_cast<uint32_t>(block_join(warp_max64(~first), m.warp_sum, [](u64 a, u64 b) { return max(a, b); }));
     if (threadIdx.x == 0) m.first = first;
     barrier();
     if (rank == 0 && threadIdx.x == 0) {

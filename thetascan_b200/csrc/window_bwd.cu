@@ -12,9 +12,9 @@
 // no f32 copy of dq.  The keys of first tokens meet all queries: their tiles are
 // split among CTAs, whose sums go to a workspace in f32 and are joined in order.
 //
-// In both, thread t of warps 0-3 and its partner in warps 4-7 own a row of the
-// tile and half of the columns; p and ds go back to tensor memory in bf16 and are
-// the operand of the next product from there.  S^T = K Q^T and dP^T = V dY^T have
+// In both, four threads share a row of the tile, with a quarter of the columns
+// each; p and ds go back to tensor memory in bf16 and are the operand of the next
+// product from there.  S^T = K Q^T and dP^T = V dY^T have
 // keys in the rows, which is how dv and dk need them.
 #include "capi_internal.h"
 #include "window.cuh"
@@ -23,30 +23,40 @@ namespace ts {
 
 namespace {
 
-// Warps 0-7: rows, 8: loads, 9: instructions, 10: tensor memory.
-constexpr int kBwdThreads = 384;
+// Warps 0-15: rows, 16: loads, 17: instructions, 18: tensor memory.  Of the 61440 registers that 640 threads of 96 are
+// launched with, the row warps take 104 each, the others 64.  (With eight row warps each tile waited for them: 16 heads x
+// 16384, width 128, window 2048 took 540 us for dq and 527 for dk and dv.)
+constexpr int kBwdRowWarps = 16;
+constexpr int kBwdThreads = 32 * (kBwdRowWarps + 4);
+constexpr int kBwdRowRegs = 104, kBwdOtherRegs = 64;
+static_assert(32 * (kBwdRowWarps * kBwdRowRegs + 4 * kBwdOtherRegs) <= kBwdThreads * 96, "registers");
 
 template <int kD>
 struct WinBwdLayout {
   static constexpr int kBoxes = kD / 64;
   static constexpr uint32_t kTileBytes = kBoxes * kSwBox;
-  static constexpr int kSlots = kD == 64 ? 8 : 4;
-  static constexpr int kPairSlots = kSlots / 2;                          // of queries and their gradients
-  static constexpr uint32_t kRingBytes = kSlots * kTileBytes;
-  static constexpr uint32_t kSmemQ = 3 * kTileBytes + kRingBytes + 1024;                      // q, dy, y; keys and values
-  static constexpr uint32_t kSmemKV = 2 * kTileBytes + kRingBytes + kPairSlots * 1024 + 1024; // k, v; q, dy; lse, delta
+  // dq: q and dy, y where there is room, rings of keys (which wait for ds) and of values
+  static constexpr bool kKeepsY = kD == 64;
+  static constexpr int kKeySlots = kD == 64 ? 4 : 3, kValueSlots = kD == 64 ? 4 : 2;
+  static constexpr uint32_t kSmemQ = (2 + (kKeepsY ? 1 : 0) + kKeySlots + kValueSlots) * kTileBytes + 1024;
+  // dk and dv: k and v, a ring of q with dy, lse and delta
+  static constexpr int kPairSlots = kD == 64 ? 4 : 2;
+  static constexpr uint32_t kSmemKV = (2 + 2 * kPairSlots) * kTileBytes + kPairSlots * 1024 + 1024;
 };
 
 struct WinBwdParams {
   CUtensorMap q, k, v, k_sink, v_sink, y, dy;
   WinSizes w;
   int units;
+  Divisor by_row;           // units of a key head
   int sink_rows;
   // dk and dv: key tiles, the ones with first tokens, and the chunks (of `chunk` query tiles) that those are split in
   int key_tiles, sink_tiles, chunks, chunk;
   const float* lse;
   float* delta;
   float* partial;           // [batch, kv_heads, sink_tiles, chunks, dk and dv, dim padded, 128]
+  const __nv_bfloat16* y_at;   // where the kernel reads y itself
+  long long y_strides[3];
   __nv_bfloat16 *dq, *dk, *dv;
   long long dq_strides[3], dk_strides[3], dv_strides[3];
 };
@@ -62,6 +72,14 @@ __device__ __forceinline__ void store_row(__nv_bfloat16* row, const uint32_t (&r
   }
 }
 
+// 2^(scale s - origin) of a pair of scores.  (A part of them by a polynomial, beside the special function unit, took
+// longer: 16 heads x 16384, width 128, window 2048 464 -> 490 us for dq with half.)
+__device__ __forceinline__ void weight_pair(uint32_t s0, uint32_t s1, Pair scale2, Pair origin, float& a, float& b) {
+  fma2(Pair(__uint_as_float(s0), __uint_as_float(s1)), scale2, origin).get(a, b);
+  a = exp2_fast(a);
+  b = exp2_fast(b);
+}
+
 // ------------------------------------------------------------------ dq
 
 // A query tile and the key tiles that it sees (as in the forward pass, for one tile).
@@ -70,11 +88,12 @@ struct WinQueryUnit {
   bool live;
   int sinks, sink_tiles, first, count;
 
-  __device__ __forceinline__ WinQueryUnit(const WinSizes& w, int unit) {
-    const int row = unit / (w.q_tiles * w.share), at = unit - row * (w.q_tiles * w.share);
-    b = row / w.kv_heads;
+  __device__ __forceinline__ WinQueryUnit(const WinBwdParams& p, int unit) {
+    const WinSizes& w = p.w;
+    const int row = p.by_row(unit), at = unit - row * static_cast<int>(p.by_row.by);
+    b = w.by_kv_heads(row);
     kv_head = row - b * w.kv_heads;
-    tile = at / w.share;
+    tile = w.by_share(at);
     head = kv_head * w.share + at - tile * w.share;
     length = win_length(w, b);
     live = w.past + 128 * tile < length;
@@ -107,13 +126,13 @@ __device__ __forceinline__ void score_gradients(const uint32_t (&p)[32], const u
   }
 }
 
-// Whether `ok` holds in all of the 256 row threads (a barrier among them).
+// Whether `ok` holds in all of the 512 row threads (a barrier among them).
 __device__ __forceinline__ bool rows_all(bool ok) {
   uint32_t all;
   asm volatile(
       "{\n\t.reg .pred p, r;\n\t"
       "setp.ne.u32 p, %1, 0;\n\t"
-      "barrier.cta.red.and.pred r, 1, 256, p;\n\t"
+      "barrier.cta.red.and.pred r, 1, 512, p;\n\t"
       "selp.u32 %0, 1, 0, r;\n\t}"
       : "=r"(all)
       : "r"(static_cast<uint32_t>(ok))
@@ -124,156 +143,197 @@ __device__ __forceinline__ bool rows_all(bool ok) {
 template <int kD>
 __global__ void __launch_bounds__(kBwdThreads, 1) window_bwd_q_kernel(const __grid_constant__ WinBwdParams p) {
   using L = WinBwdLayout<kD>;
+  constexpr uint32_t kSlotStep = L::kTileBytes >> 4;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ alignas(8) uint64_t full[L::kSlots], empty[L::kSlots], q_full, q_empty, y_full, y_empty, s_full, dp_full,
-      s_free, dp_free, ds_full, ds_free, dq_full;
+  __shared__ alignas(8) uint64_t k_full[L::kKeySlots], k_empty[L::kKeySlots], v_full[L::kValueSlots], v_empty[L::kValueSlots],
+      q_full, q_empty, y_full, y_empty, s_full, dp_full, s_free, ds_full, ds_free, dq_full;
   __shared__ uint32_t tmem_slot;
   __shared__ float halves[2][128];   // free again before the next q_full, which waits for every row warp
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  const uint32_t q_at = base, dy_at = base + L::kTileBytes, y_at = base + 2 * L::kTileBytes, ring = base + 3 * L::kTileBytes;
+  const uint32_t q_at = base, dy_at = base + L::kTileBytes, keys = base + 2 * L::kTileBytes,
+                 values = keys + L::kKeySlots * L::kTileBytes, y_at = values + L::kValueSlots * L::kTileBytes;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const WinSizes& w = p.w;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < L::kSlots; ++i) {
-      mbar_init(&full[i], 1);
-      mbar_init(&empty[i], 1);
+    for (int i = 0; i < L::kKeySlots; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 1);
+    }
+    for (int i = 0; i < L::kValueSlots; ++i) {
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_empty[i], 1);
     }
     mbar_init(&q_full, 1);
-    mbar_init(&q_empty, 9);   // the instructions, and the rows' reading of dy
+    mbar_init(&q_empty, 1 + kBwdRowWarps);   // the instructions, and the rows' reading of dy
     mbar_init(&y_full, 1);
-    mbar_init(&y_empty, 8);
+    mbar_init(&y_empty, kBwdRowWarps);
     mbar_init(&s_full, 1);
     mbar_init(&dp_full, 1);
-    mbar_init(&s_free, 8);
-    mbar_init(&dp_free, 8);
-    mbar_init(&ds_full, 8);
+    mbar_init(&s_free, kBwdRowWarps);
+    mbar_init(&ds_full, kBwdRowWarps);
     mbar_init(&ds_free, 1);
     mbar_init(&dq_full, 1);
     fence_mbar_init();
   }
-  if (warp == 10) tmem_alloc(&tmem_slot, 512);
+  if (warp == 18) tmem_alloc(&tmem_slot, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   // all of tensor memory: its addresses start at 0.  Columns: S, dP, dq, ds (bf16)
   constexpr uint32_t kDp = 128, kDq = 256, kDs = 384;
 
-  if (warp == 8) {
-    // ---- loads
-    uint32_t it = 0, q_turn = 0, y_turn = 0;
-    bool ok = true;
-    auto load = [&](const CUtensorMap* map, const CUtensorMap* sink_map, const WinQueryUnit& u, int n) {
-      const uint32_t s = it % L::kSlots;
-      if (!(ok = ok && mbar_wait_warp(&empty[s], ((it / L::kSlots) & 1) ^ 1, kErrMmaTimeout))) return;
-      const bool sink = n < u.sink_tiles;
-      if (elect_one()) {
-        mbar_expect_tx(&full[s], L::kBoxes * (sink ? p.sink_rows : 128) * 128);
-#pragma unroll
-        for (int c = 0; c < L::kBoxes; ++c)
-          tma_load_4d(ring + s * L::kTileBytes + c * kSwBox, sink ? sink_map : map, 64 * c, u.key(w, n), u.kv_head, u.b,
-                      &full[s]);
-      }
-      ++it;
-    };
-    for (int unit = blockIdx.x; unit < p.units && ok; unit += gridDim.x) {
-      const WinQueryUnit u(w, unit);
-      if (u.count == 0) continue;
-      if (!(ok = mbar_wait_warp(&q_empty, (q_turn++ & 1) ^ 1, kErrMmaTimeout))) break;
-      if (elect_one()) {
-        mbar_expect_tx(&q_full, 2 * L::kTileBytes);
-#pragma unroll
-        for (int c = 0; c < L::kBoxes; ++c) {
-          tma_load_4d(q_at + c * kSwBox, &p.q, 64 * c, 128 * u.tile, u.head, u.b, &q_full);
-          tma_load_4d(dy_at + c * kSwBox, &p.dy, 64 * c, 128 * u.tile, u.head, u.b, &q_full);
-        }
-      }
-      load(&p.k, &p.k_sink, u, 0);
-      load(&p.v, &p.v_sink, u, 0);
-      if (!(ok = ok && mbar_wait_warp(&y_empty, (y_turn++ & 1) ^ 1, kErrMmaTimeout))) break;
-      if (elect_one()) {
-        mbar_expect_tx(&y_full, L::kTileBytes);
-#pragma unroll
-        for (int c = 0; c < L::kBoxes; ++c)
-          tma_load_4d(y_at + c * kSwBox, &p.y, 64 * c, 128 * u.tile, u.head, u.b, &y_full);
-      }
-      for (int n = 1; n < u.count && ok; ++n) {
-        load(&p.k, &p.k_sink, u, n);
-        load(&p.v, &p.v_sink, u, n);
-      }
-    }
-    if (!ok) {
-      // given up: let the copies in flight land before the memory goes (for a bounded time too)
-      for (uint32_t i = it > L::kSlots ? it - L::kSlots : 0; i < it; ++i)
-        for (int poll = 0; poll < (1 << 16) && !mbar_try_wait(&full[i % L::kSlots], (i / L::kSlots) & 1); ++poll) {
-        }
-      for (int poll = 0; poll < (1 << 16) && q_turn > 0 && !mbar_try_wait(&q_full, (q_turn - 1) & 1); ++poll) {
-      }
-      for (int poll = 0; poll < (1 << 16) && y_turn > 0 && !mbar_try_wait(&y_full, (y_turn - 1) & 1); ++poll) {
-      }
-    }
-  } else if (warp == 9) {
-    // ---- instructions
-    uint32_t it = 0, q_turn = 0, n_s = 0, n_ds = 0;
-    bool ok = true;
-    constexpr uint32_t id_dq = idesc_bf16(128, kD, false, true);
-    const uint64_t q0 = win_rows(q_at), dy0 = win_rows(dy_at);
-    for (int unit = blockIdx.x; unit < p.units && ok; unit += gridDim.x) {
-      const WinQueryUnit u(w, unit);
-      if (u.count == 0) continue;
-      // a product of the query side (rows in shared memory) with ring item `item`, once its place is free
-      auto product = [&](uint32_t to, uint64_t a, uint32_t item, int n, uint64_t* free, uint64_t* done) {
-        ok = ok && mbar_wait_warp(free, (n_s & 1) ^ 1, kErrMmaTimeout) &&
-             mbar_wait_warp(&full[item % L::kSlots], (item / L::kSlots) & 1, kErrCopyTimeout);
-        if (!ok) return;
-        tc_fence_after();
-        const uint64_t b = win_rows(ring + item % L::kSlots * L::kTileBytes);
-        const uint32_t id = idesc_bf16(128, u.columns(n), false, false);
+  if (warp >= kBwdRowWarps) {
+    win_fewer_registers<kBwdOtherRegs>();
+    if (warp == 16) {
+      // ---- loads
+      uint32_t it = 0, q_turn = 0, y_turn = 0;
+      bool ok = true;
+      auto load = [&](uint32_t to, uint64_t* full, uint64_t* empty, uint32_t turn, const CUtensorMap* map,
+                      const CUtensorMap* sink_map, const WinQueryUnit& u, int n) {
+        if (!(ok = ok && mbar_wait_warp(empty, (turn & 1) ^ 1, kErrMmaTimeout))) return;
+        const bool sink = n < u.sink_tiles;
         if (elect_one()) {
+          mbar_expect_tx(full, L::kBoxes * (sink ? p.sink_rows : 128) * 128);
 #pragma unroll
-          for (int s = 0; s < kD / 16; ++s) mma_bf16(to, win_rows_step(a, s), win_rows_step(b, s), id, s > 0);
-          mma_commit(done);
+          for (int c = 0; c < L::kBoxes; ++c)
+            tma_load_4d(to + c * kSwBox, sink ? sink_map : map, 64 * c, u.key(w, n), u.kv_head, u.b, full);
         }
       };
-      if (!(ok = mbar_wait_warp(&q_full, q_turn++ & 1, kErrCopyTimeout))) break;
-      tc_fence_after();
-      product(0, q0, it, 0, &s_free, &s_full);
-      product(kDp, dy0, it + 1, 0, &dp_free, &dp_full);
-      if (ok && elect_one()) {
-        mma_commit(&empty[(it + 1) % L::kSlots]);
-        if (u.count == 1) mma_commit(&q_empty);
-      }
-      ++n_s;
-      for (int n = 0; n < u.count && ok; ++n, it += 2) {
-        if (n + 1 < u.count) {
-          product(0, q0, it + 2, n + 1, &s_free, &s_full);
-          product(kDp, dy0, it + 3, n + 1, &dp_free, &dp_full);
-          if (ok && elect_one()) {
-            mma_commit(&empty[(it + 3) % L::kSlots]);
-            if (n + 2 == u.count) mma_commit(&q_empty);
-          }
-          ++n_s;
-        }
-        if (!(ok = ok && mbar_wait_warp(&ds_full, n_ds++ & 1, kErrMmaTimeout))) break;
-        tc_fence_after();
-        const uint64_t k = win_inner(ring + it % L::kSlots * L::kTileBytes);
-        const int steps = u.columns(n) >> 4;
+      auto load_key = [&](const WinQueryUnit& u, int n) {
+        const uint32_t s = it % L::kKeySlots;
+        load(keys + s * L::kTileBytes, &k_full[s], &k_empty[s], it / L::kKeySlots, &p.k, &p.k_sink, u, n);
+      };
+      auto load_value = [&](const WinQueryUnit& u, int n) {
+        const uint32_t s = it % L::kValueSlots;
+        load(values + s * L::kTileBytes, &v_full[s], &v_empty[s], it / L::kValueSlots, &p.v, &p.v_sink, u, n);
+        ++it;
+      };
+      for (int unit = blockIdx.x; unit < p.units && ok; unit += gridDim.x) {
+        const WinQueryUnit u(p, unit);
+        if (u.count == 0) continue;
+        load_key(u, 0);
+        if (!(ok = ok && mbar_wait_warp(&q_empty, (q_turn++ & 1) ^ 1, kErrMmaTimeout))) break;
         if (elect_one()) {
+          mbar_expect_tx(&q_full, 2 * L::kTileBytes);
 #pragma unroll
-          for (int s = 0; s < 8; ++s)
-            if (s < steps) mma_bf16_ts(kDq, kDs + 8 * s, win_inner_step(k, s), id_dq, n > 0 || s > 0);
-          mma_commit(&ds_free);
-          mma_commit(&empty[it % L::kSlots]);
-          if (n == u.count - 1) mma_commit(&dq_full);
+          for (int c = 0; c < L::kBoxes; ++c) {
+            tma_load_4d(q_at + c * kSwBox, &p.q, 64 * c, 128 * u.tile, u.head, u.b, &q_full);
+            tma_load_4d(dy_at + c * kSwBox, &p.dy, 64 * c, 128 * u.tile, u.head, u.b, &q_full);
+          }
+        }
+        load_value(u, 0);
+        if (L::kKeepsY) {
+          if (!(ok = ok && mbar_wait_warp(&y_empty, (y_turn++ & 1) ^ 1, kErrMmaTimeout))) break;
+          if (elect_one()) {
+            mbar_expect_tx(&y_full, L::kTileBytes);
+#pragma unroll
+            for (int c = 0; c < L::kBoxes; ++c)
+              tma_load_4d(y_at + c * kSwBox, &p.y, 64 * c, 128 * u.tile, u.head, u.b, &y_full);
+          }
+        }
+        for (int n = 1; n < u.count && ok; ++n) {
+          load_key(u, n);
+          load_value(u, n);
+        }
+      }
+      if (!ok) {
+        // given up: let the copies in flight land before the memory goes (for a bounded time too)
+        auto landed = [](uint64_t* bar, uint32_t turn) {
+          for (int poll = 0; poll < (1 << 16) && !mbar_try_wait(bar, turn & 1); ++poll) {
+          }
+        };
+        for (uint32_t i = it > L::kKeySlots ? it - L::kKeySlots : 0; i <= it; ++i) {
+          landed(&k_full[i % L::kKeySlots], i / L::kKeySlots);
+          if (i < it) landed(&v_full[i % L::kValueSlots], i / L::kValueSlots);
+        }
+        if (q_turn > 0) landed(&q_full, q_turn - 1);
+        if (y_turn > 0) landed(&y_full, y_turn - 1);
+      }
+    } else if (warp == 17) {
+      // ---- instructions: the next S once the rows have this one in registers, the next dP and dq once they have sent ds
+      constexpr uint32_t id_dq = idesc_bf16(128, kD, false, true), id_s = idesc_bf16(128, 128, false, false);
+      const uint64_t q0 = win_rows(q_at), dy0 = win_rows(dy_at), k0 = win_rows(keys), v0 = win_rows(values), kt0 = win_inner(keys);
+      uint32_t k_slot = 0, k_parity = 0, v_slot = 0, v_parity = 0, dq_slot = 0, q_parity = 0, s_parity = 1, ds_parity = 0;
+      bool ok = true;
+      for (int unit = blockIdx.x; unit < p.units && ok; unit += gridDim.x) {
+        const WinQueryUnit u(p, unit);
+        if (u.count == 0) continue;
+        auto id_of = [&](int n) { return n < u.sink_tiles ? idesc_bf16(128, u.columns(n), false, false) : id_s; };
+        auto scores = [&](int n) {
+          const uint32_t id = id_of(n);
+          ok = ok && mbar_wait_warp(&k_full[k_slot], k_parity, kErrCopyTimeout) && mbar_wait_warp(&s_free, s_parity, kErrMmaTimeout);
+          s_parity ^= 1;
+          if (!ok) return;
+          tc_fence_after();
+          const uint64_t k = k0 + k_slot * kSlotStep;
+          if (elect_one()) {
+#pragma unroll
+            for (int s = 0; s < kD / 16; ++s) mma_bf16(0, win_rows_step(q0, s), win_rows_step(k, s), id, s > 0);
+            mma_commit(&s_full);
+          }
+          if (++k_slot == L::kKeySlots) {
+            k_slot = 0;
+            k_parity ^= 1;
+          }
+        };
+        // dP of tile n; by one lane
+        auto weights = [&](int n, uint32_t id) {
+          const uint64_t v = v0 + v_slot * kSlotStep;
+#pragma unroll
+          for (int s = 0; s < kD / 16; ++s) mma_bf16(kDp, win_rows_step(dy0, s), win_rows_step(v, s), id, s > 0);
+          mma_commit(&dp_full);
+          mma_commit(&v_empty[v_slot]);
+          if (n == u.count - 1) mma_commit(&q_empty);
+        };
+        auto next_value = [&] {
+          if (++v_slot == L::kValueSlots) {
+            v_slot = 0;
+            v_parity ^= 1;
+          }
+        };
+        ok = ok && mbar_wait_warp(&q_full, q_parity, kErrCopyTimeout);
+        q_parity ^= 1;
+        scores(0);
+        ok = ok && mbar_wait_warp(&v_full[v_slot], v_parity, kErrCopyTimeout);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) weights(0, id_of(0));
+        next_value();
+        for (int n = 0; n < u.count && ok; ++n) {
+          const bool more = n + 1 < u.count;
+          if (more) {
+            scores(n + 1);
+            ok = ok && mbar_wait_warp(&v_full[v_slot], v_parity, kErrCopyTimeout);
+          }
+          const uint32_t id = id_of(n + 1);
+          const uint64_t k = kt0 + dq_slot * kSlotStep;
+          const int steps = u.columns(n) >> 4;
+          ok = ok && mbar_wait_warp(&ds_full, ds_parity, kErrMmaTimeout);
+          ds_parity ^= 1;
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_one()) {
+            if (more) weights(n + 1, id);
+#pragma unroll
+            for (int s = 0; s < 8; ++s)
+              if (s < steps) mma_bf16_ts(kDq, kDs + 8 * s, win_inner_step(k, s), id_dq, n > 0 || s > 0);
+            mma_commit(&ds_free);
+            mma_commit(&k_empty[dq_slot]);
+            if (!more) mma_commit(&dq_full);
+          }
+          if (more) next_value();
+          if (++dq_slot == L::kKeySlots) dq_slot = 0;
         }
       }
     }
-  } else if (warp < 8) {
-    // ---- rows
-    const int half = warp >> 2, quad = warp & 3, row = 32 * quad + lane;
+  } else {
+    // ---- rows: part `part` of the columns of row `row`
+    win_more_registers<kBwdRowRegs>();
+    const int part = warp >> 2, quad = warp & 3, row = 32 * quad + lane;
     const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
-    const uint32_t s_at = lanes + 64 * half, dp_at = kDp + lanes + 64 * half, ds_at = kDs + lanes + 32 * half;
-    const float scale2 = w.scale * kLog2e;
-    uint32_t turn = 0, n_s = 0, dq_turn = 0;
+    const uint32_t s_at = lanes + 32 * part, dp_at = kDp + lanes + 32 * part, ds_at = kDs + lanes + 16 * part;
+    const Pair scale2(w.scale * kLog2e);
+    uint32_t turn = 0, it = 0, dq_turn = 0;
     bool ok = true;
     auto signal = [&](uint64_t* bar) {
       tc_fence_before();
@@ -281,136 +341,110 @@ __global__ void __launch_bounds__(kBwdThreads, 1) window_bwd_q_kernel(const __gr
       if (lane == 0) mbar_arrive(bar);
     };
     for (int unit = blockIdx.x; unit < p.units; unit += gridDim.x) {
-      const WinQueryUnit u(w, unit);
+      const WinQueryUnit u(p, unit);
       const int q_row = 128 * u.tile + row, at = w.past + q_row;
       const size_t stat = (static_cast<size_t>(u.b) * w.heads + u.head) * (128 * static_cast<size_t>(w.q_tiles)) + q_row;
       __nv_bfloat16* to = p.dq + u.b * p.dq_strides[0] + u.head * p.dq_strides[1] + q_row * p.dq_strides[2];
       if (u.count == 0) {
         // rows behind the sequence
         const uint32_t none[32] = {};
-        for (int c = 32 * half; c < w.dim; c += 64)
-          if (q_row < w.q_tokens) store_row(to, none, 0.f, c, w.dim);
-        if (half == 0) p.delta[stat] = 0.f;
+        if (q_row < w.q_tokens) store_row(to, none, 0.f, 32 * part, w.dim);
+        if (part == 0) p.delta[stat] = 0.f;
         continue;
       }
-      const float lse = p.lse[stat];
-      // delta: this thread's half of the channels, and its partner's
-      ok = ok && mbar_wait(&q_full, turn & 1, kErrCopyTimeout) && mbar_wait(&y_full, turn & 1, kErrCopyTimeout);
-      ++turn;
-      float part = 0.f;
-      if (ok) {
+      const Pair origin(-p.lse[stat]);
+      // delta: half of the channels to each of two threads
+      uint4 y[kD / 16];
+      if (!L::kKeepsY && part < 2) {
+        const __nv_bfloat16* from = p.y_at + u.b * p.y_strides[0] + u.head * p.y_strides[1] + q_row * p.y_strides[2];
 #pragma unroll
         for (int i = 0; i < kD / 16; ++i) {
-          const int c8 = half * (kD / 16) + i;
-          const uint32_t off = (c8 >> 3) * kSwBox + sw128_offset(row, c8 & 7);
-          float a[8], b[8];
-          unpack8(ld_shared_v4(dy_at + off), a);
-          unpack8(ld_shared_v4(y_at + off), b);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) part = fmaf(a[e], b[e], part);
+          const int c = 8 * (part * (kD / 16) + i);
+          y[i] = q_row < w.q_tokens && c < w.dim ? __ldg(reinterpret_cast<const uint4*>(from + c)) : make_uint4(0, 0, 0, 0);
         }
       }
-      // the row warps meet here, and only here: they go on, or give up, together
-      halves[half][row] = part;
+      ok = ok && mbar_wait(&q_full, turn & 1, kErrCopyTimeout) && (!L::kKeepsY || mbar_wait(&y_full, turn & 1, kErrCopyTimeout));
+      ++turn;
+      if (ok && part < 2) {
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < kD / 16; ++i) {
+          const int c8 = part * (kD / 16) + i;
+          const uint32_t off = (c8 >> 3) * kSwBox + sw128_offset(row, c8 & 7);
+          if (L::kKeepsY) y[i] = ld_shared_v4(y_at + off);
+          float a[8], b[8];
+          unpack8(ld_shared_v4(dy_at + off), a);
+          unpack8(y[i], b);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) sum = fmaf(a[e], b[e], sum);
+        }
+        halves[part][row] = sum;
+      }
+      // The row warps meet here, and only here: they go on, or give up, together.  (All have read the dq of the unit
+      // before, which this one's first ds lets be overwritten.)
       if (!rows_all(ok)) break;
       const float delta = halves[0][row] + halves[1][row];
-      if (half == 0) p.delta[stat] = delta;
+      if (part == 0) p.delta[stat] = delta;
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(&y_empty);
         mbar_arrive(&q_empty);
       }
       const int near = max(at - w.window + 1, u.sinks), upto = at < u.length ? at : -1;   // visible: first ones, near..upto
-      for (int n = 0; n < u.count && ok; ++n, ++n_s) {
-        const int cols = u.columns(n), key = u.key(w, n);
+      for (int n = 0; n < u.count && ok; ++n, ++it) {
+        const int key = u.key(w, n) + 32 * part;
         const bool sink = n < u.sink_tiles;
-        const int from = (sink ? 0 : near - key) - 64 * half;
-        const int until = min(min(upto, sink ? u.sinks - 1 : upto) - key, cols - 1) - 64 * half;
-        if (!(ok = mbar_wait(&s_full, n_s & 1, kErrMmaTimeout))) break;
+        const int from = sink ? 0 : near - key, until = min(upto, sink ? u.sinks - 1 : upto) - key;
+        // whether all, or any, of the warp's rows see all, or any, of its columns
+        const bool all = __all_sync(0xffffffffu, from <= 0 && until >= 31);
+        const bool some = all || __any_sync(0xffffffffu, from <= 31 && until >= 0 && from <= until);
+        if (!(ok = mbar_wait(&s_full, it & 1, kErrMmaTimeout))) break;
         tc_fence_after();
-        if (cols <= 64) {
-          // a narrow tile: 32 columns at a time, all of them the first group's
-          if (!(ok = mbar_wait(&dp_full, n_s & 1, kErrMmaTimeout) && mbar_wait(&ds_free, (n_s & 1) ^ 1, kErrMmaTimeout))) break;
-          tc_fence_after();
-          if (half == 0) {
-#pragma unroll 1
-            for (int c = 0; c < cols; c += 32) {
-              uint32_t s[32], d[32], out[16];
-              tmem_ld(s_at + c, s);
-              tmem_ld(dp_at + c, d);
-              tmem_wait();
-              tie(s);
-              tie(d);
-              hide(s, from - c, until - c);
-#pragma unroll
-              for (int e = 0; e < 32; ++e)
-                s[e] = __float_as_uint(exp2_fast(fmaf(__uint_as_float(s[e]), scale2, -lse)));
-              score_gradients(s, d, delta, out);
-              tmem_st(ds_at + c / 2, out);
-            }
-            tmem_store_wait();
-          }
-          signal(&s_free);
-          signal(&dp_free);
-          signal(&ds_full);
-          continue;
-        }
-        uint32_t s[32], t[32];
+        uint32_t s[32], d[32], out[16];
         tmem_ld(s_at, s);
-        tmem_ld(s_at + 32, t);
         tmem_wait();
         tie(s);
-        tie(t);
         signal(&s_free);
-        if (!__all_sync(0xffffffffu, from <= 0 && until >= 63)) {
-          hide(s, from, until);
-          hide(t, from - 32, until - 32);
-        }
+        if (some) {
+          if (!all) hide(s, from, until);
 #pragma unroll
-        for (int e = 0; e < 32; ++e) s[e] = __float_as_uint(exp2_fast(fmaf(__uint_as_float(s[e]), scale2, -lse)));
+          for (int e = 0; e < 32; e += 2) {
+            float a, b;
+            weight_pair(s[e], s[e + 1], scale2, origin, a, b);
+            s[e] = __float_as_uint(a);
+            s[e + 1] = __float_as_uint(b);
+          }
+        }
+        if (!(ok = mbar_wait(&dp_full, it & 1, kErrMmaTimeout) && mbar_wait(&ds_free, (it & 1) ^ 1, kErrMmaTimeout))) break;
+        tc_fence_after();
+        tmem_ld(dp_at, d);
+        tmem_wait();
+        tie(d);
+        if (some) {
+          score_gradients(s, d, delta, out);
+        } else {
 #pragma unroll
-        for (int e = 0; e < 32; ++e) t[e] = __float_as_uint(exp2_fast(fmaf(__uint_as_float(t[e]), scale2, -lse)));
-        if (!(ok = mbar_wait(&dp_full, n_s & 1, kErrMmaTimeout))) break;
-        tc_fence_after();
-        uint32_t out[2][16];
-        {
-          uint32_t d[32];
-          tmem_ld(dp_at, d);
-          tmem_wait();
-          tie(d);
-          score_gradients(s, d, delta, out[0]);
+          for (int e = 0; e < 16; ++e) out[e] = 0;
         }
-        {
-          uint32_t d[32];
-          tmem_ld(dp_at + 32, d);
-          tmem_wait();
-          tie(d);
-          signal(&dp_free);
-          score_gradients(t, d, delta, out[1]);
-        }
-        if (!(ok = mbar_wait(&ds_free, (n_s & 1) ^ 1, kErrMmaTimeout))) break;
-        tc_fence_after();
-        tmem_st(ds_at, out[0]);
-        tmem_st(ds_at + 16, out[1]);
+        tmem_st(ds_at, out);
         tmem_store_wait();
         signal(&ds_full);
       }
       if (!(ok = ok && mbar_wait(&dq_full, dq_turn++ & 1, kErrMmaTimeout))) continue;
       tc_fence_after();
-#pragma unroll 1
-      for (int c = 32 * half; c < w.dim; c += 64) {
+      if (32 * part < w.dim) {
         uint32_t r[32];
-        tmem_ld(kDq + lanes + c, r);
+        tmem_ld(kDq + lanes + 32 * part, r);
         tmem_wait();
         tie(r);
-        if (q_row < w.q_tokens) store_row(to, r, w.scale, c, w.dim);
+        if (q_row < w.q_tokens) store_row(to, r, w.scale, 32 * part, w.dim);
       }
       tc_fence_before();
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 10) {
+  if (warp == 18) {
     tc_fence_after();
     tmem_dealloc(tmem_slot, 512);
   }
@@ -426,9 +460,8 @@ struct WinKeyUnit {
 
   __device__ __forceinline__ WinKeyUnit(const WinBwdParams& p, int unit) {
     const WinSizes& w = p.w;
-    const int each = p.sink_tiles * p.chunks + p.key_tiles - p.sink_tiles;
-    const int row = unit / each, at = unit - row * each;
-    b = row / w.kv_heads;
+    const int row = p.by_row(unit), at = unit - row * static_cast<int>(p.by_row.by);
+    b = w.by_kv_heads(row);
     kv_head = row - b * w.kv_heads;
     const bool sink = at < p.sink_tiles * p.chunks;
     tile = sink ? at / p.chunks : at - p.sink_tiles * p.chunks + p.sink_tiles;
@@ -453,16 +486,22 @@ struct WinKeyUnit {
   }
 };
 
+// Threads that share a row.  (Four at width 64, where tiles are short work: 64 x 8 heads x 1024, window 256 take 310 us so
+// and 337 with two; two at width 128: 16 heads x 16384, window 2048 582 us with four.)
+constexpr int kv_parts(int d) { return d == 64 ? 4 : 2; }
+constexpr int kv_row_warps(int d) { return 4 * kv_parts(d); }
+constexpr int kv_threads(int d) { return 32 * (kv_row_warps(d) + 4); }
+
 template <int kD>
-__global__ void __launch_bounds__(kBwdThreads, 1) window_bwd_kv_kernel(const __grid_constant__ WinBwdParams p) {
+__global__ void __launch_bounds__(kv_threads(kD), 1) window_bwd_kv_kernel(const __grid_constant__ WinBwdParams p) {
   using L = WinBwdLayout<kD>;
-  constexpr int kSlots = L::kPairSlots;
+  constexpr int kSlots = L::kPairSlots, kParts = kv_parts(kD), kRowWarps = kv_row_warps(kD), kCols = 128 / kParts;
   extern __shared__ uint8_t smem_raw[];
   __shared__ alignas(8) uint64_t full[kSlots], empty[kSlots], kv_full, kv_empty, s_full, dp_full, p_full, ds_full, done;
   __shared__ uint32_t tmem_slot;
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t k_at = base, v_at = base + L::kTileBytes, ring = base + 2 * L::kTileBytes;
-  const uint32_t stats = ring + L::kRingBytes;   // of each slot: 128 lse, 128 delta
+  const uint32_t stats = ring + 2 * kSlots * L::kTileBytes;   // of each slot: 128 lse, 128 delta
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const WinSizes& w = p.w;
   if (threadIdx.x == 0) {
@@ -474,123 +513,130 @@ __global__ void __launch_bounds__(kBwdThreads, 1) window_bwd_kv_kernel(const __g
     mbar_init(&kv_empty, 1);
     mbar_init(&s_full, 1);
     mbar_init(&dp_full, 1);
-    mbar_init(&p_full, 8);
-    mbar_init(&ds_full, 8);
+    mbar_init(&p_full, kRowWarps);
+    mbar_init(&ds_full, kRowWarps);
     mbar_init(&done, 1);
     fence_mbar_init();
   }
-  if (warp == 10) tmem_alloc(&tmem_slot, 512);
+  if (warp == kRowWarps + 2) tmem_alloc(&tmem_slot, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   // all of tensor memory: its addresses start at 0.  Columns: S^T and P^T in its place (each group of warps within its
-  // half), dP^T and dS^T in its place, dv, dk
+  // columns), dP^T and dS^T in its place, dv, dk
   constexpr uint32_t kDp = 128, kDv = 256, kDk = 384;
 
-  if (warp == 8) {
-    // ---- loads
-    uint32_t it = 0, turn = 0;
-    bool ok = true;
-    for (int unit = blockIdx.x; unit < p.units && ok; unit += gridDim.x) {
-      const WinKeyUnit u(p, unit);
-      if (u.count == 0) continue;
-      if (!(ok = mbar_wait_warp(&kv_empty, (turn++ & 1) ^ 1, kErrMmaTimeout))) break;
-      if (elect_one()) {
-        mbar_expect_tx(&kv_full, 2 * L::kTileBytes);
-#pragma unroll
-        for (int c = 0; c < L::kBoxes; ++c) {
-          tma_load_4d(k_at + c * kSwBox, &p.k, 64 * c, 128 * u.tile, u.kv_head, u.b, &kv_full);
-          tma_load_4d(v_at + c * kSwBox, &p.v, 64 * c, 128 * u.tile, u.kv_head, u.b, &kv_full);
-        }
-      }
-      for (int n = 0; n < u.count; ++n, ++it) {
-        const uint32_t s = it % kSlots;
-        if (!(ok = mbar_wait_warp(&empty[s], ((it / kSlots) & 1) ^ 1, kErrMmaTimeout))) break;
-        int head, tile;
-        u.query(w, n, head, tile);
-        const size_t stat = (static_cast<size_t>(u.b) * w.heads + head) * (128 * static_cast<size_t>(w.q_tiles)) + 128 * tile;
+  if (warp >= kRowWarps) {
+    if constexpr (kParts == 4) win_fewer_registers<kBwdOtherRegs>();
+    if (warp == kRowWarps) {
+      // ---- loads
+      uint32_t it = 0, turn = 0;
+      bool ok = true;
+      for (int unit = blockIdx.x; unit < p.units && ok; unit += gridDim.x) {
+        const WinKeyUnit u(p, unit);
+        if (u.count == 0) continue;
+        if (!(ok = mbar_wait_warp(&kv_empty, (turn++ & 1) ^ 1, kErrMmaTimeout))) break;
         if (elect_one()) {
-          const uint32_t to = ring + s * 2 * L::kTileBytes;
-          mbar_expect_tx(&full[s], 2 * L::kTileBytes + 1024);
+          mbar_expect_tx(&kv_full, 2 * L::kTileBytes);
 #pragma unroll
           for (int c = 0; c < L::kBoxes; ++c) {
-            tma_load_4d(to + c * kSwBox, &p.q, 64 * c, 128 * tile, head, u.b, &full[s]);
-            tma_load_4d(to + L::kTileBytes + c * kSwBox, &p.dy, 64 * c, 128 * tile, head, u.b, &full[s]);
+            tma_load_4d(k_at + c * kSwBox, &p.k, 64 * c, 128 * u.tile, u.kv_head, u.b, &kv_full);
+            tma_load_4d(v_at + c * kSwBox, &p.v, 64 * c, 128 * u.tile, u.kv_head, u.b, &kv_full);
           }
-          bulk_load(stats + 1024 * s, p.lse + stat, 512, &full[s]);
-          bulk_load(stats + 1024 * s + 512, p.delta + stat, 512, &full[s]);
+        }
+        for (int n = 0; n < u.count; ++n, ++it) {
+          const uint32_t s = it % kSlots;
+          if (!(ok = mbar_wait_warp(&empty[s], ((it / kSlots) & 1) ^ 1, kErrMmaTimeout))) break;
+          int head, tile;
+          u.query(w, n, head, tile);
+          const size_t stat = (static_cast<size_t>(u.b) * w.heads + head) * (128 * static_cast<size_t>(w.q_tiles)) + 128 * tile;
+          if (elect_one()) {
+            const uint32_t to = ring + s * 2 * L::kTileBytes;
+            mbar_expect_tx(&full[s], 2 * L::kTileBytes + 1024);
+#pragma unroll
+            for (int c = 0; c < L::kBoxes; ++c) {
+              tma_load_4d(to + c * kSwBox, &p.q, 64 * c, 128 * tile, head, u.b, &full[s]);
+              tma_load_4d(to + L::kTileBytes + c * kSwBox, &p.dy, 64 * c, 128 * tile, head, u.b, &full[s]);
+            }
+            bulk_load(stats + 1024 * s, p.lse + stat, 512, &full[s]);
+            bulk_load(stats + 1024 * s + 512, p.delta + stat, 512, &full[s]);
+          }
         }
       }
-    }
-    if (!ok) {
-      // given up: let the copies in flight land before the memory goes (for a bounded time too)
-      for (uint32_t i = it > kSlots ? it - kSlots : 0; i < it; ++i)
-        for (int poll = 0; poll < (1 << 16) && !mbar_try_wait(&full[i % kSlots], (i / kSlots) & 1); ++poll) {
-        }
-    }
-  } else if (warp == 9) {
-    // ---- instructions
-    uint32_t it = 0, turn = 0, n_p = 0;
-    bool ok = true;
-    constexpr uint32_t id_s = idesc_bf16(128, 128, false, false), id_d = idesc_bf16(128, kD, false, true);
-    const uint64_t k0 = win_rows(k_at), v0 = win_rows(v_at);
-    // S^T or dP^T: rows of K or V with rows of the item's queries or their gradients
-    auto product = [&](uint32_t to, uint64_t a, uint32_t tile, uint64_t* finished) {
-      const uint64_t b = win_rows(tile);
-      if (elect_one()) {
+      if (!ok) {
+        // given up: let the copies in flight land before the memory goes (for a bounded time too)
+        for (uint32_t i = it > kSlots ? it - kSlots : 0; i < it; ++i)
+          for (int poll = 0; poll < (1 << 16) && !mbar_try_wait(&full[i % kSlots], (i / kSlots) & 1); ++poll) {
+          }
+      }
+    } else if (warp == kRowWarps + 1) {
+      // ---- instructions: while the rows form ds of this query tile, dv and the next S; while they form the next p, dk
+      // and the next dP
+      constexpr uint32_t id_s = idesc_bf16(128, 128, false, false), id_d = idesc_bf16(128, kD, false, true);
+      constexpr uint32_t kStep = 2 * L::kTileBytes >> 4, kHalf = L::kTileBytes >> 4;   // a slot's queries, its gradients
+      const uint64_t k0 = win_rows(k_at), v0 = win_rows(v_at), rows0 = win_rows(ring), inner0 = win_inner(ring);
+      uint32_t slot = 0, parity = 0, kv_parity = 0, p_parity = 0;
+      bool ok = true;
+      // S^T or dP^T: rows of K or V with rows of a slot's queries or their gradients; by one lane
+      auto product = [&](uint32_t to, uint64_t a, uint64_t b, uint64_t* finished) {
 #pragma unroll
         for (int s = 0; s < kD / 16; ++s) mma_bf16(to, win_rows_step(a, s), win_rows_step(b, s), id_s, s > 0);
         mma_commit(finished);
-      }
-    };
-    // dv or dk: what lies at `a` in tensor memory, 64 queries in each half of 64 columns
-    auto sum = [&](uint32_t to, uint32_t a, uint32_t tile, bool more) {
-      const uint64_t b = win_inner(tile);
-      if (elect_one()) {
+      };
+      // dv or dk: what lies at `a` in tensor memory, kCols queries in each part
+      auto sum = [&](uint32_t to, uint32_t a, uint64_t b, bool more) {
 #pragma unroll
         for (int s = 0; s < 8; ++s)
-          mma_bf16_ts(to, a + 64 * (s >> 2) + 8 * (s & 3), win_inner_step(b, s), id_d, more || s > 0);
-      }
-    };
-    for (int unit = blockIdx.x; unit < p.units && ok; unit += gridDim.x) {
-      const WinKeyUnit u(p, unit);
-      if (u.count == 0) continue;
-      auto landed = [&](uint32_t item) {
-        ok = ok && mbar_wait_warp(&full[item % kSlots], (item / kSlots) & 1, kErrCopyTimeout);
-        tc_fence_after();
-        return ok;
+          mma_bf16_ts(to, a + kCols * (16 * s / kCols) + 16 * s % kCols / 2, win_inner_step(b, s), id_d, more || s > 0);
       };
-      if (!(ok = mbar_wait_warp(&kv_full, turn++ & 1, kErrCopyTimeout)) || !landed(it)) break;
-      product(0, k0, ring + it % kSlots * 2 * L::kTileBytes, &s_full);
-      product(kDp, v0, ring + it % kSlots * 2 * L::kTileBytes + L::kTileBytes, &dp_full);
-      for (int n = 0; n < u.count && ok; ++n, ++it) {
-        const uint32_t q = ring + it % kSlots * 2 * L::kTileBytes, next = ring + (it + 1) % kSlots * 2 * L::kTileBytes;
-        const bool more = n + 1 < u.count;
-        if (!(ok = mbar_wait_warp(&p_full, n_p & 1, kErrMmaTimeout))) break;
+      for (int unit = blockIdx.x; unit < p.units && ok; unit += gridDim.x) {
+        const WinKeyUnit u(p, unit);
+        if (u.count == 0) continue;
+        ok = ok && mbar_wait_warp(&kv_full, kv_parity, kErrCopyTimeout) && mbar_wait_warp(&full[slot], parity, kErrCopyTimeout);
+        kv_parity ^= 1;
+        if (!ok) break;
         tc_fence_after();
-        sum(kDv, 0, q + L::kTileBytes, n > 0);
-        if (more) {
-          if (!landed(it + 1)) break;
-          product(0, k0, next, &s_full);
+        if (elect_one()) {
+          product(0, k0, rows0 + slot * kStep, &s_full);
+          product(kDp, v0, rows0 + slot * kStep + kHalf, &dp_full);
         }
-        if (!(ok = mbar_wait_warp(&ds_full, n_p++ & 1, kErrMmaTimeout))) break;
-        tc_fence_after();
-        sum(kDk, kDp, q, n > 0);
-        if (elect_one()) mma_commit(&empty[it % kSlots]);
-        if (more) product(kDp, v0, next + L::kTileBytes, &dp_full);
-      }
-      if (ok && elect_one()) {
-        mma_commit(&kv_empty);
-        mma_commit(&done);
+        for (int n = 0; n < u.count && ok; ++n) {
+          const bool more = n + 1 < u.count;
+          const uint32_t now = slot;
+          slot = slot + 1 == kSlots ? 0 : slot + 1;
+          parity ^= slot == 0;
+          if (more) ok = mbar_wait_warp(&full[slot], parity, kErrCopyTimeout);
+          ok = ok && mbar_wait_warp(&p_full, p_parity, kErrMmaTimeout);
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_one()) {
+            sum(kDv, 0, inner0 + now * kStep + kHalf, n > 0);
+            if (more) product(0, k0, rows0 + slot * kStep, &s_full);
+          }
+          ok = mbar_wait_warp(&ds_full, p_parity, kErrMmaTimeout);
+          p_parity ^= 1;
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_one()) {
+            sum(kDk, kDp, inner0 + now * kStep, n > 0);
+            mma_commit(&empty[now]);
+            if (more) product(kDp, v0, rows0 + slot * kStep + kHalf, &dp_full);
+          }
+        }
+        if (ok && elect_one()) {
+          mma_commit(&kv_empty);
+          mma_commit(&done);
+        }
       }
     }
-  } else if (warp < 8) {
-    // ---- rows
-    const int half = warp >> 2, quad = warp & 3, row = 32 * quad + lane;
+  } else {
+    // ---- rows: part `part` of the columns (queries) of row `row` (a key)
+    if constexpr (kParts == 4) win_more_registers<kBwdRowRegs>();
+    const int part = warp >> 2, quad = warp & 3, row = 32 * quad + lane;
     const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
-    const uint32_t s_at = lanes + 64 * half, dp_at = kDp + lanes + 64 * half;
-    const float scale2 = w.scale * kLog2e;
-    uint32_t it = 0, turn = 0;
+    const uint32_t s_at = lanes + kCols * part, dp_at = kDp + lanes + kCols * part;
+    const Pair scale2(w.scale * kLog2e);
+    uint32_t slot = 0, parity = 0, it = 0, turn = 0;
     bool ok = true;
     auto signal = [&](uint64_t* bar) {
       tmem_store_wait();
@@ -602,84 +648,89 @@ __global__ void __launch_bounds__(kBwdThreads, 1) window_bwd_kv_kernel(const __g
       const WinKeyUnit u(p, unit);
       const int key = 128 * u.tile + row;
       const bool is_key = key < u.length, everywhere = key < w.sinks;
+      const int last = is_key ? (everywhere ? u.length - 1 : min(u.length - 1, key + w.window - 1)) : -1;
+      int tile = u.first;
       for (int n = 0; n < u.count && ok; ++n, ++it) {
-        const uint32_t slot = it % kSlots;
-        int head, tile;
-        u.query(w, n, head, tile);
         // the columns (queries) that see this row's key
-        const int first = w.past + 128 * tile + 64 * half;
-        const int from = key - first;
-        const int until = is_key ? (everywhere ? u.length - 1 : min(u.length - 1, key + w.window - 1)) - first : -1;
-        const bool masked = !__all_sync(0xffffffffu, from <= 0 && until >= 63);
-        if (!(ok = mbar_wait(&full[slot], (it / kSlots) & 1, kErrCopyTimeout) && mbar_wait(&s_full, it & 1, kErrMmaTimeout)))
-          break;
+        const int first = w.past + 128 * tile + kCols * part, from = key - first, until = last - first;
+        tile = tile + 1 == u.first + u.tiles ? u.first : tile + 1;
+        const bool all = __all_sync(0xffffffffu, from <= 0 && until >= kCols - 1);
+        const bool some = all || __any_sync(0xffffffffu, from <= kCols - 1 && until >= 0 && from <= until);
+        if (!(ok = mbar_wait(&full[slot], parity, kErrCopyTimeout) && mbar_wait(&s_full, it & 1, kErrMmaTimeout))) break;
         tc_fence_after();
-        const uint32_t lse = stats + 1024 * slot + 256 * half, delta = lse + 512;
-        uint32_t s[2][32];
-        tmem_ld(s_at, s[0]);
-        tmem_ld(s_at + 32, s[1]);
+        const uint32_t lse = stats + 1024 * slot + 4 * kCols * part, delta = lse + 512;
+        slot = slot + 1 == kSlots ? 0 : slot + 1;
+        parity ^= slot == 0;
+        uint32_t s[kCols / 32][32];
+#pragma unroll
+        for (int c = 0; c < kCols / 32; ++c) tmem_ld(s_at + 32 * c, s[c]);
         tmem_wait();
-        tie(s[0]);
-        tie(s[1]);
-        if (masked) {
-          hide(s[0], from, until);
-          hide(s[1], from - 32, until - 32);
-        }
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int c = 0; c < kCols / 32; ++c) {
           uint32_t out[16];
+          tie(s[c]);
+          if (some) {
+            if (!all) hide(s[c], from - 32 * c, until - 32 * c);
 #pragma unroll
-          for (int e = 0; e < 32; e += 4) {
-            const uint4 l = ld_shared_v4(lse + 128 * h + 4 * e);
-            const uint32_t of[4] = {l.x, l.y, l.z, l.w};
-            float f[4];
+            for (int e = 0; e < 32; e += 4) {
+              const uint4 l = ld_shared_v4(lse + 128 * c + 4 * e);
+              const uint32_t of[4] = {l.x, l.y, l.z, l.w};
+              float f[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              f[i] = exp2_fast(fmaf(__uint_as_float(s[h][e + i]), scale2, -__uint_as_float(of[i])));
-              s[h][e + i] = __float_as_uint(f[i]);
+              for (int i = 0; i < 4; i += 2) {
+                weight_pair(s[c][e + i], s[c][e + i + 1], scale2, Pair(-__uint_as_float(of[i]), -__uint_as_float(of[i + 1])),
+                            f[i], f[i + 1]);
+                s[c][e + i] = __float_as_uint(f[i]);
+                s[c][e + i + 1] = __float_as_uint(f[i + 1]);
+              }
+              out[e / 2] = pack_bf16(f[0], f[1]);
+              out[e / 2 + 1] = pack_bf16(f[2], f[3]);
             }
-            out[e / 2] = pack_bf16(f[0], f[1]);
-            out[e / 2 + 1] = pack_bf16(f[2], f[3]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) out[e] = 0;
           }
-          tmem_st(s_at + 16 * h, out);
+          tmem_st(s_at + 16 * c, out);
         }
         signal(&p_full);
         if (!(ok = mbar_wait(&dp_full, it & 1, kErrMmaTimeout))) break;
         tc_fence_after();
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int c = 0; c < kCols / 32; ++c) {
           uint32_t d[32], out[16];
-          tmem_ld(dp_at + 32 * h, d);
+          tmem_ld(dp_at + 32 * c, d);
           tmem_wait();
           tie(d);
 #pragma unroll
           for (int e = 0; e < 32; e += 4) {
-            const uint4 l = ld_shared_v4(delta + 128 * h + 4 * e);
+            const uint4 l = ld_shared_v4(delta + 128 * c + 4 * e);
             const uint32_t of[4] = {l.x, l.y, l.z, l.w};
             float f[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const float weight = __uint_as_float(s[h][e + i]);
+              const float weight = some ? __uint_as_float(s[c][e + i]) : 0.f;
               f[i] = weight != 0.f ? weight * (__uint_as_float(d[e + i]) - __uint_as_float(of[i])) : 0.f;
             }
             out[e / 2] = pack_bf16(f[0], f[1]);
             out[e / 2 + 1] = pack_bf16(f[2], f[3]);
           }
-          tmem_st(dp_at + 16 * h, out);
+          tmem_st(dp_at + 16 * c, out);
         }
         signal(&ds_full);
       }
       if (!ok || (u.count > 0 && !(ok = mbar_wait(&done, turn++ & 1, kErrMmaTimeout)))) break;
       tc_fence_after();
-      // the first group's dv, the second's dk
-      const uint32_t acc = (half ? kDk : kDv) + lanes;
-      const long long* strides = half ? p.dk_strides : p.dv_strides;
-      __nv_bfloat16* to = (half ? p.dk : p.dv) + u.b * strides[0] + u.kv_head * strides[1] + key * strides[2];
-      const float scale = u.count == 0 ? 0.f : half ? w.scale : 1.f;
+      // even parts: dv, odd ones: dk; with four, half of the channels each
+      constexpr int kChannels = 2 * kD / kParts;
+      const int what = part & 1;
+      const uint32_t acc = (what ? kDk : kDv) + lanes;
+      const long long* strides = what ? p.dk_strides : p.dv_strides;
+      __nv_bfloat16* to = (what ? p.dk : p.dv) + u.b * strides[0] + u.kv_head * strides[1] + key * strides[2];
+      const float scale = u.count == 0 ? 0.f : what ? w.scale : 1.f;
       const size_t item = ((static_cast<size_t>(u.b) * w.kv_heads + u.kv_head) * p.sink_tiles + u.tile) * p.chunks + u.chunk;
-      float* sums = p.partial + (item * 2 + half) * (kD * 128) + row;
+      float* sums = p.partial + (item * 2 + what) * (kD * 128) + row;
 #pragma unroll 1
-      for (int c = 0; c < w.dim; c += 32) {
+      for (int c = kChannels * (part >> 1); c < kChannels * ((part >> 1) + 1) && c < w.dim; c += 32) {
         uint32_t r[32];
         tmem_ld(acc + c, r);
         tmem_wait();
@@ -700,31 +751,30 @@ __global__ void __launch_bounds__(kBwdThreads, 1) window_bwd_kv_kernel(const __g
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 10) {
+  if (warp == kRowWarps + 2) {
     tc_fence_after();
     tmem_dealloc(tmem_slot, 512);
   }
 }
 
-// The sums of first tokens' key tiles, chunk by chunk; a CTA for each 32 channels of a tile of dk or dv.
+// The sums of first tokens' key tiles, chunk by chunk; a CTA for each 8 channels of a tile of dk or dv.
 template <int kD>
 __global__ void __launch_bounds__(128) window_bwd_join_kernel(const __grid_constant__ WinBwdParams p) {
   const WinSizes& w = p.w;
-  const int part = blockIdx.x % (kD / 32), what = blockIdx.x / (kD / 32) & 1, tile = blockIdx.y % p.sink_tiles;
+  const int part = blockIdx.x % (kD / 8), what = blockIdx.x / (kD / 8), tile = blockIdx.y % p.sink_tiles;
   const int row = blockIdx.y / p.sink_tiles, b = row / w.kv_heads, kv_head = row - b * w.kv_heads;
-  const int key = 128 * tile + threadIdx.x, c = 32 * part;
+  const int key = 128 * tile + threadIdx.x, c = 8 * part;
   if (key >= w.kv_tokens || c >= w.dim) return;
   const float* from = p.partial + (static_cast<size_t>(blockIdx.y) * p.chunks * 2 + what) * (kD * 128) + c * 128 + threadIdx.x;
-  float sum[32] = {};
+  float sum[8] = {};
+#pragma unroll 4
   for (int i = 0; i < p.chunks; ++i) {
 #pragma unroll
-    for (int e = 0; e < 32; ++e) sum[e] += __ldcg(from + static_cast<size_t>(i) * (2 * kD * 128) + e * 128);
+    for (int e = 0; e < 8; ++e) sum[e] += __ldcg(from + static_cast<size_t>(i) * (2 * kD * 128) + e * 128);
   }
-  uint32_t r[32];
-#pragma unroll
-  for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(sum[e]);
   const long long* strides = what ? p.dk_strides : p.dv_strides;
-  store_row((what ? p.dk : p.dv) + b * strides[0] + kv_head * strides[1] + key * strides[2], r, 1.f, c, w.dim);
+  __nv_bfloat16* to = (what ? p.dk : p.dv) + b * strides[0] + kv_head * strides[1] + key * strides[2];
+  *reinterpret_cast<uint4*>(to + c) = pack8(sum);
 }
 
 size_t win_stats_bytes(const WinSizes& w) {
@@ -753,13 +803,15 @@ int window_bwd_launch(WinBwdParams& p, cudaStream_t s) {
     set = cudaFuncSetAttribute(window_bwd_kv_kernel<kD>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmemKV);
   if (set != cudaSuccess) return set_error(TS_ERR_CUDA, "window_bwd: %s", cudaGetErrorString(set));
   p.units = w.batch * w.heads * w.q_tiles;
+  p.by_row = Divisor::of(w.share * w.q_tiles);
   window_bwd_q_kernel<kD><<<p.units < 148 ? p.units : 148, kBwdThreads, L::kSmemQ, s>>>(p);
   if (const int rc = check_launch("window_bwd_q")) return rc;
-  p.units = w.batch * w.kv_heads * (p.sink_tiles * p.chunks + p.key_tiles - p.sink_tiles);
-  window_bwd_kv_kernel<kD><<<p.units < 148 ? p.units : 148, kBwdThreads, L::kSmemKV, s>>>(p);
+  p.by_row = Divisor::of(p.sink_tiles * p.chunks + p.key_tiles - p.sink_tiles);
+  p.units = w.batch * w.kv_heads * static_cast<int>(p.by_row.by);
+  window_bwd_kv_kernel<kD><<<p.units < 148 ? p.units : 148, kv_threads(kD), L::kSmemKV, s>>>(p);
   if (const int rc = check_launch("window_bwd_kv")) return rc;
   if (p.sink_tiles == 0 || p.chunks < 2) return TS_OK;
-  window_bwd_join_kernel<kD><<<dim3(kD / 32 * 2, w.batch * w.kv_heads * p.sink_tiles), 128, 0, s>>>(p);
+  window_bwd_join_kernel<kD><<<dim3(kD / 8 * 2, w.batch * w.kv_heads * p.sink_tiles), 128, 0, s>>>(p);
   return check_launch("window_bwd_join");
 }
 
@@ -797,10 +849,12 @@ int ts_b200_window_bwd(const ts_window_args* a, const ts_window_grad_args* g, ts
   p.lse = a->lse;
   p.delta = static_cast<float*>(g->workspace);
   p.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(g->workspace) + stats);
+  p.y_at = static_cast<const __nv_bfloat16*>(a->y);
   p.dq = static_cast<__nv_bfloat16*>(g->dq);
   p.dk = static_cast<__nv_bfloat16*>(g->dk);
   p.dv = static_cast<__nv_bfloat16*>(g->dv);
   for (int i = 0; i < 3; ++i) {
+    p.y_strides[i] = a->y_strides[i];
     p.dq_strides[i] = g->dq_strides[i];
     p.dk_strides[i] = g->dk_strides[i];
     p.dv_strides[i] = g->dv_strides[i];

@@ -27,7 +27,10 @@ feed-forward block is a :class:`GatedFFN` of that activation), ``fused_norms``
 (each norm takes the previous branch's addition to the residual stream with
 it), training by :class:`AdamW` with states in 32 or 8 bits, and
 :meth:`HybridLM.quantize_head` (inference logits from an 8-bit norm and an
-8-bit vocabulary projection).  ``python -m thetascan_b200.lm`` trains such a
+8-bit vocabulary projection).  With ``window`` the attention layers see a
+sliding window (:func:`thetascan_b200.window_attention`), and
+:meth:`HybridLM.generate` goes on from a prompt token by token, with ring caches
+and scan states whose size does not depend on the length.  ``python -m thetascan_b200.lm`` trains such a
 model on uniform-random tokens for a few steps and reports loss, time and the
 8-bit head's agreement.
 """
@@ -43,6 +46,9 @@ from .config import GNConfig, RoPEConfig, TemporalConfig, ThetaScanConfig
 from .ffn import GatedFFN
 from .mixer import ThetaScan
 from .norm import add_rms_norm, rms_norm, rms_norm_8bit
+from .sample import sample_tokens
+from .seqpar import ScanStream
+from .window import WindowCache, window_attention
 
 
 def gn_mixer_config(d_model: int = 512, n_heads: int = 8, memory_multiplier: int = 2) -> ThetaScanConfig:
@@ -66,27 +72,71 @@ class RMSNorm(nn.Module):
         return F.rms_norm(x, (x.shape[-1],), self.weight, self.eps)
 
 
-def _rope(x, base: float = 10_000.0):
-    """Adjacent-pair rotation of all channels of ``x [B,H,T,d]`` (f32 phases)."""
+def _rope(x, base: float = 10_000.0, start: int = 0):
+    """Adjacent-pair rotation of all channels of ``x [B,H,T,d]`` (f32 phases),
+    whose first token is at position ``start``."""
     B, H, T, d = x.shape
     inv = 1.0 / (base ** (torch.arange(0, d, 2, dtype=torch.float32, device=x.device) / d))
-    ang = torch.outer(torch.arange(T, dtype=torch.float32, device=x.device), inv)
+    ang = torch.outer(torch.arange(start, start + T, dtype=torch.float32, device=x.device), inv)
     cos, sin = ang.cos().to(x.dtype), ang.sin().to(x.dtype)
     even, odd = x[..., 0::2], x[..., 1::2]
     return torch.stack((even * cos - odd * sin, even * sin + odd * cos), dim=-1).flatten(-2)
 
 
+class AttentionStream(WindowCache):
+    """The ring cache of one layer and the tokens that the sequences, all of one
+    length, have had; ``lengths`` (int32, on the device) is the same number for
+    each, and the layers of a model share it."""
+
+    def __init__(self, lengths, n_heads: int, head_dim: int, window: int, sinks: int):
+        super().__init__(lengths.shape[0], n_heads, head_dim, window, sinks, device=lengths.device)
+        self.lengths, self.position = lengths, 0
+
+    def attend(self, q, k, v):
+        """The attention of the next tokens, ``[B,H,T,d]`` bf16, which enter the cache."""
+        T, start = q.shape[2], self.position
+        self.position += T
+        if T == 1:
+            return self.step(q, k, v, self.lengths)
+        slots = self.keys.shape[2]
+        window = slots - self.sinks
+        past_k, past_v = k, v
+        if start:
+            # what the piece still sees, in order: the first tokens, then the last ones (differences of
+            # positions within the window are right even where tokens between the two are left out)
+            order = torch.arange(start, device=q.device)
+            if start > slots:
+                order = torch.cat((order[:self.sinks], order[start - window:]))
+            order = torch.where(order < self.sinks, order, self.sinks + (order - self.sinks) % window)
+            past_k, past_v = (torch.cat((t[:, :, order], new), 2) for t, new in ((self.keys, k), (self.values, v)))
+        y = window_attention(q, past_k, past_v, window, self.sinks)
+        self.extend(k, v, self.lengths)
+        return y
+
+
 class CausalAttention(nn.Module):
-    def __init__(self, d_model: int, n_heads: int):
+    """Causal softmax attention; with a ``window`` each token sees that many last
+    tokens and the ``sinks`` first ones, in bf16 (CUDA only)."""
+
+    def __init__(self, d_model: int, n_heads: int, window: int | None = None, sinks: int = 0):
         super().__init__()
-        self.n_heads = n_heads
+        if window is None and sinks:
+            raise ValueError("first tokens that stay visible (sinks) need a window")
+        self.n_heads, self.window, self.sinks = n_heads, window, sinks
         self.qkv = nn.Linear(d_model, 3 * d_model, bias=False)
         self.out = nn.Linear(d_model, d_model, bias=False)
 
-    def forward(self, x):
+    def forward(self, x, stream: AttentionStream | None = None):
         B, T, D = x.shape
         q, k, v = self.qkv(x).view(B, T, 3, self.n_heads, D // self.n_heads).permute(2, 0, 3, 1, 4)
-        y = F.scaled_dot_product_attention(_rope(q), _rope(k), v, is_causal=True)
+        start = 0 if stream is None else stream.position
+        q, k = _rope(q, start=start), _rope(k, start=start)
+        if self.window is None:
+            y = F.scaled_dot_product_attention(q, k, v, is_causal=True)
+        else:
+            half = [t.to(torch.bfloat16) for t in (q, k, v)]
+            y = window_attention(*half, self.window, self.sinks) if stream is None else stream.attend(*half)
+            y = y.to(q.dtype)
         return self.out(y.transpose(1, 2).reshape(B, T, D))
 
 
@@ -107,16 +157,16 @@ class Block(nn.Module):
         self.mix = mixer
         self.mlp = MLP(d_model, mlp_ratio) if gated is None else GatedFFN(d_model, mlp_ratio * d_model, gated)
 
-    def forward(self, x):
-        x = x + self.mix(self.norm1(x))
+    def forward(self, x, *state):
+        x = x + self.mix(self.norm1(x), *state)
         return x + self.mlp(self.norm2(x))
 
-    def forward_fused(self, branch, stream):
+    def forward_fused(self, branch, stream, *state):
         """The block on a residual ``stream`` that the previous ``branch``
         (None: nothing) still has to be added to; returns its own last branch
         and the stream before that."""
         y, stream = _add_norm(self.norm1, branch, stream)
-        y, stream = _add_norm(self.norm2, self.mix(y), stream)
+        y, stream = _add_norm(self.norm2, self.mix(y, *state), stream)
         return self.mlp(y), stream
 
 
@@ -138,12 +188,15 @@ class HybridLM(nn.Module):
 
     def __init__(self, vocab: int = 1024, d_model: int = 512, n_layers: int = 9, n_heads: int = 8,
                  mlp_ratio: int = 2, mixer_layers=(3, 4), mixer_config: ThetaScanConfig | None = None,
-                 mixer_factory=None, gated: str | None = None, fused_norms: bool = False):
+                 mixer_factory=None, gated: str | None = None, fused_norms: bool = False, window: int | None = None,
+                 sinks: int = 0):
         """``mixer_factory(config)`` builds a mixer module (default: this
         package's ThetaScan; a test passes the reference's own to compare).
         ``gated``: the activation of gated feed-forward blocks (default: the
         plain squared-ReLU MLP).  ``fused_norms``: residual additions within
-        the norms' kernels (CUDA only)."""
+        the norms' kernels (CUDA only).  ``window``, ``sinks``: attention over
+        the last ``window`` tokens and the first ``sinks`` (CUDA only), with
+        which the model can :meth:`generate`."""
         super().__init__()
         self.fused_norms = fused_norms
         self.head_8bit = None
@@ -157,7 +210,7 @@ class HybridLM(nn.Module):
                 mixer = factory(cfg)
                 mixer.zero_output_projection_()
             else:
-                mixer = CausalAttention(d_model, n_heads)
+                mixer = CausalAttention(d_model, n_heads, window, sinks)
             blocks.append(Block(d_model, n_heads, mlp_ratio, mixer, gated))
         self.blocks = nn.ModuleList(blocks)
         self.norm = RMSNorm(d_model)
@@ -197,10 +250,74 @@ class HybridLM(nn.Module):
             branch, x = block.forward_fused(branch, x)
         return self._head(branch, x)
 
+    def stream(self, batch: int) -> "ModelStream":
+        """The start of ``batch`` sequences that come in pieces (see :meth:`extend`)."""
+        return ModelStream(self, batch)
+
+    @torch.no_grad()
+    def extend(self, tokens, stream: "ModelStream"):
+        """Logits ``[B,vocab]`` behind the last of the ``tokens [B,T]`` that the
+        sequences of the ``stream`` go on by.  The whole work on a token does not
+        depend on how many came before it."""
+        if tokens.ndim != 2 or tokens.shape[0] != stream.lengths.shape[0] or tokens.shape[1] < 1:
+            raise ValueError(f"extend: tokens must be [{stream.lengths.shape[0]}, at least 1], got {tuple(tokens.shape)}")
+        if stream.model is not self:
+            raise ValueError("extend: another model's stream")
+        if stream.broken:
+            raise RuntimeError("extend: an earlier call ended with an error, and the stream's layers are not alike")
+        stream.broken = True
+        x, branch = self.embed(tokens), None
+        for block, state in zip(self.blocks, stream.layers):
+            if self.fused_norms:
+                branch, x = block.forward_fused(branch, x, state)
+            else:
+                x = block(x, state)
+        stream.lengths += tokens.shape[1]
+        stream.broken = False
+        return self._head(None if branch is None else branch[:, -1:], x[:, -1:])[:, 0]
+
+    @torch.no_grad()
+    def generate(self, tokens, count: int, *, temperature=1.0, top_k=None, top_p=None, min_p=None,
+                 generator: torch.Generator | None = None, stream: "ModelStream | None" = None):
+        """``count`` further tokens ``[B,count]`` of the sequences that ``tokens
+        [B,T]`` begin (or, with a ``stream``, go on), drawn by
+        :func:`thetascan_b200.sample_tokens` with its settings."""
+        if count < 1:
+            raise ValueError(f"generate: count must be >= 1, got {count}")
+        stream = self.stream(tokens.shape[0]) if stream is None else stream
+        uniform = torch.rand(count, tokens.shape[0], device=tokens.device, generator=generator)
+        got = []
+        for row in uniform:
+            logits = self.extend(tokens, stream)
+            tokens = sample_tokens(logits, row, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)[:, None]
+            got.append(tokens)
+        return torch.cat(got, 1)
+
     def loss(self, tokens):
         """Next-token cross entropy of ``tokens [B,T]`` (predicting 1..T-1)."""
         logits = self(tokens[:, :-1])
         return F.cross_entropy(logits.float().reshape(-1, logits.shape[-1]), tokens[:, 1:].reshape(-1))
+
+
+class ModelStream:
+    """What a :class:`HybridLM` keeps of its sequences: a ring cache of each
+    attention layer, the scan states of each mixer."""
+
+    def __init__(self, model: HybridLM, batch: int):
+        if batch < 1:
+            raise ValueError(f"a stream needs at least one sequence, got {batch}")
+        self.model, self.broken = model, False
+        self.lengths = torch.zeros(batch, dtype=torch.int32, device=model.embed.weight.device)
+        self.layers = []
+        for block in model.blocks:
+            mix = block.mix
+            if isinstance(mix, ThetaScan):
+                self.layers.append(ScanStream())
+            elif isinstance(mix, CausalAttention) and mix.window is not None:
+                width = mix.qkv.in_features // mix.n_heads
+                self.layers.append(AttentionStream(self.lengths, mix.n_heads, width, mix.window, mix.sinks))
+            else:
+                raise TypeError("a stream needs attention with a window and this package's mixers")
 
 
 def main() -> None:
@@ -215,10 +332,17 @@ def main() -> None:
     ap.add_argument("--batch", type=int, default=8)
     ap.add_argument("--tokens", type=int, default=1024)
     ap.add_argument("--gated", default="silu", choices=("silu", "gelu", "relu2"))
+    ap.add_argument("--window", type=int, help="attention over so many last tokens")
+    ap.add_argument("--sinks", type=int, default=0, help="and over so many first ones")
+    ap.add_argument("--generate", type=int, default=0, metavar="N", help="let the model go on by N tokens (needs --window)")
     ap.add_argument("--state-bits", type=int, default=8, choices=(8, 32))
     a = ap.parse_args()
+    if a.generate and a.window is None:
+        ap.error("--generate needs --window")
+    if a.sinks and a.window is None:
+        ap.error("--sinks needs --window")
     torch.manual_seed(0)
-    model = HybridLM(gated=a.gated, fused_norms=True).cuda()
+    model = HybridLM(gated=a.gated, fused_norms=True, window=a.window, sinks=a.sinks).cuda()
     optimizer = AdamW(model.parameters(), lr=3e-4, betas=(0.9, 0.95), weight_decay=0.1, state_bits=a.state_bits)
     data = torch.randint(0, model.embed.num_embeddings, (a.batch, a.tokens + 1), device="cuda")
     for step in range(a.steps):
@@ -237,6 +361,15 @@ def main() -> None:
         got = model(data[:, :-1]).float()
     print(f"8-bit head: logits within {float((got - want).norm() / want.norm()):.3f} of the bf16 head's, "
           f"{float((got.argmax(-1) == want.argmax(-1)).float().mean()) * 100:.1f} % of the tokens the same")
+    if a.generate:
+        with torch.no_grad(), torch.autocast("cuda", dtype=torch.bfloat16):
+            stream = model.stream(a.batch)
+            first = model.generate(data, 1, top_k=50, stream=stream)
+            torch.cuda.synchronize()
+            start = time.perf_counter()
+            got = model.generate(first, a.generate, top_k=50, stream=stream)
+            torch.cuda.synchronize()
+        print(f"{got.numel()} tokens behind {tuple(data.shape)}: {(time.perf_counter() - start) * 1e3 / a.generate:.2f} ms a step")
 
 
 if __name__ == "__main__":

@@ -32,6 +32,7 @@ import torch.nn.functional as F
 
 from .config import ThetaScanConfig
 from .kernel import KernelSpec, Prologue, kernel_core, kernel_core_qkv, kernel_core_sharded
+from .seqpar import ScanStream
 
 EXPANSION_DOMAIN = "thetascan-expansion-v1"
 FINGERPRINT_MAGIC = b"TSXF"
@@ -113,13 +114,21 @@ def _rope_width(d: int, mode: str, frac: float) -> int:
     return max_rot if mode == "full" else min(max_rot, max(2, int(d * frac) // 2 * 2))
 
 
+def _rope_rows(pos0: int, T: int, rot: int, base: float, device: str):
+    """Rows ``pos0 .. pos0 + T - 1`` of the tables; behind the start, of tables
+    whose length is a power of two, so that a stream's steps share them."""
+    if pos0 == 0:
+        return _rope_tables(T, rot, base, device)
+    cos, sin = _rope_tables(1 << (pos0 + T - 1).bit_length(), rot, base, device)
+    return cos[pos0:pos0 + T], sin[pos0:pos0 + T]
+
+
 def _rope(x: torch.Tensor, rot: int, base: float, pos0: int = 0) -> torch.Tensor:
     """Adjacent-pair rotation of the first ``rot`` channels with f32 phases
     (rope.py:57-72); ``pos0`` is the position of the first token."""
     if rot == 0:
         return x
-    cos, sin = _rope_tables(pos0 + x.shape[2], rot, float(base), str(x.device))
-    cos, sin = cos[pos0:], sin[pos0:]
+    cos, sin = _rope_rows(pos0, x.shape[2], rot, float(base), str(x.device))
     even, odd = x[..., 0:rot:2], x[..., 1:rot:2]
     rotated = torch.stack((even * cos - odd * sin, even * sin + odd * cos), dim=-1).flatten(-2)
     return torch.cat((rotated, x[..., rot:]), dim=-1)
@@ -276,14 +285,13 @@ class ThetaScanCore(nn.Module):
         # earlier shards' state.
         deep = self.cfg.depth > 1 or gn.nonlinearity == "swiglu" or shard is not None
         lin = F.linear if deep else tf32_linear
-        pos0 = 0 if shard is None else shard.rank * T
+        pos0 = 0 if shard is None else shard.start(T)
         if self.cfg.key_value_heads is None and not self.cfg.share_key_query:
             # fused projection, then RoPE + L2 of q and k in one row kernel
             from . import ops  # noqa: F401  (registers the operators)
             qkv = lin(xf, self.proj_qkv.weight)
             if rot:
-                cos, sin = _rope_tables(pos0 + T, rot, float(base), str(x.device))
-                cos, sin = cos[pos0:], sin[pos0:]
+                cos, sin = _rope_rows(pos0, T, rot, float(base), str(x.device))
             else:
                 cos = sin = qkv.new_empty(0)
             q, k, v = torch.ops.thetascan_b200.gn_prep_fwd(qkv, cos, sin, rot, H, eps)
@@ -344,7 +352,7 @@ class ThetaScanCore(nn.Module):
         B, T, _ = x.shape
         H, d = self.n_heads, self.head_dim
         rot, base = self._rot, self.cfg.rope.base
-        pos0 = 0 if shard is None else shard.rank * T
+        pos0 = 0 if shard is None else shard.start(T)
         q, k, v = self.project(x)
         q, k = _l2(_rope(q, rot, base, pos0)), _l2(_rope(k, rot, base, pos0))
         if self.vmlp_in is not None:
@@ -431,7 +439,9 @@ class ThetaScanCore(nn.Module):
     def forward(self, x: torch.Tensor, shard=None) -> torch.Tensor:
         """``x [B,T,D]``; with ``shard`` (a :class:`thetascan_b200.seqpar.SeqShard`)
         ``x`` is this rank's contiguous T-slice of longer sequences, and the
-        chunk states of the earlier slices arrive through one exchange."""
+        chunk states of the earlier slices arrive through one exchange; with a
+        :class:`thetascan_b200.seqpar.ScanStream` ``x`` is the next piece of
+        the sequences that the stream has had so far."""
         if not x.is_cuda:
             raise RuntimeError("thetascan_b200 requires a CUDA input")
         if torch.is_autocast_enabled("cuda"):
@@ -447,9 +457,9 @@ class ThetaScanCore(nn.Module):
             return self._forward_gn(x, shard)
         if x.dtype == torch.float32:
             return self._forward_f32(x, shard)
-        if shard is not None and not self._fused_shards():
-            # sequence shards of the other views and reads: the float32 path,
-            # each scan entering with the earlier shards' state
+        if shard is not None and (isinstance(shard, ScanStream) or not self._fused_shards()):
+            # streams, and sequence shards of the other views and reads: the
+            # float32 path, each scan entering with the earlier shards' state
             return self._forward_f32(x.float(), shard).to(x.dtype)
         B, T, _ = x.shape
         H, d = self.n_heads, self.head_dim
@@ -459,7 +469,7 @@ class ThetaScanCore(nn.Module):
         log_alphas, etas = self.fade()
         if shard is not None:
             qkv = F.linear(xb, self.proj_qkv.weight.to(torch.bfloat16))
-            pos0 = shard.rank * T
+            pos0 = shard.start(T)
             cos = sin = None
             if self._rot:
                 cos, sin = _rope_tables(pos0 + T, self._rot, float(self.cfg.rope.base), str(x.device))
@@ -507,7 +517,12 @@ class ThetaScan(nn.Module):
                     p.requires_grad_(False)
 
     def forward(self, x: torch.Tensor, shard=None) -> torch.Tensor:
-        return self._core(x, shard)
+        if not isinstance(shard, ScanStream):
+            return self._core(x, shard)
+        if torch.is_grad_enabled():
+            raise RuntimeError("ThetaScan: a stream has no gradient: call the mixer under torch.no_grad()")
+        with shard.piece(x):
+            return self._core(x, shard)
 
     def zero_output_projection_(self) -> "ThetaScan":
         nn.init.zeros_(self._core.proj_out.weight)

@@ -27,6 +27,7 @@ tests run it around the float64 oracle scan).
 """
 from __future__ import annotations
 
+from contextlib import contextmanager
 from dataclasses import dataclass
 from typing import Callable, Sequence
 
@@ -44,6 +45,10 @@ class SeqShard:
     rank: int
     world: int
     gather: Callable[[torch.Tensor], Sequence[torch.Tensor]]
+
+    def start(self, length: int) -> int:
+        """Position of this rank's first token; every rank has ``length`` tokens."""
+        return self.rank * length
 
 
 def nccl_shard(group=None) -> SeqShard:
@@ -158,6 +163,9 @@ def sharded_reads(shard: SeqShard, scan, query, keys, payload, retentions, *, ap
         return len(base) - 1
 
     plan = [(slot(None), slot(r)) if st else (slot(r), None) for r, st in zip(retentions, stale)]
+    if isinstance(shard, ScanStream):
+        reads = shard.reads(scan, query, keys, payload, tuple(base))
+        return [(reads[a] if b is None else reads[a] - reads[b])[..., :payload.shape[-1] + bool(append_unit)] for a, b in plan]
     reads = list(scan(query, keys, payload, tuple(base), append_unit=True))
     totals = shard.gather(shard_totals(keys, payload, base))
     if shard.rank == 0:
@@ -171,6 +179,68 @@ def sharded_reads(shard: SeqShard, scan, query, keys, payload, retentions, *, ap
         o = reads[a] if b is None else reads[a] - reads[b]
         out.append(o if append_unit else o[..., :-1])
     return out
+
+
+class ScanStream:
+    """Sequences that come in pieces, down to single tokens: in place of a
+    :class:`SeqShard`, the states that a mixer's reads have reached.
+
+    A mixer reads its scans in the same order for every piece, so the states are
+    kept by their place in it: ``[B,H,R,Dk,Dv+1]`` f32 for each.  A single token
+    takes one kernel for each read, which updates the state in place
+    (:func:`thetascan_b200.scan.linattn_views_step`); a longer piece is scanned
+    from a zero state and corrected for the state it enters with, as a shard is.
+    All sequences of the batch go on by the same number of tokens.  A piece that
+    ends with an error leaves the stream unusable.  For inference."""
+
+    def __init__(self):
+        self.position = 0
+        self.states: list[torch.Tensor] = []
+        self._next = 0
+        self._batch = None
+        self._broken = False
+
+    def start(self, length: int) -> int:
+        return self.position
+
+    @contextmanager
+    def piece(self, x: torch.Tensor):
+        """Around the mixer's work on the piece ``x [B,T,D]``."""
+        if self._broken:
+            raise RuntimeError("ScanStream: an earlier piece ended with an error, and the states are not whole")
+        if x.ndim != 3 or x.shape[1] < 1:
+            raise ValueError(f"ScanStream: a piece is [batch, tokens >= 1, channels], got {tuple(x.shape)}")
+        if self._batch not in (None, x.shape[0]):
+            raise ValueError(f"ScanStream: {x.shape[0]} sequences, {self._batch} before")
+        self._next, self._batch, self._broken = 0, x.shape[0], True
+        yield self
+        if self._next != len(self.states):
+            raise RuntimeError(f"ScanStream: {self._next} reads in a piece, {len(self.states)} before: another mixer's stream")
+        self.position += x.shape[1]
+        self._broken = False
+
+    def reads(self, scan, query, keys, payload, retentions) -> list[torch.Tensor]:
+        """Reads of the piece by each retention, with the unit column, as f32."""
+        from .scan import linattn_views_step
+        fresh = self._next == len(self.states)
+        if fresh:
+            if self.position:
+                raise RuntimeError("ScanStream: more reads than in the pieces before: another mixer's stream")
+            B, H, _, m = keys.shape
+            self.states.append(torch.zeros(B, H, len(retentions), m, payload.shape[-1] + 1, dtype=torch.float32,
+                                           device=keys.device))
+        state = self.states[self._next]
+        self._next += 1
+        if query.shape[2] == 1:
+            return [r.float() for r in linattn_views_step(query, keys, payload, retentions, state, append_unit=True)]
+        slots = scan(query, keys, payload, retentions, append_unit=True)
+        totals = shard_totals(keys, payload, retentions)
+        if fresh:
+            state.copy_(totals)
+            return [r.float() for r in slots]
+        reads = add_entering(slots, query, state, retentions)
+        state.copy_(entering_state((state, totals), retentions, query.shape[2], 2))
+        return [r.float() for r in reads]
 
 
 class SequentialShards:

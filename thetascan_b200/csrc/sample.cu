@@ -20,7 +20,11 @@
 // What bounds it is the number of instructions: about 70 for each logit with
 // top-p.  The exponential is therefore in 64 bits, which run at half the rate of
 // 32 but need no compensation: the sum of a logit's product and 1.5 2^52 has the
-// rounded distance, which is the bin too, in its low word.
+// rounded distance, which is the bin too, in its low word.  Only the pass that
+// fills the histogram takes it of every logit: a cut's bin is found again by its
+// first and last logit, and kept tokens are brought side by side in shared memory
+// before their masses are summed (512 rows x 50257, top-p: 168 -> 139 us; 64 rows
+// x 128257 bf16, every filter: 69 -> 62 us).
 #include <cmath>
 #include <type_traits>
 
@@ -39,6 +43,7 @@ constexpr int kSteps = 32;                     // bins of a power of two
 constexpr int kLastStep = 41 * kSteps;         // tokens further than 2^-41 have no mass
 constexpr int kBins = 1536, kPerThread = kBins / kSampleThreads;
 constexpr int kRanked = 512;                   // tokens that are ranked against each other
+constexpr int kFew = 128;                      // kept tokens of a piece that are taken together
 constexpr int kPieces = 2048;                  // of a CTA's tokens: stretches that one warp goes over
 constexpr int kCacheMost = 66560;              // bytes of a CTA's tokens: two CTAs to an SM
 constexpr u64 kOne = 1ull << 40;
@@ -76,7 +81,12 @@ struct SampleShared {
   };
   double power[kSteps];                        // 2^(k/32) in units of 2^-40
   uint32_t key[kRanked], index[kRanked];       // tokens of a bin: this CTA's
-  u64 all_place[kRanked], all_mass[kRanked];   // and the cluster's: key and index, falling in the order
+  union {
+    struct {
+      u64 all_place[kRanked], all_mass[kRanked];   // and the cluster's: key and index, falling in the order
+    };
+    float few[kSampleWarps][kFew];             // after the cuts: kept logits of the piece that a warp is at
+  };
   u64 warp_sum[kSampleWarps], warp_sum_b[kSampleWarps];
   u64 total, total_b, smallest, largest;       // of this CTA, for the others
   float top;
@@ -84,6 +94,7 @@ struct SampleShared {
   // for this CTA's threads
   double scale, offset;                        // of the distance (see Row)
   float lowest, floor_at;
+  float edge[2];                               // a bin's logits: from the first on, below the second
   u64 before, before_b, rest;
   uint32_t bin, cut_key, cut_index, found;
   int piece_at;
@@ -179,9 +190,9 @@ struct Sampler {
     }
   }
   // f(x, first place in the slice, piece) for this thread's tokens of each piece, which are 32 places apart.  A NaN, as
-  // everything that has no mass, is `lowest`.  (The tokens of a piece are taken side by side: one after the other, with
+  // everything that has no mass, is `lowest` (not where f only asks what is above some logit that is not below `lowest`).  (The tokens of a piece are taken side by side: one after the other, with
   // what each of them may lead to between, the waits for their 64-bit operations add up.)
-  template <class F>
+  template <bool kRaise = true, class F>
   __device__ __forceinline__ void each(F f) const {
     for (int piece = threadIdx.x >> 5; piece < pieces; piece += kSampleWarps) {
       float x[kPer];
@@ -190,8 +201,10 @@ struct Sampler {
 #pragma unroll
         for (int j = 0; j < kPer; ++j) x[j] = x[j] == INFINITY ? 0.f : -INFINITY;
       }
+      if constexpr (kRaise) {
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) x[j] = fmaxf(x[j], lowest);
+        for (int j = 0; j < kPer; ++j) x[j] = fmaxf(x[j], lowest);
+      }
       f(x, piece * kPiece + static_cast<int>(threadIdx.x & 31), piece);
     }
   }
@@ -230,12 +243,29 @@ struct Sampler {
     e *= m.power[i & (kSteps - 1)];
     // times 2^(i >> 5), and the integer out of a sum with 2^52
     e = __hiloint2double(__double2hiint(e) + ((i >> 5) << 20), __double2loint(e)) + 4503599627370496.;
-    const u64 w = static_cast<u64>(__double_as_longlong(e)) & 0xfffffffffffffull;
-    return i >= -kLastStep ? w : 0;
+    const u64 w = static_cast<u64>(__double_as_longlong(e)) & 0xfffffffffffffull;   // the bits of 2^52 fall away
+    return w;   // 0 below -kLastStep: it was less than 1/2
   }
   __device__ __forceinline__ u64 mass(float x) const {
     uint32_t b;
     return mass(x, b);
+  }
+
+  // The smallest logit in the bins up to `most` (0: the largest logit is in it), by a whole warp: one that lies behind the
+  // largest logit for most < 0.
+  __device__ __forceinline__ float edge(int most, float top) const {
+    if (most < 0) return INFINITY;
+    uint32_t out = order_key(lowest) - 1, in = order_key(top);   // 32 places between the two at a time
+    while (in - out > 1) {
+      const uint32_t step = (in - out + 31) / 32, at = out + (threadIdx.x & 31) * step + step;
+      const bool past = at >= in || at < out;
+      const uint32_t yes = __ballot_sync(0xffffffffu, past || static_cast<int>(bin(key_value(past ? in : at))) <= most);
+      const int first = __ffs(yes) - 1;   // the last place is `in` or past it
+      const uint32_t here = out + first * step;
+      if (in - here > step) in = here + step;
+      out = here;
+    }
+    return key_value(in);
   }
 
   __device__ __forceinline__ void clear() {
@@ -378,12 +408,13 @@ struct Sampler {
 
   // The cluster's tokens of a bin with keys from `least` to `most`, in every CTA's m.all_place and m.all_mass, their count
   // in m.gathered; false where there are more than kRanked.
-  __device__ __forceinline__ bool gather(uint32_t cut_bin, uint32_t least, uint32_t most) {
+  template <class F>
+  __device__ __forceinline__ bool gather(F in_bin, uint32_t least, uint32_t most) {
     if (threadIdx.x == 0) m.listed = 0;
     barrier();
     const bool whole = least == 0 && most == 0xffffffffu;
-    each([&](Tokens x, int i0, int) {
-      few(x, i0, which(x, [&](float v, int) { return bin(v) == cut_bin; }), [&](float v, int i) {
+    each<false>([&](Tokens x, int i0, int) {
+      few(x, i0, which(x, [&](float v, int) { return in_bin(v); }), [&](float v, int i) {
         const uint32_t k = order_key(v);
         if (!whole && (k < least || k > most)) return;
         const uint32_t at = atomicAdd(&m.listed, 1u);
@@ -411,16 +442,24 @@ struct Sampler {
 
   // The last token that is kept when the order is cut where the count (mass) reaches `target` within the bin in m.bin:
   // m.cut_key and m.cut_index; returned: the mass of the bin's tokens up to it.  The target counts from the bin's start.
-  __device__ __forceinline__ u64 cut(bool by_mass, u64 target) {
+  __device__ __forceinline__ u64 cut(bool by_mass, u64 target, float top) {
+    // the bin's logits; where a lane has two tokens the search for them would take longer than asking each for its bin
     const uint32_t cut_bin = m.bin;
+    if (kPer > 2 && threadIdx.x < 64) {
+      const float at = edge(static_cast<int>(m.bin) - (threadIdx.x < 32 ? 0 : 1), top);
+      if ((threadIdx.x & 31) == 0) m.edge[threadIdx.x >> 5] = at;
+    }
+    __syncthreads();
+    const float from_edge = m.edge[0], to_edge = m.edge[1];
+    auto in_bin = [&](float v) { return kPer > 2 ? v >= from_edge && v < to_edge : bin(fmaxf(v, lowest)) == cut_bin; };
     uint32_t least = 0, most = 0xffffffffu;   // of the keys that are still in question
     u64 before = 0;
     auto in_question = [&](float v) {
       const uint32_t k = order_key(v);
-      return bin(v) == cut_bin && k >= least && k <= most;
+      return in_bin(v) && k >= least && k <= most;
     };
 #pragma unroll 1
-    while (!gather(cut_bin, least, most)) {
+    while (!gather(in_bin, least, most)) {
       // the largest and smallest key
       u64 low = ~0ull, high = 0;
       each([&](Tokens x, int i0, int) {
@@ -622,7 +661,7 @@ struct Sampler {
           locate(b, false, static_cast<u64>(top_k));
           if (m.bin < kBins) {
             const u64 ahead = m.before_b;
-            kept = ahead + cut(false, top_k - m.before);
+            kept = ahead + cut(false, top_k - m.before, top);
             cut_at = key_value(m.cut_key);
             cut_index = m.cut_index;
           } else if (by_mass) {
@@ -640,7 +679,7 @@ struct Sampler {
           __syncthreads();
           locate(b, true, target);
           if (m.bin < kBins) {
-            cut(true, target - m.before_b);
+            cut(true, target - m.before_b, top);
             cut_at = key_value(m.cut_key);
             cut_index = m.cut_index;
           }
@@ -656,22 +695,50 @@ struct Sampler {
     } else if (greedy) {
       first_of(top, total);
     } else {
-      const uint32_t last = cut_index - start;   // as a place in the slice; all or none of it where it lies in another
-      const bool none_here = cut_index < static_cast<uint32_t>(start);
-      auto kept = [&](float v, int i) {
-        return (v > cut_at || (v == cut_at && !none_here && static_cast<uint32_t>(i) <= last)) && v >= floor_at;
-      };
+      // kept: what is at least `least` up to the place `last` of the slice, what is above it behind that
+      const float least = fmaxf(fmaxf(cut_at, floor_at), lowest), above = nextafterf(least, INFINITY);
+      const int last = cut_at < least || cut_index - start > 0x7fffffffu
+                           ? (cut_at < least || cut_index >= static_cast<uint32_t>(start) ? 0x7fffffff : -1)
+                           : static_cast<int>(cut_index - start);
+      auto kept = [&](float v, int i) { return v >= (i <= last ? least : above); };
       u64 mine = 0;
-      each([&](Tokens x, int i0, int piece) {
-        const uint32_t bits = which(x, [&](float v, int i) { return kept(v, i0 + i); });
+      each<false>([&](Tokens x, int i0, int piece) {
+        uint32_t bits;
+        if (last < (piece + 1) * kPiece && last >= piece * kPiece) {
+          bits = which(x, [&](float v, int i) { return kept(v, i0 + i); });
+        } else {
+          const float from_here = last < piece * kPiece ? above : least;
+          bits = which(x, [&](float v, int) { return v >= from_here; });
+        }
         u64 sum = 0;
         if (__any_sync(0xffffffffu, bits)) {
+          // the kept ones side by side, where they are few: their masses are what costs
+          uint32_t upto = __popc(bits);
 #pragma unroll
-          for (int j = 0; j < kPer; ++j) {
-            const u64 w = mass(x[j]);
-            sum += bits >> j & 1 ? w : 0;
+          for (int d = 1; d < 32; d <<= 1) {
+            const uint32_t before = __shfl_up_sync(0xffffffffu, upto, d);
+            if ((threadIdx.x & 31) >= d) upto += before;
           }
-          sum = warp_sum64(sum);
+          const uint32_t all = __shfl_sync(0xffffffffu, upto, 31);
+          if (all <= kFew) {
+            float* to = m.few[threadIdx.x >> 5];
+            uint32_t at = upto - __popc(bits);
+#pragma unroll
+            for (int j = 0; j < kPer; ++j)
+              if (bits >> j & 1) to[at++] = x[j];
+            __syncwarp();
+            for (uint32_t i = threadIdx.x & 31; i < all; i += 32) sum += mass(to[i]);
+            __syncwarp();
+          } else {
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) {
+              const u64 w = mass(fmaxf(x[j], lowest));
+              sum += bits >> j & 1 ? w : 0;
+            }
+          }
+          // below 2^44 in a lane: its parts of 24 bits
+          sum = __reduce_add_sync(0xffffffffu, static_cast<uint32_t>(sum) & 0xffffffu) +
+                (static_cast<u64>(__reduce_add_sync(0xffffffffu, static_cast<uint32_t>(sum >> 24))) << 24);
           mine += sum;
         }
         if ((threadIdx.x & 31) == 0) m.piece[piece] = sum;

@@ -81,6 +81,23 @@ def test_rows_that_see_nothing_are_zero(win):
 
 
 @gpu
+@pytest.mark.parametrize("dim,past,window,sinks", [(64, 0, 100, 4), (128, 0, 300, 0), (80, 77, 150, 130), (128, 40, 64, 200)])
+@pytest.mark.parametrize("filling", [math.nan, math.inf])
+def test_what_lies_behind_a_sequence_does_not_matter(win, dim, past, window, sinks, filling):
+    q, k, v, dy, _ = _make(4, 4, 2, 330, past, dim, False, seed=dim)
+    lengths = torch.tensor([330 + past, 257 + past, 1 + past, 0], dtype=torch.int32, device="cuda")
+    behind = torch.arange(330 + past, device="cuda")[None] >= lengths[:, None]
+    got = []
+    for fill in (0.0, filling):
+        parts = [t.masked_fill(behind[:, None, -t.shape[2]:, None], fill) for t in (q, k, v, dy)]
+        leaves = [t.requires_grad_(True) for t in parts[:3]]
+        y = win.window_attention(*leaves, window, sinks, lengths=lengths)
+        got.append((y.detach(), *torch.autograd.grad(y, leaves, parts[3])))
+    for a, b in zip(*got):
+        assert torch.isfinite(b).all() and torch.equal(a, b)
+
+
+@gpu
 def test_layouts(win):
     g = torch.Generator("cuda").manual_seed(3)
     qkv = torch.randn(2, 150, 3, 4, 64, generator=g, device="cuda").to(BF16)

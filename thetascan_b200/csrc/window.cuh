@@ -101,6 +101,18 @@ __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, i
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, code));
 }
 
+// Zeros in the rows of a tile from `from` on, by the warp that issues the products, before the ones in which they would meet
+// weights of zero: what lies behind a sequence may be anything, and zero times infinity or NaN is not zero.
+template <int kBoxes>
+__device__ __forceinline__ void win_clear_rows(uint32_t tile, int from) {
+#pragma unroll 1
+  for (int at = 128 * max(from, 0) + 16 * static_cast<int>(threadIdx.x & 31); at < static_cast<int>(kSwBox); at += 512)
+#pragma unroll
+    for (int c = 0; c < kBoxes; ++c) st_shared_v4(tile + c * kSwBox + at, make_uint4(0, 0, 0, 0));
+  fence_async_smem();
+  __syncwarp();
+}
+
 // Give up registers of a warpgroup, or take more.
 template <int kRegs>
 __device__ __forceinline__ void win_fewer_registers() {

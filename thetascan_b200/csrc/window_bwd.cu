@@ -265,6 +265,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) window_bwd_q_kernel(const __gr
           s_parity ^= 1;
           if (!ok) return;
           tc_fence_after();
+          if (w.lengths && u.key(w, n) + 128 > u.length) win_clear_rows<L::kBoxes>(keys + k_slot * L::kTileBytes, u.length - u.key(w, n));
           const uint64_t k = k0 + k_slot * kSlotStep;
           if (elect_one()) {
 #pragma unroll
@@ -592,10 +593,20 @@ __global__ void __launch_bounds__(kv_threads(kD), 1) window_bwd_kv_kernel(const 
       for (int unit = blockIdx.x; unit < p.units && ok; unit += gridDim.x) {
         const WinKeyUnit u(p, unit);
         if (u.count == 0) continue;
+        int tile = u.first;   // of the queries that come next
+        auto queries_landed = [&] {
+          const int limit = u.length - w.past - 128 * tile;
+          if (w.lengths && limit < 128) {
+            win_clear_rows<L::kBoxes>(ring + 2 * slot * L::kTileBytes, limit);
+            win_clear_rows<L::kBoxes>(ring + (2 * slot + 1) * L::kTileBytes, limit);
+          }
+          tile = tile + 1 == u.first + u.tiles ? u.first : tile + 1;
+        };
         ok = ok && mbar_wait_warp(&kv_full, kv_parity, kErrCopyTimeout) && mbar_wait_warp(&full[slot], parity, kErrCopyTimeout);
         kv_parity ^= 1;
         if (!ok) break;
         tc_fence_after();
+        queries_landed();
         if (elect_one()) {
           product(0, k0, rows0 + slot * kStep, &s_full);
           product(kDp, v0, rows0 + slot * kStep + kHalf, &dp_full);
@@ -605,7 +616,7 @@ __global__ void __launch_bounds__(kv_threads(kD), 1) window_bwd_kv_kernel(const 
           const uint32_t now = slot;
           slot = slot + 1 == kSlots ? 0 : slot + 1;
           parity ^= slot == 0;
-          if (more) ok = mbar_wait_warp(&full[slot], parity, kErrCopyTimeout);
+          if (more && (ok = mbar_wait_warp(&full[slot], parity, kErrCopyTimeout))) queries_landed();
           ok = ok && mbar_wait_warp(&p_full, p_parity, kErrMmaTimeout);
           if (!ok) break;
           tc_fence_after();

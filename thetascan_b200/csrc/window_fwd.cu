@@ -5,11 +5,15 @@
 //
 // One pass over the keys with a running reference m_i and sum.  A CTA takes two
 // tiles of 128 queries at a time, A and B: of two heads that share a key head, or
-// neighbours of one head, so that both read the same keys.  Warp 8 feeds a ring of
-// key and value tiles by TMA, warps 9 and 11 issue the matrix instructions, warps 0-3 and 4-7 each own the rows of one query tile, a row to a thread.
-// S = Q K^T lies in tensor memory, 128 columns for each of A and B; P replaces it
-// there in bf16 and is the operand of O += P V from where it lies.  While one
-// group forms its P the tensor cores work for the other.
+// neighbours of one head, so that both read the same keys.  One warp feeds a ring of
+// key and value tiles by TMA, another or two issue the matrix instructions, eight
+// own the rows of each query tile, two threads to a row.  S = Q K^T lies in tensor
+// memory, 128 columns for each of A and B; P goes back there in bf16, in S's place
+// or (heads of up to 64) beside it, and is the operand of O += P V from where it
+// lies.  While one group forms its P the tensor cores work for the other: forming
+// P and issuing instructions bound it, not the products (16 heads x 16384, width
+// 128, window 2048, sinks 16: 276 us, 1.0 PFLOP/s of whole tiles; 64 x 8 heads x
+// 1024, width 64, window 256, sinks 4: 122 us, 1.2 TB/s).
 //
 // A row's reference moves only when a score exceeds it by 2^8 (P is then at most
 // 256, and bf16 keeps its relative error): O is seldom rescaled, and the row's own
@@ -127,8 +131,7 @@ __device__ __forceinline__ float ld_shared_f32(uint32_t at) {
   return v;
 }
 
-// 32 scores to weights in bf16, their sum to `part`.  A quarter of the exponentials goes by exp2_poly, beside the special
-// function unit.
+// 32 scores to weights in bf16, their sum to `part`.
 __device__ __forceinline__ void row_exp(const uint32_t (&s)[32], uint32_t to, Pair scale2, Pair origin, Pair (&part)[2]) {
   uint32_t packed[16];
 #pragma unroll
@@ -311,6 +314,8 @@ __global__ void __launch_bounds__(kFwdThreads, 1) window_fwd_kernel(const __grid
           const bool more = n + 1 < u.count;
           if (!(ok = ok && mbar_wait_warp(&full[v_slot], v_parity, kErrCopyTimeout))) break;
           if (more && !keys_landed()) break;
+          if (w.lengths && u.key(w, n) + 128 > u.length)
+            win_clear_rows<L::kBoxes>(base + L::kRing + v_slot * L::kTileBytes, u.length - u.key(w, n));
           step(0, n, more);
           step(1, n, more);
           if (ok && elect_one()) mma_commit(&empty[v_slot]);
@@ -377,6 +382,8 @@ __global__ void __launch_bounds__(kFwdThreads, 1) window_fwd_kernel(const __grid
         auto sums = [&](int n) {
           if (!(ok = ok && mbar_wait_warp(&full[v_slot], v_parity, kErrCopyTimeout))) return;
           if (active(n)) {
+            if (w.lengths && u.key(w, n) + 128 > u.length)
+              win_clear_rows<L::kBoxes>(base + L::kRing + v_slot * L::kTileBytes, u.length - u.key(w, n));
             ok = mbar_wait_warp(&p_full[x], p_parity, kErrMmaTimeout);
             p_parity ^= 1;
             if (!ok) return;

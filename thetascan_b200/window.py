@@ -20,8 +20,9 @@ gradients.  The results do not depend on timing.
 
 ``lengths`` (int32, one per sequence) ends the sequences of a padded batch:
 positions at or behind a sequence's length are seen by none and see none; their
-rows of the output and of the gradients are zero.  What lies in them must be
-finite: it is multiplied by zero within a tile of 128.
+rows of the output and of the gradients are zero, and what lies in them does not
+matter.  (An infinity or NaN within a sequence may reach the rows of other
+positions within its 128: a hidden pair's weight of zero is multiplied by it.)
 """
 from __future__ import annotations
 

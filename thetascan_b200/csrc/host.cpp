@@ -1132,10 +1132,11 @@ PyObject* py_window_extend(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// scan_step(q, k, v, retentions, append_unit, state) -> reads [views, B, H, 1, width]; the state changes in place
+// scan_step(q, k, v, retentions, append_unit, state, apart) -> reads [views, B, H, 1, width], or (apart) a tuple of each
+// view's; the state changes in place
 PyObject* py_scan_step(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  count_args(n, 6);
+  count_args(n, 7);
   const Tensor &q = tensor_arg(args[0], "q"), &k = tensor_arg(args[1], "k"), &v = tensor_arg(args[2], "v");
   THPObjectPtr list(PySequence_Fast(args[3], "retentions"));
   if (!list) throw python_error();
@@ -1147,7 +1148,12 @@ PyObject* py_scan_step(PyObject*, PyObject* const* args, Py_ssize_t n) {
   }
   TORCH_CHECK(!needs_grad({&q, &k, &v}), "linattn_views_step has no gradient: call it under torch.no_grad()");
   TORCH_CHECK_VALUE(!retentions.empty(), "b200 scan step: no retentions");
-  return wrap(scan_step_run(q, k, v, retentions, PyObject_IsTrue(args[4]) == 1, tensor_arg(args[5], "state")));
+  const Tensor reads = scan_step_run(q, k, v, retentions, PyObject_IsTrue(args[4]) == 1, tensor_arg(args[5], "state"));
+  if (PyObject_IsTrue(args[6]) != 1) return wrap(reads);
+  THPObjectPtr tuple(PyTuple_New(static_cast<Py_ssize_t>(reads.size(0))));
+  if (!tuple) throw python_error();
+  for (int64_t i = 0; i < reads.size(0); ++i) PyTuple_SET_ITEM(tuple.get(), i, wrap(reads.select(0, i)));
+  return tuple.release();
   END_HANDLE_TH_ERRORS
 }
 

@@ -469,7 +469,7 @@ def scan_views_step(q: Tensor, k: Tensor, v: Tensor, log_alphas: list[Tensor], p
     """One token of each sequence: reads ``[R,B,H,1,Dv(+unit)]`` in the type of
     the streams; ``state`` moves on in place."""
     _require_cuda(q, k, v, state, *log_alphas)
-    return _lib.host().scan_step(q, k, v, _retentions(log_alphas, present), append_unit, state)
+    return _lib.host().scan_step(q, k, v, _retentions(log_alphas, present), append_unit, state, False)
 
 
 @scan_views_step.register_fake

@@ -363,4 +363,4 @@ def linattn_views_step(q, k, v, retentions, state, *, append_unit: bool = False)
         return torch.ops.thetascan_b200.scan_views_step(
             q, k, v, [r for r in retentions if r is not None], [r is not None for r in retentions], bool(append_unit),
             state).unbind(0)
-    return tuple(_lib.host().scan_step(q, k, v, retentions, append_unit, state).unbind(0))
+    return _lib.host().scan_step(q, k, v, retentions, append_unit, state, True)

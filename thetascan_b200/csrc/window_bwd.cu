@@ -16,6 +16,12 @@
 // each; p and ds go back to tensor memory in bf16 and are the operand of the next
 // product from there.  S^T = K Q^T and dP^T = V dY^T have
 // keys in the rows, which is how dv and dk need them.
+//
+// Forming p and ds bounds it where tiles are narrow, the products and the turns
+// between the two where they are wide: 64 x 8 heads x 1024, width 64, window 256,
+// sinks 4: 197 us for dq, 310 for dk and dv, 44 % of the issue slots; 16 heads x
+// 16384, width 128, window 2048, sinks 16: 465 and 560 us, tensor cores at work for
+// 43 and 56 % of them.
 #include "capi_internal.h"
 #include "window.cuh"
 

@@ -778,11 +778,11 @@ __global__ void __launch_bounds__(kv_threads(kD), 1) window_bwd_kv_kernel(const 
 template <int kD>
 __global__ void __launch_bounds__(128) window_bwd_join_kernel(const __grid_constant__ WinBwdParams p) {
   const WinSizes& w = p.w;
-  const int part = blockIdx.x % (kD / 8), what = blockIdx.x / (kD / 8), tile = blockIdx.y % p.sink_tiles;
-  const int row = blockIdx.y / p.sink_tiles, b = row / w.kv_heads, kv_head = row - b * w.kv_heads;
+  const int part = blockIdx.y % (kD / 8), what = blockIdx.y / (kD / 8), tile = blockIdx.x % p.sink_tiles;
+  const int row = blockIdx.x / p.sink_tiles, b = row / w.kv_heads, kv_head = row - b * w.kv_heads;
   const int key = 128 * tile + threadIdx.x, c = 8 * part;
   if (key >= w.kv_tokens || c >= w.dim) return;
-  const float* from = p.partial + (static_cast<size_t>(blockIdx.y) * p.chunks * 2 + what) * (kD * 128) + c * 128 + threadIdx.x;
+  const float* from = p.partial + (static_cast<size_t>(blockIdx.x) * p.chunks * 2 + what) * (kD * 128) + c * 128 + threadIdx.x;
   float sum[8] = {};
 #pragma unroll 4
   for (int i = 0; i < p.chunks; ++i) {
@@ -828,7 +828,7 @@ int window_bwd_launch(WinBwdParams& p, cudaStream_t s) {
   window_bwd_kv_kernel<kD><<<p.units < 148 ? p.units : 148, kv_threads(kD), L::kSmemKV, s>>>(p);
   if (const int rc = check_launch("window_bwd_kv")) return rc;
   if (p.sink_tiles == 0 || p.chunks < 2) return TS_OK;
-  window_bwd_join_kernel<kD><<<dim3(kD / 8 * 2, w.batch * w.kv_heads * p.sink_tiles), 128, 0, s>>>(p);
+  window_bwd_join_kernel<kD><<<dim3(w.batch * w.kv_heads * p.sink_tiles, kD / 8 * 2), 128, 0, s>>>(p);
   return check_launch("window_bwd_join");
 }
 
@@ -858,8 +858,6 @@ int ts_b200_window_bwd(const ts_window_args* a, const ts_window_grad_args* g, ts
   const size_t stats = win_stats_bytes(w);
   if (!g->workspace || g->workspace_bytes < stats + win_partial_bytes(w, p))
     return set_error(TS_ERR_VALUE, "window_bwd: workspace too small");
-  if (static_cast<long long>(w.batch) * w.kv_heads * p.sink_tiles > 65535)
-    return set_error(TS_ERR_NOT_IMPLEMENTED, "window_bwd: too many tiles of first tokens");
   if (static_cast<long long>(w.batch) * w.kv_heads * (static_cast<long long>(p.sink_tiles) * p.chunks + p.key_tiles) > 0x3fffffffll)
     return set_error(TS_ERR_NOT_IMPLEMENTED, "window_bwd: too many key tiles");
   p.sink_rows = w.sinks >= 128 ? 128 : round_up(w.sinks > 0 ? w.sinks : 1, 16);

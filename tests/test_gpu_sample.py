@@ -164,6 +164,34 @@ def test_masked_tokens(sample):
 
 
 @gpu
+def test_logits_and_temperatures_at_the_ends_of_f32(sample):
+    least = torch.finfo(F32).min
+    logits = torch.full((8, 3000), -math.inf, device="cuda")
+    logits[:, 7] = math.nan
+    logits[0, 1000:1010] = least                                   # a mask of the type's lowest value, and nothing else
+    logits[1, ::3] = least
+    logits[1, 1] = torch.nextafter(torch.tensor(least), torch.tensor(0.0))
+    logits[2, 100:1100] = torch.randn(1000, generator=torch.Generator("cuda").manual_seed(1), device="cuda")
+    logits[3, ::2] = torch.linspace(-1, 1, 1500, device="cuda") * 3.4e38
+    logits[4, 5:9] = torch.tensor([-3e38, 3e38, 0.0, 1.0], device="cuda")
+    logits[5, 2000:] = least
+    logits[5, 2001] = 1.0
+    logits[6, 50:60] = math.inf
+    logits[7, ::5] = least / 2
+    temperature = torch.tensor([1.0, 0.5, 3e38, 1e38, 2e38, 1.0, 3e38, 0.0], device="cuda")
+    clean = logits.clone()
+    clean[6] = torch.where(logits[6] == math.inf, 0.0, -math.inf)   # infinities share a row's probability
+    for seed in range(4):
+        uniform = torch.rand(8, generator=torch.Generator("cuda").manual_seed(seed), device="cuda")
+        for settings in (dict(), dict(top_k=4), dict(top_p=0.6), dict(top_k=600, top_p=0.9, min_p=0.01), dict(min_p=0.3)):
+            tokens, logprobs = sample(logits, uniform, temperature=temperature, return_logprobs=True, **settings)
+            _check(tokens, clean, uniform, temperature=temperature, logprobs=logprobs, **settings)
+    temperature[:] = math.inf
+    tokens = sample(logits, uniform, temperature=temperature)
+    assert (clean[torch.arange(8), tokens] > -math.inf).all()
+
+
+@gpu
 def test_uniform_at_its_ends(sample):
     logits, _ = _logits(4, 300, F32, seed=4)
     ends = torch.tensor([0.0, 1 - 2.0 ** -24, 1.0, math.nan], device="cuda")

@@ -152,6 +152,7 @@ struct Sampler {
   uint32_t rank, ranks;
   int row, start, size, pieces;
   bool infinite;                               // the largest logit is infinite: its tokens are 0, and alone
+  bool scaled;                                 // logits are taken times 2^-20: f32 has room below the ones with mass
   float lowest;                                // what lies below has no mass, and is this
   double scale, offset;                        // distance in 32nds of a power of two: scale x + offset, 0 at the top
 
@@ -178,6 +179,9 @@ struct Sampler {
     if constexpr (kBf16) return bf2f(r);
     else return r;
   }
+  __device__ __forceinline__ float meant(float x) const {
+    return infinite ? (x == INFINITY ? 0.f : -INFINITY) : scaled ? x * 0x1p-20f : x;
+  }
   // A piece's logits as they are; behind the slice minus infinity.
   __device__ __forceinline__ void load(const Raw* at, int piece, float (&x)[kPer]) const {
     const int i0 = piece * kPiece + static_cast<int>(threadIdx.x & 31);
@@ -197,9 +201,9 @@ struct Sampler {
     for (int piece = threadIdx.x >> 5; piece < pieces; piece += kSampleWarps) {
       float x[kPer];
       load(p.cache ? cache : from, piece, x);
-      if (infinite) {
+      if (infinite || scaled) {
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) x[j] = x[j] == INFINITY ? 0.f : -INFINITY;
+        for (int j = 0; j < kPer; ++j) x[j] = meant(x[j]);
       }
       if constexpr (kRaise) {
 #pragma unroll
@@ -388,7 +392,7 @@ struct Sampler {
       for (int j = 0; j < kPer; ++j) {
         const int i = m.piece_at * kPiece + 32 * j + static_cast<int>(threadIdx.x);
         float x = i < size ? value(tokens[i]) : -INFINITY;
-        if (infinite) x = x == INFINITY ? 0.f : -INFINITY;
+        x = meant(x);
         const u64 w = f(fmaxf(x, lowest), i);
         u64 upto = w;
 #pragma unroll
@@ -571,7 +575,7 @@ struct Sampler {
   __device__ __forceinline__ void run() {
     const double given = p.temperature ? static_cast<double>(__ldg(p.temperature + row)) : p.temperature_value;
     const bool greedy = !(given > 0.);
-    const double temperature = greedy ? 1. : given;
+    double temperature = greedy ? 1. : fmin(given, 3.4028234663852886e38);
     if (threadIdx.x < kSteps) m.power[threadIdx.x] = exp2(static_cast<int>(threadIdx.x) * (1. / kSteps) + 40.);
     // the largest logit; the slice into shared memory, where each thread reads again what it has put there
     float top = -INFINITY;
@@ -592,7 +596,17 @@ struct Sampler {
     }
     const bool nothing = top == -INFINITY;
     infinite = top == INFINITY;
-    if (infinite) top = 0.f;
+    if (infinite) {
+      top = 0.f;
+      temperature = 1.;
+    }
+    // What has no mass is a logit below the rest, which these leave no room for.  (Where two logits then become one, they
+    // are less than a 2^100th of the temperature or of the largest apart.)
+    scaled = top < -1e38f || temperature > 1e36;
+    if (scaled) {
+      top *= 0x1p-20f;
+      temperature *= 0x1p-20;
+    }
     int top_k = greedy ? 0 : p.top_k ? __ldg(p.top_k + row) : p.top_k_value;
     const double top_p = greedy ? 1. : p.top_p ? static_cast<double>(__ldg(p.top_p + row)) : p.top_p_value;
     if (threadIdx.x == 0) {
@@ -778,7 +792,7 @@ struct Sampler {
   __device__ __forceinline__ void finish(uint32_t token, double temperature, float top, u64 total) {
     p.tokens[row] = token;
     if (!p.logprobs) return;
-    const float v = value(static_cast<const Raw*>(p.logits)[row * p.row_stride + token]);
+    const float v = meant(value(static_cast<const Raw*>(p.logits)[row * p.row_stride + token]));
     const double distance = infinite || v == top ? 0. : (static_cast<double>(v) - top) / temperature;
     p.logprobs[row] = static_cast<float>(distance - log(static_cast<double>(total) / static_cast<double>(kOne)));
   }

@@ -51,7 +51,8 @@ def sample_tokens(logits: Tensor, uniform: Tensor, *, temperature: Union[float, 
     Numbers out of range raise ``ValueError``; in a tensor they have a meaning
     (which is cheaper than looking): a temperature that is not above 0 is 0,
     ``top_k`` below 1, ``top_p`` from 1 on and ``min_p`` up to 0 do not filter,
-    ``top_p`` up to 0 keeps one token and ``min_p`` above 1 is 1.
+    ``top_p`` up to 0 keeps one token, ``min_p`` above 1 is 1, and an infinite
+    temperature is the largest number.
 
     A NaN or minus infinity is a masked token; a row of nothing else gives -1.
     Infinities share a row's probability.  A token under 2^-41 of the largest

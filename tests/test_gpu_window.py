@@ -68,6 +68,19 @@ def test_forward_and_backward(win, case):
 
 
 @gpu
+@pytest.mark.parametrize("batch,heads,kv_heads,tokens,past,dim,sinks", [(64, 2, 1, 300, 0, 64, 3), (65, 2, 2, 200, 30, 64, 0), (33, 3, 1, 140, 7, 72, 140)])
+def test_many_sequences_of_any_length(win, batch, heads, kv_heads, tokens, past, dim, sinks):
+    q, k, v, dy, lengths = _make(batch, heads, kv_heads, tokens, past, dim, True, seed=batch)
+    lengths[5:9], lengths[20:24] = tokens + past, 0   # equal ones among them
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    y = win.window_attention(*leaves, 90, sinks, lengths=lengths)
+    grads = torch.autograd.grad(y, leaves, dy)
+    want, want_grads, bounds = attention(*(t.double() for t in (q, k, v)), 90, sinks, 1 / math.sqrt(dim), lengths, dy.double())
+    for got, w, bound in zip((y.detach(), *grads), (want, *want_grads), bounds):
+        _within(got, w, bound)
+
+
+@gpu
 def test_rows_that_see_nothing_are_zero(win):
     q, k, v, dy, _ = _make(3, 4, 2, 200, 100, 64, False)
     lengths = torch.tensor([0, 150, 100], dtype=torch.int32, device="cuda")   # none, 50 queries, keys but no query

@@ -45,6 +45,87 @@ __device__ __forceinline__ int win_length(const WinSizes& w, int b) {
   return w.lengths ? max(0, min(__ldg(w.lengths + b), w.kv_tokens)) : w.kv_tokens;
 }
 
+// The order of the units of a padded batch, in shared memory.  CTAs take every 148th unit; with the sequences one after
+// another their lengths would leave some CTAs twice the work of others.  Of each key head of sequence b the units 0 ..
+// live(b) - 1 have work, the last ones most: units come by falling index, those of all sequences that have one together,
+// and what has no work at the end.
+struct WinOrder {
+  static constexpr int kMost = 64;   // sequences; more are taken one after another
+  int begin[kMost + 1];              // first unit of those that the sequences 0 .. j, by falling length, have together
+  uint16_t live[kMost];
+  uint8_t sequence[kMost];
+};
+
+// By one warp, before a barrier.
+template <class F>
+__device__ __forceinline__ void win_order(WinOrder& o, const WinSizes& w, F live) {
+  const int lane = threadIdx.x & 31;
+  int n[2], rank[2] = {0, 0};
+#pragma unroll
+  for (int h = 0; h < 2; ++h) n[h] = lane + 32 * h < w.batch ? live(lane + 32 * h) : 0;
+  for (int i = 0; i < 32; ++i) {
+    const int x[2] = {__shfl_sync(0xffffffffu, n[0], i), __shfl_sync(0xffffffffu, n[1], i)};
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int g = 0; g < 2; ++g) rank[h] += x[g] > n[h] || (x[g] == n[h] && i + 32 * g < lane + 32 * h);
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    o.live[rank[h]] = static_cast<uint16_t>(n[h]);
+    o.sequence[rank[h]] = static_cast<uint8_t>(lane + 32 * h);
+  }
+  __syncwarp();
+  int before = 0;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int j = lane + 32 * h;
+    int upto = (o.live[j] - (j + 1 < WinOrder::kMost ? o.live[j + 1] : 0)) * (j + 1) * w.kv_heads;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, upto, d);
+      if (lane >= d) upto += x;
+    }
+    o.begin[j + 1] = before + upto;
+    before += __shfl_sync(0xffffffffu, upto, 31);
+  }
+  if (lane == 0) o.begin[0] = 0;
+}
+
+// A unit's sequence, key head and index of the `each` units that a key head has; `by_each` divides by that.
+__device__ __forceinline__ void win_place(const WinOrder& o, bool ordered, const WinSizes& w, Divisor by_each, int unit, int& b,
+                                          int& kv_head, int& at) {
+  const int each = static_cast<int>(by_each.by);
+  if (!ordered) {
+    const int row = by_each(unit);
+    at = unit - row * each;
+    b = w.by_kv_heads(row);
+    kv_head = row - b * w.kv_heads;
+    return;
+  }
+  int j = 0, rest = unit - o.begin[WinOrder::kMost];
+  if (rest < 0) {
+#pragma unroll
+    for (int s = WinOrder::kMost / 2; s > 0; s >>= 1) j += o.begin[j + s] <= unit ? s : 0;
+    rest = unit - o.begin[j];
+    const int row = rest / ((j + 1) * w.kv_heads);
+    rest -= row * (j + 1) * w.kv_heads;
+    at = o.live[j] - 1 - row;
+    j = w.by_kv_heads(rest);
+    kv_head = rest - j * w.kv_heads;
+  } else {
+    for (; j < WinOrder::kMost - 1; ++j) {
+      const int none = (each - o.live[j]) * w.kv_heads;
+      if (rest < none) break;
+      rest -= none;
+    }
+    const int row = w.by_kv_heads(rest);
+    at = o.live[j] + row;
+    kv_head = rest - row * w.kv_heads;
+  }
+  b = o.sequence[j];
+}
+
 // ---- instructions
 
 // D (+)= A B with A [128 x 16 per step] in tensor memory (bf16, two to a column) and B in shared memory.

@@ -55,6 +55,7 @@ struct WinBwdParams {
   WinSizes w;
   int units;
   Divisor by_row;           // units of a key head
+  bool ordered;
   int sink_rows;
   // dk and dv: key tiles, the ones with first tokens, and the chunks (of `chunk` query tiles) that those are split in
   int key_tiles, sink_tiles, chunks, chunk;
@@ -94,11 +95,10 @@ struct WinQueryUnit {
   bool live;
   int sinks, sink_tiles, first, count;
 
-  __device__ __forceinline__ WinQueryUnit(const WinBwdParams& p, int unit) {
+  __device__ __forceinline__ WinQueryUnit(const WinBwdParams& p, const WinOrder& order, int unit) {
     const WinSizes& w = p.w;
-    const int row = p.by_row(unit), at = unit - row * static_cast<int>(p.by_row.by);
-    b = w.by_kv_heads(row);
-    kv_head = row - b * w.kv_heads;
+    int at;
+    win_place(order, p.ordered, w, p.by_row, unit, b, kv_head, at);
     tile = w.by_share(at);
     head = kv_head * w.share + at - tile * w.share;
     length = win_length(w, b);
@@ -154,6 +154,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) window_bwd_q_kernel(const __gr
   __shared__ alignas(8) uint64_t k_full[L::kKeySlots], k_empty[L::kKeySlots], v_full[L::kValueSlots], v_empty[L::kValueSlots],
       q_full, q_empty, y_full, y_empty, s_full, dp_full, s_free, ds_full, ds_free, dq_full;
   __shared__ uint32_t tmem_slot;
+  __shared__ WinOrder order;
   __shared__ float halves[2][128];   // free again before the next q_full, which waits for every row warp
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t q_at = base, dy_at = base + L::kTileBytes, keys = base + 2 * L::kTileBytes,
@@ -182,6 +183,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1) window_bwd_q_kernel(const __gr
     fence_mbar_init();
   }
   if (warp == 18) tmem_alloc(&tmem_slot, 512);
+  if (warp == 1 && p.ordered)
+    win_order(order, w, [&](int b) { return ((max(0, win_length(w, b) - w.past) + 127) >> 7) * w.share; });
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -215,7 +218,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) window_bwd_q_kernel(const __gr
         ++it;
       };
       for (int unit = blockIdx.x; unit < p.units && ok; unit += gridDim.x) {
-        const WinQueryUnit u(p, unit);
+        const WinQueryUnit u(p, order, unit);
         if (u.count == 0) continue;
         load_key(u, 0);
         if (!(ok = ok && mbar_wait_warp(&q_empty, (q_turn++ & 1) ^ 1, kErrMmaTimeout))) break;
@@ -262,7 +265,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) window_bwd_q_kernel(const __gr
       uint32_t k_slot = 0, k_parity = 0, v_slot = 0, v_parity = 0, dq_slot = 0, q_parity = 0, s_parity = 1, ds_parity = 0;
       bool ok = true;
       for (int unit = blockIdx.x; unit < p.units && ok; unit += gridDim.x) {
-        const WinQueryUnit u(p, unit);
+        const WinQueryUnit u(p, order, unit);
         if (u.count == 0) continue;
         auto id_of = [&](int n) { return n < u.sink_tiles ? idesc_bf16(128, u.columns(n), false, false) : id_s; };
         auto scores = [&](int n) {
@@ -348,7 +351,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) window_bwd_q_kernel(const __gr
       if (lane == 0) mbar_arrive(bar);
     };
     for (int unit = blockIdx.x; unit < p.units; unit += gridDim.x) {
-      const WinQueryUnit u(p, unit);
+      const WinQueryUnit u(p, order, unit);
       const int q_row = 128 * u.tile + row, at = w.past + q_row;
       const size_t stat = (static_cast<size_t>(u.b) * w.heads + u.head) * (128 * static_cast<size_t>(w.q_tiles)) + q_row;
       __nv_bfloat16* to = p.dq + u.b * p.dq_strides[0] + u.head * p.dq_strides[1] + q_row * p.dq_strides[2];
@@ -465,11 +468,10 @@ struct WinKeyUnit {
   int first, tiles, count;   // query tiles first .. first + tiles - 1 of each head that shares the keys
   bool split;
 
-  __device__ __forceinline__ WinKeyUnit(const WinBwdParams& p, int unit) {
+  __device__ __forceinline__ WinKeyUnit(const WinBwdParams& p, const WinOrder& order, int unit) {
     const WinSizes& w = p.w;
-    const int row = p.by_row(unit), at = unit - row * static_cast<int>(p.by_row.by);
-    b = w.by_kv_heads(row);
-    kv_head = row - b * w.kv_heads;
+    int at;
+    win_place(order, p.ordered, w, p.by_row, unit, b, kv_head, at);
     const bool sink = at < p.sink_tiles * p.chunks;
     tile = sink ? at / p.chunks : at - p.sink_tiles * p.chunks + p.sink_tiles;
     chunk = sink ? at - tile * p.chunks : 0;
@@ -506,6 +508,7 @@ __global__ void __launch_bounds__(kv_threads(kD), 1) window_bwd_kv_kernel(const 
   extern __shared__ uint8_t smem_raw[];
   __shared__ alignas(8) uint64_t full[kSlots], empty[kSlots], kv_full, kv_empty, s_full, dp_full, p_full, ds_full, done;
   __shared__ uint32_t tmem_slot;
+  __shared__ WinOrder order;
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t k_at = base, v_at = base + L::kTileBytes, ring = base + 2 * L::kTileBytes;
   const uint32_t stats = ring + 2 * kSlots * L::kTileBytes;   // of each slot: 128 lse, 128 delta
@@ -526,6 +529,11 @@ __global__ void __launch_bounds__(kv_threads(kD), 1) window_bwd_kv_kernel(const 
     fence_mbar_init();
   }
   if (warp == kRowWarps + 2) tmem_alloc(&tmem_slot, 512);
+  if (warp == 1 && p.ordered)
+    win_order(order, w, [&](int b) {   // first tokens' chunks, and the tiles behind them that hold keys
+      const int length = win_length(w, b);
+      return length > 0 ? p.sink_tiles * p.chunks + max(0, ((length + 127) >> 7) - p.sink_tiles) : 0;
+    });
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -540,7 +548,7 @@ __global__ void __launch_bounds__(kv_threads(kD), 1) window_bwd_kv_kernel(const 
       uint32_t it = 0, turn = 0;
       bool ok = true;
       for (int unit = blockIdx.x; unit < p.units && ok; unit += gridDim.x) {
-        const WinKeyUnit u(p, unit);
+        const WinKeyUnit u(p, order, unit);
         if (u.count == 0) continue;
         if (!(ok = mbar_wait_warp(&kv_empty, (turn++ & 1) ^ 1, kErrMmaTimeout))) break;
         if (elect_one()) {
@@ -597,7 +605,7 @@ __global__ void __launch_bounds__(kv_threads(kD), 1) window_bwd_kv_kernel(const 
           mma_bf16_ts(to, a + kCols * (16 * s / kCols) + 16 * s % kCols / 2, win_inner_step(b, s), id_d, more || s > 0);
       };
       for (int unit = blockIdx.x; unit < p.units && ok; unit += gridDim.x) {
-        const WinKeyUnit u(p, unit);
+        const WinKeyUnit u(p, order, unit);
         if (u.count == 0) continue;
         int tile = u.first;   // of the queries that come next
         auto queries_landed = [&] {
@@ -662,7 +670,7 @@ __global__ void __launch_bounds__(kv_threads(kD), 1) window_bwd_kv_kernel(const 
       if (lane == 0) mbar_arrive(bar);
     };
     for (int unit = blockIdx.x; unit < p.units && ok; unit += gridDim.x) {
-      const WinKeyUnit u(p, unit);
+      const WinKeyUnit u(p, order, unit);
       const int key = 128 * u.tile + row;
       const bool is_key = key < u.length, everywhere = key < w.sinks;
       const int last = is_key ? (everywhere ? u.length - 1 : min(u.length - 1, key + w.window - 1)) : -1;
@@ -821,10 +829,12 @@ int window_bwd_launch(WinBwdParams& p, cudaStream_t s) {
   if (set != cudaSuccess) return set_error(TS_ERR_CUDA, "window_bwd: %s", cudaGetErrorString(set));
   p.units = w.batch * w.heads * w.q_tiles;
   p.by_row = Divisor::of(w.share * w.q_tiles);
+  p.ordered = w.lengths && w.batch <= WinOrder::kMost && p.by_row.by <= 0xffff;
   window_bwd_q_kernel<kD><<<p.units < 148 ? p.units : 148, kBwdThreads, L::kSmemQ, s>>>(p);
   if (const int rc = check_launch("window_bwd_q")) return rc;
   p.by_row = Divisor::of(p.sink_tiles * p.chunks + p.key_tiles - p.sink_tiles);
   p.units = w.batch * w.kv_heads * static_cast<int>(p.by_row.by);
+  p.ordered = w.lengths && w.batch <= WinOrder::kMost && p.by_row.by <= 0xffff;
   window_bwd_kv_kernel<kD><<<p.units < 148 ? p.units : 148, kv_threads(kD), L::kSmemKV, s>>>(p);
   if (const int rc = check_launch("window_bwd_kv")) return rc;
   if (p.sink_tiles == 0 || p.chunks < 2) return TS_OK;

@@ -53,6 +53,7 @@ struct WinFwdParams {
   WinSizes w;
   int each, pairs, units;   // query tiles of a unit (1 or 2), units of a key head, units
   Divisor by_pairs;
+  bool ordered;
   int sink_rows;         // rows of a sink box
   float* lse;            // or null
 };
@@ -80,11 +81,10 @@ struct WinFwdUnit {
     t.live = t.exists && w.past + 128 * t.tile < length;
     return t;
   }
-  __device__ __forceinline__ WinFwdUnit(const WinFwdParams& p, int unit) {
+  __device__ __forceinline__ WinFwdUnit(const WinFwdParams& p, const WinOrder& order, int unit) {
     const WinSizes& w = p.w;
-    const int row = p.by_pairs(unit), pair = unit - row * p.pairs;
-    b = w.by_kv_heads(row);
-    kv_head = row - b * w.kv_heads;
+    int pair;
+    win_place(order, p.ordered, w, p.by_pairs, unit, b, kv_head, pair);
     length = win_length(w, b);
     a = place(w, p.each * pair);
     z = place(w, p.each == 2 ? 2 * pair + 1 : w.q_tiles * w.share);   // or none
@@ -154,6 +154,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) window_fwd_kernel(const __grid
   __shared__ alignas(8) uint64_t full[L::kSlots], empty[L::kSlots], q_full[2], q_empty[2], s_full[2], s_free[2], p_full[2],
       p_free[2], o_full[2];
   __shared__ uint32_t tmem_slot;
+  __shared__ WinOrder order;
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const WinSizes& w = p.w;
@@ -174,6 +175,10 @@ __global__ void __launch_bounds__(kFwdThreads, 1) window_fwd_kernel(const __grid
     fence_mbar_init();
   }
   if (warp == 18) tmem_alloc(&tmem_slot, 512);
+  if (warp == 1 && p.ordered)
+    win_order(order, w, [&](int b) {
+      return (((max(0, win_length(w, b) - w.past) + 127) >> 7) * w.share + p.each - 1) / p.each;
+    });
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -202,7 +207,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) window_fwd_kernel(const __grid
         ++it;
       };
       for (int unit = blockIdx.x; unit < p.units && ok; unit += gridDim.x) {
-        const WinFwdUnit u(p, unit);
+        const WinFwdUnit u(p, order, unit);
         auto queries = [&](int x) {
           if (!u.of(x).live || !(ok = ok && mbar_wait_warp(&q_empty[x], (q_turn[x]++ & 1) ^ 1, kErrMmaTimeout))) return;
           if (elect_one()) {
@@ -246,7 +251,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) window_fwd_kernel(const __grid
       uint32_t q_parity[2] = {0, 0}, p_parity[2] = {0, 0};
       bool ok = true;
       for (int unit = blockIdx.x; unit < p.units && ok; unit += gridDim.x) {
-        const WinFwdUnit u(p, unit);
+        const WinFwdUnit u(p, order, unit);
         // tile x takes part in the first tokens' (n < sink_tiles) and from `low` to `last`
         const int low[2] = {0, u.sink_tiles + u.z.low - u.first}, last[2] = {u.a.live ? u.a.last : -1, u.z.live ? u.z.last : -1};
         auto active = [&](int x, int n) { return n <= last[x] && (x == 0 || n < u.sink_tiles || n >= low[x]); };
@@ -342,7 +347,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) window_fwd_kernel(const __grid
       uint32_t q_parity = 0, s_parity = 1, p_parity = 0;
       bool ok = true;
       for (int unit = blockIdx.x; unit < p.units && ok; unit += gridDim.x) {
-        const WinFwdUnit u(p, unit);
+        const WinFwdUnit u(p, order, unit);
         const WinFwdTile mine = u.of(x);
         // this tile takes part in the first tokens' (n < sink_tiles) and from `low` to `last`
         const int low = u.sink_tiles + mine.low - u.first, last = mine.live ? mine.last : -1;
@@ -441,11 +446,11 @@ __global__ void __launch_bounds__(kFwdThreads, 1) window_fwd_kernel(const __grid
       asm volatile("bar.sync %0, 64;" ::"r"(1 + 4 * x + quad) : "memory");
       return ld_shared_f32(partner + 128 * slot + 4 * lane);
     };
-    WinFwdUnit next(p, blockIdx.x);
+    WinFwdUnit next(p, order, blockIdx.x);
     for (int unit = blockIdx.x; unit < p.units; unit += gridDim.x) {
       const WinFwdUnit u = next;
       const WinFwdTile mine = u.of(x);
-      if (unit + gridDim.x < p.units) next = WinFwdUnit(p, unit + gridDim.x);
+      if (unit + gridDim.x < p.units) next = WinFwdUnit(p, order, unit + gridDim.x);
       if (!mine.exists) continue;
       if (lane == 0) tma_store_read_wait<0>();   // the last store has read the stage, which carries exchanges now
       __syncwarp();
@@ -667,6 +672,7 @@ int ts_b200_window_fwd(const ts_window_args* a, ts_stream_t stream) {
   p.pairs = (tiles + p.each - 1) / p.each;
   p.by_pairs = Divisor::of(p.pairs);
   p.units = rows * p.pairs;
+  p.ordered = w.lengths && w.batch <= WinOrder::kMost && p.pairs <= 0xffff;
   p.sink_rows = w.sinks >= 128 ? 128 : round_up(w.sinks > 0 ? w.sinks : 1, 16);
   p.lse = a->lse;
   const bool ok = win_map(&p.q, a->q, a->q_strides, w.batch, w.heads, w.q_tokens, w.dim, 128) &&

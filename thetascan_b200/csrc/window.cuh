@@ -45,16 +45,37 @@ __device__ __forceinline__ int win_length(const WinSizes& w, int b) {
   return w.lengths ? max(0, min(__ldg(w.lengths + b), w.kv_tokens)) : w.kv_tokens;
 }
 
-// The order of the units of a padded batch, in shared memory.  CTAs take every 148th unit; with the sequences one after
-// another their lengths would leave some CTAs twice the work of others.  Of each key head of sequence b the units 0 ..
-// live(b) - 1 have work, the last ones most: units come by falling index, those of all sequences that have one together,
-// and what has no work at the end.
+// The order in which the units (query or key tiles, or pairs) of the key heads are taken.  CTAs take every 148th, and units
+// differ: by the window's start, by a sequence's end.  One key head after another would leave some CTAs up to twice the
+// work of others, so units of one index come together, through all key heads, the ones with most work first (64 x 8 heads x
+// 1024, width 64, window 256, forward and backward: 635 us one after another, 544 so).
+enum WinHow {
+  kWinApart,   // one key head after another
+  kWinLevel,   // all key heads alike
+  kWinTable    // sequences of different lengths: by a WinOrder
+};
+struct WinUnits {
+  int units;
+  Divisor by_each, by_rows;   // units of a key head; key heads of all sequences
+  WinHow how;
+};
+
+// For a padded batch, in shared memory.  Of each key head of sequence b the units 0 .. live(b) - 1 have work: they come by
+// falling index, those of all sequences that have one together, and what has no work at the end.
 struct WinOrder {
   static constexpr int kMost = 64;   // sequences; more are taken one after another
   int begin[kMost + 1];              // first unit of those that the sequences 0 .. j, by falling length, have together
   uint16_t live[kMost];
   uint8_t sequence[kMost];
 };
+
+inline WinUnits win_units(const WinSizes& w, int each) {
+  const int rows = w.batch * w.kv_heads;
+  WinUnits n = {rows * each, Divisor::of(each), Divisor::of(rows), kWinLevel};
+  if (w.lengths) n.how = w.batch <= WinOrder::kMost && each <= 0xffff ? kWinTable : kWinApart;
+  if (n.units <= 148) n.how = kWinApart;   // each has an SM of its own
+  return n;
+}
 
 // By one warp, before a barrier.
 template <class F>
@@ -92,13 +113,21 @@ __device__ __forceinline__ void win_order(WinOrder& o, const WinSizes& w, F live
   if (lane == 0) o.begin[0] = 0;
 }
 
-// A unit's sequence, key head and index of the `each` units that a key head has; `by_each` divides by that.
-__device__ __forceinline__ void win_place(const WinOrder& o, bool ordered, const WinSizes& w, Divisor by_each, int unit, int& b,
-                                          int& kv_head, int& at) {
-  const int each = static_cast<int>(by_each.by);
-  if (!ordered) {
-    const int row = by_each(unit);
-    at = unit - row * each;
+// A unit's sequence, key head and index among the units of a key head.  kRising: the first ones have most work.
+template <bool kRising>
+__device__ __forceinline__ void win_place(const WinOrder& o, const WinUnits& n, const WinSizes& w, int unit, int& b, int& kv_head,
+                                          int& at) {
+  const int each = static_cast<int>(n.by_each.by);
+  if (n.how != kWinTable) {
+    int row;
+    if (n.how == kWinApart) {
+      row = n.by_each(unit);
+      at = unit - row * each;
+    } else {
+      at = n.by_rows(unit);
+      row = unit - at * static_cast<int>(n.by_rows.by);
+      if (!kRising) at = each - 1 - at;
+    }
     b = w.by_kv_heads(row);
     kv_head = row - b * w.kv_heads;
     return;

@@ -53,9 +53,7 @@ struct WinBwdLayout {
 struct WinBwdParams {
   CUtensorMap q, k, v, k_sink, v_sink, y, dy;
   WinSizes w;
-  int units;
-  Divisor by_row;           // units of a key head
-  bool ordered;
+  WinUnits n;
   int sink_rows;
   // dk and dv: key tiles, the ones with first tokens, and the chunks (of `chunk` query tiles) that those are split in
   int key_tiles, sink_tiles, chunks, chunk;
@@ -98,7 +96,7 @@ struct WinQueryUnit {
   __device__ __forceinline__ WinQueryUnit(const WinBwdParams& p, const WinOrder& order, int unit) {
     const WinSizes& w = p.w;
     int at;
-    win_place(order, p.ordered, w, p.by_row, unit, b, kv_head, at);
+    win_place<false>(order, p.n, w, unit, b, kv_head, at);
     tile = w.by_share(at);
     head = kv_head * w.share + at - tile * w.share;
     length = win_length(w, b);
@@ -183,7 +181,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) window_bwd_q_kernel(const __gr
     fence_mbar_init();
   }
   if (warp == 18) tmem_alloc(&tmem_slot, 512);
-  if (warp == 1 && p.ordered)
+  if (warp == 1 && p.n.how == kWinTable)
     win_order(order, w, [&](int b) { return ((max(0, win_length(w, b) - w.past) + 127) >> 7) * w.share; });
   tc_fence_before();
   __syncthreads();
@@ -217,7 +215,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) window_bwd_q_kernel(const __gr
         load(values + s * L::kTileBytes, &v_full[s], &v_empty[s], it / L::kValueSlots, &p.v, &p.v_sink, u, n);
         ++it;
       };
-      for (int unit = blockIdx.x; unit < p.units && ok; unit += gridDim.x) {
+      for (int unit = blockIdx.x; unit < p.n.units && ok; unit += gridDim.x) {
         const WinQueryUnit u(p, order, unit);
         if (u.count == 0) continue;
         load_key(u, 0);
@@ -264,7 +262,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) window_bwd_q_kernel(const __gr
       const uint64_t q0 = win_rows(q_at), dy0 = win_rows(dy_at), k0 = win_rows(keys), v0 = win_rows(values), kt0 = win_inner(keys);
       uint32_t k_slot = 0, k_parity = 0, v_slot = 0, v_parity = 0, dq_slot = 0, q_parity = 0, s_parity = 1, ds_parity = 0;
       bool ok = true;
-      for (int unit = blockIdx.x; unit < p.units && ok; unit += gridDim.x) {
+      for (int unit = blockIdx.x; unit < p.n.units && ok; unit += gridDim.x) {
         const WinQueryUnit u(p, order, unit);
         if (u.count == 0) continue;
         auto id_of = [&](int n) { return n < u.sink_tiles ? idesc_bf16(128, u.columns(n), false, false) : id_s; };
@@ -350,7 +348,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) window_bwd_q_kernel(const __gr
       __syncwarp();
       if (lane == 0) mbar_arrive(bar);
     };
-    for (int unit = blockIdx.x; unit < p.units; unit += gridDim.x) {
+    for (int unit = blockIdx.x; unit < p.n.units; unit += gridDim.x) {
       const WinQueryUnit u(p, order, unit);
       const int q_row = 128 * u.tile + row, at = w.past + q_row;
       const size_t stat = (static_cast<size_t>(u.b) * w.heads + u.head) * (128 * static_cast<size_t>(w.q_tiles)) + q_row;
@@ -471,7 +469,7 @@ struct WinKeyUnit {
   __device__ __forceinline__ WinKeyUnit(const WinBwdParams& p, const WinOrder& order, int unit) {
     const WinSizes& w = p.w;
     int at;
-    win_place(order, p.ordered, w, p.by_row, unit, b, kv_head, at);
+    win_place<true>(order, p.n, w, unit, b, kv_head, at);
     const bool sink = at < p.sink_tiles * p.chunks;
     tile = sink ? at / p.chunks : at - p.sink_tiles * p.chunks + p.sink_tiles;
     chunk = sink ? at - tile * p.chunks : 0;
@@ -529,7 +527,7 @@ __global__ void __launch_bounds__(kv_threads(kD), 1) window_bwd_kv_kernel(const 
     fence_mbar_init();
   }
   if (warp == kRowWarps + 2) tmem_alloc(&tmem_slot, 512);
-  if (warp == 1 && p.ordered)
+  if (warp == 1 && p.n.how == kWinTable)
     win_order(order, w, [&](int b) {   // first tokens' chunks, and the tiles behind them that hold keys
       const int length = win_length(w, b);
       return length > 0 ? p.sink_tiles * p.chunks + max(0, ((length + 127) >> 7) - p.sink_tiles) : 0;
@@ -547,7 +545,7 @@ __global__ void __launch_bounds__(kv_threads(kD), 1) window_bwd_kv_kernel(const 
       // ---- loads
       uint32_t it = 0, turn = 0;
       bool ok = true;
-      for (int unit = blockIdx.x; unit < p.units && ok; unit += gridDim.x) {
+      for (int unit = blockIdx.x; unit < p.n.units && ok; unit += gridDim.x) {
         const WinKeyUnit u(p, order, unit);
         if (u.count == 0) continue;
         if (!(ok = mbar_wait_warp(&kv_empty, (turn++ & 1) ^ 1, kErrMmaTimeout))) break;
@@ -604,7 +602,7 @@ __global__ void __launch_bounds__(kv_threads(kD), 1) window_bwd_kv_kernel(const 
         for (int s = 0; s < 8; ++s)
           mma_bf16_ts(to, a + kCols * (16 * s / kCols) + 16 * s % kCols / 2, win_inner_step(b, s), id_d, more || s > 0);
       };
-      for (int unit = blockIdx.x; unit < p.units && ok; unit += gridDim.x) {
+      for (int unit = blockIdx.x; unit < p.n.units && ok; unit += gridDim.x) {
         const WinKeyUnit u(p, order, unit);
         if (u.count == 0) continue;
         int tile = u.first;   // of the queries that come next
@@ -669,7 +667,7 @@ __global__ void __launch_bounds__(kv_threads(kD), 1) window_bwd_kv_kernel(const 
       __syncwarp();
       if (lane == 0) mbar_arrive(bar);
     };
-    for (int unit = blockIdx.x; unit < p.units && ok; unit += gridDim.x) {
+    for (int unit = blockIdx.x; unit < p.n.units && ok; unit += gridDim.x) {
       const WinKeyUnit u(p, order, unit);
       const int key = 128 * u.tile + row;
       const bool is_key = key < u.length, everywhere = key < w.sinks;
@@ -827,15 +825,11 @@ int window_bwd_launch(WinBwdParams& p, cudaStream_t s) {
   if (set == cudaSuccess)
     set = cudaFuncSetAttribute(window_bwd_kv_kernel<kD>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmemKV);
   if (set != cudaSuccess) return set_error(TS_ERR_CUDA, "window_bwd: %s", cudaGetErrorString(set));
-  p.units = w.batch * w.heads * w.q_tiles;
-  p.by_row = Divisor::of(w.share * w.q_tiles);
-  p.ordered = w.lengths && w.batch <= WinOrder::kMost && p.by_row.by <= 0xffff;
-  window_bwd_q_kernel<kD><<<p.units < 148 ? p.units : 148, kBwdThreads, L::kSmemQ, s>>>(p);
+  p.n = win_units(w, w.share * w.q_tiles);
+  window_bwd_q_kernel<kD><<<p.n.units < 148 ? p.n.units : 148, kBwdThreads, L::kSmemQ, s>>>(p);
   if (const int rc = check_launch("window_bwd_q")) return rc;
-  p.by_row = Divisor::of(p.sink_tiles * p.chunks + p.key_tiles - p.sink_tiles);
-  p.units = w.batch * w.kv_heads * static_cast<int>(p.by_row.by);
-  p.ordered = w.lengths && w.batch <= WinOrder::kMost && p.by_row.by <= 0xffff;
-  window_bwd_kv_kernel<kD><<<p.units < 148 ? p.units : 148, kv_threads(kD), L::kSmemKV, s>>>(p);
+  p.n = win_units(w, p.sink_tiles * p.chunks + p.key_tiles - p.sink_tiles);
+  window_bwd_kv_kernel<kD><<<p.n.units < 148 ? p.n.units : 148, kv_threads(kD), L::kSmemKV, s>>>(p);
   if (const int rc = check_launch("window_bwd_kv")) return rc;
   if (p.sink_tiles == 0 || p.chunks < 2) return TS_OK;
   window_bwd_join_kernel<kD><<<dim3(w.batch * w.kv_heads * p.sink_tiles, kD / 8 * 2), 128, 0, s>>>(p);

@@ -51,9 +51,8 @@ struct WinFwdLayout {
 struct WinFwdParams {
   CUtensorMap q, k, v, k_sink, v_sink, y;
   WinSizes w;
-  int each, pairs, units;   // query tiles of a unit (1 or 2), units of a key head, units
-  Divisor by_pairs;
-  bool ordered;
+  int each;              // query tiles of a unit: 1 or 2
+  WinUnits n;
   int sink_rows;         // rows of a sink box
   float* lse;            // or null
 };
@@ -84,7 +83,7 @@ struct WinFwdUnit {
   __device__ __forceinline__ WinFwdUnit(const WinFwdParams& p, const WinOrder& order, int unit) {
     const WinSizes& w = p.w;
     int pair;
-    win_place(order, p.ordered, w, p.by_pairs, unit, b, kv_head, pair);
+    win_place<false>(order, p.n, w, unit, b, kv_head, pair);
     length = win_length(w, b);
     a = place(w, p.each * pair);
     z = place(w, p.each == 2 ? 2 * pair + 1 : w.q_tiles * w.share);   // or none
@@ -175,7 +174,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) window_fwd_kernel(const __grid
     fence_mbar_init();
   }
   if (warp == 18) tmem_alloc(&tmem_slot, 512);
-  if (warp == 1 && p.ordered)
+  if (warp == 1 && p.n.how == kWinTable)
     win_order(order, w, [&](int b) {
       return (((max(0, win_length(w, b) - w.past) + 127) >> 7) * w.share + p.each - 1) / p.each;
     });
@@ -206,7 +205,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) window_fwd_kernel(const __grid
         }
         ++it;
       };
-      for (int unit = blockIdx.x; unit < p.units && ok; unit += gridDim.x) {
+      for (int unit = blockIdx.x; unit < p.n.units && ok; unit += gridDim.x) {
         const WinFwdUnit u(p, order, unit);
         auto queries = [&](int x) {
           if (!u.of(x).live || !(ok = ok && mbar_wait_warp(&q_empty[x], (q_turn[x]++ & 1) ^ 1, kErrMmaTimeout))) return;
@@ -250,7 +249,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) window_fwd_kernel(const __grid
       uint32_t k_slot = 0, k_parity = 0, v_slot = 1, v_parity = 0;
       uint32_t q_parity[2] = {0, 0}, p_parity[2] = {0, 0};
       bool ok = true;
-      for (int unit = blockIdx.x; unit < p.units && ok; unit += gridDim.x) {
+      for (int unit = blockIdx.x; unit < p.n.units && ok; unit += gridDim.x) {
         const WinFwdUnit u(p, order, unit);
         // tile x takes part in the first tokens' (n < sink_tiles) and from `low` to `last`
         const int low[2] = {0, u.sink_tiles + u.z.low - u.first}, last[2] = {u.a.live ? u.a.last : -1, u.z.live ? u.z.last : -1};
@@ -346,7 +345,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) window_fwd_kernel(const __grid
       uint32_t k_slot = 0, k_parity = 0, v_slot = 1, v_parity = 0;
       uint32_t q_parity = 0, s_parity = 1, p_parity = 0;
       bool ok = true;
-      for (int unit = blockIdx.x; unit < p.units && ok; unit += gridDim.x) {
+      for (int unit = blockIdx.x; unit < p.n.units && ok; unit += gridDim.x) {
         const WinFwdUnit u(p, order, unit);
         const WinFwdTile mine = u.of(x);
         // this tile takes part in the first tokens' (n < sink_tiles) and from `low` to `last`
@@ -447,10 +446,10 @@ __global__ void __launch_bounds__(kFwdThreads, 1) window_fwd_kernel(const __grid
       return ld_shared_f32(partner + 128 * slot + 4 * lane);
     };
     WinFwdUnit next(p, order, blockIdx.x);
-    for (int unit = blockIdx.x; unit < p.units; unit += gridDim.x) {
+    for (int unit = blockIdx.x; unit < p.n.units; unit += gridDim.x) {
       const WinFwdUnit u = next;
       const WinFwdTile mine = u.of(x);
-      if (unit + gridDim.x < p.units) next = WinFwdUnit(p, order, unit + gridDim.x);
+      if (unit + gridDim.x < p.n.units) next = WinFwdUnit(p, order, unit + gridDim.x);
       if (!mine.exists) continue;
       if (lane == 0) tma_store_read_wait<0>();   // the last store has read the stage, which carries exchanges now
       __syncwarp();
@@ -595,7 +594,7 @@ int window_fwd_launch(const WinFwdParams& p, cudaStream_t s) {
   constexpr int smem = WinFwdLayout<kD>::kSmem;
   const cudaError_t set = cudaFuncSetAttribute(window_fwd_kernel<kD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (set != cudaSuccess) return set_error(TS_ERR_CUDA, "window_fwd: %s", cudaGetErrorString(set));
-  window_fwd_kernel<kD><<<p.units < 148 ? p.units : 148, kFwdThreads, smem, s>>>(p);
+  window_fwd_kernel<kD><<<p.n.units < 148 ? p.n.units : 148, kFwdThreads, smem, s>>>(p);
   return check_launch("window_fwd");
 }
 
@@ -667,12 +666,9 @@ int ts_b200_window_fwd(const ts_window_args* a, ts_stream_t stream) {
   const WinSizes& w = p.w;
   // two tiles to a CTA, which then seldom waits; one where all of them find an SM of their own (2 x 8 heads, 1000 queries:
   // 27 us, 34 in pairs)
-  const int tiles = w.q_tiles * w.share, rows = w.batch * w.kv_heads;
-  p.each = static_cast<long long>(rows) * tiles <= 148 ? 1 : 2;
-  p.pairs = (tiles + p.each - 1) / p.each;
-  p.by_pairs = Divisor::of(p.pairs);
-  p.units = rows * p.pairs;
-  p.ordered = w.lengths && w.batch <= WinOrder::kMost && p.pairs <= 0xffff;
+  const int tiles = w.q_tiles * w.share;
+  p.each = static_cast<long long>(w.batch) * w.kv_heads * tiles <= 148 ? 1 : 2;
+  p.n = win_units(w, (tiles + p.each - 1) / p.each);
   p.sink_rows = w.sinks >= 128 ? 128 : round_up(w.sinks > 0 ? w.sinks : 1, 16);
   p.lse = a->lse;
   const bool ok = win_map(&p.q, a->q, a->q_strides, w.batch, w.heads, w.q_tokens, w.dim, 128) &&

@@ -19,7 +19,7 @@
 //
 // Forming p and ds bounds it where tiles are narrow, the products and the turns
 // between the two where they are wide: 64 x 8 heads x 1024, width 64, window 256,
-// sinks 4: 197 us for dq, 310 for dk and dv, 44 % of the issue slots; 16 heads x
+// sinks 4: 185 us for dq, 220 for dk and dv, 44 % of the issue slots; 16 heads x
 // 16384, width 128, window 2048, sinks 16: 465 and 560 us, tensor cores at work for
 // 43 and 56 % of them.
 #include "capi_internal.h"
@@ -493,8 +493,8 @@ struct WinKeyUnit {
   }
 };
 
-// Threads that share a row.  (Four at width 64, where tiles are short work: 64 x 8 heads x 1024, window 256 take 310 us so
-// and 337 with two; two at width 128: 16 heads x 16384, window 2048 582 us with four.)
+// Threads that share a row.  (Four at width 64, where tiles are short work: 64 x 8 heads x 1024, window 256 took 310 us so
+// and 337 with two, one key head after another; two at width 128: 16 heads x 16384, window 2048 582 us with four.)
 constexpr int kv_parts(int d) { return d == 64 ? 4 : 2; }
 constexpr int kv_row_warps(int d) { return 4 * kv_parts(d); }
 constexpr int kv_threads(int d) { return 32 * (kv_row_warps(d) + 4); }

@@ -13,7 +13,7 @@
 // lies.  While one group forms its P the tensor cores work for the other: forming
 // P and issuing instructions bound it, not the products (16 heads x 16384, width
 // 128, window 2048, sinks 16: 276 us, 1.0 PFLOP/s of whole tiles; 64 x 8 heads x
-// 1024, width 64, window 256, sinks 4: 122 us, 1.2 TB/s).
+// 1024, width 64, window 256, sinks 4: 115 us, 1.2 TB/s).
 //
 // A row's reference moves only when a score exceeds it by 2^8 (P is then at most
 // 256, and bf16 keeps its relative error): O is seldom rescaled, and the row's own

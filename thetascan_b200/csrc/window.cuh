@@ -61,7 +61,7 @@ struct WinUnits {
 };
 
 // For a padded batch, in shared memory.  Of each key head of sequence b the units 0 .. live(b) - 1 have work: they come by
-// falling index, those of all sequences that have one together, and what has no work at the end.
+// falling index (or rising: backwards), those of all sequences that have one together, and what has no work at the end.
 struct WinOrder {
   static constexpr int kMost = 64;   // sequences; more are taken one after another
   int begin[kMost + 1];              // first unit of those that the sequences 0 .. j, by falling length, have together
@@ -132,8 +132,10 @@ __device__ __forceinline__ void win_place(const WinOrder& o, const WinUnits& n, 
     kv_head = row - b * w.kv_heads;
     return;
   }
-  int j = 0, rest = unit - o.begin[WinOrder::kMost];
+  const int working = o.begin[WinOrder::kMost];
+  int j = 0, rest = unit - working;
   if (rest < 0) {
+    if (kRising) unit = working - 1 - unit;
 #pragma unroll
     for (int s = WinOrder::kMost / 2; s > 0; s >>= 1) j += o.begin[j + s] <= unit ? s : 0;
     rest = unit - o.begin[j];

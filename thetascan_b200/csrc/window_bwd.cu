@@ -12,8 +12,12 @@
 // no f32 copy of dq.  The keys of first tokens meet all queries: their tiles are
 // split among CTAs, whose sums go to a workspace in f32 and are joined in order.
 //
-// In both, four threads share a row of the tile, with a quarter of the columns
-// each; p and ds go back to tensor memory in bf16 and are the operand of the next
+// delta is formed of y as the forward stored it, in bf16: with the rounding of ds
+// and the result's own a gradient is off by 2.6e-3 of its norm (1.7e-3 is its own
+// rounding's), and no second copy of y is kept.
+//
+// Two or four threads share a row of a tile, with a part of the columns each; p
+// and ds go back to tensor memory in bf16 and are the operand of the next
 // product from there.  S^T = K Q^T and dP^T = V dY^T have
 // keys in the rows, which is how dv and dk need them.
 //

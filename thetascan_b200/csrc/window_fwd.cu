@@ -438,11 +438,14 @@ __global__ void __launch_bounds__(kFwdThreads, 1) window_fwd_kernel(const __grid
       __syncwarp();
       if (lane == 0) mbar_arrive(bar);
     };
-    // the value of the other thread of the row, by two places in turn
+    // the two warps of these rows
+    auto pair_meets = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + 4 * x + quad) : "memory"); };
+    // the value of the other thread of the row, by two places in turn: one is written again once both warps have met
+    // over the other, and so have read this one
     auto exchange = [&](float v) {
       const uint32_t slot = exchanges++ & 1;
       st_shared_f32(stage + 128 * slot + 4 * lane, v);
-      asm volatile("bar.sync %0, 64;" ::"r"(1 + 4 * x + quad) : "memory");
+      pair_meets();
       return ld_shared_f32(partner + 128 * slot + 4 * lane);
     };
     WinFwdUnit next(p, order, blockIdx.x);
@@ -541,6 +544,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) window_fwd_kernel(const __grid
         signal(&p_full[x]);
       }
       sum += exchange(sum);
+      pair_meets();   // both have read the other's: the stage takes the results
       ok = ok && (!mine.live || mbar_wait(&o_full[x], o_turn++ & 1, kErrMmaTimeout));
       if (!ok) break;
       tc_fence_after();

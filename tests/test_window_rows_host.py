@@ -3,7 +3,8 @@ order that their steps can come in, without a GPU.
 
 The steps are taken from the source, in its order: each warp puts a value into its stage, meets the other at a barrier and
 reads the other's stage (``exchange``); at a unit's end it writes its results over its stage.  A value that is written
-over before the other warp has read it is a race."""
+over before the other warp has read it is a race.  A wait for the copies or the tensor cores gives up after a while, in
+either warp; a warp that meets one that has left waits for ever."""
 from __future__ import annotations
 
 import os
@@ -12,11 +13,14 @@ import re
 import pytest
 
 SOURCE = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "thetascan_b200", "csrc", "window_fwd.cu")
-# what each step is made of; "meet" is the barrier of the two warps
+# what each step is made of; "meet" is the barrier of the two warps, "agree" one at which either can say that both leave
 STEPS = {
-    "exchange": ("put", "meet", "read"),
-    "pair_meets": ("meet",),
-    "store": ("over",),
+    r"\bexchange\(": ("put", "meet", "read"),
+    r"\bpair_meets\(": ("meet",),
+    r"\bthreads_agree<64>\(": ("agree",),
+    r"\bmbar_wait(?:_warp)?\(": ("wait",),
+    r"\bif \(!ok\) break": ("leave",),
+    r"\bst_shared_v4\(stage": ("over",),
 }
 
 
@@ -26,11 +30,11 @@ def _steps():
         text = f.read()
     text = re.sub(r"//.*", "", text[text.index("// ---- rows: two threads"):])
     text = text[text.index("for (int unit = blockIdx.x"):text.index("window_fwd_launch(")]
-    found = [(m.start(), m.group()) for m in re.finditer(r"\bexchange\(|\bpair_meets\(|\bst_shared_v4\(stage", text)]
-    names = ["store" if n.startswith("st_") else n[:-1] for _, n in found]
-    assert names.count("exchange") == 2 and names.count("store") == 1
-    tile = names.index("exchange") + 1
-    return names[:tile], names[tile:]
+    found = sorted((m.start(), name) for name in STEPS for m in re.finditer(name, text))
+    names = [name for _, name in found]
+    last_of_tile = text.index("signal(&p_full[x])")
+    assert names.count(r"\bexchange\(") == 2 and names.count(r"\bst_shared_v4\(stage") == 1
+    return [n for at, n in found if at < last_of_tile], [n for at, n in found if at > last_of_tile]
 
 
 def _program(tiles, units=2):
@@ -40,45 +44,73 @@ def _program(tiles, units=2):
     for _ in range(units):
         for name in tile * tiles + end:
             out += [(what, turn & 1) for what in STEPS[name]]
-            turn += name == "exchange"
+            turn += name == r"\bexchange\("
     return out
 
 
-def _races(program):
-    """Whether some order of the two warps' steps writes over a value that the other has still to read."""
-    seen, todo = set(), [((0, 0), (frozenset(), frozenset()))]   # next steps; places that hold a value not yet read
+def _faults(program):
+    """What some order of the two warps' steps, with waits that give up in either, leads to: "race" where one writes over a
+    value that the other has still to read, "hang" where one meets the other after that has left."""
+    faults, seen, end = set(), set(), len(program)
+    # next steps; places that hold a value not yet read; whether no wait has given up
+    todo = [((0, 0), (frozenset(), frozenset()), (True, True))]
     while todo:
         state = todo.pop()
         if state in seen:
             continue
         seen.add(state)
-        at, held = state
-        what = [program[i][0] if i < len(program) else None for i in at]
-        if what[0] == what[1] == "meet":
-            todo.append(((at[0] + 1, at[1] + 1), held))
+        at, held, ok = state
+        what = [program[i][0] if i < end else None for i in at]
+        meets = [x in ("meet", "agree") for x in what]
+        if all(meets):
+            assert what[0] == what[1] and at[0] == at[1]
+            both = at[0] + 1 if what[0] == "meet" or all(ok) else end
+            todo.append(((both, both), held, ok))
+        elif any(meets) and what[meets.index(False)] is None:
+            faults.add("hang")
         for w in range(2):
-            if what[w] in (None, "meet"):
+            if what[w] is None or meets[w]:
                 continue
+
+            def go(step=at[w] + 1, now=held, fine=ok[w]):
+                todo.append((tuple(step if n == w else i for n, i in enumerate(at)), tuple(now),
+                             tuple(fine if n == w else o for n, o in enumerate(ok))))
+
             place, now = program[at[w]][1], list(held)
-            if what[w] == "put":
+            if what[w] == "wait":
+                go()
+                go(fine=False)
+            elif what[w] == "leave":
+                go(step=at[w] + 1 if ok[w] else end)
+            elif what[w] == "put":
                 if place in held[w]:
-                    return True
+                    faults.add("race")
                 now[w] = held[w] | {place}
+                go(now=now)
             elif what[w] == "read":
                 now[1 - w] = held[1 - w] - {place}
-            elif held[w]:
-                return True
-            todo.append((tuple(i + (n == w) for n, i in enumerate(at)), tuple(now)))
-    return False
+                go(now=now)
+            else:
+                if held[w]:
+                    faults.add("race")
+                go()
+    return faults
 
 
-@pytest.mark.parametrize("tiles", [0, 1, 2, 5])   # none: a tile behind its sequence
+@pytest.mark.parametrize("tiles", [0, 1, 2, 4])   # none: a tile behind its sequence
 def test_nothing_is_written_over_before_it_is_read(tiles):
-    assert not _races(_program(tiles))
+    assert "race" not in _faults(_program(tiles))
 
 
-def test_a_missing_barrier_is_found():
-    assert _races([("put", 0), ("meet", 0), ("read", 0), ("over", 0)])
-    assert _races([("put", 0), ("meet", 0), ("read", 0), ("put", 0)])
-    assert not _races([("put", 0), ("meet", 0), ("read", 0), ("meet", 0), ("over", 0)])
-    assert not _races([("put", 0), ("meet", 0), ("read", 0), ("put", 1), ("meet", 1), ("read", 1), ("put", 0)])
+@pytest.mark.parametrize("tiles", [0, 1, 2, 4])
+def test_a_wait_that_gives_up_ends_both(tiles):
+    assert "hang" not in _faults(_program(tiles))
+
+
+def test_faults_are_found():
+    unread = [("put", 0), ("meet", 0), ("read", 0)]
+    assert _faults(unread + [("over", 0)]) == {"race"} and _faults(unread + [("put", 0)]) == {"race"}
+    assert not _faults(unread + [("meet", 0), ("over", 0)])
+    assert not _faults(unread + [("put", 1), ("meet", 1), ("read", 1), ("put", 0)])
+    assert _faults([("wait", 0), ("leave", 0), ("meet", 0)]) == {"hang"}
+    assert not _faults([("wait", 0), ("agree", 0), ("meet", 0)])

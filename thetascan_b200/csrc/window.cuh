@@ -213,6 +213,21 @@ __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, i
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, code));
 }
 
+// Whether `ok` holds in all of the kThreads threads that meet at the barrier `id`.
+template <int kThreads>
+__device__ __forceinline__ bool threads_agree(int id, bool ok) {
+  uint32_t all;
+  asm volatile(
+      "{\n\t.reg .pred p, r;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.and.pred r, %2, %3, p;\n\t"
+      "selp.u32 %0, 1, 0, r;\n\t}"
+      : "=r"(all)
+      : "r"(static_cast<uint32_t>(ok)), "r"(id), "n"(kThreads)
+      : "memory");
+  return all != 0;
+}
+
 // Zeros in the rows of a tile from `from` on, by the warp that issues the products, before the ones in which they would meet
 // weights of zero: what lies behind a sequence may be anything, and zero times infinity or NaN is not zero.
 template <int kBoxes>

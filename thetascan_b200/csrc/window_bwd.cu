@@ -134,20 +134,6 @@ __device__ __forceinline__ void score_gradients(const uint32_t (&p)[32], const u
   }
 }
 
-// Whether `ok` holds in all of the 512 row threads (a barrier among them).
-__device__ __forceinline__ bool rows_all(bool ok) {
-  uint32_t all;
-  asm volatile(
-      "{\n\t.reg .pred p, r;\n\t"
-      "setp.ne.u32 p, %1, 0;\n\t"
-      "barrier.cta.red.and.pred r, 1, 512, p;\n\t"
-      "selp.u32 %0, 1, 0, r;\n\t}"
-      : "=r"(all)
-      : "r"(static_cast<uint32_t>(ok))
-      : "memory");
-  return all != 0;
-}
-
 template <int kD>
 __global__ void __launch_bounds__(kBwdThreads, 1) window_bwd_q_kernel(const __grid_constant__ WinBwdParams p) {
   using L = WinBwdLayout<kD>;
@@ -394,7 +380,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) window_bwd_q_kernel(const __gr
       }
       // The row warps meet here, and only here: they go on, or give up, together.  (All have read the dq of the unit
       // before, which this one's first ds lets be overwritten.)
-      if (!rows_all(ok)) break;
+      if (!threads_agree<32 * kBwdRowWarps>(1, ok)) break;
       const float delta = halves[0][row] + halves[1][row];
       if (part == 0) p.delta[stat] = delta;
       __syncwarp();

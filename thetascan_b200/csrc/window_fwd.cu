@@ -544,9 +544,10 @@ __global__ void __launch_bounds__(kFwdThreads, 1) window_fwd_kernel(const __grid
         signal(&p_full[x]);
       }
       sum += exchange(sum);
-      pair_meets();   // both have read the other's: the stage takes the results
       ok = ok && (!mine.live || mbar_wait(&o_full[x], o_turn++ & 1, kErrMmaTimeout));
-      if (!ok) break;
+      // Both have read the other's sum: the stage takes the results.  They go on, or give up, together: the next unit's
+      // exchanges are waits for one another.
+      if (!threads_agree<64>(1 + 4 * x + quad, ok)) break;
       tc_fence_after();
       // a row that sees nothing has no sum: zero
       const float inverse = sum != 0.f ? 1.f / sum : 0.f;

@@ -12,7 +12,8 @@ import re
 
 import pytest
 
-SOURCE = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "thetascan_b200", "csrc", "window_fwd.cu")
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "thetascan_b200", "csrc")
+SOURCE = os.path.join(CSRC, "window_fwd.cu")
 # what each step is made of; "meet" is the barrier of the two warps, "agree" one at which either can say that both leave
 STEPS = {
     r"\bexchange\(": ("put", "meet", "read"),
@@ -105,6 +106,22 @@ def test_nothing_is_written_over_before_it_is_read(tiles):
 @pytest.mark.parametrize("tiles", [0, 1, 2, 4])
 def test_a_wait_that_gives_up_ends_both(tiles):
     assert "hang" not in _faults(_program(tiles))
+
+
+@pytest.mark.parametrize("name,kernels", [("window_fwd.cu", 1), ("window_bwd.cu", 2)])
+def test_the_lanes_of_a_warp_leave_together(name, kernels):
+    """Each lane has its own outcome of a wait; those that stayed behind would wait for the others at the next instruction
+    of the whole warp.  What ends or skips a turn of the row warps' loops is the same in all lanes."""
+    with open(os.path.join(CSRC, name)) as f:
+        text = re.sub(r"//.*", lambda m: m.group() if "---- rows" in m.group() else "", f.read())
+    rows = re.findall(r"// ---- rows:.*?tmem_dealloc", text, re.S)
+    assert len(rows) == kernels
+    alike = ("!threads_agree<", "!__all_sync(", "!mine.exists)", "!some[c])", "channel >= w.dim)")
+    for part in rows:
+        for condition in re.findall(r"if \((.*)(?:break|continue);", part):
+            assert condition.startswith(alike), condition
+        for condition in re.findall(r"for \(int n = 0;([^;]*);", part):
+            assert "ok" not in condition
 
 
 def test_faults_are_found():

@@ -389,14 +389,15 @@ __global__ void __launch_bounds__(kBwdThreads, 1) window_bwd_q_kernel(const __gr
         mbar_arrive(&q_empty);
       }
       const int near = max(at - w.window + 1, u.sinks), upto = at < u.length ? at : -1;   // visible: first ones, near..upto
-      for (int n = 0; n < u.count && ok; ++n, ++it) {
+      // (a wait that has given up does not end this: lanes leave together, at the barrier above)
+      for (int n = 0; n < u.count; ++n, ++it) {
         const int key = u.key(w, n) + 32 * part;
         const bool sink = n < u.sink_tiles;
         const int from = sink ? 0 : near - key, until = min(upto, sink ? u.sinks - 1 : upto) - key;
         // whether all, or any, of the warp's rows see all, or any, of its columns
         const bool all = __all_sync(0xffffffffu, from <= 0 && until >= 31);
         const bool some = all || __any_sync(0xffffffffu, from <= 31 && until >= 0 && from <= until);
-        if (!(ok = mbar_wait(&s_full, it & 1, kErrMmaTimeout))) break;
+        ok = ok && mbar_wait(&s_full, it & 1, kErrMmaTimeout);
         tc_fence_after();
         uint32_t s[32], d[32], out[16];
         tmem_ld(s_at, s);
@@ -413,7 +414,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) window_bwd_q_kernel(const __gr
             s[e + 1] = __float_as_uint(b);
           }
         }
-        if (!(ok = mbar_wait(&dp_full, it & 1, kErrMmaTimeout) && mbar_wait(&ds_free, (it & 1) ^ 1, kErrMmaTimeout))) break;
+        ok = ok && mbar_wait(&dp_full, it & 1, kErrMmaTimeout) && mbar_wait(&ds_free, (it & 1) ^ 1, kErrMmaTimeout);
         tc_fence_after();
         tmem_ld(dp_at, d);
         tmem_wait();
@@ -428,14 +429,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1) window_bwd_q_kernel(const __gr
         tmem_store_wait();
         signal(&ds_full);
       }
-      if (!(ok = ok && mbar_wait(&dq_full, dq_turn++ & 1, kErrMmaTimeout))) continue;
+      ok = ok && mbar_wait(&dq_full, dq_turn++ & 1, kErrMmaTimeout);
       tc_fence_after();
       if (32 * part < w.dim) {
         uint32_t r[32];
         tmem_ld(kDq + lanes + 32 * part, r);
         tmem_wait();
         tie(r);
-        if (q_row < w.q_tokens) store_row(to, r, w.scale, 32 * part, w.dim);
+        if (ok && q_row < w.q_tokens) store_row(to, r, w.scale, 32 * part, w.dim);
       }
       tc_fence_before();
     }
@@ -663,13 +664,14 @@ __global__ void __launch_bounds__(kv_threads(kD), 1) window_bwd_kv_kernel(const 
       const bool is_key = key < u.length, everywhere = key < w.sinks;
       const int last = is_key ? (everywhere ? u.length - 1 : min(u.length - 1, key + w.window - 1)) : -1;
       int tile = u.first;
-      for (int n = 0; n < u.count && ok; ++n, ++it) {
+      // (a wait that has given up does not end this: the lanes of a warp leave together, below)
+      for (int n = 0; n < u.count; ++n, ++it) {
         // the columns (queries) that see this row's key
         const int first = w.past + 128 * tile + kCols * part, from = key - first, until = last - first;
         tile = tile + 1 == u.first + u.tiles ? u.first : tile + 1;
         const bool all = __all_sync(0xffffffffu, from <= 0 && until >= kCols - 1);
         const bool some = all || __any_sync(0xffffffffu, from <= kCols - 1 && until >= 0 && from <= until);
-        if (!(ok = mbar_wait(&full[slot], parity, kErrCopyTimeout) && mbar_wait(&s_full, it & 1, kErrMmaTimeout))) break;
+        ok = ok && mbar_wait(&full[slot], parity, kErrCopyTimeout) && mbar_wait(&s_full, it & 1, kErrMmaTimeout);
         tc_fence_after();
         const uint32_t lse = stats + 1024 * slot + 4 * kCols * part, delta = lse + 512;
         slot = slot + 1 == kSlots ? 0 : slot + 1;
@@ -706,7 +708,7 @@ __global__ void __launch_bounds__(kv_threads(kD), 1) window_bwd_kv_kernel(const 
           tmem_st(s_at + 16 * c, out);
         }
         signal(&p_full);
-        if (!(ok = mbar_wait(&dp_full, it & 1, kErrMmaTimeout))) break;
+        ok = ok && mbar_wait(&dp_full, it & 1, kErrMmaTimeout);
         tc_fence_after();
 #pragma unroll
         for (int c = 0; c < kCols / 32; ++c) {
@@ -731,7 +733,8 @@ __global__ void __launch_bounds__(kv_threads(kD), 1) window_bwd_kv_kernel(const 
         }
         signal(&ds_full);
       }
-      if (!ok || (u.count > 0 && !(ok = mbar_wait(&done, turn++ & 1, kErrMmaTimeout)))) break;
+      ok = ok && (u.count == 0 || mbar_wait(&done, turn++ & 1, kErrMmaTimeout));
+      if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
       // even parts: dv, odd ones: dk; with four, half of the channels each
       constexpr int kChannels = 2 * kD / kParts;

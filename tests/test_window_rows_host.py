@@ -1,5 +1,6 @@
-"""The two warps that share the rows of a query tile in the windowed attention's forward (csrc/window_fwd.cu), in every
-order that their steps can come in, without a GPU.
+"""What the warps of the windowed attention wait for (csrc/window_fwd.cu, window_bwd.cu), without a GPU: the two warps that
+share the rows of a query tile in the forward, in every order that their steps can come in, and what each kind of warp
+does when a wait gives up.
 
 The steps are taken from the source, in its order: each warp puts a value into its stage, meets the other at a barrier and
 reads the other's stage (``exchange``); at a unit's end it writes its results over its stage.  A value that is written
@@ -122,6 +123,17 @@ def test_the_lanes_of_a_warp_leave_together(name, kernels):
             assert condition.startswith(alike), condition
         for condition in re.findall(r"for \(int n = 0;([^;]*);", part):
             assert "ok" not in condition
+
+
+@pytest.mark.parametrize("name,kernels", [("window_fwd.cu", 1), ("window_bwd.cu", 2)])
+def test_copies_in_flight_land_before_the_memory_goes(name, kernels):
+    """A warp of loads that gives up waits, for a bounded time, on every barrier that a copy of its own may still complete."""
+    with open(os.path.join(CSRC, name)) as f:
+        parts = re.findall(r"// ---- loads(.*?)(// given up.*?)\} else if", f.read(), re.S)
+    assert len(parts) == kernels
+    for loads, given_up in parts:
+        started = set(re.findall(r"&(\w*full)\b", loads))
+        assert started and started == set(re.findall(r"&(\w*full)\b", given_up))
 
 
 def test_faults_are_found():

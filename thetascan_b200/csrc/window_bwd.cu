@@ -572,6 +572,8 @@ __global__ void __launch_bounds__(kv_threads(kD), 1) window_bwd_kv_kernel(const 
         for (uint32_t i = it > kSlots ? it - kSlots : 0; i < it; ++i)
           for (int poll = 0; poll < (1 << 16) && !mbar_try_wait(&full[i % kSlots], (i / kSlots) & 1); ++poll) {
           }
+        for (int poll = 0; poll < (1 << 16) && turn > 0 && !mbar_try_wait(&kv_full, (turn - 1) & 1); ++poll) {
+        }
       }
     } else if (warp == kRowWarps + 1) {
       // ---- instructions: while the rows form ds of this query tile, dv and the next S; while they form the next p, dk

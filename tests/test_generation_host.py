@@ -154,3 +154,27 @@ def test_definition_agrees_with_differences():
         at = [[t + (s * step if n == i else 0) for n, t in enumerate((q, k, v))] for s in (1, -1)]
         up, down = (float((attention(*a, 2, 1, 0.3, lengths, dy)[0] * dy).sum()) for a in at)
         assert abs((up - down) / 2 - float((grad * step).sum())) <= 1e-8 * float(step.norm() * grad.norm())
+
+
+def _generating(monkeypatch, chosen):
+    """A model whose work and choice are replaced; what reaches each of the two."""
+    from thetascan_b200 import lm
+    model = lm.HybridLM(vocab=16, d_model=64, n_layers=1, n_heads=1, mixer_layers=(), window=4)
+    fed, drawn = [], []
+    monkeypatch.setattr(model, "extend", lambda tokens, stream: (fed.append(tokens.clone()), torch.zeros(2, 16))[1])
+
+    def choose(logits, uniform, **settings):
+        drawn.append(uniform)
+        return chosen.clone()
+
+    monkeypatch.setattr(lm, "sample_tokens", choose)
+    return model, fed, drawn
+
+
+def test_a_row_without_a_token_goes_on(monkeypatch):
+    """A row of masked logits has no token: -1, which is no place in the embedding."""
+    model, fed, _ = _generating(monkeypatch, torch.tensor([-1, 5]))
+    got = model.generate(torch.tensor([[1, 2], [3, 4]]), 3)
+    assert got.tolist() == [[-1] * 3, [5] * 3]
+    model.generate(got[:, -1:], 1, stream=model.stream(2))   # as a caller goes on from there
+    assert [t.tolist() for t in fed] == [[[1, 2], [3, 4]], [[0], [5]], [[0], [5]], [[0], [5]]]

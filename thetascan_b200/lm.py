@@ -281,14 +281,16 @@ class HybridLM(nn.Module):
                  generator: torch.Generator | None = None, stream: "ModelStream | None" = None):
         """``count`` further tokens ``[B,count]`` of the sequences that ``tokens
         [B,T]`` begin (or, with a ``stream``, go on), drawn by
-        :func:`thetascan_b200.sample_tokens` with its settings."""
+        :func:`thetascan_b200.sample_tokens` with its settings.  A row of logits
+        that are all NaN or minus infinity gives -1, and that sequence goes on as
+        if it had been token 0, as it does for a -1 among the ``tokens``."""
         if count < 1:
             raise ValueError(f"generate: count must be >= 1, got {count}")
         stream = self.stream(tokens.shape[0]) if stream is None else stream
         uniform = torch.rand(count, tokens.shape[0], device=tokens.device, generator=generator)
         got = []
         for row in uniform:
-            logits = self.extend(tokens, stream)
+            logits = self.extend(tokens.clamp_min(0), stream)
             tokens = sample_tokens(logits, row, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)[:, None]
             got.append(tokens)
         return torch.cat(got, 1)

@@ -178,3 +178,14 @@ def test_a_row_without_a_token_goes_on(monkeypatch):
     assert got.tolist() == [[-1] * 3, [5] * 3]
     model.generate(got[:, -1:], 1, stream=model.stream(2))   # as a caller goes on from there
     assert [t.tolist() for t in fed] == [[[1, 2], [3, 4]], [[0], [5]], [[0], [5]], [[0], [5]]]
+
+
+def test_uniform_numbers_are_f32_whatever_the_default(monkeypatch):
+    model, _, drawn = _generating(monkeypatch, torch.tensor([1, 5]))
+    was = torch.get_default_dtype()
+    try:
+        torch.set_default_dtype(torch.float64)
+        model.generate(torch.tensor([[1, 2], [3, 4]]), 2)
+    finally:
+        torch.set_default_dtype(was)
+    assert [u.dtype for u in drawn] == [torch.float32] * 2   # what the choice takes

@@ -287,7 +287,7 @@ class HybridLM(nn.Module):
         if count < 1:
             raise ValueError(f"generate: count must be >= 1, got {count}")
         stream = self.stream(tokens.shape[0]) if stream is None else stream
-        uniform = torch.rand(count, tokens.shape[0], device=tokens.device, generator=generator)
+        uniform = torch.rand(count, tokens.shape[0], dtype=torch.float32, device=tokens.device, generator=generator)
         got = []
         for row in uniform:
             logits = self.extend(tokens.clamp_min(0), stream)

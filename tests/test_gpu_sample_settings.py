@@ -1,0 +1,27 @@
+"""Settings of the choice of tokens: every integer type of ``top_k``, refusals of compiled calls, masses at the precision
+that the choice states."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from test_gpu_sample import sample  # noqa: F401  (a fixture)
+
+gpu = pytest.mark.gpu
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.int8, torch.int16, torch.uint16, torch.int32, torch.uint32, torch.int64,
+                                   torch.uint64])
+def test_top_k_of_any_integer_type(sample, dtype):  # noqa: F811
+    g = torch.Generator("cuda").manual_seed(0)
+    logits, uniform = torch.randn(5, 400, generator=g, device="cuda"), torch.rand(5, generator=g, device="cuda")
+    wanted = [1, 2, 50, 127, 0]
+    want = torch.cat([sample(logits[i:i + 1], uniform[i:i + 1], top_k=k or None) for i, k in enumerate(wanted)])
+    assert torch.equal(sample(logits, uniform, top_k=torch.tensor(wanted).to(dtype).cuda()), want)
+    # more than there are tokens, or less than one: no filter
+    open_ = sample(logits, uniform)
+    for limit in (torch.iinfo(dtype).max, torch.iinfo(dtype).min):
+        if 1 <= limit < 400:
+            continue
+        assert torch.equal(sample(logits, uniform, top_k=torch.tensor([limit] * 5, dtype=dtype).cuda()), open_)

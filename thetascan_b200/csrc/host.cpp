@@ -823,8 +823,10 @@ struct Setting {
     TORCH_CHECK_VALUE(type == at::kInt ? at::isIntegralType(t->scalar_type(), false) : t->scalar_type() == type, name,
                       " must be a number or a tensor of ", type, ", got ", t->scalar_type());
     TORCH_CHECK_VALUE(t->numel() == count, name, " must have one value for each of the ", count, " rows, got ", t->sizes());
+    // 64-bit integers end at the ones that 32 bits hold; an unsigned one above them is negative then, and as little of a
+    // limit as it was
     rows = t->scalar_type() == type ? t->contiguous()
-                                    : t->clamp(INT_MIN, INT_MAX).to(type).contiguous();   // of 64-bit integers
+                                    : (t->element_size() > 4 ? t->to(at::kLong).clamp(INT_MIN, INT_MAX) : *t).to(type).contiguous();
   }
 };
 

@@ -25,3 +25,17 @@ def test_top_k_of_any_integer_type(sample, dtype):  # noqa: F811
         if 1 <= limit < 400:
             continue
         assert torch.equal(sample(logits, uniform, top_k=torch.tensor([limit] * 5, dtype=dtype).cuda()), open_)
+
+
+@gpu
+def test_compiled_calls_refuse_what_eager_ones_refuse(sample):  # noqa: F811
+    torch._dynamo.reset()
+    logits, uniform = torch.randn(3, 10, device="cuda"), torch.rand(3, device="cuda")
+    for settings in (dict(temperature=-0.5), dict(top_k=0), dict(top_k=-3), dict(top_p=0.0), dict(top_p=1.5), dict(min_p=-0.1), dict(min_p=1.1)):
+        compiled = torch.compile(lambda x, u, s=settings: sample(x, u, **s), fullgraph=True, backend="aot_eager")
+        for call in (lambda x, u: sample(x, u, **settings), compiled):
+            with pytest.raises(ValueError):
+                call(logits, uniform)
+    for settings in (dict(), dict(top_k=4), dict(top_k=10 ** 9), dict(top_k=torch.full((3,), 4, device="cuda"))):
+        compiled = torch.compile(lambda x, u, s=settings: sample(x, u, **s), fullgraph=True, backend="aot_eager")
+        assert torch.equal(compiled(logits, uniform), sample(logits, uniform, **settings))

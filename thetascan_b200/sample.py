@@ -18,11 +18,11 @@ LIB = "thetascan_b200"
 
 
 @torch.library.custom_op(f"{LIB}::sample", mutates_args=())
-def _sample(logits: Tensor, uniform: Tensor, temperature: float, temperatures: Optional[Tensor], top_k: int,
+def _sample(logits: Tensor, uniform: Tensor, temperature: float, temperatures: Optional[Tensor], top_k: Optional[int],
             top_ks: Optional[Tensor], top_p: float, top_ps: Optional[Tensor], min_p: float, min_ps: Optional[Tensor],
             logprobs: bool) -> tuple[Tensor, Tensor]:
     """Tokens and their log-probabilities (empty unless wanted); each setting as a number or a tensor."""
-    settings = (temperatures if temperatures is not None else temperature, top_ks if top_ks is not None else top_k or None,
+    settings = (temperatures if temperatures is not None else temperature, top_ks if top_ks is not None else top_k,
                 top_ps if top_ps is not None else top_p, min_ps if min_ps is not None else min_p)
     got = _lib.host().sample(logits, uniform, *settings, logprobs)
     return got if logprobs else (got, logits.new_empty(0, dtype=torch.float32))
@@ -67,6 +67,6 @@ def sample_tokens(logits: Tensor, uniform: Tensor, *, temperature: Union[float, 
     def split(value, off):
         return (off, value) if isinstance(value, Tensor) else (off if value is None else value, None)
 
-    tokens, logprobs = _sample(logits.detach(), uniform, *split(temperature, 1.0), *split(top_k, 0), *split(top_p, 1.0),
+    tokens, logprobs = _sample(logits.detach(), uniform, *split(temperature, 1.0), *split(top_k, None), *split(top_p, 1.0),
                                *split(min_p, 0.0), return_logprobs)
     return (tokens, logprobs) if return_logprobs else tokens

@@ -19,8 +19,9 @@
 //
 // What bounds it is the number of instructions: about 70 for each logit with
 // top-p.  The exponential is therefore in 64 bits, which run at half the rate of
-// 32 but need no compensation: the sum of a logit's product and 1.5 2^52 has the
-// rounded distance, which is the bin too, in its low word.  Only the pass that
+// 32 but need no compensation: the sum of 1.5 2^52 and the product of a logit's
+// difference from the largest has the rounded distance, which is the bin too, in
+// its low word.  Only the pass that
 // fills the histogram takes it of every logit: a cut's bin is found again by its
 // first and last logit, and kept tokens are brought side by side in shared memory
 // before their masses are summed (512 rows x 50257, top-p: 168 -> 139 us; 64 rows
@@ -92,7 +93,7 @@ struct SampleShared {
   float top;
   uint32_t listed, gathered, first;
   // for this CTA's threads
-  double scale, offset;                        // of the distance (see Row)
+  double scale;                                // of the distance (see Sampler)
   float lowest, floor_at;
   float edge[2];                               // a bin's logits: from the first on, below the second
   u64 before, before_b, rest;
@@ -154,7 +155,7 @@ struct Sampler {
   bool infinite;                               // the largest logit is infinite: its tokens are 0, and alone
   bool scaled;                                 // logits are taken times 2^-20: f32 has room below the ones with mass
   float lowest;                                // what lies below has no mass, and is this
-  double scale, offset;                        // distance in 32nds of a power of two: scale x + offset, 0 at the top
+  double scale, peak;                          // distance in 32nds of a power of two: scale (x - peak), 0 at the top
 
   __device__ __forceinline__ Sampler(const SampleParams& p_, SampleShared& m_, void* cache_)
       : p(p_), m(m_), cache(static_cast<Raw*>(cache_)) {
@@ -232,17 +233,17 @@ struct Sampler {
 
   // 32 log2 of a token's mass, rounded, times -1: its bin.
   __device__ __forceinline__ uint32_t bin(float x) const {
-    return static_cast<uint32_t>(-__double2loint(fma(static_cast<double>(x), scale, offset + 6755399441055744.)));
+    return static_cast<uint32_t>(-__double2loint(fma(x - peak, scale, 6755399441055744.)));
   }
   __device__ __forceinline__ u64 mass(float x, uint32_t& bin) const {
-    const double d = x, near = fma(d, scale, offset + 6755399441055744.);
+    const double d = x - peak, near = fma(d, scale, 6755399441055744.);
     const int i = __double2loint(near);
     bin = static_cast<uint32_t>(-i);
-    // 2^(i/32) 2^(r/32), |r| <= 1/2: the second by its series, within 2e-12
-    const double r = fma(d, scale, offset - (near - 6755399441055744.));
-    double e = fma(r, 9.172562701e-9, 1.693850975e-6);
-    e = fma(e, r, 2.345964913e-4);
-    e = fma(e, r, 2.166084939388e-2);
+    // 2^(i/32) 2^(r/32), |r| <= 1/2: the second by a polynomial fitted there, within 1e-13
+    const double r = fma(d, scale, 6755399441055744. - near);
+    double e = fma(r, 9.172621781784e-9, 1.693863388074e-6);
+    e = fma(e, r, 2.345961981964e-4);
+    e = fma(e, r, 2.166084939172e-2);
     e = fma(e, r, 1.);
     e *= m.power[i & (kSteps - 1)];
     // times 2^(i >> 5), and the integer out of a sum with 2^52
@@ -615,13 +616,12 @@ struct Sampler {
       // the next smaller logit is 4096 steps away at most: further is without mass too, and the low word holds it
       const double s = min(kSteps * 1.4426950408889634 / temperature, 4096. / (static_cast<double>(top) - below));
       m.scale = s;
-      m.offset = -(top * s);
       m.lowest = min(__double2float_rd(top - (kLastStep + kSteps) / s), below);
       m.floor_at = min_p > 0. ? __double2float_ru(top + temperature * log(min(min_p, 1.))) : -INFINITY;
     }
     __syncthreads();
     scale = m.scale;
-    offset = m.offset;
+    peak = top;
     lowest = m.lowest;
     const float floor_at = m.floor_at;
 

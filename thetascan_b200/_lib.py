@@ -401,6 +401,14 @@ def check(code: int) -> None:
     raise ThetaScanB200Error(message)
 
 
+def refuse_gradient(name: str, *tensors) -> None:
+    """For a call without a gradient that a compiler traces; the host side of
+    eager calls (``csrc/host.cpp``) looks for itself."""
+    import torch
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad()")
+
+
 def device_status(stream_handle: int) -> int:
     """Synchronize the stream and return (and clear) the device status word."""
     status = ctypes.c_int(0)

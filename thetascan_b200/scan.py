@@ -360,7 +360,8 @@ def linattn_views_step(q, k, v, retentions, state, *, append_unit: bool = False)
         return ()
     if torch.compiler.is_compiling():
         from . import ops  # noqa: F401  (registers the operators)
+        given = [r for r in retentions if r is not None]
+        _lib.refuse_gradient("linattn_views_step", q, k, v, state, *given)
         return torch.ops.thetascan_b200.scan_views_step(
-            q, k, v, [r for r in retentions if r is not None], [r is not None for r in retentions], bool(append_unit),
-            state).unbind(0)
+            q, k, v, given, [r is not None for r in retentions], bool(append_unit), state).unbind(0)
     return _lib.host().scan_step(q, k, v, retentions, append_unit, state, True)

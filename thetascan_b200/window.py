@@ -142,6 +142,7 @@ def window_attention_step(q: Tensor, k: Tensor, v: Tensor, keys: Tensor, values:
     negative one marks a row without a sequence, for which nothing is written and
     the output is zero.  For inference: no gradient."""
     if torch.compiler.is_compiling():
+        _lib.refuse_gradient("window_attention_step", q, k, v, keys, values)
         return window_step(q, k, v, keys, values, lengths, sinks, _scale(scale, q))
     return _lib.host().window_step(q, k, v, keys, values, lengths, sinks, scale)
 
@@ -154,6 +155,7 @@ def window_cache_extend(k: Tensor, v: Tensor, keys: Tensor, values: Tensor, leng
     ``lengths`` is not changed; slots that no new token falls into are left as
     they were, and so is the whole row of a negative length."""
     if torch.compiler.is_compiling():
+        _lib.refuse_gradient("window_cache_extend", k, v, keys, values)
         return window_extend(k, v, keys, values, lengths, sinks, new)
     return _lib.host().window_extend(k, v, keys, values, lengths, sinks, new)
 

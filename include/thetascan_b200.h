@@ -681,7 +681,7 @@ typedef struct ts_window_args {
   void* y;
   long long y_strides[3];
   float* lse;               /* [batch, heads, q_tokens rounded up to 128]: written by the forward (NULL in inference),
-                             * read by the backward */
+                             * read by the backward, which wants it 16-byte aligned */
 } ts_window_args;
 
 typedef struct ts_window_grad_args {

@@ -189,3 +189,18 @@ def test_uniform_numbers_are_f32_whatever_the_default(monkeypatch):
     finally:
         torch.set_default_dtype(was)
     assert [u.dtype for u in drawn] == [torch.float32] * 2   # what the choice takes
+
+
+@pytest.mark.parametrize("over,said", [(dict(lse=THERE + 4), "lse"), (dict(workspace=THERE + 8), "workspace")])
+def test_window_backward_refuses_what_its_copies_cannot_read(over, said):
+    """Both are read by copies of 16-byte pieces, which end the context at another address."""
+    lib = _lib.load()
+    a, g = _window(lse=THERE), _lib.WindowGradArgs()
+    g.dy = g.dq = g.dk = g.dv = g.workspace = THERE
+    for n in ("dy", "dq", "dk", "dv"):
+        setattr(g, f"{n}_strides", _lib.c_longlong_3(1024, 64, 128))
+    g.workspace_bytes = lib.ts_b200_window_bwd_workspace_bytes(ctypes.byref(a))
+    for n, x in over.items():
+        setattr(a if hasattr(a, n) else g, n, x)
+    assert lib.ts_b200_window_bwd(ctypes.byref(a), ctypes.byref(g), None) == BAD
+    assert said in _lib.last_error()[1] and "16-byte" in _lib.last_error()[1]

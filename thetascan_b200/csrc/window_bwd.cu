@@ -857,6 +857,9 @@ int ts_b200_window_bwd(const ts_window_args* a, const ts_window_grad_args* g, ts
   const size_t stats = win_stats_bytes(w);
   if (!g->workspace || g->workspace_bytes < stats + win_partial_bytes(w, p))
     return set_error(TS_ERR_VALUE, "window_bwd: workspace too small");
+  // the kernel of dk and dv copies lse and delta in pieces of 16 bytes
+  if (reinterpret_cast<uintptr_t>(a->lse) % 16 || reinterpret_cast<uintptr_t>(g->workspace) % 16)
+    return set_error(TS_ERR_VALUE, "window_bwd: lse and workspace must be 16-byte aligned");
   if (static_cast<long long>(w.batch) * w.kv_heads * (static_cast<long long>(p.sink_tiles) * p.chunks + p.key_tiles) > 0x3fffffffll)
     return set_error(TS_ERR_NOT_IMPLEMENTED, "window_bwd: too many key tiles");
   p.sink_rows = w.sinks >= 128 ? 128 : round_up(w.sinks > 0 ? w.sinks : 1, 16);

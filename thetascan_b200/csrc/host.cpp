@@ -564,9 +564,10 @@ struct WindowCall {
 };
 
 // [batch, heads, tokens, dim] whose memory is [batch, tokens, heads, dim]: the heads of a token lie together, as the
-// projections around an attention have them.
+// projections around an attention have them.  No view: autograd lets the result of a function be changed in place only then.
 Tensor token_major(const Tensor& like) {
-  return at::empty({like.size(0), like.size(2), like.size(1), like.size(3)}, like.options()).transpose(1, 2);
+  const int64_t h = like.size(1), n = like.size(2), d = like.size(3);
+  return at::empty_strided(like.sizes(), {n * h * d, d, h * d, 1}, like.options());
 }
 
 std::pair<Tensor, Tensor> window_run(const Tensor& q, const Tensor& k, const Tensor& v, int64_t window, int64_t sinks,

@@ -97,3 +97,15 @@ def test_gn_state_dict_and_seeded_init_match_reference(name):
         if n not in GN_OVERWRITTEN:
             assert torch.equal(t.to(theirs[n].dtype), theirs[n]), n
     module.load_state_dict({"_core." + n: t.float() for n, t in theirs.items()})
+
+
+def test_rotary_rows_of_a_stream_do_not_grow_with_its_position():
+    from thetascan_b200 import mixer
+    whole = mixer._rope_tables(9000, 32, 10_000.0, "cpu")
+    for pos0, T in [(0, 1), (0, 70), (1, 1), (63, 2), (1023, 1), (1024, 1), (1000, 300), (4095, 3), (8191, 1), (8999, 1), (5000, 4000)]:
+        got = mixer._rope_rows(pos0, T, 32, 10_000.0, "cpu")
+        for a, b in zip(got, whole):
+            assert torch.equal(a, b[pos0:pos0 + T]), (pos0, T)
+    for pos0 in (3000, 1 << 17, 1 << 22):
+        for rows in mixer._rope_rows(pos0, 1, 32, 10_000.0, "cpu"):
+            assert rows.shape == (1, 16) and rows.untyped_storage().nbytes() <= 1024 * 16 * 4, pos0

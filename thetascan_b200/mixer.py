@@ -98,11 +98,20 @@ class _OutGate(nn.Module):
         self.g = _HeadLinear(d_model, n_heads, d, bias_init=1.0)
 
 
+def _rope_angles(start: int, T: int, rot: int, base: float, device: str):
+    inv = 1.0 / (base ** (torch.arange(0, rot, 2, dtype=torch.float32, device=device) / rot))
+    angles = torch.outer(torch.arange(start, start + T, dtype=torch.float32, device=device), inv)
+    return angles.cos(), angles.sin()
+
+
 @lru_cache(maxsize=32)
 def _rope_tables(T: int, rot: int, base: float, device: str):
-    inv = 1.0 / (base ** (torch.arange(0, rot, 2, dtype=torch.float32, device=device) / rot))
-    angles = torch.outer(torch.arange(T, dtype=torch.float32, device=device), inv)
-    return angles.cos(), angles.sin()
+    return _rope_angles(0, T, rot, base, device)
+
+
+@lru_cache(maxsize=8)
+def _rope_piece(start: int, T: int, rot: int, base: float, device: str):
+    return _rope_angles(start, T, rot, base, device)
 
 
 def _rope_width(d: int, mode: str, frac: float) -> int:
@@ -114,13 +123,20 @@ def _rope_width(d: int, mode: str, frac: float) -> int:
     return max_rot if mode == "full" else min(max_rot, max(2, int(d * frac) // 2 * 2))
 
 
+ROPE_BLOCK = 1024
+
+
 def _rope_rows(pos0: int, T: int, rot: int, base: float, device: str):
-    """Rows ``pos0 .. pos0 + T - 1`` of the tables; behind the start, of tables
-    whose length is a power of two, so that a stream's steps share them."""
+    """Rows ``pos0 .. pos0 + T - 1`` of the tables.  Behind the start only those,
+    or the block of 1024 positions that they lie in, so that a stream's steps
+    share them and hold no more as it goes on."""
     if pos0 == 0:
         return _rope_tables(T, rot, base, device)
-    cos, sin = _rope_tables(1 << (pos0 + T - 1).bit_length(), rot, base, device)
-    return cos[pos0:pos0 + T], sin[pos0:pos0 + T]
+    at = pos0 % ROPE_BLOCK
+    if at + T > ROPE_BLOCK:
+        return _rope_piece(pos0, T, rot, base, device)
+    cos, sin = _rope_piece(pos0 - at, ROPE_BLOCK, rot, base, device)
+    return cos[at:at + T], sin[at:at + T]
 
 
 def _rope(x: torch.Tensor, rot: int, base: float, pos0: int = 0) -> torch.Tensor:

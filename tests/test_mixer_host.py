@@ -109,3 +109,19 @@ def test_rotary_rows_of_a_stream_do_not_grow_with_its_position():
     for pos0 in (3000, 1 << 17, 1 << 22):
         for rows in mixer._rope_rows(pos0, 1, 32, 10_000.0, "cpu"):
             assert rows.shape == (1, 16) and rows.untyped_storage().nbytes() <= 1024 * 16 * 4, pos0
+
+
+@pytest.mark.parametrize("pos0", [0, 70])
+def test_rotary_rows_first_made_in_inference_mode_serve_training(pos0):
+    from thetascan_b200 import mixer
+    for cached in (mixer._rope_tables, mixer._rope_piece):
+        cached.cache_clear()
+    x = torch.randn(1, 2, 37, 16, generator=torch.Generator().manual_seed(0))
+    with torch.inference_mode():   # a model that answers between two steps of its training
+        want = mixer._rope(x, 16, 10_000.0, pos0).clone()
+    leaf = x.clone().requires_grad_(True)
+    y = mixer._rope(leaf, 16, 10_000.0, pos0)
+    assert torch.equal(y, want)
+    grad, = torch.autograd.grad((y * y).sum(), leaf)
+    # a rotation keeps lengths: each of its roundings is 2^-24 of a value
+    assert float((grad - 2 * x).abs().max()) <= 16 * 2.0 ** -24 * 2 * float(x.abs().max())

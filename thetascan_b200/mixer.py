@@ -98,6 +98,7 @@ class _OutGate(nn.Module):
         self.g = _HeadLinear(d_model, n_heads, d, bias_init=1.0)
 
 
+@torch.inference_mode(False)   # they are kept, and serve calls with gradients too
 def _rope_angles(start: int, T: int, rot: int, base: float, device: str):
     inv = 1.0 / (base ** (torch.arange(0, rot, 2, dtype=torch.float32, device=device) / rot))
     angles = torch.outer(torch.arange(start, start + T, dtype=torch.float32, device=device), inv)

@@ -204,3 +204,15 @@ def test_window_backward_refuses_what_its_copies_cannot_read(over, said):
         setattr(a if hasattr(a, n) else g, n, x)
     assert lib.ts_b200_window_bwd(ctypes.byref(a), ctypes.byref(g), None) == BAD
     assert said in _lib.last_error()[1] and "16-byte" in _lib.last_error()[1]
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_workspace_of_many_first_tokens_is_bounded(dim):
+    """Sums of first tokens' key tiles, [channels x 128] f32 of dk and dv for each chunk of queries: no more of them than
+    keep the SMs at work, whatever the sizes."""
+    lib = _lib.load()
+    for batch, kv_heads, tokens, sinks in [(1, 1, 1 << 20, 128), (1, 8, 16384, 4096), (64, 8, 16384, 4096), (4, 8, 1 << 20, 1 << 19), (512, 16, 4096, 1)]:
+        a = _window(batch=batch, heads=kv_heads, kv_heads=kv_heads, dim=dim, q_tokens=tokens, kv_tokens=tokens, window=100, sinks=sinks)
+        stats = batch * kv_heads * tokens * 4
+        got = lib.ts_b200_window_bwd_workspace_bytes(ctypes.byref(a))
+        assert stats <= got <= stats + 16 * 148 * 2 * dim * 128 * 4, (batch, kv_heads, tokens, sinks, got - stats)

@@ -84,3 +84,12 @@ def test_a_sequence_alone_and_in_a_batch(win):  # noqa: F811
     for b in range(5):
         s = slice(b, b + 1)
         assert all(torch.equal(a[s], one) for a, one in zip(together, step(s)))
+
+
+@gpu
+@pytest.mark.parametrize("batch,kv_heads,tokens,dim", [(20, 8, 1300, 64), (8, 8, 5000, 64), (8, 8, 5000, 128)])
+@pytest.mark.parametrize("ragged", [False, True])
+def test_first_tokens_in_fewer_chunks(win, batch, kv_heads, tokens, dim, ragged):  # noqa: F811
+    # 1280 and 512 key tiles of first tokens: their queries in one and in four chunks, in place of two and five
+    q, k, v, dy, lengths = _make(batch, kv_heads, kv_heads, tokens, 0, dim, ragged, seed=2)
+    _check(win, q, k, v, dy, 100, 1000, lengths)

@@ -806,6 +806,14 @@ void win_split(const WinSizes& w, WinBwdParams* p) {
   const int usual = (w.window + 126) / 128 + 1;
   p->chunk = usual < 8 ? 8 : usual;
   p->chunks = ceil_div(w.q_tiles, p->chunk);
+  // their sums are kept until they are joined: no more chunks than 16 for each SM, of all key tiles together (310 MB at
+  // width 128; 64 sequences x 8 heads x 16384 with 4096 first tokens would take 34 GB)
+  const long long rows = static_cast<long long>(w.batch) * w.kv_heads * p->sink_tiles;
+  if (p->chunks > 1 && rows * p->chunks > 16 * 148) {
+    const long long most = rows < 16 * 148 ? 16 * 148 / rows : 1;
+    p->chunk = static_cast<int>((w.q_tiles + most - 1) / most);
+    p->chunks = ceil_div(w.q_tiles, p->chunk);
+  }
 }
 size_t win_partial_bytes(const WinSizes& w, const WinBwdParams& p) {
   if (p.chunks < 2) return 0;

@@ -10,13 +10,14 @@
 // time straight from memory into the operands of mma.sync (16 slots, then 16
 // channels, by 8 query heads): the score's inner index and the output's rows may
 // come in any order, so each lane's 16-byte loads already are the fragments (the
-// values' pairs of slots take one byte permutation each, the weights one transposition).  tcgen05 would want the
-// tiles in shared memory and 128 rows where there are at most 16.  The warps of a
-// CTA and the CTAs of a cluster go over different slots; their sums, with each
-// one's largest score, are joined through shared memory, in order.  The heads are
-// the products' columns because 8 of them then cost no padding: with the heads as
-// 16 rows the accumulators did not fit into registers (64 sequences x 32 heads of
-// 128 channels, 4160 slots: 332 us; now 190, and 6.2 TB/s where 148 sequences fill the SMs evenly).
+// values' pairs of slots take one byte permutation each, the weights one
+// transposition).  tcgen05 would want the tiles in shared memory and 128 rows where
+// there are at most 16.  The warps of a CTA and the CTAs of a cluster go over
+// different slots; their sums, with each one's largest score, are joined through
+// shared memory, in order.  The heads are the products' columns because 8 of them
+// then cost no padding: with the heads as 16 rows the accumulators did not fit into
+// registers (64 sequences x 32 heads of 128 channels, 4160 slots: 332 us; now 176,
+// 5.4 TB/s, and 6.2 where the sequences fill the SMs evenly).
 #include <cmath>
 
 #include "capi_internal.h"

@@ -17,16 +17,17 @@
 // more is cut into parts by its logits' bits until it is not, or has one value
 // left, whose tokens then count in the order of their index.
 //
-// What bounds it is the number of instructions: about 120 for each logit with
-// top-p (512 rows x 50257: 140 us at 58 % of the issue slots).  The exponential is
-// in 64 bits, which run at half the rate of 32 but need no compensation: the sum of
-// 1.5 2^52 and the product of a logit's difference from the largest has the rounded
-// distance, which is the bin too, in its low word.  Only the pass that fills the
-// histogram takes it of every logit: a cut's bin is found again by its first and
-// last logit, and kept tokens are brought side by side in shared memory before
-// their masses are summed (512 rows x 50257, top-p: 168 -> 140 us; 64 rows x 128257
-// bf16, every filter: 69 -> 62 us).  A mass is right to half a unit and 1e-13 of
-// itself.
+// What bounds it is the number of instructions: 104 for each logit with top-p (512
+// rows x 50257: 140 us at 58 % of the issue slots), 120 with every filter, whose
+// cluster of CTAs also waits at its barriers (64 rows x 128257: 62 us at 50 %).  The
+// exponential is in 64 bits, which run at half the rate of 32 but need no
+// compensation: the sum of 1.5 2^52 and the product of a logit's difference from
+// the largest has the rounded distance, which is the bin too, in its low word.
+// Only the pass that fills the histogram takes it of every logit: a cut's bin is
+// found again by its first and last logit, and kept tokens are brought side by side
+// in shared memory before their masses are summed (512 rows x 50257, top-p: 168 ->
+// 140 us; 64 rows x 128257 bf16, every filter: 69 -> 62 us).  A mass is right to
+// half a unit and 1e-13 of itself.
 #include <cmath>
 #include <type_traits>
 

@@ -216,3 +216,29 @@ def test_workspace_of_many_first_tokens_is_bounded(dim):
         stats = batch * kv_heads * tokens * 4
         got = lib.ts_b200_window_bwd_workspace_bytes(ctypes.byref(a))
         assert stats <= got <= stats + 16 * 148 * 2 * dim * 128 * 4, (batch, kv_heads, tokens, sinks, got - stats)
+
+
+def test_a_stream_begun_in_inference_mode_goes_on_outside():
+    """What a stream keeps is changed in place by later calls, which PyTorch refuses for tensors made in inference mode."""
+    from thetascan_b200 import lm, seqpar
+    model = lm.HybridLM(vocab=16, d_model=64, n_layers=2, n_heads=1, mixer_layers=(1,), window=4,
+                        mixer_config=lm.gn_mixer_config(64, 1))
+    g = torch.Generator().manual_seed(1)
+    q, k, v = (torch.randn(2, 1, 9, n, generator=g) for n in (6, 6, 4))
+
+    def scan(q, k, v, retentions, *, append_unit=False):
+        return [(q @ k.transpose(-1, -2)).tril() @ torch.cat((v, torch.ones_like(v[..., :1])), -1) for _ in retentions]
+
+    def piece(scans, s):
+        with scans.piece(q[:, 0, s]):
+            return seqpar.sharded_reads(scans, scan, q[:, :, s], k[:, :, s], v[:, :, s], (None,), append_unit=True)[0]
+
+    with torch.inference_mode():
+        stream, scans = model.stream(2), seqpar.ScanStream()
+        first = piece(scans, slice(0, 5)).clone()
+    with torch.no_grad():
+        stream.lengths += 3
+        stream.layers[0].keys.zero_()
+        got = torch.cat((first, piece(scans, slice(5, 9))), 2)
+    want, = scan(q, k, v, (None,))
+    assert float((got - want).abs().max()) <= 9 * 6 * 2.0 ** -23 * float(want.abs().max())   # sums of 54 products

@@ -123,3 +123,18 @@ def test_streams_side_by_side(win, sample):  # noqa: F811
     torch.cuda.synchronize()
     for many, one in zip(got, want):
         assert all(torch.equal(a, b) for each in many for a, b in zip(each, one))
+
+
+@gpu
+def test_a_stream_through_inference_mode_and_out_of_it():
+    model = _model(24, 2, gated="silu", fused_norms=True).cuda()
+    tokens = torch.randint(0, 256, (2, 80), generator=torch.Generator().manual_seed(0)).cuda()
+    stream = model.stream(2)
+    want = [model.extend(tokens[:, s], stream) for s in (slice(0, 40), slice(40, 41), slice(41, 80))]
+    for inside in ((True, False, True), (False, True, False), (True, True, False)):
+        with torch.inference_mode(inside[0]):
+            stream = model.stream(2)
+        for one, s, w in zip(inside, (slice(0, 40), slice(40, 41), slice(41, 80)), want):
+            with torch.inference_mode(one):
+                got = model.extend(tokens[:, s], stream)
+            assert torch.equal(got, w)

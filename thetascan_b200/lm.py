@@ -305,6 +305,7 @@ class ModelStream:
     """What a :class:`HybridLM` keeps of its sequences: a ring cache of each
     attention layer, the scan states of each mixer."""
 
+    @torch.inference_mode(False)   # what it keeps is changed in place, in that mode or not
     def __init__(self, model: HybridLM, batch: int):
         if batch < 1:
             raise ValueError(f"a stream needs at least one sequence, got {batch}")

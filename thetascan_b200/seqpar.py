@@ -227,8 +227,9 @@ class ScanStream:
             if self.position:
                 raise RuntimeError("ScanStream: more reads than in the pieces before: another mixer's stream")
             B, H, _, m = keys.shape
-            self.states.append(torch.zeros(B, H, len(retentions), m, payload.shape[-1] + 1, dtype=torch.float32,
-                                           device=keys.device))
+            with torch.inference_mode(False):   # they are changed in place, in that mode or not
+                self.states.append(torch.zeros(B, H, len(retentions), m, payload.shape[-1] + 1, dtype=torch.float32,
+                                               device=keys.device))
         state = self.states[self._next]
         self._next += 1
         if query.shape[2] == 1:

@@ -165,6 +165,7 @@ class WindowCache:
     sequences: ``keys`` and ``values``, without the lengths, which the layers of a
     model share."""
 
+    @torch.inference_mode(False)   # what it keeps is changed in place, in that mode or not
     def __init__(self, batch: int, heads: int, head_dim: int, window: int, sinks: int = 0, *, device=None):
         if window < 1 or sinks < 0:
             raise ValueError(f"window must be >= 1 and sinks >= 0, got {window} and {sinks}")

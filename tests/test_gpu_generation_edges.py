@@ -138,3 +138,25 @@ def test_a_stream_through_inference_mode_and_out_of_it():
             with torch.inference_mode(one):
                 got = model.extend(tokens[:, s], stream)
             assert torch.equal(got, w)
+
+
+@gpu
+@pytest.mark.parametrize("dim", [64, 128])
+def test_scores_of_minus_infinity_alone_give_no_number(win, dim):  # noqa: F811
+    # a row whose visible scores are all minus infinity: 0 / 0, not the zero of a row that sees nothing; in every form
+    g = torch.Generator("cuda").manual_seed(0)
+    q, k, v = (torch.randn(2, 2, 150, dim, generator=g, device="cuda").to(BF16) for _ in range(3))
+    q[1, :, 149] = 0
+    q[1, :, 149, 0] = math.inf
+    k[..., 0] = -1
+    lengths = torch.tensor([100, 150], dtype=torch.int32, device="cuda")
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    y = win.window_attention(*leaves, 40, 2, lengths=lengths)
+    with torch.no_grad():
+        cache = win.WindowCache(2, 2, dim, 40, 2, device="cuda")
+        cache.extend(k[:, :, :149], v[:, :, :149], torch.zeros_like(lengths), new=lengths - 1)
+        step = cache.step(q[:, :, 149:], k[:, :, 149:], v[:, :, 149:], lengths - 1)
+    assert torch.isnan(y[1, :, 149]).all() and torch.isnan(step[1]).all()
+    assert torch.isfinite(y[:, :, :149]).all() and not y[0, :, 100:].any()
+    dq, = torch.autograd.grad(y, leaves[0], torch.ones_like(y))
+    assert torch.isnan(dq[1, :, 149]).all() and torch.isfinite(dq[0]).all() and not dq[0, :, 100:].any()

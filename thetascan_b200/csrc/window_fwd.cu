@@ -549,8 +549,10 @@ __global__ void __launch_bounds__(kFwdThreads, 1) window_fwd_kernel(const __grid
       // exchanges are waits for one another.
       if (!threads_agree<64>(1 + 4 * x + quad, ok)) break;
       tc_fence_after();
-      // a row that sees nothing has no sum: zero
-      const float inverse = sum != 0.f ? 1.f / sum : 0.f;
+      // A row behind its sequence sees nothing: zero.  All others see themselves at least; scores of minus infinity alone
+      // sum to zero there, and 0 / 0 is no number.
+      const bool sees = to >= 0;
+      const float inverse = 1.f / sum;
 #pragma unroll 1
       for (int c = 0; c < kD / 2; c += 32) {
         const int channel = kD / 2 * half + c;
@@ -565,7 +567,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) window_fwd_kernel(const __grid
         for (int i = 0; i < 4; ++i) {
           float f[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) f[e] = inverse != 0.f ? __uint_as_float(o[8 * i + e]) * inverse : 0.f;
+          for (int e = 0; e < 8; ++e) f[e] = sees ? __uint_as_float(o[8 * i + e]) * inverse : 0.f;
           // 64-byte rows, swizzled as the store expects: the 16-byte piece's index XORed with bits 1-2 of the row
           st_shared_v4(stage + 64 * lane + ((i ^ (lane >> 1 & 3)) << 4), pack8(f));
         }
@@ -580,7 +582,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) window_fwd_kernel(const __grid
       tc_fence_before();
       if (p.lse && half == 0) {
         // of the scores in units of log 2; +infinity, which makes every weight zero, for a row that sees nothing
-        const float l = sum != 0.f ? (ref == -INFINITY ? 0.f : ref) + log2f(sum) : INFINITY;
+        const float l = sees ? (ref == -INFINITY ? 0.f : ref) + log2f(sum) : INFINITY;
         p.lse[(static_cast<size_t>(u.b) * w.heads + mine.head) * (128 * static_cast<size_t>(w.q_tiles)) + q_row] = l;
       }
     }

@@ -21,11 +21,11 @@
 // product from there.  S^T = K Q^T and dP^T = V dY^T have
 // keys in the rows, which is how dv and dk need them.
 //
-// Forming p and ds bounds it where tiles are narrow, the products and the turns
-// between the two where they are wide: 64 x 8 heads x 1024, width 64, window 256,
-// sinks 4: 185 us for dq, 220 for dk and dv, 44 % of the issue slots; 16 heads x
-// 16384, width 128, window 2048, sinks 16: 465 and 560 us, tensor cores at work for
-// 43 and 56 % of them.
+// The rows and the products of a tile wait for one another: narrow tiles are mostly
+// forming p and ds, wide ones mostly products: 64 x 8 heads x 1024, width 64, window
+// 256, sinks 4: 188 us for dq, 215 for dk and dv, 45 % of the issue slots, tensor
+// cores at work for 18 and 25 %; 16 heads x 16384, width 128, window 2048, sinks 16:
+// 489 and 576 us, 42 and 38 % of the issue slots, tensor cores 40 and 55 %.
 #include "capi_internal.h"
 #include "window.cuh"
 

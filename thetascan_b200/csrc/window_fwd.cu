@@ -12,7 +12,7 @@
 // or (heads of up to 64) beside it, and is the operand of O += P V from where it
 // lies.  While one group forms its P the tensor cores work for the other: forming
 // P and issuing instructions bound it, not the products (16 heads x 16384, width
-// 128, window 2048, sinks 16: 276 us, 1.0 PFLOP/s of whole tiles; 64 x 8 heads x
+// 128, window 2048, sinks 16: 284 us, 1.0 PFLOP/s of whole tiles; 64 x 8 heads x
 // 1024, width 64, window 256, sinks 4: 115 us, 1.2 TB/s).
 //
 // A row's reference moves only when a score exceeds it by 2^8 (P is then at most
